@@ -54,7 +54,8 @@ extern "C" {
 #define RTXB_TENSOR_SCALE_EXACT 0
 #define RTXB_TENSOR_SCALE_POWER2 1
 
-/* codes a kernel leaves in the caller's `status` word when one of its bounded waits runs out */
+/* codes a kernel leaves in the caller's `status` word when one of its bounded waits runs out (or, the last one, when a
+ * list on the device is not one) */
 #define RTXB_DEV_OK 0
 #define RTXB_DEV_WAIT_PRODUCER 1   /* TMA producer: no free ring slot */
 #define RTXB_DEV_WAIT_MMA 2        /* MMA issuer: operands or accumulator columns never arrived */
@@ -62,6 +63,7 @@ extern "C" {
 #define RTXB_DEV_WAIT_QUANT 4      /* in-kernel quantizer warps */
 #define RTXB_DEV_WAIT_SELFTEST 5   /* rtxb_selftest_wait_timeout */
 #define RTXB_DEV_WAIT_PEER 6       /* rtxb_peer_barrier: another rank's flag never arrived */
+#define RTXB_DEV_GROUP_OFFSETS 7   /* grouped operators: offsets outside [0, rows] or decreasing */
 
 int rtxb_version(void);
 const char* rtxb_error_string(int code);
@@ -240,6 +242,40 @@ size_t rtxb_mxfp8_backward_workspace_bytes(int64_t m, int64_t n, int64_t k);
 int rtxb_mxfp8_linear_bwd(const void* dy_bf16, const void* x_bf16, const void* w_bf16, void* dx_bf16, void* dw,
                           int dw_dtype, int64_t m, int64_t n, int64_t k, void* workspace, size_t workspace_bytes,
                           void* stream, int* status);
+
+/* ---- grouped (experts') MXFP8 linear ----------------------------------------------------------
+ * No counterpart in the reference (its linears are dense).  Rows offsets[g] .. offsets[g + 1] - 1 of x (offsets:
+ * int32 [groups + 1] in device memory, non-decreasing, inside [0, rows]; groups may be empty) belong to group g, whose
+ * weight is w[g] [n, k]:
+ *     out[r] = bf16( deq(q(x[r])) deq(q(w[g]))^T )        both quantized in blocks of 32 along k
+ * Rows before offsets[0] and from offsets[groups] on belong to no group: they are not read and are zero in the result.
+ * The list stays on the device: shapes of the launches depend on rows and groups alone, so a captured graph may be
+ * replayed with other offsets.  Offsets that break the rule are held inside it by the kernels and reported as
+ * RTXB_DEV_GROUP_OFFSETS.  At most 512 groups; x has a row pitch ldx >= k, out a row pitch ldo >= n (elements).
+ * Two launches on `stream`: one quantizer launch (x by group and, for BF16 weights, every weight), one GEMM for all
+ * groups behind it as a programmatic dependent.  workspace: rtxb_mxfp8_grouped_linear_workspace_bytes(rows, n, k,
+ * groups, dynamic_w), dynamic_w = 1 for the BF16 form. */
+size_t rtxb_mxfp8_grouped_linear_workspace_bytes(int64_t rows, int64_t n, int64_t k, int64_t groups, int dynamic_w);
+int rtxb_mxfp8_grouped_linear_fwd(const void* x_bf16, int64_t ldx, const void* w_bf16, const int* offsets, int64_t groups,
+                                  void* out_bf16, int64_t ldo, int64_t rows, int64_t n, int64_t k, int rounding,
+                                  void* workspace, size_t workspace_bytes, void* stream, int* status);
+/* The same with packed weights: qw [groups * n, storage k] and its mma128 scale tiles, the quantization of the weights
+ * viewed as [groups * n, k].  A scale tile covers 128 rows, so more than one group needs n % 128 == 0. */
+int rtxb_mxfp8_grouped_linear_fwd_prequant_w(const void* x_bf16, int64_t ldx, const void* qw, const void* sw,
+                                             const int* offsets, int64_t groups, void* out_bf16, int64_t ldo, int64_t rows,
+                                             int64_t n, int64_t k, int rounding, void* workspace, size_t workspace_bytes,
+                                             void* stream, int* status);
+/* Its backward, the products of rtxb_mxfp8_linear_bwd per group:
+ *     dx[r] = dy[r] w[g]                    operands quantized in blocks of 32 along n
+ *     dw[g] = dy_g^T x_g                    blocks of 32 along the group's rows, counted from its first row
+ * dx BF16 [rows, k] (zero in rows of no group), dw BF16 [groups, n, k] (zero for a group without rows), contiguous;
+ * either may be NULL to leave that product out (then w, respectively x, is not read).  One quantizer launch, one GEMM
+ * per product. */
+size_t rtxb_mxfp8_grouped_backward_workspace_bytes(int64_t rows, int64_t n, int64_t k, int64_t groups, int need_dx,
+                                                   int need_dw);
+int rtxb_mxfp8_grouped_linear_bwd(const void* dy_bf16, int64_t lddy, const void* x_bf16, int64_t ldx, const void* w_bf16,
+                                  const int* offsets, int64_t groups, void* dx_bf16, void* dw_bf16, int64_t rows, int64_t n,
+                                  int64_t k, void* workspace, size_t workspace_bytes, void* stream, int* status);
 
 /* compile_mxfp8_workspace_reduce(m, n, split, algorithm="serial", ...) -> (ws f32 [split, m, n], out bf16)
  *   rtx/kernels/mxfp8_reduce.py:20-104; bound at rtx/fp8_bwd.py:351-386, :464-495.

@@ -58,6 +58,9 @@ _LAZY_EXPORTS = {
     # sm_100a additions
     "mxfp8_glu_mlp": ("glu", "mxfp8_glu_mlp"),
     "SwiGLU": ("glu", "SwiGLU"),
+    "MXFP8GroupedLinear": ("grouped", "MXFP8GroupedLinear"),
+    "mxfp8_grouped_linear": ("grouped", "mxfp8_grouped_linear"),
+    "mxfp8_grouped_linear_backward": ("grouped", "mxfp8_grouped_linear_backward"),
     "quantized_weight_cache": ("weight_cache", "quantized_weight_cache"),
     "KernelAdapter": ("autotune", "KernelAdapter"),
     "data_parallel_linear_backward": ("parallel", "data_parallel_linear_backward"),

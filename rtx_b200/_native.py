@@ -30,6 +30,7 @@ DEVICE_STATUS_NAMES = {
     4: "quantizer wait ran out",
     5: "self-test wait ran out (expected: nothing completes its barrier)",
     6: "node barrier: another rank's flag never arrived",
+    7: "group offsets are not non-decreasing inside [0, rows]",
 }
 
 _P, _I, _L, _Z = c_void_p, c_int, c_int64, c_size_t
@@ -63,6 +64,11 @@ SIGNATURES = {
     "rtxb_mxfp8_glu_mlp_fwd": (_I, [_P, _P, _P, _P, _P, _L, _L, _L, _L, _P, _Z, _P, _P]),
     "rtxb_mxfp8_backward_workspace_bytes": (_Z, [_L, _L, _L]),
     "rtxb_mxfp8_linear_bwd": (_I, [_P, _P, _P, _P, _P, _I, _L, _L, _L, _P, _Z, _P, _P]),
+    "rtxb_mxfp8_grouped_linear_workspace_bytes": (_Z, [_L, _L, _L, _L, _I]),
+    "rtxb_mxfp8_grouped_linear_fwd": (_I, [_P, _L, _P, _P, _L, _P, _L, _L, _L, _L, _I, _P, _Z, _P, _P]),
+    "rtxb_mxfp8_grouped_linear_fwd_prequant_w": (_I, [_P, _L, _P, _P, _P, _L, _P, _L, _L, _L, _L, _I, _P, _Z, _P, _P]),
+    "rtxb_mxfp8_grouped_backward_workspace_bytes": (_Z, [_L, _L, _L, _L, _I, _I]),
+    "rtxb_mxfp8_grouped_linear_bwd": (_I, [_P, _L, _P, _L, _P, _P, _L, _P, _P, _L, _L, _L, _P, _Z, _P, _P]),
     "rtxb_sum_parts_f32_to_bf16": (_I, [_P, _I, _L, _L, _P, _P]),
     "rtxb_selftest_wait_timeout": (_I, [_L, _P, _P, _P]),
     "rtxb_peer_barrier": (_I, [_P, _I, _I, _P, _L, _P, _P]),

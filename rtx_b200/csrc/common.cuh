@@ -23,6 +23,7 @@ enum DeviceStatus : int {
   kStatusWaitQuant = 4,      // quantizer warps gave up waiting for a BF16 tile
   kStatusWaitSelfTest = 5,   // the wait self-test's barrier (which nothing ever completes) ran out, as it must
   kStatusWaitPeer = 6,       // node barrier: another rank's flag never arrived
+  kStatusGroupOffsets = 7,   // grouped operators: offsets not non-decreasing inside [0, rows] (held inside by the kernel)
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {

@@ -1,0 +1,305 @@
+// extern "C" entry points of the grouped (experts') MXFP8 linear: argument checks, workspace layout, launches.
+#include "launch.cuh"
+#include "gemm_grouped.cuh"
+#include "grouped.cuh"
+
+using namespace rtxb;
+
+namespace {
+
+// output [groups][rows][cols] of BF16, row pitch ldo and group pitch `group_elems` elements; boxes of 32 rows x 32
+// columns in the 64-byte swizzle the epilogue stages
+int make_out_map_groups(CUtensorMap* map, const void* base, int64_t groups, int64_t rows, int64_t cols, int64_t ldo,
+                        int64_t group_elems) {
+  MapKey k = blank_key(base);
+  k.rank = 3;
+  k.words = 2;
+  k.dim[0] = static_cast<uint64_t>(cols);
+  k.dim[1] = static_cast<uint64_t>(rows);
+  k.dim[2] = static_cast<uint64_t>(groups);
+  k.stride[0] = static_cast<uint64_t>(ldo) * 2;
+  k.stride[1] = static_cast<uint64_t>(group_elems) * 2;
+  k.box[0] = 32u;
+  k.box[1] = 32u;
+  k.box[2] = 1u;
+  return encode_map(map, k, "grouped output");
+}
+
+// most 128-row (256-row) tiles that `groups` groups of `rows` rows in all can have: a started tile per group that has
+// rows, beside the full ones
+int64_t most_tiles(int64_t rows, int64_t groups, int64_t tile) { return rows / tile + (groups < rows ? groups : rows); }
+
+struct Operand {
+  const void* q;
+  const void* s;
+  int64_t rows;        // rows of its tensor map
+  int64_t sf_tiles;    // 512-byte scale tiles in all
+};
+
+int launch_grouped(GroupedGemmParams p, const Operand& a, const Operand& b, int64_t row_bytes_a, int64_t row_bytes_b,
+                   int64_t out_groups, int64_t out_rows, int64_t most, cudaStream_t stream) {
+  using P = PairTraits<kKindMxfp8>;
+  constexpr int KS = P::kStepsPerBarrierP;
+  CUtensorMap map_a, map_sfa, map_sfb, map_out;
+  GroupedMapsB maps_b;
+  int rc;
+  p.map3d = row_bytes_a % 128 == 0 && row_bytes_b % 128 == 0;
+  if (p.map3d) rc = make_payload_map_ksteps(&map_a, a.q, a.rows, row_bytes_a, 128, KS);
+  else rc = make_payload_map(&map_a, a.q, a.rows, row_bytes_a, 128);
+  for (int i = 0; i < 4 && !rc; ++i) {
+    if (p.map3d) rc = make_payload_map_ksteps(&maps_b.m[i], b.q, b.rows, row_bytes_b, 128 >> i, KS);
+    else rc = make_payload_map(&maps_b.m[i], b.q, b.rows, row_bytes_b, 128 >> i);
+  }
+  if (rc || (rc = make_scale_map(&map_sfa, a.s, a.sf_tiles, KS)) || (rc = make_scale_map(&map_sfb, b.s, b.sf_tiles, KS)))
+    return rc;
+  p.tma_out = aligned(p.out, 16) && (p.ldo * 2) % 16 == 0;
+  memset(&map_out, 0, sizeof(map_out));
+  if (p.tma_out && (rc = make_out_map_groups(&map_out, p.out, out_groups, out_rows, p.out_cols, p.ldo,
+                                             out_groups > 1 ? p.out_group : p.ldo * out_rows)))
+    return rc;
+  cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(gemm_grouped_pair_kernel), P::kSmemBytes);
+  if (e != cudaSuccess) return fail_cuda(e, "cudaFuncSetAttribute(grouped gemm)");
+  const int64_t max_pairs = sm_count() / 2;
+  const int pairs = static_cast<int>(most < max_pairs ? most : max_pairs);
+  e = launch_dependent(gemm_grouped_pair_kernel, 2 * pairs, kGemmThreads, P::kSmemBytes, stream, true, map_a, maps_b, map_sfa,
+                       map_sfb, map_out, p);
+  if (e != cudaSuccess) return fail_cuda(e, "gemm_grouped_pair_kernel launch");
+  return RTXB_OK;
+}
+
+int check_grouped(const int* offsets, int64_t rows, int64_t n, int64_t k, int64_t groups) {
+  if (!offsets) return fail_msg(RTXB_E_INVALID_ARGUMENT, "null offsets");
+  if (!aligned(offsets, 4)) return fail_msg(RTXB_E_ALIGNMENT, "offsets must be int32 aligned");
+  if (rows <= 0 || n <= 0 || k <= 0 || groups <= 0) return fail_msg(RTXB_E_INVALID_ARGUMENT, "rows, n, k, groups must be positive");
+  if (groups > kMaxGroups) return fail_msg(RTXB_E_UNSUPPORTED, "at most 512 groups");
+  // tile numbers, rows of the tensor maps and columns of the transposed operands are 32-bit
+  const int64_t lim = INT32_MAX / 2;
+  const int64_t rt = most_tiles(rows, groups, 128), nt = (n + 127) / 128, kt = (k + 127) / 128;
+  if (rows > lim || n > lim || k > lim || groups * n > lim || groups * k > lim || rt * 128 > lim || rt * nt > lim ||
+      rt * kt > lim || groups * nt * kt > lim)
+    return fail_msg(RTXB_E_UNSUPPORTED, "grouped operand exceeds the 32-bit tile count");
+  return RTXB_OK;
+}
+
+size_t scale_tiles_bytes(int64_t row_tiles, int64_t k) { return static_cast<size_t>(row_tiles * ((round_up(k, 32) / 32 + 3) / 4) * 512); }
+
+// the plan in a workspace
+struct PlanMemory {
+  GroupPlan plan;
+  PlanMemory(Carver& c, int64_t rows, int64_t groups) {
+    plan.row_tiles = reinterpret_cast<int*>(c.take(16));
+    plan.tiles = reinterpret_cast<int4*>(c.take(most_tiles(rows, groups, 256) * sizeof(int4)));
+    plan.k_tiles = reinterpret_cast<int*>(c.take((groups + 1) * sizeof(int)));
+  }
+};
+
+struct FwdMemory {
+  PlanMemory plan;
+  uint8_t *qx, *sx, *qw, *sw;
+  FwdMemory(Carver& c, int64_t rows, int64_t n, int64_t k, int64_t groups, bool dynamic_w) : plan(c, rows, groups) {
+    qx = c.take(rows * round_up(k, 32));
+    sx = c.take(scale_tiles_bytes(most_tiles(rows, groups, 128), k));
+    qw = dynamic_w ? c.take(groups * n * round_up(k, 32)) : nullptr;
+    sw = dynamic_w ? c.take(scale_tiles_bytes(groups * ((n + 127) / 128), k)) : nullptr;
+  }
+};
+
+struct BwdMemory {
+  PlanMemory plan;
+  uint8_t *q_dy = nullptr, *s_dy = nullptr, *q_wt = nullptr, *s_wt = nullptr;   // dX
+  uint8_t *q_dyt = nullptr, *s_dyt = nullptr, *q_xt = nullptr, *s_xt = nullptr; // dW
+  BwdMemory(Carver& c, int64_t rows, int64_t n, int64_t k, int64_t groups, bool need_dx, bool need_dw)
+      : plan(c, rows, groups) {
+    const int64_t tiles = most_tiles(rows, groups, 128);
+    if (need_dx) {
+      q_dy = c.take(rows * round_up(n, 32));
+      s_dy = c.take(scale_tiles_bytes(tiles, n));
+      q_wt = c.take(groups * k * round_up(n, 32));
+      s_wt = c.take(scale_tiles_bytes(groups * ((k + 127) / 128), n));
+    }
+    if (need_dw) {
+      q_dyt = c.take(n * tiles * 128);
+      s_dyt = c.take((n + 127) / 128 * tiles * 512);
+      q_xt = c.take(k * tiles * 128);
+      s_xt = c.take((k + 127) / 128 * tiles * 512);
+    }
+  }
+};
+
+QuantMxParams rows_params(const void* src, int64_t rows, int64_t k, int64_t ld, void* q, void* s, int rounding) {
+  QuantMxParams p = {};
+  p.src = static_cast<const __nv_bfloat16*>(src);
+  p.q = static_cast<uint8_t*>(q);
+  p.scales = static_cast<uint8_t*>(s);
+  p.rows = static_cast<int>(rows);
+  p.k = static_cast<int>(k);
+  p.kp = static_cast<int>(round_up(k, 32));
+  p.ld = ld;
+  p.nb = p.kp / 32;
+  p.sf_chunks = (p.nb + 3) / 4;
+  p.layout = RTXB_SCALE_MMA128;
+  p.round_to_infinity = rounding != RTXB_ROUND_FLOOR;
+  return p;
+}
+
+GroupedGemmParams gemm_params(const GroupPlan& plan, void* out, int64_t ldo, int64_t out_cols, int* status) {
+  GroupedGemmParams g = {};
+  g.plan_rows = plan.row_tiles;
+  g.plan_tiles = plan.tiles;
+  g.plan_k = plan.k_tiles;
+  g.out = static_cast<__nv_bfloat16*>(out);
+  g.ldo = ldo;
+  g.out_cols = static_cast<int>(out_cols);
+  g.status = status;
+  return g;
+}
+
+// D[r, a] = sum_k B[r, k] A_g[a, k]
+int launch_rows_form(const GroupPlan& plan, const void* q_rows, const void* s_rows, int64_t rows, const void* qa,
+                     const void* sa, int64_t a_rows, int64_t k, int64_t groups, void* out, int64_t ldo, int* status,
+                     cudaStream_t stream) {
+  const int64_t kp = round_up(k, 32), chunks = (kp / 32 + 3) / 4, a_sf = (a_rows + 127) / 128;
+  GroupedGemmParams g = gemm_params(plan, out, ldo, a_rows, status);
+  g.a_rows = static_cast<int>(a_rows);
+  g.a_tiles = static_cast<int>((a_rows + 255) / 256);
+  g.a_sf_tiles = static_cast<int>(a_sf);
+  g.groups = static_cast<int>(groups);
+  g.k_tiles = static_cast<int>((kp + 127) / 128);
+  g.sf_chunks_a = g.sf_chunks_b = static_cast<int>(chunks);
+  const Operand a{qa, sa, groups * a_rows, groups * a_sf * chunks};
+  const Operand b{q_rows, s_rows, rows, most_tiles(rows, groups, 128) * chunks};
+  return launch_grouped(g, a, b, kp, kp, 1, rows, most_tiles(rows, groups, 256) * g.a_tiles, stream);
+}
+
+int grouped_fwd(const void* x, int64_t ldx, const void* w, const void* qw, const void* sw, const int* offsets,
+                int64_t groups, void* out, int64_t ldo, int64_t rows, int64_t n, int64_t k, int rounding, void* workspace,
+                size_t workspace_bytes, void* stream, int* status) {
+  int rc = check_grouped(offsets, rows, n, k, groups);
+  if (rc) return rc;
+  if (!x || !out || !(w || (qw && sw))) return fail_msg(RTXB_E_INVALID_ARGUMENT, "null operand");
+  if (ldx < k || ldo < n) return fail_msg(RTXB_E_INVALID_ARGUMENT, "row pitch smaller than the row");
+  if (!aligned(x, 2) || !aligned(out, 2) || (w && !aligned(w, 2)))
+    return fail_msg(RTXB_E_ALIGNMENT, "pointer is not element aligned");
+  Carver c(workspace);
+  FwdMemory mem(c, rows, n, k, groups, w != nullptr);
+  if (!workspace || workspace_bytes < c.off) return fail_msg(RTXB_E_WORKSPACE, "workspace too small for the grouped forward");
+  if (!aligned(workspace, 256)) return fail_msg(RTXB_E_ALIGNMENT, "workspace must be 256-byte aligned");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  GroupedRowsParams q = {};
+  q.x = rows_params(x, rows, k, ldx, mem.qx, mem.sx, rounding);
+  q.list = GroupList{offsets, static_cast<int>(groups), static_cast<int>(rows)};
+  const int64_t col_tiles = (q.x.kp + 127) / 128;
+  int64_t tiles = most_tiles(rows, groups, 128) * col_tiles;
+  if (w) {
+    q.w = rows_params(w, n, k, k, mem.qw, mem.sw, rounding);
+    q.batches = static_cast<int>(groups);
+    tiles += groups * ((n + 127) / 128) * col_tiles;
+    qw = mem.qw;
+    sw = mem.sw;
+  }
+  q.plan = mem.plan.plan;
+  q.out = static_cast<__nv_bfloat16*>(out);
+  q.out_cols = static_cast<int>(n);
+  q.ldo = ldo;
+  q.status = status;
+  quant_mxfp8_grouped_rows_kernel<<<quant_grid(tiles, 6), kQuantThreads, 0, s>>>(q);
+  RTXB_CHECK_LAUNCH("quant_mxfp8_grouped_rows_kernel");
+  return launch_rows_form(mem.plan.plan, mem.qx, mem.sx, rows, qw, sw, n, k, groups, out, ldo, status, s);
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t rtxb_mxfp8_grouped_linear_workspace_bytes(int64_t rows, int64_t n, int64_t k, int64_t groups, int dynamic_w) {
+  Carver c(nullptr);
+  FwdMemory mem(c, rows, n, k, groups, dynamic_w != 0);
+  return c.off;
+}
+
+int rtxb_mxfp8_grouped_linear_fwd(const void* x, int64_t ldx, const void* w, const int* offsets, int64_t groups, void* out,
+                                  int64_t ldo, int64_t rows, int64_t n, int64_t k, int rounding, void* workspace,
+                                  size_t workspace_bytes, void* stream, int* status) {
+  if (!w) return fail_msg(RTXB_E_INVALID_ARGUMENT, "null operand");
+  return grouped_fwd(x, ldx, w, nullptr, nullptr, offsets, groups, out, ldo, rows, n, k, rounding, workspace, workspace_bytes,
+                     stream, status);
+}
+
+int rtxb_mxfp8_grouped_linear_fwd_prequant_w(const void* x, int64_t ldx, const void* qw, const void* sw, const int* offsets,
+                                             int64_t groups, void* out, int64_t ldo, int64_t rows, int64_t n, int64_t k,
+                                             int rounding, void* workspace, size_t workspace_bytes, void* stream,
+                                             int* status) {
+  if (!qw || !sw) return fail_msg(RTXB_E_INVALID_ARGUMENT, "null operand");
+  if (groups > 1 && n % 128 != 0)
+    return fail_msg(RTXB_E_UNSUPPORTED, "packed group weights need n % 128 == 0 (scale tiles of 128 rows per group)");
+  if (!aligned(qw, 16) || !aligned(sw, 16)) return fail_msg(RTXB_E_ALIGNMENT, "packed operands must be 16-byte aligned");
+  return grouped_fwd(x, ldx, nullptr, qw, sw, offsets, groups, out, ldo, rows, n, k, rounding, workspace, workspace_bytes,
+                     stream, status);
+}
+
+size_t rtxb_mxfp8_grouped_backward_workspace_bytes(int64_t rows, int64_t n, int64_t k, int64_t groups, int need_dx,
+                                                   int need_dw) {
+  Carver c(nullptr);
+  BwdMemory mem(c, rows, n, k, groups, need_dx != 0, need_dw != 0);
+  return c.off;
+}
+
+int rtxb_mxfp8_grouped_linear_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w,
+                                  const int* offsets, int64_t groups, void* dx, void* dw, int64_t rows, int64_t n, int64_t k,
+                                  void* workspace, size_t workspace_bytes, void* stream, int* status) {
+  int rc = check_grouped(offsets, rows, n, k, groups);
+  if (rc) return rc;
+  if (!dy || (!dx && !dw) || (dx && !w) || (dw && !x)) return fail_msg(RTXB_E_INVALID_ARGUMENT, "null operand");
+  if (lddy < n || (dw && ldx < k)) return fail_msg(RTXB_E_INVALID_ARGUMENT, "row pitch smaller than the row");
+  if (!aligned(dy, 2) || !aligned(x, 2) || !aligned(w, 2) || !aligned(dx, 2) || !aligned(dw, 2))
+    return fail_msg(RTXB_E_ALIGNMENT, "pointer is not element aligned");
+  Carver c(workspace);
+  BwdMemory mem(c, rows, n, k, groups, dx != nullptr, dw != nullptr);
+  if (!workspace || workspace_bytes < c.off) return fail_msg(RTXB_E_WORKSPACE, "workspace too small for the grouped backward");
+  if (!aligned(workspace, 256)) return fail_msg(RTXB_E_ALIGNMENT, "workspace must be 256-byte aligned");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int64_t tiles128 = most_tiles(rows, groups, 128), nt = (n + 127) / 128, kt = (k + 127) / 128;
+  GroupedBackwardParams q = {};
+  q.list = GroupList{offsets, static_cast<int>(groups), static_cast<int>(rows)};
+  q.dy = GroupedSource{static_cast<const __nv_bfloat16*>(dy), static_cast<int>(n), lddy, mem.q_dy, mem.s_dy, mem.q_dyt, mem.s_dyt};
+  if (dw) q.x = GroupedSource{static_cast<const __nv_bfloat16*>(x), static_cast<int>(k), ldx, nullptr, nullptr, mem.q_xt, mem.s_xt};
+  q.pitch_t = tiles128 * 128;
+  q.chunks_t = static_cast<int>(tiles128);
+  q.n = static_cast<int>(n);
+  q.k = static_cast<int>(k);
+  if (dx) {
+    q.w = static_cast<const __nv_bfloat16*>(w);
+    q.q_wt = mem.q_wt;
+    q.s_wt = mem.s_wt;
+    q.batches = static_cast<int>(groups);
+    q.dx = static_cast<__nv_bfloat16*>(dx);
+    q.lddx = k;
+  }
+  q.plan = mem.plan.plan;
+  q.status = status;
+  const int64_t tiles = tiles128 * nt + (dw ? tiles128 * kt : 0) + (dx ? groups * nt * kt : 0);
+  cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(quant_mxfp8_grouped_backward_kernel), kQtSmemBytes);
+  if (e != cudaSuccess) return fail_cuda(e, "cudaFuncSetAttribute(grouped backward quantizer)");
+  quant_mxfp8_grouped_backward_kernel<<<quant_grid(tiles, kQtOccupancy), kQuantThreads, kQtSmemBytes, s>>>(q);
+  RTXB_CHECK_LAUNCH("quant_mxfp8_grouped_backward_kernel");
+  if (dx && (rc = launch_rows_form(mem.plan.plan, mem.q_dy, mem.s_dy, rows, mem.q_wt, mem.s_wt, k, n, groups, dx, k, status, s)))
+    return rc;
+  if (dw) {
+    // dW_g[n, k] = sum over the rows of g: operand A = X^T (output columns), operand B = dY^T (output rows)
+    GroupedGemmParams g = gemm_params(mem.plan.plan, dw, k, k, status);
+    g.contraction = 1;
+    g.a_rows = static_cast<int>(k);
+    g.a_tiles = static_cast<int>((k + 255) / 256);
+    g.b_rows = static_cast<int>(n);
+    g.b_tiles = static_cast<int>((n + 255) / 256);
+    g.groups = static_cast<int>(groups);
+    g.sf_chunks_a = g.sf_chunks_b = static_cast<int>(tiles128);
+    g.out_group = n * k;
+    const Operand a{mem.q_xt, mem.s_xt, k, kt * tiles128};
+    const Operand b{mem.q_dyt, mem.s_dyt, n, nt * tiles128};
+    return launch_grouped(g, a, b, tiles128 * 128, tiles128 * 128, groups, n, groups * g.a_tiles * g.b_tiles, s);
+  }
+  return RTXB_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,371 @@
+// Operands split into groups of consecutive rows (the experts of a mixture): the list of groups, and the MXFP8
+// quantizers that lay a grouped operand out for the grouped GEMM (gemm_grouped.cuh).
+//
+// Group g holds rows offsets[g] .. offsets[g + 1] - 1.  Two things have to start on a 128-row boundary for the
+// block-scaled MMA: the 512-byte scale tiles (128 rows each) when the rows are an MMA operand's rows, and the K steps
+// (128 bytes) when the rows are the contraction (dW).  The payload of a row operand needs no such boundary, because a
+// TMA box may start at any row.  So
+//   rows        payload stays in place, [rows, kp]; scale tiles are counted per group: tile[g] .. tile[g + 1] - 1;
+//   transposed  payload and scales are [columns, 128 * tiles], group g at columns 128 * tile[g], zero behind its end:
+//               one 128-byte K step is one 128-row tile, one 512-byte scale tile belongs to it.
+// Rows of no group are never read; the kernels here set them to zero in the result.
+#pragma once
+
+#include "quant_tiles.cuh"
+
+namespace rtxb {
+
+constexpr int kMaxGroups = 512;   // the list is scanned in shared memory beside the staged tiles (4 KB at 512)
+
+struct GroupList {
+  const int* offsets;   // [groups + 1]
+  int groups;
+  int rows;             // rows of the operand; offsets are held inside [0, rows] and non-decreasing
+};
+
+struct GroupScan {
+  int start[kMaxGroups + 1];   // first row of the group; [groups] = end of the last one
+  int tile[kMaxGroups + 1];    // 128-row tiles of the groups before it
+  int warp_part[8];
+};
+
+// What the quantizer leaves for the GEMM behind it (global memory, written by block 0).
+struct GroupPlan {
+  int* row_tiles;    // [0] = number of 256-row tiles over all groups
+  int4* tiles;       // per 256-row tile: {first row, live rows, first scale tile, group}
+  int* k_tiles;      // [groups + 1] = GroupScan::tile
+};
+
+__device__ __forceinline__ int block_scan_max(int v, int* part) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int o = __shfl_up_sync(0xffffffffu, v, d);
+    if (lane >= d) v = max(v, o);
+  }
+  if (lane == 31) part[warp] = v;
+  __syncthreads();
+  for (int w = 0; w < warp; ++w) v = max(v, part[w]);
+  __syncthreads();
+  return v;   // inclusive
+}
+__device__ __forceinline__ int block_scan_sum(int v, int* part) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int o = __shfl_up_sync(0xffffffffu, v, d);
+    if (lane >= d) v += o;
+  }
+  if (lane == 31) part[warp] = v;
+  __syncthreads();
+  for (int w = 0; w < warp; ++w) v += part[w];
+  __syncthreads();
+  return v;   // inclusive
+}
+
+// All kQuantThreads threads of a block: the list from memory into `s`.  Offsets outside [0, rows] or below an earlier
+// one are brought back inside (and reported in the status word), so that no list makes a kernel leave its buffers.
+__device__ __forceinline__ void scan_groups(const GroupList& l, GroupScan& s, int* status) {
+  constexpr int kPer = (kMaxGroups + 1 + kQuantThreads - 1) / kQuantThreads;
+  const int first = threadIdx.x * kPer;
+  int v[kPer], m = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int raw = first + i <= l.groups ? l.offsets[first + i] : 0;
+    v[i] = raw;
+    m = max(m, min(raw, l.rows));
+  }
+  const int incl = block_scan_max(m, s.warp_part);
+  const int lane = threadIdx.x & 31;
+  // exclusive value of this thread: the inclusive one of the thread before it
+  __shared__ int edge[kQuantThreads / 32];
+  if (lane == 31) edge[threadIdx.x >> 5] = incl;
+  int run = __shfl_up_sync(0xffffffffu, incl, 1);
+  __syncthreads();
+  if (lane == 0) run = threadIdx.x ? edge[(threadIdx.x >> 5) - 1] : 0;
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    run = max(run, min(v[i], l.rows));
+    if (first + i <= l.groups) {
+      s.start[first + i] = run;
+      bad |= run != v[i];
+    }
+  }
+  if (bad && status && blockIdx.x == 0) atomicCAS(status, 0, kStatusGroupOffsets);
+  __syncthreads();
+  int n[kPer], sum = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    n[i] = first + i < l.groups ? (s.start[first + i + 1] - s.start[first + i] + 127) >> 7 : 0;
+    sum += n[i];
+  }
+  int before = block_scan_sum(sum, s.warp_part) - sum;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    if (first + i <= l.groups) s.tile[first + i] = before;
+    before += n[i];
+  }
+  __syncthreads();
+}
+
+// the last group g with before[g] <= t, where before[] counts the tiles of the groups ahead of each group: the one
+// that holds tile t
+__device__ __forceinline__ int group_before(const int* before, int groups, int t) {
+  int lo = 0, hi = groups;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (before[mid] <= t) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+// The plan for the GEMM behind the quantizer, written by one block; `wide` is shared scratch of kMaxGroups + 1 ints.
+__device__ __forceinline__ void write_group_plan(const GroupList& l, GroupScan& s, const GroupPlan& plan, int* wide) {
+  constexpr int kPer = (kMaxGroups + 1 + kQuantThreads - 1) / kQuantThreads;
+  const int first = threadIdx.x * kPer;
+  int n[kPer], sum = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    n[i] = first + i < l.groups ? (s.start[first + i + 1] - s.start[first + i] + 255) >> 8 : 0;
+    sum += n[i];
+  }
+  int before = block_scan_sum(sum, s.warp_part) - sum;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    if (first + i <= l.groups) {
+      wide[first + i] = before;
+      plan.k_tiles[first + i] = s.tile[first + i];
+    }
+    before += n[i];
+  }
+  __syncthreads();
+  const int total = wide[l.groups];
+  if (threadIdx.x == 0) plan.row_tiles[0] = total;
+  for (int t = threadIdx.x; t < total; t += kQuantThreads) {
+    const int g = group_before(wide, l.groups, t);
+    const int j = t - wide[g], row = s.start[g] + 256 * j;
+    plan.tiles[t] = make_int4(row, min(256, s.start[g + 1] - row), s.tile[g] + 2 * j, g);
+  }
+  __syncthreads();
+}
+
+// rows of no group: zero in `out` [rows, cols]
+__device__ __forceinline__ void zero_rows_of_no_group(const GroupList& l, const GroupScan& s, __nv_bfloat16* out,
+                                                      int cols, int64_t ldo) {
+  const int head = s.start[0], dead = head + l.rows - s.start[l.groups];
+  const bool vec = (reinterpret_cast<uintptr_t>(out) & 15) == 0 && ldo % 8 == 0;
+  for (int i = blockIdx.x; i < dead; i += gridDim.x) {
+    const int row = i < head ? i : s.start[l.groups] + i - head;
+    __nv_bfloat16* dst = out + static_cast<int64_t>(row) * ldo;
+    const int vecs = vec ? cols / 8 : 0;
+    for (int c = threadIdx.x; c < vecs; c += blockDim.x) reinterpret_cast<uint4*>(dst)[c] = make_uint4(0, 0, 0, 0);
+    for (int c = vecs * 8 + threadIdx.x; c < cols; c += blockDim.x) dst[c] = __float2bfloat16_rn(0.0f);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Forward operands in one launch: the rows of x by group, then (dynamic weights) the `batches` weight matrices
+// [w.rows, k], each with scale tiles of its own.
+// ---------------------------------------------------------------------------
+struct GroupedRowsParams {
+  QuantMxParams x;            // scales: 128-row tiles counted per group
+  GroupList list;
+  QuantMxParams w;            // one matrix; src nullptr = packed weights, nothing to do
+  int batches;
+  GroupPlan plan;
+  __nv_bfloat16* out;         // result whose rows of no group become zero
+  int out_cols;
+  int64_t ldo;
+  int* status;
+};
+
+__global__ void __launch_bounds__(kQuantThreads, 6) quant_mxfp8_grouped_rows_kernel(const GroupedRowsParams p) {
+  __shared__ GroupScan scan;
+  __shared__ __align__(16) uint8_t tile_scales[128][4];
+  griddep_launch_dependents();
+  scan_groups(p.list, scan, p.status);
+  if (blockIdx.x == 0) {
+    __shared__ int wide[kMaxGroups + 1];
+    write_group_plan(p.list, scan, p.plan, wide);
+  }
+  zero_rows_of_no_group(p.list, scan, p.out, p.out_cols, p.ldo);
+  const int col_tiles = (p.x.kp + 127) / 128;
+  const int x_tiles = scan.tile[p.list.groups] * col_tiles;
+  const int w_row_tiles = (p.w.rows + 127) / 128;
+  const int w_tiles = p.w.src ? w_row_tiles * col_tiles : 0;   // per matrix
+  const int64_t total = x_tiles + static_cast<int64_t>(p.batches) * w_tiles;
+  for (int64_t t = blockIdx.x; t < total; t += gridDim.x) {
+    if (t < x_tiles) {
+      const int rt = static_cast<int>(t) / col_tiles, ct = static_cast<int>(t) - rt * col_tiles;
+      const int g = group_before(scan.tile, p.list.groups, rt);
+      const int64_t row0 = scan.start[g] + 128 * (rt - scan.tile[g]);
+      QuantMxParams q = p.x;
+      q.src += row0 * q.ld;
+      q.q += row0 * q.kp;
+      q.scales += static_cast<size_t>(rt) * q.sf_chunks * 512;
+      q.rows = min(128, scan.start[g + 1] - static_cast<int>(row0));
+      quant_mxfp8_rows_tile(q, ct, tile_scales);
+    } else {
+      const int64_t u = t - x_tiles;
+      const int64_t e = u / w_tiles;
+      QuantMxParams q = p.w;
+      q.src += e * q.rows * q.ld;
+      q.q += e * q.rows * q.kp;
+      q.scales += static_cast<size_t>(e) * w_row_tiles * q.sf_chunks * 512;
+      quant_mxfp8_rows_tile(q, static_cast<int>(u - e * w_tiles), tile_scales);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Backward operands in one launch, all walked as 128 x 128 tiles of their source:
+//   dy   by group: rows (blocks along n, for dX) and transposed (blocks along the tokens, for dW), one read;
+//   x    by group: transposed (for dW);
+//   w    `batches` matrices [n, k]: transposed (blocks along n, for dX), each with scale tiles of its own.
+// A null destination leaves that product out.
+// ---------------------------------------------------------------------------
+struct GroupedSource {
+  const __nv_bfloat16* src;   // nullptr = absent
+  int cols;
+  int64_t ld;
+  uint8_t* q_rows;            // [rows, round_up(cols, 32)]
+  uint8_t* s_rows;
+  uint8_t* q_t;               // [cols, pitch_t]
+  uint8_t* s_t;               // [ceil(cols / 128)][chunks_t][512]
+};
+struct GroupedBackwardParams {
+  GroupedSource dy, x;
+  GroupList list;
+  int64_t pitch_t;            // 128 * (most tiles the list can have)
+  int chunks_t;               // pitch_t / 128
+  const __nv_bfloat16* w;     // nullptr = absent
+  uint8_t* q_wt;              // [batches][k, round_up(n, 32)]
+  uint8_t* s_wt;
+  int batches, n, k;
+  GroupPlan plan;
+  __nv_bfloat16* dx;          // result whose rows of no group become zero; nullptr = none
+  int64_t lddx;
+  int* status;
+};
+
+// one tile: where it is read and where its two quantizations go
+struct BackwardTile {
+  QuantMxTParams f;           // what the fetch needs (src, rows = source columns, k = live source rows, ld)
+  int row0;                   // first source column
+  uint8_t* q_t;
+  uint8_t* s_t;
+  int64_t pitch_t;            // payload pitch and limit of q_t
+  int k0, chunks_t, blk0;
+  uint8_t* q_rows;
+  uint8_t* s_rows;
+};
+
+__device__ __forceinline__ BackwardTile backward_tile(const GroupedBackwardParams& p, const GroupScan& scan, int64_t t,
+                                                      int dy_tiles, int x_tiles, int w_tiles) {
+  BackwardTile b;
+  if (t < dy_tiles + static_cast<int64_t>(x_tiles)) {
+    const bool is_x = t >= dy_tiles;
+    const GroupedSource& s = is_x ? p.x : p.dy;
+    const int u = static_cast<int>(is_x ? t - dy_tiles : t);
+    const int ct = (s.cols + 127) / 128;
+    const int rt = u / ct;
+    const int g = group_before(scan.tile, p.list.groups, rt);
+    const int64_t first = scan.start[g] + 128 * (rt - scan.tile[g]);
+    const int chunks_rows = ((s.cols + 31) / 32 + 3) / 4, np = (s.cols + 31) / 32 * 32;
+    b.row0 = (u - rt * ct) * 128;
+    b.f.src = s.src + first * s.ld;
+    b.f.rows = s.cols;
+    b.f.k = min(128, scan.start[g + 1] - static_cast<int>(first));
+    b.f.ld = s.ld;
+    b.q_t = s.q_t ? s.q_t + static_cast<int64_t>(rt) * 128 : nullptr;
+    b.s_t = s.s_t;
+    b.pitch_t = p.pitch_t;
+    b.k0 = 0;
+    b.chunks_t = p.chunks_t;
+    b.blk0 = rt * 4;
+    b.q_rows = s.q_rows ? s.q_rows + first * np : nullptr;
+    b.s_rows = s.q_rows ? s.s_rows + static_cast<size_t>(rt) * chunks_rows * 512 : nullptr;
+  } else {
+    const int64_t u = t - dy_tiles - x_tiles;
+    const int64_t e = u / w_tiles;
+    const int v = static_cast<int>(u - e * w_tiles);
+    const int ct = (p.k + 127) / 128, np = (p.n + 31) / 32 * 32;
+    const int nt = v / ct;
+    b.row0 = (v - nt * ct) * 128;
+    b.f.src = p.w + (e * p.n + 128 * nt) * p.k;
+    b.f.rows = p.k;
+    b.f.k = min(128, p.n - 128 * nt);
+    b.f.ld = p.k;
+    b.q_t = p.q_wt + e * p.k * np;
+    b.pitch_t = np;
+    b.k0 = 128 * nt;
+    b.chunks_t = (np / 32 + 3) / 4;
+    b.s_t = p.s_wt + static_cast<size_t>(e) * ct * b.chunks_t * 512;
+    b.blk0 = nt * 4;
+    b.q_rows = b.s_rows = nullptr;
+  }
+  return b;
+}
+
+__global__ void __launch_bounds__(kQuantThreads, kQtOccupancy)
+quant_mxfp8_grouped_backward_kernel(const GroupedBackwardParams p) {
+  extern __shared__ __align__(16) uint8_t qt_smem[];
+  uint16_t (*tiles[2])[kQtPitch] = {reinterpret_cast<uint16_t (*)[kQtPitch]>(qt_smem),
+                                    reinterpret_cast<uint16_t (*)[kQtPitch]>(qt_smem + kQtTileBytes)};
+  __shared__ GroupScan scan;
+  __shared__ __align__(16) uint8_t tile_scales[128][4];
+  __shared__ __align__(16) uint8_t tile_scales_rows[128][4];
+  scan_groups(p.list, scan, p.status);
+  if (blockIdx.x == 0) write_group_plan(p.list, scan, p.plan, reinterpret_cast<int*>(qt_smem));
+  if (p.dx) zero_rows_of_no_group(p.list, scan, p.dx, p.k, p.lddx);
+  const int row_tiles = scan.tile[p.list.groups];
+  const int dy_tiles = row_tiles * ((p.dy.cols + 127) / 128);
+  const int x_tiles = p.x.src ? row_tiles * ((p.x.cols + 127) / 128) : 0;
+  const int w_tiles = p.w ? (p.n + 127) / 128 * ((p.k + 127) / 128) : 0;   // per matrix
+  const int64_t total = static_cast<int64_t>(dy_tiles) + x_tiles + static_cast<int64_t>(p.batches) * w_tiles;
+  int buf = 0;
+  BackwardTile b;
+  auto fetch = [&](const BackwardTile& f, uint16_t (*dst)[kQtPitch]) {
+    const bool vec_ok = (f.f.ld % 8 == 0) && ((reinterpret_cast<uintptr_t>(f.f.src) & 15) == 0);
+    quant_mxfp8_t_fetch(f.f, dst, f.row0, 0, vec_ok);
+  };
+  if (blockIdx.x < total) {
+    b = backward_tile(p, scan, blockIdx.x, dy_tiles, x_tiles, w_tiles);
+    fetch(b, tiles[0]);
+  }
+  for (int64_t t = blockIdx.x; t < total; t += gridDim.x) {
+    const int64_t tn = t + gridDim.x;
+    BackwardTile next = b;
+    if (tn < total) {
+      next = backward_tile(p, scan, tn, dy_tiles, x_tiles, w_tiles);
+      fetch(next, tiles[buf ^ 1]);
+      cp_async_wait<1>();   // everything but the newest group (the next tile) has landed
+    } else {
+      cp_async_wait<0>();
+    }
+    __syncthreads();
+    uint32_t o[2][8];
+    if (b.q_t)
+      quant_mxfp8_tile_columns(tiles[buf], tile_scales, o, static_cast<int>(min(b.pitch_t, int64_t(INT32_MAX))), b.f.rows,
+                               b.row0, b.k0, true);
+    if (b.q_rows)
+      quant_mxfp8_tile_rows(tiles[buf], tile_scales_rows, b.q_rows, (b.f.rows + 31) / 32 * 32, b.f.k, b.f.rows, 0, b.row0,
+                            true);
+    __syncthreads();   // every thread has read the staged tile: its storage now collects the transposed payload
+    if (b.q_t) {
+      quant_mxfp8_tile_columns_store(reinterpret_cast<uint8_t*>(tiles[buf]), o, b.q_t, static_cast<int>(b.pitch_t), b.f.rows,
+                                     b.row0, b.k0);
+      store_scale_tile<4>(tile_scales, b.s_t, kScaleMma128, b.row0, b.blk0, b.f.rows, 0, b.chunks_t);
+    }
+    if (b.q_rows)
+      store_scale_tile<4>(tile_scales_rows, b.s_rows, kScaleMma128, 0, b.row0 / 32, b.f.k, 0,
+                          ((b.f.rows + 31) / 32 + 3) / 4);
+    __syncthreads();   // the scale tiles and this buffer are free again
+    buf ^= 1;
+    b = next;
+  }
+}
+
+}  // namespace rtxb

@@ -308,6 +308,131 @@ def mxfp8_linear_bwd(dy, x, w, ws: Workspace, *, need_dx: bool = True, need_dw: 
     return dx, dw
 
 
+MAX_GROUPS = 512
+
+
+def _require_rows(t: torch.Tensor, cols: Optional[int], name: str) -> None:
+    """A BF16 CUDA matrix whose rows are contiguous (any row pitch)."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if t.device.type != "cuda":
+        raise ValueError(f"{name} must be a CUDA tensor")
+    if t.dtype != torch.bfloat16:
+        raise TypeError(f"{name} must have dtype {torch.bfloat16}, got {t.dtype}")
+    if t.dim() != 2 or (cols is not None and t.shape[1] != cols):
+        raise ValueError(f"{name} must be two-dimensional" + (f" with {cols} columns" if cols is not None else ""))
+    if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+        raise ValueError(f"{name} must have contiguous rows that do not overlap")
+
+
+def _pitch(t: torch.Tensor) -> int:
+    """Row pitch in elements; a single row's stride says nothing and is replaced by its width."""
+    return t.stride(0) if t.shape[0] > 1 else max(int(t.shape[1]), 1)
+
+
+def _require_offsets(offsets: torch.Tensor, groups: int, device: torch.device) -> None:
+    if not isinstance(offsets, torch.Tensor):
+        raise TypeError("offsets must be a torch.Tensor")
+    if offsets.dtype is not torch.int32:
+        raise TypeError(f"offsets must have dtype torch.int32, got {offsets.dtype}")
+    if offsets.device != device:
+        raise ValueError("offsets must be on the operands' device")
+    if offsets.dim() != 1 or offsets.numel() != groups + 1 or not offsets.is_contiguous():
+        raise ValueError(f"offsets must be a contiguous vector of groups + 1 = {groups + 1} row numbers")
+    if groups > MAX_GROUPS:
+        raise ValueError(f"at most {MAX_GROUPS} groups, got {groups}")
+
+
+def mxfp8_grouped_linear_fwd(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, *,
+                             rounding: int = N.ROUND_INFINITY, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """x bf16 [T, K] (any row pitch), w bf16 [E, N, K], offsets int32 [E + 1] -> out bf16 [T, N]: row r of group g is
+    q(x[r]) q(w[g])^T, rows of no group are zero.  The scratch is a fresh allocation of the calling stream, so calls on
+    several streams and captured graphs share nothing."""
+    if w.dim() != 3 or w.dtype is not torch.bfloat16 or not w.is_contiguous():
+        raise ValueError("weight must be a contiguous BF16 tensor [groups, N, K]")
+    groups, n, k = (int(v) for v in w.shape)
+    _require_rows(x, k, "x")
+    if w.device != x.device:
+        raise ValueError("x and weight must share one device")
+    _require_offsets(offsets, groups, x.device)
+    rows = int(x.shape[0])
+    out = _grouped_out(out, rows, n, x.device)
+    if out.numel() == 0:
+        return out
+    nbytes = N.query("rtxb_mxfp8_grouped_linear_workspace_bytes", rows, n, k, groups, 1)
+    with _on(x.device):
+        buf = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        N.call("rtxb_mxfp8_grouped_linear_fwd", x.data_ptr(), _pitch(x), w.data_ptr(), offsets.data_ptr(), groups,
+               out.data_ptr(), _pitch(out), rows, n, k, rounding, buf.data_ptr(), nbytes, _stream_ptr(),
+               status_word(x.device).data_ptr())
+    return out
+
+
+def _grouped_out(out: Optional[torch.Tensor], rows: int, n: int, device: torch.device) -> torch.Tensor:
+    if out is None:
+        return torch.empty(rows, n, dtype=torch.bfloat16, device=device)
+    _require_rows(out, n, "out")
+    if out.shape[0] != rows or out.device != device:
+        raise ValueError(f"out must be [{rows}, {n}] on the operands' device")
+    return out
+
+
+def mxfp8_grouped_linear_fwd_prequant_w(x: torch.Tensor, qw: torch.Tensor, sw: torch.Tensor, offsets: torch.Tensor, n: int,
+                                        *, rounding: int = N.ROUND_INFINITY,
+                                        out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The same with packed weights: qw u8 [E * N, Kp] and mma128 scale tiles, N a multiple of 128 when E > 1."""
+    _require_rows(x, None, "x")
+    rows, k = (int(v) for v in x.shape)
+    groups = int(offsets.numel()) - 1
+    _require_offsets(offsets, groups, x.device)
+    if qw.device != x.device or sw.device != x.device:
+        raise ValueError("x and the packed weight must share one device")
+    if qw.element_size() != 1 or qw.numel() != groups * n * mx_storage_k(k) or not qw.is_contiguous():
+        raise ValueError(f"packed weight must hold {groups} x {n} rows of {mx_storage_k(k)} values")
+    if sw.element_size() != 1 or sw.numel() != mxfp8_scale_numel(groups * n, k, N.SCALE_MMA128) or not sw.is_contiguous():
+        raise ValueError("packed weight scales must be mma128 tiles")
+    out = _grouped_out(out, rows, n, x.device)
+    if out.numel() == 0:
+        return out
+    nbytes = N.query("rtxb_mxfp8_grouped_linear_workspace_bytes", rows, n, k, groups, 0)
+    with _on(x.device):
+        buf = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        N.call("rtxb_mxfp8_grouped_linear_fwd_prequant_w", x.data_ptr(), _pitch(x), qw.data_ptr(), sw.data_ptr(),
+               offsets.data_ptr(), groups, out.data_ptr(), _pitch(out), rows, n, k, rounding, buf.data_ptr(), nbytes,
+               _stream_ptr(), status_word(x.device).data_ptr())
+    return out
+
+
+def mxfp8_grouped_linear_bwd(dy: torch.Tensor, x: Optional[torch.Tensor], w: Optional[torch.Tensor], offsets: torch.Tensor,
+                             groups: int, k: int, *, need_dx: bool = True, need_dw: bool = True):
+    """(dY [T, N], X [T, K], W [E, N, K]) -> (dX bf16 [T, K] | None, dW bf16 [E, N, K] | None); X is read for dW only,
+    W for dX only."""
+    _require_rows(dy, None, "grad_output")
+    rows, n = (int(v) for v in dy.shape)
+    _require_offsets(offsets, groups, dy.device)
+    if need_dw:
+        _require_rows(x, k, "x")
+        if x.shape[0] != rows or x.device != dy.device:
+            raise ValueError("grad_output and x disagree on the rows or the device")
+    if need_dx and (tuple(w.shape) != (groups, n, k) or w.dtype is not torch.bfloat16 or not w.is_contiguous()
+                    or w.device != dy.device):
+        raise ValueError("weight must be a contiguous BF16 tensor [groups, N, K] on grad_output's device")
+    dx = torch.empty(rows, k, dtype=torch.bfloat16, device=dy.device) if need_dx else None
+    dw = torch.empty(groups, n, k, dtype=torch.bfloat16, device=dy.device) if need_dw else None
+    if not (need_dx or need_dw):
+        return dx, dw
+    if min(rows, n, k, groups) == 0:      # an empty sum is zero
+        return (dx.zero_() if need_dx else None), (dw.zero_() if need_dw else None)
+    nbytes = N.query("rtxb_mxfp8_grouped_backward_workspace_bytes", rows, n, k, groups, int(need_dx), int(need_dw))
+    with _on(dy.device):
+        buf = torch.empty(nbytes, dtype=torch.uint8, device=dy.device)
+        N.call("rtxb_mxfp8_grouped_linear_bwd", dy.data_ptr(), _pitch(dy), x.data_ptr() if need_dw else None,
+               _pitch(x) if need_dw else k, w.data_ptr() if need_dx else None, offsets.data_ptr(), groups,
+               dx.data_ptr() if need_dx else None, dw.data_ptr() if need_dw else None, rows, n, k, buf.data_ptr(), nbytes,
+               _stream_ptr(), status_word(dy.device).data_ptr())
+    return dx, dw
+
+
 def peer_barrier(flag_ptrs, rank: int, epoch_counter: torch.Tensor, limit_ns: int = 2_000_000_000) -> None:
     """Node barrier through flag words in peer-mapped memory on the current stream: `flag_ptrs[t]` is the address
     of rank t's array of eight int32 words as mapped into this process; `epoch_counter` is one int32 of this
