@@ -51,6 +51,13 @@ extern "C" {
 #define RTXB_OUT_BF16 0
 #define RTXB_OUT_F32 1
 
+#define RTXB_ACT_NONE 0
+#define RTXB_ACT_RELU 1
+#define RTXB_ACT_RELU2 2      /* max(z, 0)^2 */
+#define RTXB_ACT_SILU 3       /* z / (1 + e^-z) */
+#define RTXB_ACT_GELU 4       /* z (1 + erf(z / sqrt 2)) / 2 */
+#define RTXB_ACT_GELU_TANH 5  /* z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) / 2 */
+
 #define RTXB_TENSOR_SCALE_EXACT 0
 #define RTXB_TENSOR_SCALE_POWER2 1
 
@@ -242,6 +249,36 @@ size_t rtxb_mxfp8_backward_workspace_bytes(int64_t m, int64_t n, int64_t k);
 int rtxb_mxfp8_linear_bwd(const void* dy_bf16, const void* x_bf16, const void* w_bf16, void* dx_bf16, void* dw,
                           int dw_dtype, int64_t m, int64_t n, int64_t k, void* workspace, size_t workspace_bytes,
                           void* stream, int* status);
+
+/* ---- MXFP8 linear with bias, activation and residual -------------------------------------------
+ * No counterpart in the reference (its linears are no-bias, rtx/fp8.py:2389).
+ *     z   = deq(q(x)) deq(q(w))^T + bias            FP32 accumulator, bias BF16 [n] or NULL
+ *     out = bf16( act(z) + residual )               one rounding; residual BF16 [m, n], pitch ldr >= n, or NULL
+ *     z_bf16 (optional, [m, n]) keeps z rounded to BF16 for the backward; the activation takes the FP32 value.
+ * out and z are contiguous; no input may overlap them.  Two launches on `stream`: quantizer of x (and of a BF16 w),
+ * GEMM with the epilogue as a programmatic dependent.  workspace: rtxb_mxfp8_linear_epilogue_workspace_bytes(m, n, k, dynamic_w). */
+size_t rtxb_mxfp8_linear_epilogue_workspace_bytes(int64_t m, int64_t n, int64_t k, int dynamic_w);
+int rtxb_mxfp8_linear_epilogue_fwd(const void* x_bf16, int64_t ldx, const void* w_bf16, const void* bias_bf16,
+                                   const void* residual_bf16, int64_t ldr, void* out_bf16, void* z_bf16, int64_t m, int64_t n,
+                                   int64_t k, int activation, int rounding, void* workspace, size_t workspace_bytes,
+                                   void* stream, int* status);
+/* The same with a packed weight: qw [n, storage k] and its mma128 scale tiles. */
+int rtxb_mxfp8_linear_epilogue_fwd_prequant_w(const void* x_bf16, int64_t ldx, const void* qw, const void* sw,
+                                              const void* bias_bf16, const void* residual_bf16, int64_t ldr, void* out_bf16,
+                                              int64_t m, int64_t n, int64_t k, int activation, int rounding, void* workspace,
+                                              size_t workspace_bytes, void* stream, int* status);
+/* Its backward:
+ *     dz    = bf16( dy act'(z) )                    z as kept by the forward; for RTXB_ACT_NONE dz = dy, z may be NULL
+ *     dx    = dz w, dw = dz^T x                     as rtxb_mxfp8_linear_bwd of dz
+ *     dbias = bf16( sum over the rows of dy act'(z) )   FP32 sums in a fixed order
+ * (the residual's gradient is dy itself).  dx [m, k], dw [n, k], dbias [n], any of them NULL to leave it out; w is read
+ * for dx only, x for dw only.  dz never reaches memory: one launch reads dy and z once and writes both quantizations. */
+size_t rtxb_mxfp8_linear_epilogue_backward_workspace_bytes(int64_t m, int64_t n, int64_t k, int need_dx, int need_dw,
+                                                           int need_dbias);
+int rtxb_mxfp8_linear_epilogue_bwd(const void* dy_bf16, int64_t lddy, const void* z_bf16, const void* x_bf16, int64_t ldx,
+                                   const void* w_bf16, void* dx_bf16, void* dw_bf16, void* dbias_bf16, int64_t m, int64_t n,
+                                   int64_t k, int activation, void* workspace, size_t workspace_bytes, void* stream,
+                                   int* status);
 
 /* ---- grouped (experts') MXFP8 linear ----------------------------------------------------------
  * No counterpart in the reference (its linears are dense).  Rows offsets[g] .. offsets[g + 1] - 1 of x (offsets:

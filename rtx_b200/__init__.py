@@ -58,6 +58,9 @@ _LAZY_EXPORTS = {
     # sm_100a additions
     "mxfp8_glu_mlp": ("glu", "mxfp8_glu_mlp"),
     "SwiGLU": ("glu", "SwiGLU"),
+    "MXFP8LinearEpilogue": ("epilogue", "MXFP8LinearEpilogue"),
+    "mxfp8_linear_epilogue": ("epilogue", "mxfp8_linear_epilogue"),
+    "mxfp8_linear_epilogue_backward": ("epilogue", "mxfp8_linear_epilogue_backward"),
     "MXFP8GroupedLinear": ("grouped", "MXFP8GroupedLinear"),
     "mxfp8_grouped_linear": ("grouped", "mxfp8_grouped_linear"),
     "mxfp8_grouped_linear_backward": ("grouped", "mxfp8_grouped_linear_backward"),

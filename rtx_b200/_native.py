@@ -64,6 +64,11 @@ SIGNATURES = {
     "rtxb_mxfp8_glu_mlp_fwd": (_I, [_P, _P, _P, _P, _P, _L, _L, _L, _L, _P, _Z, _P, _P]),
     "rtxb_mxfp8_backward_workspace_bytes": (_Z, [_L, _L, _L]),
     "rtxb_mxfp8_linear_bwd": (_I, [_P, _P, _P, _P, _P, _I, _L, _L, _L, _P, _Z, _P, _P]),
+    "rtxb_mxfp8_linear_epilogue_workspace_bytes": (_Z, [_L, _L, _L, _I]),
+    "rtxb_mxfp8_linear_epilogue_fwd": (_I, [_P, _L, _P, _P, _P, _L, _P, _P, _L, _L, _L, _I, _I, _P, _Z, _P, _P]),
+    "rtxb_mxfp8_linear_epilogue_fwd_prequant_w": (_I, [_P, _L, _P, _P, _P, _P, _L, _P, _L, _L, _L, _I, _I, _P, _Z, _P, _P]),
+    "rtxb_mxfp8_linear_epilogue_backward_workspace_bytes": (_Z, [_L, _L, _L, _I, _I, _I]),
+    "rtxb_mxfp8_linear_epilogue_bwd": (_I, [_P, _L, _P, _P, _L, _P, _P, _P, _P, _L, _L, _L, _I, _P, _Z, _P, _P]),
     "rtxb_mxfp8_grouped_linear_workspace_bytes": (_Z, [_L, _L, _L, _L, _I]),
     "rtxb_mxfp8_grouped_linear_fwd": (_I, [_P, _L, _P, _P, _L, _P, _L, _L, _L, _L, _I, _P, _Z, _P, _P]),
     "rtxb_mxfp8_grouped_linear_fwd_prequant_w": (_I, [_P, _L, _P, _P, _P, _L, _P, _L, _L, _L, _L, _I, _P, _Z, _P, _P]),

@@ -9,6 +9,7 @@
 #include "quant.cuh"
 #include "gemm_decode_fused.cuh"
 #include "gemm_fused_quant.cuh"
+#include "quant_act.cuh"
 #include "reduce.cuh"
 #include "peer.cuh"
 
@@ -70,12 +71,21 @@ struct RegionScales {
   int x_rows, w_rows;
 };
 
+// bias, activation, residual and kept pre-activation of kEpiAct
+struct ActEpilogue {
+  const void* bias;
+  const void* residual;
+  int64_t ldr;
+  void* z;
+  int act;
+};
+
 template <int KIND, int EPI>
 int launch_gemm(const void* qa, const void* sa, const void* qb, const void* sb, void* out, int64_t m, int64_t n_rows_b,
                 int64_t row_bytes, int64_t sf_k_chunks, int64_t ldo, int64_t out_cols, int64_t glu_inter,
                 const float* out_scale, cudaStream_t stream, int* status, void* q_out = nullptr,
                 void* sf_out = nullptr, bool overlap_previous = false, const RegionScales* regions = nullptr,
-                const BlockOutputs* blocks = nullptr, bool after_quantizer = false) {
+                const BlockOutputs* blocks = nullptr, bool after_quantizer = false, const ActEpilogue* act = nullptr) {
   // after_quantizer: EVERY operand comes from the kernel enqueued just before this one (the composite forwards'
   // quantizer); the pair and single-CTA kernels are then launched as programmatic dependents — they wait for that
   // grid before their first load, their set-up runs beside its tail.  The streaming kernel is launched normally.
@@ -113,6 +123,14 @@ int launch_gemm(const void* qa, const void* sa, const void* qb, const void* sb, 
   p.q_out = static_cast<uint8_t*>(q_out);
   p.sf_out = static_cast<uint8_t*>(sf_out);
   p.sf_out_chunks = static_cast<int>((out_cols / 32 + 3) / 4);
+  p.bias = static_cast<const __nv_bfloat16*>(act ? act->bias : nullptr);
+  p.residual = static_cast<const __nv_bfloat16*>(act ? act->residual : nullptr);
+  p.ldr = act ? act->ldr : 0;
+  p.residual_vec_ok = aligned(p.residual, 16) && p.ldr % 8 == 0;
+  p.bias_vec_ok = aligned(p.bias, 16);
+  p.z_out = static_cast<__nv_bfloat16*>(act ? act->z : nullptr);
+  if (p.z_out && !aligned(p.z_out, 16)) p.out_vec_ok = 0;
+  p.act = act ? act->act : 0;
   p.status = status;
   p.a_box_rows = 128;
   p.slots = 0;
@@ -147,7 +165,7 @@ int launch_gemm(const void* qa, const void* sa, const void* qb, const void* sb, 
       if (rc) return rc;
     }
     p.n_tiles = static_cast<int>((n_rows_b + kSkinnyN - 1) / kSkinnyN);
-    auto sk = gemm_skinny_kernel<KIND, EPI == kEpiF32 ? kEpiF32 : kEpiBf16>;
+    auto sk = gemm_skinny_kernel<KIND, EPI == kEpiF32 || EPI == kEpiAct ? EPI : static_cast<int>(kEpiBf16)>;
     cudaError_t se = ensure_dynamic_smem(reinterpret_cast<const void*>(sk), kSkinnySmemBudget);
     if (se != cudaSuccess) return fail_cuda(se, "cudaFuncSetAttribute(skinny gemm)");
     se = launch_dependent(sk, p.n_tiles < sm_count() ? p.n_tiles : sm_count(), kGemmThreads,
@@ -175,6 +193,7 @@ int launch_gemm(const void* qa, const void* sa, const void* qb, const void* sb, 
     } else if (p.tma_out) {
       rc = make_out_map(&maps_out.m[0], out, m, out_cols, ldo, EPI == kEpiF32 ? 4 : 2);
       if (rc) return rc;
+      if (p.z_out && (rc = make_out_map(&maps_out.m[1], p.z_out, m, out_cols, ldo, 2))) return rc;
     }
     // one load per operand brings the KS K steps of a barrier group
     p.map3d = row_bytes % 128 == 0 ? 1 : 0;
@@ -842,6 +861,169 @@ int rtxb_mxfp8_linear_bwd(const void* dy, const void* x, const void* w, void* dx
     if ((rc = rtxb_mxfp8_quantize_transposed(x, k, m, k, qd, sd, RTXB_SCALE_MMA128, RTXB_ROUND_INFINITY, stream)))
       return rc;
     if ((rc = rtxb_mxfp8_gemm(qc, sc, qd, sd, dw, n, k, m, k, dw_dtype, stream, status))) return rc;
+  }
+  return RTXB_OK;
+}
+
+// ---- linear with bias, activation and residual ------------------------------------------------------------
+
+static int check_epilogue(int64_t m, int64_t n, int64_t k, int act) {
+  if (m <= 0 || n <= 0 || k <= 0) return fail_msg(RTXB_E_INVALID_ARGUMENT, "m, n, k must be positive");
+  if (m > INT32_MAX - 256 || n > INT32_MAX - 256 || k > INT32_MAX - 256)
+    return fail_msg(RTXB_E_UNSUPPORTED, "dimension exceeds int32");
+  if (act < RTXB_ACT_NONE || act > RTXB_ACT_GELU_TANH) return fail_msg(RTXB_E_INVALID_ARGUMENT, "unknown activation");
+  return RTXB_OK;
+}
+
+size_t rtxb_mxfp8_linear_epilogue_workspace_bytes(int64_t m, int64_t n, int64_t k, int dynamic_w) {
+  Carver c(nullptr);
+  c.take(m * round_up(k, 32));
+  c.take(rtxb_mxfp8_scale_bytes(m, k, RTXB_SCALE_MMA128));
+  if (dynamic_w) {
+    c.take(n * round_up(k, 32));
+    c.take(rtxb_mxfp8_scale_bytes(n, k, RTXB_SCALE_MMA128));
+  }
+  return c.off;
+}
+
+// exactly one of `w` (BF16, quantized here) and `qw` / `sw` is given
+static int linear_epilogue(const void* x, int64_t ldx, const void* w, const void* qw, const void* sw, const void* bias,
+                           const void* residual, int64_t ldr, void* out, void* z, int64_t m, int64_t n, int64_t k, int act,
+                           int rounding, void* workspace, size_t workspace_bytes, void* stream, int* status) {
+  int rc = check_epilogue(m, n, k, act);
+  if (rc) return rc;
+  if (!x || !out) return fail_msg(RTXB_E_INVALID_ARGUMENT, "null operand");
+  if (ldx < k || (residual && ldr < n)) return fail_msg(RTXB_E_INVALID_ARGUMENT, "row pitch smaller than the row");
+  if (!aligned(x, 2) || !aligned(w, 2) || !aligned(bias, 2) || !aligned(residual, 2) || !aligned(out, 2) || !aligned(z, 2))
+    return fail_msg(RTXB_E_ALIGNMENT, "pointer is not element aligned");
+  if (!workspace || workspace_bytes < rtxb_mxfp8_linear_epilogue_workspace_bytes(m, n, k, w != nullptr))
+    return fail_msg(RTXB_E_WORKSPACE, "workspace too small for rtxb_mxfp8_linear_epilogue_fwd");
+  if (!aligned(workspace, 256)) return fail_msg(RTXB_E_ALIGNMENT, "workspace must be 256-byte aligned");
+  Carver c(workspace);
+  const int64_t kp = round_up(k, 32), chunks = (kp / 32 + 3) / 4;
+  QuantMxParams p[2] = {};
+  for (int i = 0; i < 2; ++i) {
+    p[i].src = static_cast<const __nv_bfloat16*>(i ? w : x);
+    p[i].rows = static_cast<int>(i ? (w ? n : 0) : m);   // packed weights: no tiles of the second operand
+    p[i].k = static_cast<int>(k);
+    p[i].kp = static_cast<int>(kp);
+    p[i].ld = i ? k : ldx;
+    p[i].nb = static_cast<int>(kp / 32);
+    p[i].sf_chunks = static_cast<int>(chunks);
+    p[i].layout = RTXB_SCALE_MMA128;
+    p[i].round_to_infinity = rounding != RTXB_ROUND_FLOOR;
+    if (i == 0 || w) {
+      p[i].q = c.take(p[i].rows * kp);
+      p[i].scales = c.take(rtxb_mxfp8_scale_bytes(p[i].rows, k, RTXB_SCALE_MMA128));
+    }
+  }
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int64_t tiles = (round_up(m, 128) + (w ? round_up(n, 128) : 0)) / 128 * ((kp + 127) / 128);
+  quant_mxfp8_rows2_kernel<<<quant_grid(tiles, 6), kQuantThreads, 0, s>>>(p[0], p[1]);
+  RTXB_CHECK_LAUNCH("quant_mxfp8_rows2_kernel");
+  const ActEpilogue e{bias, residual, ldr, z, act};
+  // packed weights do not come from the quantizer just launched: on small layers the GEMM streams them beside it
+  return launch_gemm<kKindMxfp8, kEpiAct>(p[0].q, p[0].scales, w ? p[1].q : qw, w ? p[1].scales : sw, out, m, n, kp, chunks, n,
+                                          n, 0, nullptr, s, status, nullptr, nullptr, w == nullptr, nullptr, nullptr,
+                                          w != nullptr, &e);
+}
+
+int rtxb_mxfp8_linear_epilogue_fwd(const void* x, int64_t ldx, const void* w, const void* bias, const void* residual,
+                                   int64_t ldr, void* out, void* z, int64_t m, int64_t n, int64_t k, int activation,
+                                   int rounding, void* workspace, size_t workspace_bytes, void* stream, int* status) {
+  if (!w) return fail_msg(RTXB_E_INVALID_ARGUMENT, "null operand");
+  return linear_epilogue(x, ldx, w, nullptr, nullptr, bias, residual, ldr, out, z, m, n, k, activation, rounding, workspace,
+                         workspace_bytes, stream, status);
+}
+
+int rtxb_mxfp8_linear_epilogue_fwd_prequant_w(const void* x, int64_t ldx, const void* qw, const void* sw, const void* bias,
+                                              const void* residual, int64_t ldr, void* out, int64_t m, int64_t n, int64_t k,
+                                              int activation, int rounding, void* workspace, size_t workspace_bytes,
+                                              void* stream, int* status) {
+  if (!qw || !sw) return fail_msg(RTXB_E_INVALID_ARGUMENT, "null operand");
+  if (!aligned(qw, 16) || !aligned(sw, 16)) return fail_msg(RTXB_E_ALIGNMENT, "packed operands must be 16-byte aligned");
+  return linear_epilogue(x, ldx, nullptr, qw, sw, bias, residual, ldr, out, nullptr, m, n, k, activation, rounding, workspace,
+                         workspace_bytes, stream, status);
+}
+
+namespace {
+struct EpilogueBwdMemory {
+  uint8_t *q_dz = nullptr, *s_dz = nullptr, *q_wt = nullptr, *s_wt = nullptr;     // dX
+  uint8_t *q_dzt = nullptr, *s_dzt = nullptr, *q_xt = nullptr, *s_xt = nullptr;   // dW
+  float* partial = nullptr;                                                       // dbias
+  EpilogueBwdMemory(Carver& c, int64_t m, int64_t n, int64_t k, bool dx, bool dw, bool db) {
+    if (dx) {
+      q_dz = c.take(m * round_up(n, 32));
+      s_dz = c.take(rtxb_mxfp8_scale_bytes(m, n, RTXB_SCALE_MMA128));
+      q_wt = c.take(k * round_up(n, 32));
+      s_wt = c.take(rtxb_mxfp8_scale_bytes(k, n, RTXB_SCALE_MMA128));
+    }
+    if (dw) {
+      q_dzt = c.take(n * round_up(m, 32));
+      s_dzt = c.take(rtxb_mxfp8_scale_bytes(n, m, RTXB_SCALE_MMA128));
+      q_xt = c.take(k * round_up(m, 32));
+      s_xt = c.take(rtxb_mxfp8_scale_bytes(k, m, RTXB_SCALE_MMA128));
+    }
+    if (db) partial = reinterpret_cast<float*>(c.take((m + 127) / 128 * n * 4));
+  }
+};
+}  // namespace
+
+size_t rtxb_mxfp8_linear_epilogue_backward_workspace_bytes(int64_t m, int64_t n, int64_t k, int need_dx, int need_dw,
+                                                           int need_dbias) {
+  Carver c(nullptr);
+  EpilogueBwdMemory mem(c, m, n, k, need_dx != 0, need_dw != 0, need_dbias != 0);
+  return c.off;
+}
+
+int rtxb_mxfp8_linear_epilogue_bwd(const void* dy, int64_t lddy, const void* z, const void* x, int64_t ldx, const void* w,
+                                   void* dx, void* dw, void* dbias, int64_t m, int64_t n, int64_t k, int activation,
+                                   void* workspace, size_t workspace_bytes, void* stream, int* status) {
+  int rc = check_epilogue(m, n, k, activation);
+  if (rc) return rc;
+  if (!dy || (!dx && !dw && !dbias) || (dx && !w) || (dw && !x)) return fail_msg(RTXB_E_INVALID_ARGUMENT, "null operand");
+  if (activation != RTXB_ACT_NONE && !z) return fail_msg(RTXB_E_INVALID_ARGUMENT, "an activation's backward needs z");
+  if (lddy < n || (dw && ldx < k)) return fail_msg(RTXB_E_INVALID_ARGUMENT, "row pitch smaller than the row");
+  if (!aligned(dy, 2) || !aligned(z, 2) || !aligned(x, 2) || !aligned(w, 2) || !aligned(dx, 2) || !aligned(dw, 2) ||
+      !aligned(dbias, 2))
+    return fail_msg(RTXB_E_ALIGNMENT, "pointer is not element aligned");
+  Carver c(workspace);
+  EpilogueBwdMemory mem(c, m, n, k, dx != nullptr, dw != nullptr, dbias != nullptr);
+  if (!workspace || workspace_bytes < c.off)
+    return fail_msg(RTXB_E_WORKSPACE, "workspace too small for rtxb_mxfp8_linear_epilogue_bwd");
+  if (!aligned(workspace, 256)) return fail_msg(RTXB_E_ALIGNMENT, "workspace must be 256-byte aligned");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  QuantActParams q = {};
+  q.dy = static_cast<const __nv_bfloat16*>(dy);
+  q.z = activation == RTXB_ACT_NONE ? nullptr : static_cast<const __nv_bfloat16*>(z);
+  q.m = static_cast<int>(m);
+  q.n = static_cast<int>(n);
+  q.act = activation;
+  q.lddy = lddy;
+  q.q_rows = mem.q_dz;
+  q.s_rows = mem.s_dz;
+  q.q_t = mem.q_dzt;
+  q.s_t = mem.s_dzt;
+  q.partial = mem.partial;
+  const int64_t row_tiles = (m + 127) / 128, tiles = row_tiles * ((n + 127) / 128);
+  cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(quant_mxfp8_act_backward_kernel), kQtTileBytes);
+  if (e != cudaSuccess) return fail_cuda(e, "cudaFuncSetAttribute(activation backward quantizer)");
+  quant_mxfp8_act_backward_kernel<<<quant_grid(tiles, 4), kQuantThreads, kQtTileBytes, s>>>(q);
+  RTXB_CHECK_LAUNCH("quant_mxfp8_act_backward_kernel");
+  if (dbias) {
+    bias_grad_kernel<<<static_cast<int>((n + 31) / 32), 256, 0, s>>>(mem.partial, static_cast<int>(row_tiles),
+                                                                     static_cast<int>(n), static_cast<__nv_bfloat16*>(dbias));
+    RTXB_CHECK_LAUNCH("bias_grad_kernel");
+  }
+  if (dx) {
+    if ((rc = rtxb_mxfp8_quantize_transposed(w, k, n, k, mem.q_wt, mem.s_wt, RTXB_SCALE_MMA128, RTXB_ROUND_INFINITY, stream)))
+      return rc;
+    if ((rc = rtxb_mxfp8_gemm(mem.q_dz, mem.s_dz, mem.q_wt, mem.s_wt, dx, m, k, n, k, RTXB_OUT_BF16, stream, status))) return rc;
+  }
+  if (dw) {
+    if ((rc = rtxb_mxfp8_quantize_transposed(x, k, m, ldx, mem.q_xt, mem.s_xt, RTXB_SCALE_MMA128, RTXB_ROUND_INFINITY, stream)))
+      return rc;
+    if ((rc = rtxb_mxfp8_gemm(mem.q_dzt, mem.s_dzt, mem.q_xt, mem.s_xt, dw, n, k, m, k, RTXB_OUT_BF16, stream, status))) return rc;
   }
   return RTXB_OK;
 }

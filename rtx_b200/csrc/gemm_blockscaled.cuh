@@ -25,6 +25,7 @@
 // the next tile's MMAs start, so the rest of the drain overlaps the next main loop.
 #pragma once
 
+#include "activation.cuh"
 #include "common.cuh"
 
 namespace rtxb {
@@ -35,6 +36,7 @@ enum GemmEpilogue : int {
   kEpiF32 = 1,    // D f32  = acc * out_scale
   kEpiGluBf16 = 2, // D bf16[M, N/2] = silu(acc[:, gate]) * acc[:, up]
   kEpiGluMx = 3,   // the same H, also (or only) emitted as MXFP8: E4M3 payload + E8M0 scale tiles
+  kEpiAct = 5,     // z = acc + bias[col], D bf16 = act(z) + residual; z optionally kept in BF16
   kEpiRegionBf16 = 4  // D bf16 = acc * (x_region_scale[row / Rx] * w_region_scale[col / Rw])  (NVFP4 row-region policy)
 };
 __host__ __device__ constexpr bool epi_is_glu(int epi) { return epi == kEpiGluBf16 || epi == kEpiGluMx; }
@@ -121,6 +123,13 @@ struct GemmParams {
   uint8_t* q_out;         // kEpiGluMx: E4M3 payload of H, [M, out_cols] (out may then be nullptr)
   uint8_t* sf_out;        // kEpiGluMx: E8M0 scales of H in 128-row tiles, sf_out_chunks tiles per row block
   int sf_out_chunks;
+  const __nv_bfloat16* bias;      // kEpiAct: [out_cols] or nullptr
+  const __nv_bfloat16* residual;  // kEpiAct: [M, out_cols], pitch ldr, or nullptr
+  int64_t ldr;
+  int residual_vec_ok;            // residual and its pitch are 16-byte aligned
+  int bias_vec_ok;
+  __nv_bfloat16* z_out;           // kEpiAct: pre-activation for the backward, pitch ldo, or nullptr
+  int act;
   int* status;            // device status word or nullptr
   int a_box_rows;         // kernels for one row block (M <= 128): rows of A fetched per K step (M rounded up to 8)
   int slots;              // streaming kernel: ring slots that fit shared memory with that A box
@@ -154,6 +163,75 @@ __device__ __forceinline__ void store_bf16x8(__nv_bfloat16* out, int col, int ou
     for (int e = 0; e < 8; ++e)
       if (col + e < out_cols) out[col + e] = reinterpret_cast<const __nv_bfloat16*>(w)[e];
   }
+}
+
+// kEpiAct, 32 columns of one row: v (accumulators) -> z = v + bias.  Every lane of a warp reads the same 64 bytes.
+__device__ __forceinline__ void act_add_bias(const GemmParams& p, float (&v)[32], int col) {
+  if (p.bias == nullptr) return;
+  if (p.bias_vec_ok && col + 32 <= p.out_cols) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint4 b = __ldg(reinterpret_cast<const uint4*>(p.bias + col) + j);
+      const uint32_t w[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        v[8 * j + 2 * e] += bf16_lo(w[e]);
+        v[8 * j + 2 * e + 1] += bf16_hi(w[e]);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 32; ++e)
+      if (col + e < p.out_cols) v[e] += __bfloat162float(p.bias[col + e]);
+  }
+}
+__device__ __forceinline__ void act_apply(int act, float (&v)[32]) {
+  with_activation(act, [&](auto tag) {
+#pragma unroll
+    for (int e = 0; e < 32; ++e) v[e] = act_value<decltype(tag)::value>(v[e]);
+  });
+}
+__device__ __forceinline__ void act_add_residual(const GemmParams& p, float (&v)[32], int row, bool row_ok, int col) {
+  if (p.residual == nullptr || !row_ok) return;
+  const __nv_bfloat16* src = p.residual + static_cast<int64_t>(row) * p.ldr + col;
+  if (p.residual_vec_ok && col + 32 <= p.out_cols) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint4 b = __ldg(reinterpret_cast<const uint4*>(src) + j);
+      const uint32_t w[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        v[8 * j + 2 * e] += bf16_lo(w[e]);
+        v[8 * j + 2 * e + 1] += bf16_hi(w[e]);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 32; ++e)
+      if (col + e < p.out_cols) v[e] += __bfloat162float(src[e]);
+  }
+}
+__device__ __forceinline__ void pack_bf16x32(const float (&v)[32], uint32_t (&w)[16]) {
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
+    w[e] = *reinterpret_cast<uint32_t*>(&b);
+  }
+}
+__device__ __forceinline__ void store_bf16x32(__nv_bfloat16* row_ptr, int col, int out_cols, bool vec_ok,
+                                              const uint32_t (&w)[16]) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const uint32_t ww[4] = {w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]};
+    store_bf16x8(row_ptr, col + 8 * q, out_cols, vec_ok, ww);
+  }
+}
+// 32 rows x 64 bytes (one row per lane) into a staging buffer in the 64-byte swizzle of the output map
+__device__ __forceinline__ void stage_bf16x32(uint8_t* buf, int lane, const uint32_t (&w)[16]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    *reinterpret_cast<uint4*>(buf + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) =
+        make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
 }
 
 // Drains one 128 x 256 accumulator window of this warp's 32 TMEM lanes.  `tacc` already holds the
@@ -286,7 +364,45 @@ __device__ __forceinline__ void epilogue_drain(const GemmParams& p, uint32_t tac
 #pragma unroll
         for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(r[e]) * out_scale;
       }
-      if (EPI == kEpiF32) {
+      if (EPI == kEpiAct) {
+        // z is rounded to BF16 only for the backward; the activation takes the FP32 value
+        act_add_bias(p, v, col);
+        uint32_t w[16];
+        if (staged) {
+          // with z both staging buffers of the warp are used by a chunk (0: z, 1: the result), without it they alternate
+          uint8_t* buf = stage + (p.z_out ? 1 : (i & 1)) * kEpiStageBufBytes;
+          if (lane == 0) {
+            if (p.z_out) tma_store_wait_read<0>();
+            else tma_store_wait_read<1>();
+          }
+          __syncwarp();
+          if (p.z_out) {
+            pack_bf16x32(v, w);
+            stage_bf16x32(stage, lane, w);
+          }
+          act_apply(p.act, v);
+          act_add_residual(p, v, row, row_ok, col);
+          pack_bf16x32(v, w);
+          stage_bf16x32(buf, lane, w);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            if (p.z_out) tma_store_2d(map_out + 1, stage, col, row - lane - out_row0);
+            tma_store_2d(map_out, buf, col, row - lane - out_row0);
+            tma_store_commit();
+          }
+        } else {
+          const int64_t at = static_cast<int64_t>(row) * p.ldo;
+          if (p.z_out) {
+            pack_bf16x32(v, w);
+            store_bf16x32(p.z_out + at, col, p.out_cols, p.out_vec_ok != 0, w);
+          }
+          act_apply(p.act, v);
+          act_add_residual(p, v, row, row_ok, col);
+          pack_bf16x32(v, w);
+          store_bf16x32(reinterpret_cast<__nv_bfloat16*>(p.out) + at, col, p.out_cols, p.out_vec_ok != 0, w);
+        }
+      } else if (EPI == kEpiF32) {
         if (staged) {
           // 32 rows x 128 bytes = both staging buffers as one box (128-byte swizzle: 16-byte chunk j of row r at
           // chunk j ^ (r % 8)), one store: whole 128-byte lines leave the SM, which is what a write over NVLink wants

@@ -310,7 +310,23 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         const uint32_t (&r)[32] = half ? r1 : r0;
-        if (EPI == kEpiBf16) {
+        if (EPI == kEpiAct) {
+          const int c = col + 32 * half;
+          const int64_t at = static_cast<int64_t>(row) * p.ldo;
+          float v[32];
+          uint32_t w[16];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(r[e]) * out_scale;
+          act_add_bias(p, v, c);
+          if (p.z_out) {
+            pack_bf16x32(v, w);
+            store_bf16x32(p.z_out + at, c, p.out_cols, p.out_vec_ok != 0, w);
+          }
+          act_apply(p.act, v);
+          act_add_residual(p, v, row, true, c);
+          pack_bf16x32(v, w);
+          store_bf16x32(reinterpret_cast<__nv_bfloat16*>(p.out) + at, c, p.out_cols, p.out_vec_ok != 0, w);
+        } else if (EPI == kEpiBf16) {
           __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(p.out) + static_cast<int64_t>(row) * p.ldo;
 #pragma unroll
           for (int v = 0; v < 32; v += 8) {

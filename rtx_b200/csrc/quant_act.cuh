@@ -1,0 +1,130 @@
+// Backward of the linear with an epilogue, its elementwise half fused with the quantizers:
+//   dz = dy act'(z)                          [m, n], FP32, rounded once to BF16 (the gradient autograd would carry)
+//   q_rows  MXFP8 of dz, blocks along n      (A operand of dX = dz W)
+//   q_t     MXFP8 of dz^T, blocks along m    (A operand of dW = dz^T X)
+//   partial[m / 128][n] = sum of 128 rows of dz in FP32, before the rounding   (dbias, finished by the kernel below)
+// dy and z are read once (4 bytes per value), 2 bytes of payload leave: without the fusion dz is written and read again
+// (4 more).  HBM bound; one 128 x 128 tile per block step, three blocks per SM overlap one another's loads and stores.
+#pragma once
+
+#include "activation.cuh"
+#include "quant_tiles.cuh"
+
+namespace rtxb {
+
+struct QuantActParams {
+  const __nv_bfloat16* dy;   // [m, n], pitch lddy
+  const __nv_bfloat16* z;    // [m, n], pitch n; nullptr when act is none
+  int m, n, act;
+  int64_t lddy;
+  uint8_t* q_rows;           // [m, np] or nullptr
+  uint8_t* s_rows;
+  uint8_t* q_t;              // [n, mp] or nullptr
+  uint8_t* s_t;
+  float* partial;            // [ceil(m / 128)][n] or nullptr
+};
+
+constexpr int kActSumRows = kQuantThreads / 32;   // partial column sums per tile before the last step, one per warp
+
+__global__ void __launch_bounds__(kQuantThreads, 4) quant_mxfp8_act_backward_kernel(const QuantActParams p) {
+  extern __shared__ __align__(16) uint8_t qt_smem[];
+  uint16_t (*tile)[kQtPitch] = reinterpret_cast<uint16_t (*)[kQtPitch]>(qt_smem);
+  __shared__ __align__(16) uint8_t scales_t[128][4];
+  __shared__ __align__(16) uint8_t scales_rows[128][4];
+  __shared__ float sums[kActSumRows][128];
+  const int col_tiles = (p.n + 127) / 128, row_tiles = (p.m + 127) / 128;
+  const int np = (p.n + 31) / 32 * 32, mp = (p.m + 31) / 32 * 32;
+  const bool vec_dy = (p.lddy % 8 == 0) && ((reinterpret_cast<uintptr_t>(p.dy) & 15) == 0);
+  const bool vec_z = (p.n % 8 == 0) && ((reinterpret_cast<uintptr_t>(p.z) & 15) == 0);
+  const int c8 = (threadIdx.x & 15) * 8, r0 = threadIdx.x >> 4;
+  const int64_t total = static_cast<int64_t>(row_tiles) * col_tiles;
+  for (int64_t t = blockIdx.x; t < total; t += gridDim.x) {
+    const int rt = static_cast<int>(t / col_tiles);
+    const int row0 = rt * 128, col0 = static_cast<int>(t - static_cast<int64_t>(rt) * col_tiles) * 128;
+    const int col = col0 + c8;
+    float sum[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum[e] = 0.0f;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      uint4 g[4], z[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int row = row0 + r0 + 16 * (half * 4 + j);
+        const bool live = row < p.m && col < p.n;
+        g[j] = live ? load8_raw(p.dy + row * p.lddy, col, p.n, vec_dy) : make_uint4(0, 0, 0, 0);
+        z[j] = live && p.z ? load8_raw(p.z + static_cast<int64_t>(row) * p.n, col, p.n, vec_z) : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float v[8];
+        unpack8(g[j], v);
+        if (p.z) {
+          float zz[8];
+          unpack8(z[j], zz);
+          with_activation(p.act, [&](auto tag) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] *= act_slope<decltype(tag)::value>(zz[e]);
+          });
+        }
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          sum[2 * e] += v[2 * e];
+          sum[2 * e + 1] += v[2 * e + 1];
+          __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
+          w[e] = *reinterpret_cast<uint32_t*>(&b);
+        }
+        *reinterpret_cast<uint4*>(&tile[r0 + 16 * (half * 4 + j)][c8]) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+    if (p.partial) {
+      // the two row halves of a warp, then one row of sums per warp
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], 16);
+      if ((threadIdx.x & 16) == 0) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sums[threadIdx.x >> 5][c8 + e] = sum[e];
+      }
+    }
+    __syncthreads();
+    uint32_t o[2][8];
+    if (p.q_t) quant_mxfp8_tile_columns(tile, scales_t, o, mp, p.n, col0, row0, true);
+    if (p.q_rows) quant_mxfp8_tile_rows(tile, scales_rows, p.q_rows, np, p.m, p.n, row0, col0, true);
+    if (p.partial && threadIdx.x < 128 && col0 + threadIdx.x < p.n) {
+      float s = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kActSumRows; ++w) s += sums[w][threadIdx.x];
+      p.partial[static_cast<int64_t>(rt) * p.n + col0 + threadIdx.x] = s;
+    }
+    __syncthreads();   // every thread has read the staged tile: its storage now collects the transposed payload
+    if (p.q_t) {
+      quant_mxfp8_tile_columns_store(qt_smem, o, p.q_t, mp, p.n, col0, row0);
+      store_scale_tile<4>(scales_t, p.s_t, kScaleMma128, col0, row0 / 32, p.n, mp / 32, (mp / 32 + 3) / 4);
+    }
+    if (p.q_rows)
+      store_scale_tile<4>(scales_rows, p.s_rows, kScaleMma128, row0, col0 / 32, p.m, np / 32, (np / 32 + 3) / 4);
+    __syncthreads();   // the tile, the sums and the scale tiles are free again
+  }
+}
+
+// dbias[c] = bf16( sum over the row tiles of partial[t][c] ): eight threads per column add every eighth tile, the eight
+// sums are added in a fixed order
+__global__ void __launch_bounds__(256) bias_grad_kernel(const float* __restrict__ partial, int row_tiles, int n,
+                                                        __nv_bfloat16* __restrict__ out) {
+  __shared__ float part[8][33];
+  const int lane = threadIdx.x & 31, k = threadIdx.x >> 5;
+  const int col = blockIdx.x * 32 + lane;
+  float s = 0.0f;
+  if (col < n)
+    for (int t = k; t < row_tiles; t += 8) s += partial[static_cast<int64_t>(t) * n + col];
+  part[k][lane] = s;
+  __syncthreads();
+  if (k == 0 && col < n) {
+#pragma unroll
+    for (int i = 1; i < 8; ++i) s += part[i][lane];
+    out[col] = __float2bfloat16_rn(s);
+  }
+}
+
+}  // namespace rtxb

@@ -8,6 +8,7 @@ librtxb.  PyTorch is used only for device memory and the stream handle.
 
 from __future__ import annotations
 
+import functools
 import threading
 from typing import Optional, Tuple
 
@@ -306,6 +307,128 @@ def mxfp8_linear_bwd(dy, x, w, ws: Workspace, *, need_dx: bool = True, need_dw: 
                dw.data_ptr() if need_dw else None, N.OUT_BF16 if dw_dtype == torch.bfloat16 else N.OUT_F32, m, n, k,
                buf.data_ptr(), buf.numel(), _stream_ptr(), status_word(dy.device).data_ptr())
     return dx, dw
+
+
+ACTIVATIONS = {"none": 0, "relu": 1, "relu2": 2, "silu": 3, "gelu": 4, "gelu_tanh": 5}   # RTXB_ACT_* of the header
+
+
+def activation_code(name: str) -> int:
+    try:
+        return ACTIVATIONS[name]
+    except (KeyError, TypeError):
+        raise ValueError(f"unknown activation {name!r}; built: {', '.join(ACTIVATIONS)}") from None
+
+
+def _require_vector(t: torch.Tensor, n: int, device: torch.device, name: str) -> None:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if t.dtype is not torch.bfloat16:
+        raise TypeError(f"{name} must have dtype {torch.bfloat16}, got {t.dtype}")
+    if t.dim() != 1 or t.numel() != n or not t.is_contiguous() or t.device != device:
+        raise ValueError(f"{name} must be a contiguous vector of {n} values on the operands' device")
+
+
+def _epilogue_operands(x, n, k, bias, residual):
+    _require_rows(x, k, "x")
+    if bias is not None:
+        _require_vector(bias, n, x.device, "bias")
+    if residual is not None:
+        _require_rows(residual, n, "residual")
+        if residual.shape[0] != x.shape[0] or residual.device != x.device:
+            raise ValueError("residual must have the result's shape and device")
+    return int(x.shape[0])
+
+
+def mxfp8_linear_epilogue_fwd(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                              residual: Optional[torch.Tensor] = None, *, activation: str = "none", keep_z: bool = False,
+                              rounding: int = N.ROUND_INFINITY):
+    """x bf16 [M, K] (any row pitch), w bf16 [N, K] -> (out, z): z = q(x) q(w)^T + bias, out = bf16(act(z) + residual);
+    z in BF16 with `keep_z`, else None.  The scratch is a fresh allocation of the calling stream."""
+    _require(w, torch.bfloat16, "weight")
+    n, k = (int(v) for v in w.shape)
+    m = _epilogue_operands(x, n, k, bias, residual)
+    if w.device != x.device:
+        raise ValueError("x and weight must share one device")
+    code = activation_code(activation)
+    out = torch.empty(m, n, dtype=torch.bfloat16, device=x.device)
+    z = torch.empty_like(out) if keep_z else None
+    if out.numel() == 0:
+        return out, z
+    nbytes = N.query("rtxb_mxfp8_linear_epilogue_workspace_bytes", m, n, k, 1)
+    with _on(x.device):
+        buf = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        N.call("rtxb_mxfp8_linear_epilogue_fwd", x.data_ptr(), _pitch(x), w.data_ptr(),
+               bias.data_ptr() if bias is not None else None, residual.data_ptr() if residual is not None else None,
+               _pitch(residual) if residual is not None else n, out.data_ptr(), z.data_ptr() if keep_z else None, m, n, k,
+               code, rounding, buf.data_ptr(), nbytes, _stream_ptr(), status_word(x.device).data_ptr())
+    return out, z
+
+
+def mxfp8_linear_epilogue_fwd_prequant_w(x: torch.Tensor, qw: torch.Tensor, sw: torch.Tensor, n: int,
+                                         bias: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None, *,
+                                         activation: str = "none", rounding: int = N.ROUND_INFINITY) -> torch.Tensor:
+    """The same with a packed weight (qw u8 [N, Kp], mma128 scale tiles)."""
+    k = int(x.shape[1]) if x.dim() == 2 else 0
+    m = _epilogue_operands(x, n, k, bias, residual)
+    if qw.device != x.device or sw.device != x.device:
+        raise ValueError("x and the packed weight must share one device")
+    if qw.element_size() != 1 or qw.numel() != n * mx_storage_k(k) or not qw.is_contiguous():
+        raise ValueError(f"packed weight must hold {n} rows of {mx_storage_k(k)} values")
+    if sw.element_size() != 1 or sw.numel() != mxfp8_scale_numel(n, k, N.SCALE_MMA128) or not sw.is_contiguous():
+        raise ValueError("packed weight scales must be mma128 tiles")
+    code = activation_code(activation)
+    out = torch.empty(m, n, dtype=torch.bfloat16, device=x.device)
+    if out.numel() == 0:
+        return out
+    nbytes = N.query("rtxb_mxfp8_linear_epilogue_workspace_bytes", m, n, k, 0)
+    with _on(x.device):
+        buf = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        N.call("rtxb_mxfp8_linear_epilogue_fwd_prequant_w", x.data_ptr(), _pitch(x), qw.data_ptr(), sw.data_ptr(),
+               bias.data_ptr() if bias is not None else None, residual.data_ptr() if residual is not None else None,
+               _pitch(residual) if residual is not None else n, out.data_ptr(), m, n, k, code, rounding, buf.data_ptr(),
+               nbytes, _stream_ptr(), status_word(x.device).data_ptr())
+    return out
+
+
+def mxfp8_linear_epilogue_bwd(dy: torch.Tensor, z: Optional[torch.Tensor], x: Optional[torch.Tensor],
+                              w: Optional[torch.Tensor], k: int, *, activation: str = "none", need_dx: bool = True,
+                              need_dw: bool = True, need_dbias: bool = False):
+    """(dY [M, N], z [M, N] of the forward, X [M, K], W [N, K]) -> (dX | None, dW | None, dbias [N] | None); z is read
+    unless activation is none, X for dW only, W for dX only."""
+    code = activation_code(activation)
+    _require_rows(dy, None, "grad_output")
+    m, n = (int(v) for v in dy.shape)
+    if code:
+        _require(z, torch.bfloat16, "z")
+        if z.shape != dy.shape or z.device != dy.device:
+            raise ValueError("z must have grad_output's shape and device")
+    if need_dw:
+        _require_rows(x, k, "x")
+        if x.shape[0] != m or x.device != dy.device:
+            raise ValueError("grad_output and x disagree on the rows or the device")
+    if need_dx:
+        _require(w, torch.bfloat16, "weight")
+        if tuple(w.shape) != (n, k) or w.device != dy.device:
+            raise ValueError("weight must be [N, K] on grad_output's device")
+    new = functools.partial(torch.empty, dtype=torch.bfloat16, device=dy.device)
+    dx = new(m, k) if need_dx else None
+    dw = new(n, k) if need_dw else None
+    db = new(n) if need_dbias else None
+    outs = (dx, dw, db)
+    if all(t is None for t in outs):
+        return outs
+    if min(m, n, k) == 0:                 # an empty sum is zero
+        return tuple(None if t is None else t.zero_() for t in outs)
+    nbytes = N.query("rtxb_mxfp8_linear_epilogue_backward_workspace_bytes", m, n, k, int(need_dx), int(need_dw),
+                     int(need_dbias))
+    with _on(dy.device):
+        buf = torch.empty(nbytes, dtype=torch.uint8, device=dy.device)
+        N.call("rtxb_mxfp8_linear_epilogue_bwd", dy.data_ptr(), _pitch(dy), z.data_ptr() if code else None,
+               x.data_ptr() if need_dw else None, _pitch(x) if need_dw else k, w.data_ptr() if need_dx else None,
+               dx.data_ptr() if need_dx else None, dw.data_ptr() if need_dw else None,
+               db.data_ptr() if need_dbias else None, m, n, k, code, buf.data_ptr(), nbytes, _stream_ptr(),
+               status_word(dy.device).data_ptr())
+    return outs
 
 
 MAX_GROUPS = 512
