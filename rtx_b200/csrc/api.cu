@@ -230,7 +230,7 @@ int launch_gemm(const void* qa, const void* sa, const void* qb, const void* sb, 
       const int64_t start_pair = static_cast<int64_t>(blocks->first_block) * (blocks->block_rows / 256);
       p.tile_shift = static_cast<int>(((start_pair / p.group_m) * p.group_m * p.n_tiles) % pair_tiles);
     }
-    cudaError_t le = launch_dependent(pk, 2 * pairs, kGemmThreads, P::kSmemBytes, stream,
+    cudaError_t le = launch_dependent(pk, 2 * pairs, kPairThreads<EPI>, P::kSmemBytes, stream,
                                       overlap_previous || after_quantizer, map_a, map_b, map_sfa, map_sfb, maps_out, p);
     if (le != cudaSuccess) return fail_cuda(le, "gemm_blockscaled_pair_kernel launch");
     return RTXB_OK;
@@ -1006,9 +1006,9 @@ int rtxb_mxfp8_linear_epilogue_bwd(const void* dy, int64_t lddy, const void* z, 
   q.s_t = mem.s_dzt;
   q.partial = mem.partial;
   const int64_t row_tiles = (m + 127) / 128, tiles = row_tiles * ((n + 127) / 128);
-  cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(quant_mxfp8_act_backward_kernel), kQtTileBytes);
+  cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(quant_mxfp8_act_backward_kernel), kActSmemBytes);
   if (e != cudaSuccess) return fail_cuda(e, "cudaFuncSetAttribute(activation backward quantizer)");
-  quant_mxfp8_act_backward_kernel<<<quant_grid(tiles, 4), kQuantThreads, kQtTileBytes, s>>>(q);
+  quant_mxfp8_act_backward_kernel<<<quant_grid(tiles, kActOccupancy), kQuantThreads, kActSmemBytes, s>>>(q);
   RTXB_CHECK_LAUNCH("quant_mxfp8_act_backward_kernel");
   if (dbias) {
     bias_grad_kernel<<<static_cast<int>((n + 31) / 32), 256, 0, s>>>(mem.partial, static_cast<int>(row_tiles),

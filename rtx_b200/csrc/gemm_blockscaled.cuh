@@ -191,24 +191,34 @@ __device__ __forceinline__ void act_apply(int act, float (&v)[32]) {
     for (int e = 0; e < 32; ++e) v[e] = act_value<decltype(tag)::value>(v[e]);
   });
 }
-__device__ __forceinline__ void act_add_residual(const GemmParams& p, float (&v)[32], int row, bool row_ok, int col) {
+// 32 columns of one residual row, packed two per word; loaded ahead of the activation so that the latency is covered
+__device__ __forceinline__ void act_load_residual(const GemmParams& p, uint32_t (&w)[16], int row, bool row_ok, int col) {
+#pragma unroll
+  for (int e = 0; e < 16; ++e) w[e] = 0;
   if (p.residual == nullptr || !row_ok) return;
   const __nv_bfloat16* src = p.residual + static_cast<int64_t>(row) * p.ldr + col;
   if (p.residual_vec_ok && col + 32 <= p.out_cols) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const uint4 b = __ldg(reinterpret_cast<const uint4*>(src) + j);
-      const uint32_t w[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        v[8 * j + 2 * e] += bf16_lo(w[e]);
-        v[8 * j + 2 * e + 1] += bf16_hi(w[e]);
-      }
+      w[4 * j] = b.x; w[4 * j + 1] = b.y; w[4 * j + 2] = b.z; w[4 * j + 3] = b.w;
     }
   } else {
+    const uint16_t* bits = reinterpret_cast<const uint16_t*>(src);
 #pragma unroll
-    for (int e = 0; e < 32; ++e)
-      if (col + e < p.out_cols) v[e] += __bfloat162float(src[e]);
+    for (int e = 0; e < 16; ++e) {
+      const uint32_t lo = col + 2 * e < p.out_cols ? bits[2 * e] : 0u;
+      const uint32_t hi = col + 2 * e + 1 < p.out_cols ? bits[2 * e + 1] : 0u;
+      w[e] = lo | (hi << 16);
+    }
+  }
+}
+__device__ __forceinline__ void act_add_residual(const GemmParams& p, float (&v)[32], const uint32_t (&w)[16]) {
+  if (p.residual == nullptr) return;   // v + 0 would turn -0 into 0
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    v[2 * e] += bf16_lo(w[e]);
+    v[2 * e + 1] += bf16_hi(w[e]);
   }
 }
 __device__ __forceinline__ void pack_bf16x32(const float (&v)[32], uint32_t (&w)[16]) {
@@ -365,43 +375,19 @@ __device__ __forceinline__ void epilogue_drain(const GemmParams& p, uint32_t tac
         for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(r[e]) * out_scale;
       }
       if (EPI == kEpiAct) {
-        // z is rounded to BF16 only for the backward; the activation takes the FP32 value
+        // single-CTA kernel only (one row block): direct stores, one row per lane
+        uint32_t res[16], w[16];
+        act_load_residual(p, res, row, row_ok, col);
         act_add_bias(p, v, col);
-        uint32_t w[16];
-        if (staged) {
-          // with z both staging buffers of the warp are used by a chunk (0: z, 1: the result), without it they alternate
-          uint8_t* buf = stage + (p.z_out ? 1 : (i & 1)) * kEpiStageBufBytes;
-          if (lane == 0) {
-            if (p.z_out) tma_store_wait_read<0>();
-            else tma_store_wait_read<1>();
-          }
-          __syncwarp();
-          if (p.z_out) {
-            pack_bf16x32(v, w);
-            stage_bf16x32(stage, lane, w);
-          }
-          act_apply(p.act, v);
-          act_add_residual(p, v, row, row_ok, col);
+        const int64_t at = static_cast<int64_t>(row) * p.ldo;
+        if (p.z_out) {
           pack_bf16x32(v, w);
-          stage_bf16x32(buf, lane, w);
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            if (p.z_out) tma_store_2d(map_out + 1, stage, col, row - lane - out_row0);
-            tma_store_2d(map_out, buf, col, row - lane - out_row0);
-            tma_store_commit();
-          }
-        } else {
-          const int64_t at = static_cast<int64_t>(row) * p.ldo;
-          if (p.z_out) {
-            pack_bf16x32(v, w);
-            store_bf16x32(p.z_out + at, col, p.out_cols, p.out_vec_ok != 0, w);
-          }
-          act_apply(p.act, v);
-          act_add_residual(p, v, row, row_ok, col);
-          pack_bf16x32(v, w);
-          store_bf16x32(reinterpret_cast<__nv_bfloat16*>(p.out) + at, col, p.out_cols, p.out_vec_ok != 0, w);
+          store_bf16x32(p.z_out + at, col, p.out_cols, p.out_vec_ok != 0, w);
         }
+        act_apply(p.act, v);
+        act_add_residual(p, v, res);
+        pack_bf16x32(v, w);
+        store_bf16x32(reinterpret_cast<__nv_bfloat16*>(p.out) + at, col, p.out_cols, p.out_vec_ok != 0, w);
       } else if (EPI == kEpiF32) {
         if (staged) {
           // 32 rows x 128 bytes = both staging buffers as one box (128-byte swizzle: 16-byte chunk j of row r at
@@ -474,6 +460,130 @@ __device__ __forceinline__ void epilogue_drain(const GemmParams& p, uint32_t tac
       emit(c, i, r);
     }
   }
+}
+
+// kEpiAct in the pair kernel: one tile of this warp's 32 rows, columns [128 half, 128 half + 128) of the accumulator.
+// Eight warps drain a tile (two per lane quadrant): an activation costs some thirty instructions per value and every
+// chunk waits for TMEM, for the residual and for its staging buffer, more than four warps can hide behind the next
+// tile's MMAs (8192 x 4096 x 8192 with gelu, residual and z: 304 us with four warps).  A chunk is 32 rows x 32 columns:
+//   z = acc + bias, staged and stored while act(z) is computed (training only; rounded to BF16 for the backward, the
+//   activation takes the FP32 value), then act(z) + residual through the same 2 KB buffer.
+// The residual of the next chunk is fetched before the current one is finished.
+// Overlap barrier: the two windows share one chunk, which belongs to half 1 of an even window and half 0 of an odd one;
+// its warps signal when they hold it in registers, the others at once.  All signal only after they have seen this tile
+// accumulated, so that no signal can be counted for the tile before it.
+constexpr int kActEpiWarps = 8;
+constexpr int kActGemmThreads = 64 + 32 * kActEpiWarps;
+
+// 32 rows x 32 columns from the staging buffer (64-byte swizzle) to rows of any alignment: 64-byte segments
+__device__ __forceinline__ void act_store_rows(const uint8_t* buf, __nv_bfloat16* out, int64_t ldo, int row0, int rows,
+                                               int col, int cols, int lane) {
+  if (col + lane >= cols) return;
+  __nv_bfloat16* dst = out + static_cast<int64_t>(row0) * ldo + col + lane;
+#pragma unroll 8
+  for (int j = 0; j < 32; ++j)
+    if (row0 + j < rows)
+      dst[j * ldo] = *reinterpret_cast<const __nv_bfloat16*>(buf + j * 64 + (((lane >> 3) ^ ((j >> 1) & 3)) << 4) + (lane & 7) * 2);
+}
+// the reverse for a residual of any alignment: through the buffer into one row per lane
+__device__ __forceinline__ void act_load_rows(const GemmParams& p, uint8_t* buf, uint32_t (&w)[16], int row0, int col, int lane) {
+  const uint16_t* src = reinterpret_cast<const uint16_t*>(p.residual) + static_cast<int64_t>(row0) * p.ldr + col + lane;
+  const bool col_ok = col + lane < p.out_cols;
+#pragma unroll 8
+  for (int j = 0; j < 32; ++j)
+    *reinterpret_cast<uint16_t*>(buf + j * 64 + (((lane >> 3) ^ ((j >> 1) & 3)) << 4) + (lane & 7) * 2) =
+        col_ok && row0 + j < p.m ? src[j * p.ldr] : static_cast<uint16_t>(0);
+  __syncwarp();
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint4 v = *reinterpret_cast<const uint4*>(buf + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4));
+    w[4 * j] = v.x; w[4 * j + 1] = v.y; w[4 * j + 2] = v.z; w[4 * j + 3] = v.w;
+  }
+  __syncwarp();
+}
+
+template <int KIND>
+__device__ __forceinline__ bool act_epilogue_tile(const GemmParams& p, uint32_t tacc, int row0, int n_idx, bool odd, int half,
+                                                  uint64_t* acc_full_bar, uint32_t parity, volatile int* abort_flag,
+                                                  uint32_t overlap_bar_addr, float out_scale, int lane,
+                                                  const CUtensorMap* map_out, uint8_t* buf) {
+  using TP = TmemPlan<KIND>;
+  static_assert(TP::kOverlapChunks == 1, "one chunk shared by the two windows");
+  const bool holder = odd ? half == 0 : half == 1;
+  const int first = odd ? 0 : 3;                   // the shared chunk within its half
+  const int col_base = n_idx * kBlockN + half * 128;
+  const int row = row0 + lane;
+  const bool row_ok = row < p.m;
+  const bool res_ahead = p.residual != nullptr && p.residual_vec_ok;
+  uint32_t res[16], next[16];
+  if (res_ahead) act_load_residual(p, res, row, row_ok && col_base + 32 * first < p.out_cols, col_base + 32 * first);
+  if (!mbar_wait(acc_full_bar, parity, abort_flag)) return false;
+  tc_fence_after_sync();
+  if (!holder && lane == 0) mbar_arrive_cluster(overlap_bar_addr);
+#pragma unroll 1
+  for (int i = 0; i < 4; ++i) {
+    const int c = 32 * ((first + i) & 3), col = col_base + c;
+    uint32_t r[32];
+    tmem_ld_32x32(tacc + half * 128 + c, r);
+    if (res_ahead && i < 3) {
+      const int cn = col_base + 32 * ((first + i + 1) & 3);
+      act_load_residual(p, next, row, row_ok && cn < p.out_cols, cn);
+    }
+    tmem_ld_wait();
+    if (holder && i == 0) {
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(overlap_bar_addr);
+    }
+    if (col < p.out_cols) {                        // warp-uniform
+      float v[32];
+      uint32_t w[16];
+#pragma unroll
+      for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(r[e]) * out_scale;
+      act_add_bias(p, v, col);
+      if (p.z_out) {
+        pack_bf16x32(v, w);
+        if (p.tma_out && lane == 0) tma_store_wait_read<0>();
+        __syncwarp();
+        stage_bf16x32(buf, lane, w);
+        if (p.tma_out) {
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_2d(map_out + 1, buf, col, row0);
+            tma_store_commit();
+          }
+        } else {
+          __syncwarp();
+          act_store_rows(buf, p.z_out, p.ldo, row0, p.m, col, p.out_cols, lane);
+        }
+      }
+      act_apply(p.act, v);
+      if (p.tma_out && lane == 0) tma_store_wait_read<0>();
+      __syncwarp();
+      if (p.residual != nullptr && !p.residual_vec_ok) act_load_rows(p, buf, res, row0, col, lane);
+      act_add_residual(p, v, res);
+      pack_bf16x32(v, w);
+      stage_bf16x32(buf, lane, w);
+      if (p.tma_out) {
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          tma_store_2d(map_out, buf, col, row0);
+          tma_store_commit();
+        }
+      } else {
+        __syncwarp();
+        act_store_rows(buf, reinterpret_cast<__nv_bfloat16*>(p.out), p.ldo, row0, p.m, col, p.out_cols, lane);
+        __syncwarp();
+      }
+    }
+    if (res_ahead) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) res[e] = next[e];
+    }
+  }
+  return true;
 }
 
 // shared -> TMEM copy of one K step's scale factors into scale set `set`.
@@ -788,8 +898,12 @@ struct PairTraits {
       idesc_block_scaled(256, 256, KIND == kKindMxfp8 ? 0u : 1u, KIND == kKindMxfp8 ? 1u : 0u);
 };
 
+// threads of the pair kernel: two roles and the epilogue warps
+template <int EPI>
+constexpr int kPairThreads = EPI == kEpiAct ? kActGemmThreads : kGemmThreads;
+
 template <int KIND, int EPI>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads<EPI>, 1)
 gemm_blockscaled_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                              const __grid_constant__ CUtensorMap map_sfa, const __grid_constant__ CUtensorMap map_sfb,
                              const __grid_constant__ OutMaps maps_out, const GemmParams p) {
@@ -822,7 +936,7 @@ gemm_blockscaled_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __
       mbar_init(&empty_bar[s], 1);
     }
     mbar_init(acc_full_bar, 1);
-    mbar_init(acc_overlap_bar, 8);
+    mbar_init(acc_overlap_bar, 2 * (kPairThreads<EPI> / 32 - 2));   // every epilogue warp of both CTAs
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -938,6 +1052,16 @@ gemm_blockscaled_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __
       const int row = (mp_idx * 2 + static_cast<int>(rank)) * 128 + quad * 32 + lane;
       const bool row_ok = row < p.m;
       const uint32_t acc_col = (local_tile & 1) ? TP::kAccWindow1 : 0;
+      if constexpr (EPI == kEpiAct) {
+        if (!act_epilogue_tile<KIND>(p, tmem_base + lane_base + acc_col, row - lane, n_idx, (local_tile & 1) != 0,
+                                     (warp - 2) >> 2, acc_full_bar, local_tile & 1, abort_flag, overlap_addr, out_scale, lane,
+                                     maps_out.m, smem + T::kOffStage + (warp - 2) * kEpiStageBufBytes)) {
+          if (p.status && lane == 0) atomicCAS(p.status, 0, kStatusWaitEpilogue);
+          *abort_flag = 1;
+          break;
+        }
+        continue;
+      }
       if (!mbar_wait(acc_full_bar, local_tile & 1, abort_flag)) {
         if (p.status && lane == 0) atomicCAS(p.status, 0, kStatusWaitEpilogue);
         *abort_flag = 1;

@@ -314,7 +314,8 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
           const int c = col + 32 * half;
           const int64_t at = static_cast<int64_t>(row) * p.ldo;
           float v[32];
-          uint32_t w[16];
+          uint32_t res[16], w[16];
+          act_load_residual(p, res, row, true, c);
 #pragma unroll
           for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(r[e]) * out_scale;
           act_add_bias(p, v, c);
@@ -323,7 +324,7 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
             store_bf16x32(p.z_out + at, c, p.out_cols, p.out_vec_ok != 0, w);
           }
           act_apply(p.act, v);
-          act_add_residual(p, v, row, true, c);
+          act_add_residual(p, v, res);
           pack_bf16x32(v, w);
           store_bf16x32(reinterpret_cast<__nv_bfloat16*>(p.out) + at, c, p.out_cols, p.out_vec_ok != 0, w);
         } else if (EPI == kEpiBf16) {

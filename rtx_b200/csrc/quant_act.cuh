@@ -4,7 +4,8 @@
 //   q_t     MXFP8 of dz^T, blocks along m    (A operand of dW = dz^T X)
 //   partial[m / 128][n] = sum of 128 rows of dz in FP32, before the rounding   (dbias, finished by the kernel below)
 // dy and z are read once (4 bytes per value), 2 bytes of payload leave: without the fusion dz is written and read again
-// (4 more).  HBM bound; one 128 x 128 tile per block step, three blocks per SM overlap one another's loads and stores.
+// (4 more).  HBM bound; one 128 x 128 tile per block step, the next one
+// is fetched asynchronously while this one is quantized.
 #pragma once
 
 #include "activation.cuh"
@@ -24,11 +25,34 @@ struct QuantActParams {
   float* partial;            // [ceil(m / 128)][n] or nullptr
 };
 
+constexpr int kActOccupancy = 2;                  // resident blocks per SM (three staged tiles each)
 constexpr int kActSumRows = kQuantThreads / 32;   // partial column sums per tile before the last step, one per warp
+constexpr int kActSmemBytes = 3 * kQtTileBytes;   // raw dy, raw z, dz
 
-__global__ void __launch_bounds__(kQuantThreads, 4) quant_mxfp8_act_backward_kernel(const QuantActParams p) {
+// Raw tile of dy or z into `raw`: thread t copies the 8 columns (t & 15) of the rows (t >> 4) + 16 j, the ones it will
+// read back itself, so no barrier stands between the copy and its use.
+__device__ __forceinline__ void act_fetch(const __nv_bfloat16* src, int64_t ld, bool vec_ok, int m, int n, int row0, int col0,
+                                          uint16_t (*raw)[kQtPitch]) {
+  const int c8 = (threadIdx.x & 15) * 8, r0 = threadIdx.x >> 4;
+  const int col = col0 + c8;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int row = row0 + r0 + 16 * j;
+    const bool live = row < m && col < n;
+    if (vec_ok && (!live || col + 8 <= n)) {
+      cp_async_16(&raw[r0 + 16 * j][c8], src + (live ? row * ld + col : 0), live);
+    } else {
+      *reinterpret_cast<uint4*>(&raw[r0 + 16 * j][c8]) = live ? load8_raw(src + row * ld, col, n, false) : make_uint4(0, 0, 0, 0);
+    }
+  }
+}
+
+__global__ void __launch_bounds__(kQuantThreads, kActOccupancy) quant_mxfp8_act_backward_kernel(const QuantActParams p) {
   extern __shared__ __align__(16) uint8_t qt_smem[];
-  uint16_t (*tile)[kQtPitch] = reinterpret_cast<uint16_t (*)[kQtPitch]>(qt_smem);
+  uint16_t (*raw_g)[kQtPitch] = reinterpret_cast<uint16_t (*)[kQtPitch]>(qt_smem);
+  uint16_t (*raw_z)[kQtPitch] = reinterpret_cast<uint16_t (*)[kQtPitch]>(qt_smem + kQtTileBytes);
+  uint8_t* stage = qt_smem + 2 * kQtTileBytes;
+  uint16_t (*tile)[kQtPitch] = reinterpret_cast<uint16_t (*)[kQtPitch]>(stage);
   __shared__ __align__(16) uint8_t scales_t[128][4];
   __shared__ __align__(16) uint8_t scales_rows[128][4];
   __shared__ float sums[kActSumRows][128];
@@ -38,46 +62,44 @@ __global__ void __launch_bounds__(kQuantThreads, 4) quant_mxfp8_act_backward_ker
   const bool vec_z = (p.n % 8 == 0) && ((reinterpret_cast<uintptr_t>(p.z) & 15) == 0);
   const int c8 = (threadIdx.x & 15) * 8, r0 = threadIdx.x >> 4;
   const int64_t total = static_cast<int64_t>(row_tiles) * col_tiles;
+  auto fetch = [&](int64_t t) {
+    const int rt = static_cast<int>(t / col_tiles), ct = static_cast<int>(t - static_cast<int64_t>(rt) * col_tiles);
+    act_fetch(p.dy, p.lddy, vec_dy, p.m, p.n, rt * 128, ct * 128, raw_g);
+    if (p.z) act_fetch(p.z, p.n, vec_z, p.m, p.n, rt * 128, ct * 128, raw_z);
+    cp_async_commit();
+  };
+  if (blockIdx.x < total) fetch(blockIdx.x);
   for (int64_t t = blockIdx.x; t < total; t += gridDim.x) {
     const int rt = static_cast<int>(t / col_tiles);
     const int row0 = rt * 128, col0 = static_cast<int>(t - static_cast<int64_t>(rt) * col_tiles) * 128;
-    const int col = col0 + c8;
+    cp_async_wait<0>();
     float sum[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) sum[e] = 0.0f;
+#pragma unroll 4
+    for (int j = 0; j < 8; ++j) {
+      float v[8];
+      unpack8(*reinterpret_cast<const uint4*>(&raw_g[r0 + 16 * j][c8]), v);
+      if (p.z) {
+        float z[8];
+        unpack8(*reinterpret_cast<const uint4*>(&raw_z[r0 + 16 * j][c8]), z);
+        with_activation(p.act, [&](auto tag) {
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      uint4 g[4], z[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int row = row0 + r0 + 16 * (half * 4 + j);
-        const bool live = row < p.m && col < p.n;
-        g[j] = live ? load8_raw(p.dy + row * p.lddy, col, p.n, vec_dy) : make_uint4(0, 0, 0, 0);
-        z[j] = live && p.z ? load8_raw(p.z + static_cast<int64_t>(row) * p.n, col, p.n, vec_z) : make_uint4(0, 0, 0, 0);
+          for (int e = 0; e < 8; ++e) v[e] *= act_slope<decltype(tag)::value>(z[e]);
+        });
       }
+      uint32_t w[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        float v[8];
-        unpack8(g[j], v);
-        if (p.z) {
-          float zz[8];
-          unpack8(z[j], zz);
-          with_activation(p.act, [&](auto tag) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] *= act_slope<decltype(tag)::value>(zz[e]);
-          });
-        }
-        uint32_t w[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          sum[2 * e] += v[2 * e];
-          sum[2 * e + 1] += v[2 * e + 1];
-          __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
-          w[e] = *reinterpret_cast<uint32_t*>(&b);
-        }
-        *reinterpret_cast<uint4*>(&tile[r0 + 16 * (half * 4 + j)][c8]) = make_uint4(w[0], w[1], w[2], w[3]);
+      for (int e = 0; e < 4; ++e) {
+        sum[2 * e] += v[2 * e];
+        sum[2 * e + 1] += v[2 * e + 1];
+        __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
+        w[e] = *reinterpret_cast<uint32_t*>(&b);
       }
+      *reinterpret_cast<uint4*>(&tile[r0 + 16 * j][c8]) = make_uint4(w[0], w[1], w[2], w[3]);
     }
+    // this thread's part of the raw tiles is read: the next tile's may come in while this one is quantized
+    if (t + gridDim.x < total) fetch(t + gridDim.x);
     if (p.partial) {
       // the two row halves of a warp, then one row of sums per warp
 #pragma unroll
@@ -99,12 +121,12 @@ __global__ void __launch_bounds__(kQuantThreads, 4) quant_mxfp8_act_backward_ker
     }
     __syncthreads();   // every thread has read the staged tile: its storage now collects the transposed payload
     if (p.q_t) {
-      quant_mxfp8_tile_columns_store(qt_smem, o, p.q_t, mp, p.n, col0, row0);
+      quant_mxfp8_tile_columns_store(stage, o, p.q_t, mp, p.n, col0, row0);
       store_scale_tile<4>(scales_t, p.s_t, kScaleMma128, col0, row0 / 32, p.n, mp / 32, (mp / 32 + 3) / 4);
     }
     if (p.q_rows)
       store_scale_tile<4>(scales_rows, p.s_rows, kScaleMma128, row0, col0 / 32, p.m, np / 32, (np / 32 + 3) / 4);
-    __syncthreads();   // the tile, the sums and the scale tiles are free again
+    __syncthreads();   // the staged tile, the sums and the scale tiles are free again
   }
 }
 
