@@ -25,65 +25,98 @@ constexpr float kInvSqrt2Pi = 0.39894228040143268f;
 constexpr float kGeluTanhA = 0.79788456080286536f;   // sqrt(2 / pi)
 constexpr float kGeluTanhB = 0.044715f;
 
-__device__ __forceinline__ float fast_rcp(float x) {
-  float r;
-  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
+// 1 / x and 2^x of both halves by the special-function unit
+__device__ __forceinline__ f32x2 rcp2(f32x2 v) {
+  float a, b;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"(lo(v)));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(b) : "f"(hi(v)));
+  return pack2(a, b);
 }
-// 1 / (1 + e^-z): 0 and 1 at the ends (e^-z overflows to infinity, whose reciprocal is 0)
-__device__ __forceinline__ float sigmoid(float z) { return fast_rcp(1.0f + __expf(-z)); }
-
-// Phi(z); `e` receives e^(-z^2 / 2)
-__device__ __forceinline__ float normal_cdf(float z, float& e) {
-  const float x = fabsf(z) * kSqrtHalf;
-  const float t = fast_rcp(fmaf(0.3275911f, x, 1.0f));
-  e = __expf(-x * x);
-  float c = fmaf(1.061405429f, t, -1.453152027f);
-  c = fmaf(c, t, 1.421413741f);
-  c = fmaf(c, t, -0.284496736f);
-  c = fmaf(c, t, 0.254829592f);
-  const float lower = 0.5f * c * t * e;
-  return z < 0.0f ? lower : 1.0f - lower;
+__device__ __forceinline__ f32x2 exp2_2(f32x2 v) {
+  float a, b;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"(lo(v)));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(b) : "f"(hi(v)));
+  return pack2(a, b);
 }
+constexpr float kLog2E = 1.4426950408889634f;
 
-// Beyond +-128 silu and the two gelus are their limits to the last bit (e^128 overflows, e^-8192 is 0), so the arguments
-// are held there: infinities and the type's lowest value give the limit (0, z, slope 0 or 1) and not inf * 0.
-// NaN passes through (the comparisons are false).
+// s(z) for both; 0 and 1 at the ends (e^-z overflows to infinity, whose reciprocal is 0)
+__device__ __forceinline__ f32x2 sigmoid2(f32x2 z) { return rcp2(add2(exp2_2(mul2(z, both(-kLog2E))), both(1.0f))); }
+// s(2 a (z + b z^3)): the exponent is -2 a log2(e) z (1 + b z^2)
+__device__ __forceinline__ f32x2 gelu_tanh_gate2(f32x2 z, f32x2 zz) {
+  constexpr float k = -2.0f * kGeluTanhA * kLog2E;
+  return rcp2(add2(exp2_2(mul2(z, fma2(zz, both(k * kGeluTanhB), both(k)))), both(1.0f)));
+}
+// -Phi(-a) for a >= 0; `e` receives e^(-a^2 / 2).  The 1/2 and the sign are in the coefficients.
+__device__ __forceinline__ f32x2 minus_tail2(f32x2 a, f32x2& e) {
+  const f32x2 t = rcp2(fma2(a, both(0.3275911f * kSqrtHalf), both(1.0f)));
+  e = exp2_2(mul2(mul2(a, a), both(-0.5f * kLog2E)));
+  f32x2 c = fma2(t, both(-0.5f * 1.061405429f), both(0.5f * 1.453152027f));
+  c = fma2(c, t, both(-0.5f * 1.421413741f));
+  c = fma2(c, t, both(0.5f * 0.284496736f));
+  c = fma2(c, t, both(-0.5f * 0.254829592f));
+  return mul2(c, mul2(t, e));
+}
+__device__ __forceinline__ float abs_upto_128(float z) { return fmin_nan(fabsf(z), 128.0f); }
+
+// Beyond +-128 silu and the two gelus are their limits to the last bit (e^128 overflows, e^-8192 is 0), so what could
+// become inf * 0 is held there: infinities and the type's lowest value give the limit (0, z, slope 0 or 1).  NaN passes
+// through every step.
 template <int ACT>
-__device__ __forceinline__ float act_value(float z) {
-  if (ACT == kActRelu) return z < 0.0f ? 0.0f : z;
-  if (ACT == kActRelu2) return z < 0.0f ? 0.0f : z * z;
-  if (ACT != kActNone) z = z < -128.0f ? -128.0f : z;
-  if (ACT == kActSilu) return z * sigmoid(z);
-  if (ACT == kActGelu) {
-    float e;
-    return z * normal_cdf(z, e);
+__device__ __forceinline__ void act_value2(float& x, float& y) {
+  if (ACT == kActRelu || ACT == kActRelu2) {
+    x = fmax_nan(x, 0.0f);
+    y = fmax_nan(y, 0.0f);
+    if (ACT == kActRelu2) { x *= x; y *= y; }
+    return;
   }
-  if (ACT == kActGeluTanh) return z * sigmoid(2.0f * kGeluTanhA * z * fmaf(kGeluTanhB * z, z, 1.0f));
-  return z;
+  f32x2 r;
+  if (ACT == kActGelu) {
+    // z Phi(z) = max(z, 0) - |z| Phi(-|z|)
+    f32x2 e;
+    const f32x2 a = pack2(abs_upto_128(x), abs_upto_128(y));
+    r = fma2(a, minus_tail2(a, e), pack2(fmax_nan(x, 0.0f), fmax_nan(y, 0.0f)));
+  } else {
+    const f32x2 z = pack2(fmax_nan(x, -128.0f), fmax_nan(y, -128.0f));
+    r = mul2(z, ACT == kActSilu ? sigmoid2(z) : gelu_tanh_gate2(z, mul2(z, z)));
+  }
+  x = lo(r);
+  y = hi(r);
 }
 
-// act'(z); relu has slope 0 at 0
+// g * act'(z) for a pair; relu has slope 0 at 0
 template <int ACT>
-__device__ __forceinline__ float act_slope(float z) {
-  if (ACT == kActRelu) return z > 0.0f ? 1.0f : (z == z ? 0.0f : z);
-  if (ACT == kActRelu2) return z > 0.0f ? 2.0f * z : (z == z ? 0.0f : z);
-  z = z < -128.0f ? -128.0f : z > 128.0f ? 128.0f : z;
+__device__ __forceinline__ void act_slope2(float& gx, float& gy, float x, float y) {
+  if (ACT == kActRelu || ACT == kActRelu2) {
+    const float k = ACT == kActRelu ? 1.0f : 2.0f;
+    gx *= x > 0.0f ? (ACT == kActRelu ? k : k * x) : (x == x ? 0.0f : x);
+    gy *= y > 0.0f ? (ACT == kActRelu ? k : k * y) : (y == y ? 0.0f : y);
+    return;
+  }
+  const f32x2 one = both(1.0f);
+  const f32x2 z = pack2(fmin_nan(fmax_nan(x, -128.0f), 128.0f), fmin_nan(fmax_nan(y, -128.0f), 128.0f));
+  f32x2 d;
   if (ACT == kActSilu) {
-    const float s = sigmoid(z);
-    return s * fmaf(z, 1.0f - s, 1.0f);
+    // s (1 + z (1 - s))
+    const f32x2 s = sigmoid2(z);
+    d = mul2(s, fma2(z, fma2(s, both(-1.0f), one), one));
+  } else if (ACT == kActGelu) {
+    // Phi(z) + z phi(z)
+    f32x2 e;
+    const f32x2 m = minus_tail2(pack2(fabsf(lo(z)), fabsf(hi(z))), e);
+    const f32x2 up = add2(m, one);
+    const f32x2 cdf = pack2(x < 0.0f ? -lo(m) : lo(up), y < 0.0f ? -hi(m) : hi(up));
+    d = fma2(mul2(z, both(kInvSqrt2Pi)), e, cdf);
+  } else {
+    // s + z s (1 - s) 2 a (1 + 3 b z^2)
+    const f32x2 zz = mul2(z, z);
+    const f32x2 s = gelu_tanh_gate2(z, zz);
+    const f32x2 w = mul2(mul2(z, s), fma2(zz, both(6.0f * kGeluTanhA * kGeluTanhB), both(2.0f * kGeluTanhA)));
+    d = fma2(w, fma2(s, both(-1.0f), one), s);
   }
-  if (ACT == kActGelu) {
-    float e;
-    const float cdf = normal_cdf(z, e);
-    return fmaf(z * kInvSqrt2Pi, e, cdf);
-  }
-  if (ACT == kActGeluTanh) {
-    // d(2u)/dz = 2 a (1 + 3 b z^2)
-    const float s = sigmoid(2.0f * kGeluTanhA * z * fmaf(kGeluTanhB * z, z, 1.0f));
-    return fmaf(z * s * (1.0f - s), 2.0f * kGeluTanhA * fmaf(3.0f * kGeluTanhB * z, z, 1.0f), s);
-  }
-  return 1.0f;
+  d = mul2(pack2(gx, gy), d);
+  gx = lo(d);
+  gy = hi(d);
 }
 
 template <int ACT>

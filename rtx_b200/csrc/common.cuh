@@ -373,8 +373,56 @@ __device__ __forceinline__ float fmin_nan(float a, float b) {
   asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
+// magnitudes of two packed BF16 values against a running maximum; NaN wins
+__device__ __forceinline__ uint32_t absmax_bf16x2(uint32_t m, uint32_t w) {
+  const __nv_bfloat162 r = __hmax2_nan(*reinterpret_cast<const __nv_bfloat162*>(&m),
+                                       __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w)));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+// FP32 pairs in one 64-bit register: the packed multiply-add handles two values per instruction
+struct f32x2 {
+  uint64_t bits;
+};
+__device__ __forceinline__ f32x2 pack2(float a, float b) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.bits) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 both(float a) { return pack2(a, a); }
+__device__ __forceinline__ float lo(f32x2 v) {
+  float a, b;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v.bits));
+  return a;
+}
+__device__ __forceinline__ float hi(f32x2 v) {
+  float a, b;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v.bits));
+  return b;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits));
+  return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits));
+  return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits), "l"(c.bits));
+  return r;
+}
 __device__ __forceinline__ float bf16_lo(uint32_t packed) { return __uint_as_float(packed << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t packed) { return __uint_as_float(packed & 0xFFFF0000u); }
+
+__device__ __forceinline__ f32x2 unpack_bf16x2(uint32_t w) { return pack2(bf16_lo(w), bf16_hi(w)); }
+// two words of two BF16 values each -> four E4M3 codes of value * recip
+__device__ __forceinline__ uint32_t cvt_e4m3x4_bf16(uint32_t w0, uint32_t w1, f32x2 recip) {
+  const f32x2 a = mul2(unpack_bf16x2(w0), recip), b = mul2(unpack_bf16x2(w1), recip);
+  return cvt_e4m3x2(lo(a), hi(a)) | (cvt_e4m3x2(lo(b), hi(b)) << 16);
+}
 
 // physical byte of (row, block) inside the 128-row scale tiles:
 // tiles [row/128][block/4] of 512 bytes, byte (row%32)*16 + ((row/32)%4)*4 + block%4

@@ -188,7 +188,7 @@ __device__ __forceinline__ void act_add_bias(const GemmParams& p, float (&v)[32]
 __device__ __forceinline__ void act_apply(int act, float (&v)[32]) {
   with_activation(act, [&](auto tag) {
 #pragma unroll
-    for (int e = 0; e < 32; ++e) v[e] = act_value<decltype(tag)::value>(v[e]);
+    for (int e = 0; e < 32; e += 2) act_value2<decltype(tag)::value>(v[e], v[e + 1]);
   });
 }
 // 32 columns of one residual row, packed two per word; loaded ahead of the activation so that the latency is covered

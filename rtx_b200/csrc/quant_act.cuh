@@ -85,7 +85,7 @@ __global__ void __launch_bounds__(kQuantThreads, kActOccupancy) quant_mxfp8_act_
         unpack8(*reinterpret_cast<const uint4*>(&raw_z[r0 + 16 * j][c8]), z);
         with_activation(p.act, [&](auto tag) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] *= act_slope<decltype(tag)::value>(z[e]);
+          for (int e = 0; e < 8; e += 2) act_slope2<decltype(tag)::value>(v[e], v[e + 1], z[e], z[e + 1]);
         });
       }
       uint32_t w[4];

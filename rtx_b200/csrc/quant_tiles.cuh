@@ -115,17 +115,17 @@ __device__ __forceinline__ void quant_mxfp8_rows_tile(const QuantMxParams& p, in
       const int r = rsel + 16 * (half * 4 + j);
       const int row = row0 + r;
       const bool live = row < p.rows && col_ok;
-      float v[8];
-      unpack8(raw[j], v);
-      float a = amax8(v);
-      a = fmax_nan(a, __shfl_xor_sync(0xffffffffu, a, 1));
-      a = fmax_nan(a, __shfl_xor_sync(0xffffffffu, a, 2));
-      const uint32_t code = e8m0_from_amax(a, rinf);
-      const float recip = e8m0_reciprocal(code);
+      // |max| of the block on packed pairs; 4 lanes hold its 32 values
+      uint32_t m2 = absmax_bf16x2(absmax_bf16x2(0u, raw[j].x), raw[j].y);
+      m2 = absmax_bf16x2(absmax_bf16x2(m2, raw[j].z), raw[j].w);
+      m2 = absmax_bf16x2(m2, __shfl_xor_sync(0xffffffffu, m2, 1));
+      m2 = absmax_bf16x2(m2, __shfl_xor_sync(0xffffffffu, m2, 2));
+      const uint32_t code = e8m0_from_amax(fmax_nan(bf16_lo(m2), bf16_hi(m2)), rinf);
+      const f32x2 recip = both(e8m0_reciprocal(code));
       if ((sub & 3) == 0) tile_scales[r][sub >> 2] = live ? static_cast<uint8_t>(code) : 0;
       if (live) {
-        const uint32_t lo = cvt_e4m3x2(v[0] * recip, v[1] * recip) | (cvt_e4m3x2(v[2] * recip, v[3] * recip) << 16);
-        const uint32_t hi = cvt_e4m3x2(v[4] * recip, v[5] * recip) | (cvt_e4m3x2(v[6] * recip, v[7] * recip) << 16);
+        const uint32_t lo = cvt_e4m3x4_bf16(raw[j].x, raw[j].y, recip);
+        const uint32_t hi = cvt_e4m3x4_bf16(raw[j].z, raw[j].w, recip);
         uint8_t* dst = p.q + static_cast<int64_t>(row) * p.kp + col;
         if (q_vec_ok) {
           *reinterpret_cast<uint2*>(dst) = make_uint2(lo, hi);
@@ -184,22 +184,21 @@ __device__ __forceinline__ void quant_mxfp8_tile_columns(const uint16_t (*tile)[
 #pragma unroll
   for (int e = 0; e < 32; ++e) w[e] = *reinterpret_cast<const uint32_t*>(&tile[j * 32 + e][2 * rp]);
   const int kcol = k0 + j * 32;
+  uint32_t m2 = 0;   // |max| of both rows at once
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    float a = 0.0f;
+  for (int e = 0; e < 32; ++e) m2 = absmax_bf16x2(m2, w[e]);
+  const uint32_t code0 = e8m0_from_amax(bf16_lo(m2), round_to_infinity), code1 = e8m0_from_amax(bf16_hi(m2), round_to_infinity);
+  const f32x2 recip = pack2(e8m0_reciprocal(code0), e8m0_reciprocal(code1));
+  const int row = row0 + 2 * rp;
+  tile_scales[2 * rp][j] = row < rows && kcol < kp ? static_cast<uint8_t>(code0) : 0;
+  tile_scales[2 * rp + 1][j] = row + 1 < rows && kcol < kp ? static_cast<uint8_t>(code1) : 0;
 #pragma unroll
-    for (int e = 0; e < 32; ++e) a = fmax_nan(a, fabsf(h ? bf16_hi(w[e]) : bf16_lo(w[e])));
-    const uint32_t code = e8m0_from_amax(a, round_to_infinity);
-    const float recip = e8m0_reciprocal(code);
-    const int r = 2 * rp + h, row = row0 + r;
-    const bool live = row < rows && kcol < kp;
-    tile_scales[r][j] = live ? static_cast<uint8_t>(code) : 0;
+  for (int e = 0; e < 8; ++e) {
+    f32x2 v[4];   // four values of k, both rows
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float v0 = h ? bf16_hi(w[4 * e]) : bf16_lo(w[4 * e]), v1 = h ? bf16_hi(w[4 * e + 1]) : bf16_lo(w[4 * e + 1]);
-      const float v2 = h ? bf16_hi(w[4 * e + 2]) : bf16_lo(w[4 * e + 2]), v3 = h ? bf16_hi(w[4 * e + 3]) : bf16_lo(w[4 * e + 3]);
-      o[h][e] = cvt_e4m3x2(v0 * recip, v1 * recip) | (cvt_e4m3x2(v2 * recip, v3 * recip) << 16);
-    }
+    for (int i = 0; i < 4; ++i) v[i] = mul2(unpack_bf16x2(w[4 * e + i]), recip);
+    o[0][e] = cvt_e4m3x2(lo(v[0]), lo(v[1])) | (cvt_e4m3x2(lo(v[2]), lo(v[3])) << 16);
+    o[1][e] = cvt_e4m3x2(hi(v[0]), hi(v[1])) | (cvt_e4m3x2(hi(v[2]), hi(v[3])) << 16);
   }
 }
 
@@ -243,21 +242,19 @@ __device__ __forceinline__ void quant_mxfp8_tile_rows(const uint16_t (*tile)[kQt
       const uint4 v = *reinterpret_cast<const uint4*>(&tile[r][part * 16 + 8 * c]);
       w[4 * c] = v.x; w[4 * c + 1] = v.y; w[4 * c + 2] = v.z; w[4 * c + 3] = v.w;
     }
-    float a = 0.0f;
+    uint32_t m2 = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) a = fmax_nan(a, fmax_nan(fabsf(bf16_lo(w[e])), fabsf(bf16_hi(w[e]))));
-    a = fmax_nan(a, __shfl_xor_sync(0xffffffffu, a, 1));
-    const uint32_t code = e8m0_from_amax(a, round_to_infinity);
-    const float recip = e8m0_reciprocal(code);
+    for (int e = 0; e < 8; ++e) m2 = absmax_bf16x2(m2, w[e]);
+    m2 = absmax_bf16x2(m2, __shfl_xor_sync(0xffffffffu, m2, 1));
+    const uint32_t code = e8m0_from_amax(fmax_nan(bf16_lo(m2), bf16_hi(m2)), round_to_infinity);
+    const f32x2 recip = both(e8m0_reciprocal(code));
     const int row = k0 + r, col = col0 + part * 16;
     const bool live = row < k_rows && col < np;
     if ((part & 1) == 0) tile_scales[r][part >> 1] = live ? static_cast<uint8_t>(code) : 0;
     if (live) {
       uint32_t o[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        o[e] = cvt_e4m3x2(bf16_lo(w[2 * e]) * recip, bf16_hi(w[2 * e]) * recip) |
-               (cvt_e4m3x2(bf16_lo(w[2 * e + 1]) * recip, bf16_hi(w[2 * e + 1]) * recip) << 16);
+      for (int e = 0; e < 4; ++e) o[e] = cvt_e4m3x4_bf16(w[2 * e], w[2 * e + 1], recip);
       *reinterpret_cast<uint4*>(q + static_cast<int64_t>(row) * np + col) = make_uint4(o[0], o[1], o[2], o[3]);
     }
   }
