@@ -1006,9 +1006,10 @@ int rtxb_mxfp8_linear_epilogue_bwd(const void* dy, int64_t lddy, const void* z, 
   q.s_t = mem.s_dzt;
   q.partial = mem.partial;
   const int64_t row_tiles = (m + 127) / 128, tiles = row_tiles * ((n + 127) / 128);
-  cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(quant_mxfp8_act_backward_kernel), kActSmemBytes);
+  auto kernel = activation >= RTXB_ACT_SILU ? quant_mxfp8_act_backward_kernel<true> : quant_mxfp8_act_backward_kernel<false>;
+  cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), kActSmemBytes);
   if (e != cudaSuccess) return fail_cuda(e, "cudaFuncSetAttribute(activation backward quantizer)");
-  quant_mxfp8_act_backward_kernel<<<quant_grid(tiles, kActOccupancy), kQuantThreads, kActSmemBytes, s>>>(q);
+  kernel<<<quant_grid(tiles, kActOccupancy), kQuantThreads, kActSmemBytes, s>>>(q);
   RTXB_CHECK_LAUNCH("quant_mxfp8_act_backward_kernel");
   if (dbias) {
     bias_grad_kernel<<<static_cast<int>((n + 31) / 32), 256, 0, s>>>(mem.partial, static_cast<int>(row_tiles),

@@ -4,8 +4,8 @@
 //   q_t     MXFP8 of dz^T, blocks along m    (A operand of dW = dz^T X)
 //   partial[m / 128][n] = sum of 128 rows of dz in FP32, before the rounding   (dbias, finished by the kernel below)
 // dy and z are read once (4 bytes per value), 2 bytes of payload leave: without the fusion dz is written and read again
-// (4 more).  HBM bound; one 128 x 128 tile per block step, the next one
-// is fetched asynchronously while this one is quantized.
+// (4 more).  One 128 x 128 tile per block step, three blocks per SM
+// overlap one another's loads, arithmetic and stores.
 #pragma once
 
 #include "activation.cuh"
@@ -25,88 +25,130 @@ struct QuantActParams {
   float* partial;            // [ceil(m / 128)][n] or nullptr
 };
 
-constexpr int kActOccupancy = 2;                  // resident blocks per SM (three staged tiles each)
+constexpr int kActOccupancy = 3;                  // resident blocks per SM (registers)
 constexpr int kActSumRows = kQuantThreads / 32;   // partial column sums per tile before the last step, one per warp
-constexpr int kActSmemBytes = 3 * kQtTileBytes;   // raw dy, raw z, dz
 
-// Raw tile of dy or z into `raw`: thread t copies the 8 columns (t & 15) of the rows (t >> 4) + 16 j, the ones it will
-// read back itself, so no barrier stands between the copy and its use.
-__device__ __forceinline__ void act_fetch(const __nv_bfloat16* src, int64_t ld, bool vec_ok, int m, int n, int row0, int col0,
-                                          uint16_t (*raw)[kQtPitch]) {
-  const int c8 = (threadIdx.x & 15) * 8, r0 = threadIdx.x >> 4;
-  const int col = col0 + c8;
+// z has eight significant bits, so between 2^-21 and 32 it takes 26 x 128 magnitudes: the slopes of silu and the gelus
+// are looked up.  Each of them is 1/2 plus an odd function (f(z) - f(-z) = z), so the table holds act'(|z|) - 1/2 and the
+// sign of z is put on it.  Below 2^-21 the slope is within 4e-7 of 1/2, from 32 on it is 1.  That is a third of the
+// instructions of an evaluation, and instructions are what bounds the pass.
+constexpr int kSlopeLow = 106 << 7, kSlopeHigh = 132 << 7;     // BF16 magnitudes of 2^-21 and 32
+constexpr int kSlopeEntries = kSlopeHigh - kSlopeLow + 1;
+constexpr int kActSmemBytes = kQtTileBytes + (kSlopeEntries * 4 + 15) / 16 * 16;
+
+// Eight gradients dy act'(z) as four pairs.  LOOKUP: from the table; else relu, relu2 or none by `act`.
+template <bool LOOKUP>
+__device__ __forceinline__ void act_gradient8(const float* table, int act, const uint4 dy, const uint4 z, f32x2 (&v)[4]) {
+  const uint32_t g[4] = {dy.x, dy.y, dy.z, dy.w}, w[4] = {z.x, z.y, z.z, z.w};
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const int row = row0 + r0 + 16 * j;
-    const bool live = row < m && col < n;
-    if (vec_ok && (!live || col + 8 <= n)) {
-      cp_async_16(&raw[r0 + 16 * j][c8], src + (live ? row * ld + col : 0), live);
-    } else {
-      *reinterpret_cast<uint4*>(&raw[r0 + 16 * j][c8]) = live ? load8_raw(src + row * ld, col, n, false) : make_uint4(0, 0, 0, 0);
+  for (int e = 0; e < 4; ++e) v[e] = unpack_bf16x2(g[e]);
+  if (LOOKUP) {
+    uint32_t m2 = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t mag = __vminu2(__vmaxu2(w[e] & 0x7FFF7FFFu, kSlopeLow * 0x10001u), kSlopeHigh * 0x10001u);
+      const uint32_t u0 = __float_as_uint(table[mag & 0xFFFFu]) ^ ((w[e] << 16) & 0x80000000u);
+      const uint32_t u1 = __float_as_uint(table[mag >> 16]) ^ (w[e] & 0x80000000u);
+      v[e] = mul2(v[e], add2(pack2(__uint_as_float(u0), __uint_as_float(u1)), both(0.5f)));
+      m2 = absmax_bf16x2(m2, w[e]);
+    }
+    if (bf16_lo(m2) != bf16_lo(m2) || bf16_hi(m2) != bf16_hi(m2)) {   // a NaN among them: it goes on to dz
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float z0 = bf16_lo(w[e]), z1 = bf16_hi(w[e]);
+        v[e] = pack2(z0 != z0 ? z0 : lo(v[e]), z1 != z1 ? z1 : hi(v[e]));
+      }
+    }
+  } else if (act != kActNone) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float a = lo(v[e]), b = hi(v[e]);
+      if (act == kActRelu) act_slope2<kActRelu>(a, b, bf16_lo(w[e]), bf16_hi(w[e]));
+      else act_slope2<kActRelu2>(a, b, bf16_lo(w[e]), bf16_hi(w[e]));
+      v[e] = pack2(a, b);
     }
   }
 }
 
+template <bool LOOKUP>
 __global__ void __launch_bounds__(kQuantThreads, kActOccupancy) quant_mxfp8_act_backward_kernel(const QuantActParams p) {
   extern __shared__ __align__(16) uint8_t qt_smem[];
-  uint16_t (*raw_g)[kQtPitch] = reinterpret_cast<uint16_t (*)[kQtPitch]>(qt_smem);
-  uint16_t (*raw_z)[kQtPitch] = reinterpret_cast<uint16_t (*)[kQtPitch]>(qt_smem + kQtTileBytes);
-  uint8_t* stage = qt_smem + 2 * kQtTileBytes;
-  uint16_t (*tile)[kQtPitch] = reinterpret_cast<uint16_t (*)[kQtPitch]>(stage);
+  uint16_t (*tile)[kQtPitch] = reinterpret_cast<uint16_t (*)[kQtPitch]>(qt_smem);
+  float* slopes = reinterpret_cast<float*>(qt_smem + kQtTileBytes) - kSlopeLow;   // indexed by magnitude
   __shared__ __align__(16) uint8_t scales_t[128][4];
   __shared__ __align__(16) uint8_t scales_rows[128][4];
   __shared__ float sums[kActSumRows][128];
+  if (LOOKUP) {
+    with_activation(p.act, [&](auto tag) {
+      for (int i = kSlopeLow + threadIdx.x; i <= kSlopeHigh; i += kQuantThreads) {
+        const float z = __uint_as_float(static_cast<uint32_t>(i) << 16);
+        float a = 1.0f, b = 0.0f;
+        act_slope2<decltype(tag)::value>(a, b, z, 0.0f);
+        slopes[i] = a - 0.5f;
+      }
+    });
+    __syncthreads();
+  }
   const int col_tiles = (p.n + 127) / 128, row_tiles = (p.m + 127) / 128;
   const int np = (p.n + 31) / 32 * 32, mp = (p.m + 31) / 32 * 32;
   const bool vec_dy = (p.lddy % 8 == 0) && ((reinterpret_cast<uintptr_t>(p.dy) & 15) == 0);
-  const bool vec_z = (p.n % 8 == 0) && ((reinterpret_cast<uintptr_t>(p.z) & 15) == 0);
+  const bool vec_z = (p.n % 8 == 0) && ((reinterpret_cast<uintptr_t>(p.z) & 15) == 0);   // true without z
   const int c8 = (threadIdx.x & 15) * 8, r0 = threadIdx.x >> 4;
   const int64_t total = static_cast<int64_t>(row_tiles) * col_tiles;
-  auto fetch = [&](int64_t t) {
-    const int rt = static_cast<int>(t / col_tiles), ct = static_cast<int>(t - static_cast<int64_t>(rt) * col_tiles);
-    act_fetch(p.dy, p.lddy, vec_dy, p.m, p.n, rt * 128, ct * 128, raw_g);
-    if (p.z) act_fetch(p.z, p.n, vec_z, p.m, p.n, rt * 128, ct * 128, raw_z);
-    cp_async_commit();
-  };
-  if (blockIdx.x < total) fetch(blockIdx.x);
   for (int64_t t = blockIdx.x; t < total; t += gridDim.x) {
     const int rt = static_cast<int>(t / col_tiles);
     const int row0 = rt * 128, col0 = static_cast<int>(t - static_cast<int64_t>(rt) * col_tiles) * 128;
-    cp_async_wait<0>();
-    float sum[8];
+    const int col = col0 + c8;
+    f32x2 sum[4];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) sum[e] = 0.0f;
-#pragma unroll 4
-    for (int j = 0; j < 8; ++j) {
-      float v[8];
-      unpack8(*reinterpret_cast<const uint4*>(&raw_g[r0 + 16 * j][c8]), v);
-      if (p.z) {
-        float z[8];
-        unpack8(*reinterpret_cast<const uint4*>(&raw_z[r0 + 16 * j][c8]), z);
-        with_activation(p.act, [&](auto tag) {
+    for (int e = 0; e < 4; ++e) sum[e] = both(0.0f);
+    const bool whole = vec_dy && vec_z && row0 + 128 <= p.m && col0 + 128 <= p.n;
+    const __nv_bfloat16* gp = p.dy + static_cast<int64_t>(row0 + r0) * p.lddy + col;
+    const __nv_bfloat16* zp = p.z + static_cast<int64_t>(row0 + r0) * p.n + col;
+#pragma unroll 1
+    for (int half = 0; half < 2; ++half) {
+      uint4 g[4], z[4];
+      if (whole) {
 #pragma unroll
-          for (int e = 0; e < 8; e += 2) act_slope2<decltype(tag)::value>(v[e], v[e + 1], z[e], z[e + 1]);
-        });
+        for (int j = 0; j < 4; ++j) {
+          g[j] = __ldg(reinterpret_cast<const uint4*>(gp));
+          z[j] = p.z ? __ldg(reinterpret_cast<const uint4*>(zp)) : make_uint4(0, 0, 0, 0);
+          gp += 16 * p.lddy;
+          zp += 16 * static_cast<int64_t>(p.n);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int64_t row = row0 + r0 + 16 * (half * 4 + j);
+          const bool live = row < p.m && col < p.n;
+          g[j] = live ? load8_raw(p.dy + row * p.lddy, col, p.n, vec_dy) : make_uint4(0, 0, 0, 0);
+          z[j] = live && p.z ? load8_raw(p.z + row * p.n, col, p.n, vec_z) : make_uint4(0, 0, 0, 0);
+        }
       }
-      uint32_t w[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        sum[2 * e] += v[2 * e];
-        sum[2 * e + 1] += v[2 * e + 1];
-        __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
-        w[e] = *reinterpret_cast<uint32_t*>(&b);
+      for (int j = 0; j < 4; ++j) {
+        f32x2 v[4];
+        act_gradient8<LOOKUP>(slopes, p.act, g[j], z[j], v);
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          sum[e] = add2(sum[e], v[e]);
+          __nv_bfloat162 b = __floats2bfloat162_rn(lo(v[e]), hi(v[e]));
+          w[e] = *reinterpret_cast<uint32_t*>(&b);
+        }
+        *reinterpret_cast<uint4*>(&tile[r0 + 16 * (half * 4 + j)][c8]) = make_uint4(w[0], w[1], w[2], w[3]);
       }
-      *reinterpret_cast<uint4*>(&tile[r0 + 16 * j][c8]) = make_uint4(w[0], w[1], w[2], w[3]);
     }
-    // this thread's part of the raw tiles is read: the next tile's may come in while this one is quantized
-    if (t + gridDim.x < total) fetch(t + gridDim.x);
     if (p.partial) {
       // the two row halves of a warp, then one row of sums per warp
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], 16);
-      if ((threadIdx.x & 16) == 0) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) sums[threadIdx.x >> 5][c8 + e] = sum[e];
+      for (int e = 0; e < 4; ++e) {
+        const float a = lo(sum[e]), b = hi(sum[e]);
+        const float sa = a + __shfl_xor_sync(0xffffffffu, a, 16), sb = b + __shfl_xor_sync(0xffffffffu, b, 16);
+        if ((threadIdx.x & 16) == 0) {
+          sums[threadIdx.x >> 5][c8 + 2 * e] = sa;
+          sums[threadIdx.x >> 5][c8 + 2 * e + 1] = sb;
+        }
       }
     }
     __syncthreads();
@@ -121,7 +163,7 @@ __global__ void __launch_bounds__(kQuantThreads, kActOccupancy) quant_mxfp8_act_
     }
     __syncthreads();   // every thread has read the staged tile: its storage now collects the transposed payload
     if (p.q_t) {
-      quant_mxfp8_tile_columns_store(stage, o, p.q_t, mp, p.n, col0, row0);
+      quant_mxfp8_tile_columns_store(qt_smem, o, p.q_t, mp, p.n, col0, row0);
       store_scale_tile<4>(scales_t, p.s_t, kScaleMma128, col0, row0 / 32, p.n, mp / 32, (mp / 32 + 3) / 4);
     }
     if (p.q_rows)
