@@ -9,6 +9,7 @@
 #include "quant.cuh"
 #include "gemm_decode_fused.cuh"
 #include "gemm_fused_quant.cuh"
+#include "grouped_params.cuh"
 #include "quant_act.cuh"
 #include "reduce.cuh"
 #include "peer.cuh"
@@ -901,31 +902,22 @@ static int linear_epilogue(const void* x, int64_t ldx, const void* w, const void
   if (!aligned(workspace, 256)) return fail_msg(RTXB_E_ALIGNMENT, "workspace must be 256-byte aligned");
   Carver c(workspace);
   const int64_t kp = round_up(k, 32), chunks = (kp / 32 + 3) / 4;
-  QuantMxParams p[2] = {};
-  for (int i = 0; i < 2; ++i) {
-    p[i].src = static_cast<const __nv_bfloat16*>(i ? w : x);
-    p[i].rows = static_cast<int>(i ? (w ? n : 0) : m);   // packed weights: no tiles of the second operand
-    p[i].k = static_cast<int>(k);
-    p[i].kp = static_cast<int>(kp);
-    p[i].ld = i ? k : ldx;
-    p[i].nb = static_cast<int>(kp / 32);
-    p[i].sf_chunks = static_cast<int>(chunks);
-    p[i].layout = RTXB_SCALE_MMA128;
-    p[i].round_to_infinity = rounding != RTXB_ROUND_FLOOR;
-    if (i == 0 || w) {
-      p[i].q = c.take(p[i].rows * kp);
-      p[i].scales = c.take(rtxb_mxfp8_scale_bytes(p[i].rows, k, RTXB_SCALE_MMA128));
-    }
+  RowsParams p = {};
+  p.x = RowsOperand{static_cast<const __nv_bfloat16*>(x), ldx, c.take(m * kp),
+                    c.take(rtxb_mxfp8_scale_bytes(m, k, RTXB_SCALE_MMA128)), static_cast<int>(m)};
+  if (w) {
+    p.w = RowsOperand{static_cast<const __nv_bfloat16*>(w), k, c.take(n * kp),
+                      c.take(rtxb_mxfp8_scale_bytes(n, k, RTXB_SCALE_MMA128)), static_cast<int>(n)};
+    p.batches = 1;
+    qw = p.w.q;
+    sw = p.w.scales;
   }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const int64_t tiles = (round_up(m, 128) + (w ? round_up(n, 128) : 0)) / 128 * ((kp + 127) / 128);
-  quant_mxfp8_rows2_kernel<<<quant_grid(tiles, 6), kQuantThreads, 0, s>>>(p[0], p[1]);
-  RTXB_CHECK_LAUNCH("quant_mxfp8_rows2_kernel");
+  if ((rc = launch_quantize_rows(p, (m + 127) / 128, k, rounding, s))) return rc;
   const ActEpilogue e{bias, residual, ldr, z, act};
   // packed weights do not come from the quantizer just launched: on small layers the GEMM streams them beside it
-  return launch_gemm<kKindMxfp8, kEpiAct>(p[0].q, p[0].scales, w ? p[1].q : qw, w ? p[1].scales : sw, out, m, n, kp, chunks, n,
-                                          n, 0, nullptr, s, status, nullptr, nullptr, w == nullptr, nullptr, nullptr,
-                                          w != nullptr, &e);
+  return launch_gemm<kKindMxfp8, kEpiAct>(p.x.q, p.x.scales, qw, sw, out, m, n, kp, chunks, n, n, 0, nullptr, s, status,
+                                          nullptr, nullptr, w == nullptr, nullptr, nullptr, w != nullptr, &e);
 }
 
 int rtxb_mxfp8_linear_epilogue_fwd(const void* x, int64_t ldx, const void* w, const void* bias, const void* residual,

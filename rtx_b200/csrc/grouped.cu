@@ -5,6 +5,24 @@
 
 using namespace rtxb;
 
+namespace rtxb {
+
+int launch_quantize_rows(RowsParams& p, int64_t x_tiles, int64_t k, int rounding, cudaStream_t stream) {
+  p.k = static_cast<int>(k);
+  p.kp = static_cast<int>(round_up(k, 32));
+  p.chunks = static_cast<int>((p.kp / 32 + 3) / 4);
+  p.lanes = 4;
+  while (p.lanes < 32 && p.lanes < p.kp / 32) p.lanes *= 2;
+  p.round_to_infinity = rounding != RTXB_ROUND_FLOOR;
+  const int64_t w_tiles = p.w.src ? static_cast<int64_t>(p.batches) * ((p.w.rows + 127) / 128) : 0;
+  const int64_t units = (x_tiles + w_tiles) * p.lanes * ((4 * p.chunks + p.lanes - 1) / p.lanes);
+  quant_mxfp8_rows_units_kernel<<<quant_grid((units + 7) / 8, kRowsOccupancy), kQuantThreads, 0, stream>>>(p);
+  RTXB_CHECK_LAUNCH("quant_mxfp8_rows_units_kernel");
+  return RTXB_OK;
+}
+
+}  // namespace rtxb
+
 namespace {
 
 // output [groups][rows][cols] of BF16, row pitch ldo and group pitch `group_elems` elements; boxes of 32 rows x 32
@@ -126,22 +144,6 @@ struct BwdMemory {
   }
 };
 
-QuantMxParams rows_params(const void* src, int64_t rows, int64_t k, int64_t ld, void* q, void* s, int rounding) {
-  QuantMxParams p = {};
-  p.src = static_cast<const __nv_bfloat16*>(src);
-  p.q = static_cast<uint8_t*>(q);
-  p.scales = static_cast<uint8_t*>(s);
-  p.rows = static_cast<int>(rows);
-  p.k = static_cast<int>(k);
-  p.kp = static_cast<int>(round_up(k, 32));
-  p.ld = ld;
-  p.nb = p.kp / 32;
-  p.sf_chunks = (p.nb + 3) / 4;
-  p.layout = RTXB_SCALE_MMA128;
-  p.round_to_infinity = rounding != RTXB_ROUND_FLOOR;
-  return p;
-}
-
 GroupedGemmParams gemm_params(const GroupPlan& plan, void* out, int64_t ldo, int64_t out_cols, int* status) {
   GroupedGemmParams g = {};
   g.plan_rows = plan.row_tiles;
@@ -185,15 +187,12 @@ int grouped_fwd(const void* x, int64_t ldx, const void* w, const void* qw, const
   if (!workspace || workspace_bytes < c.off) return fail_msg(RTXB_E_WORKSPACE, "workspace too small for the grouped forward");
   if (!aligned(workspace, 256)) return fail_msg(RTXB_E_ALIGNMENT, "workspace must be 256-byte aligned");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  GroupedRowsParams q = {};
-  q.x = rows_params(x, rows, k, ldx, mem.qx, mem.sx, rounding);
+  RowsParams q = {};
+  q.x = RowsOperand{static_cast<const __nv_bfloat16*>(x), ldx, mem.qx, mem.sx, static_cast<int>(rows)};
   q.list = GroupList{offsets, static_cast<int>(groups), static_cast<int>(rows)};
-  const int64_t col_tiles = (q.x.kp + 127) / 128;
-  int64_t tiles = most_tiles(rows, groups, 128) * col_tiles;
   if (w) {
-    q.w = rows_params(w, n, k, k, mem.qw, mem.sw, rounding);
+    q.w = RowsOperand{static_cast<const __nv_bfloat16*>(w), k, mem.qw, mem.sw, static_cast<int>(n)};
     q.batches = static_cast<int>(groups);
-    tiles += groups * ((n + 127) / 128) * col_tiles;
     qw = mem.qw;
     sw = mem.sw;
   }
@@ -202,8 +201,7 @@ int grouped_fwd(const void* x, int64_t ldx, const void* w, const void* qw, const
   q.out_cols = static_cast<int>(n);
   q.ldo = ldo;
   q.status = status;
-  quant_mxfp8_grouped_rows_kernel<<<quant_grid(tiles, 6), kQuantThreads, 0, s>>>(q);
-  RTXB_CHECK_LAUNCH("quant_mxfp8_grouped_rows_kernel");
+  if ((rc = launch_quantize_rows(q, most_tiles(rows, groups, 128), k, rounding, s))) return rc;
   return launch_rows_form(mem.plan.plan, mem.qx, mem.sx, rows, qw, sw, n, k, groups, out, ldo, status, s);
 }
 

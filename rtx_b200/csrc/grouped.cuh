@@ -11,29 +11,17 @@
 // Rows of no group are never read; the kernels here set them to zero in the result.
 #pragma once
 
+#include "grouped_params.cuh"
 #include "quant_tiles.cuh"
 
 namespace rtxb {
 
 constexpr int kMaxGroups = 512;   // the list is scanned in shared memory beside the staged tiles (4 KB at 512)
 
-struct GroupList {
-  const int* offsets;   // [groups + 1]
-  int groups;
-  int rows;             // rows of the operand; offsets are held inside [0, rows] and non-decreasing
-};
-
 struct GroupScan {
   int start[kMaxGroups + 1];   // first row of the group; [groups] = end of the last one
   int tile[kMaxGroups + 1];    // 128-row tiles of the groups before it
   int warp_part[8];
-};
-
-// What the quantizer leaves for the GEMM behind it (global memory, written by block 0).
-struct GroupPlan {
-  int* row_tiles;    // [0] = number of 256-row tiles over all groups
-  int4* tiles;       // per 256-row tile: {first row, live rows, first scale tile, group}
-  int* k_tiles;      // [groups + 1] = GroupScan::tile
 };
 
 __device__ __forceinline__ int block_scan_max(int v, int* part) {
@@ -166,56 +154,142 @@ __device__ __forceinline__ void zero_rows_of_no_group(const GroupList& l, const 
 }
 
 // ---------------------------------------------------------------------------
-// Forward operands in one launch: the rows of x by group, then (dynamic weights) the `batches` weight matrices
-// [w.rows, k], each with scale tiles of its own.
+// Row quantizer of the grouped forward and of the linear with an epilogue, both operands in one launch: the rows of x
+// (by group), then the `batches` weight matrices [w.rows, k], each with scale tiles of its own.
+//
+// One lane owns one block of 32 values (two 32-byte loads, one 32-byte store), so a block's maximum needs no exchange
+// between lanes and its scale is computed once: 5 instructions a value, where eight values per lane (quant_mxfp8_rows_tile)
+// take 17, and those bound that form (70 % issue at 4.2 TB/s).  A warp takes 32 blocks of the four rows r, r + 32, r + 64,
+// r + 96 of a 128-row tile: their scale bytes are whole 16-byte segments of the scale tiles, put together by four
+// shuffles; no shared memory, no barrier.  Narrow rows (fewer than 32 blocks) share a warp.
+// Rows of a tile behind the operand's last row: payload and scales stay unwritten; they reach only accumulator entries
+// that are never stored.
 // ---------------------------------------------------------------------------
-struct GroupedRowsParams {
-  QuantMxParams x;            // scales: 128-row tiles counted per group
-  GroupList list;
-  QuantMxParams w;            // one matrix; src nullptr = packed weights, nothing to do
-  int batches;
-  GroupPlan plan;
-  __nv_bfloat16* out;         // result whose rows of no group become zero
-  int out_cols;
-  int64_t ldo;
-  int* status;
-};
+constexpr int kRowsOccupancy = 4;
 
-__global__ void __launch_bounds__(kQuantThreads, 6) quant_mxfp8_grouped_rows_kernel(const GroupedRowsParams p) {
-  __shared__ GroupScan scan;
-  __shared__ __align__(16) uint8_t tile_scales[128][4];
-  griddep_launch_dependents();
-  scan_groups(p.list, scan, p.status);
-  if (blockIdx.x == 0) {
-    __shared__ int wide[kMaxGroups + 1];
-    write_group_plan(p.list, scan, p.plan, wide);
-  }
-  zero_rows_of_no_group(p.list, scan, p.out, p.out_cols, p.ldo);
-  const int col_tiles = (p.x.kp + 127) / 128;
-  const int x_tiles = scan.tile[p.list.groups] * col_tiles;
-  const int w_row_tiles = (p.w.rows + 127) / 128;
-  const int w_tiles = p.w.src ? w_row_tiles * col_tiles : 0;   // per matrix
-  const int64_t total = x_tiles + static_cast<int64_t>(p.batches) * w_tiles;
-  for (int64_t t = blockIdx.x; t < total; t += gridDim.x) {
-    if (t < x_tiles) {
-      const int rt = static_cast<int>(t) / col_tiles, ct = static_cast<int>(t) - rt * col_tiles;
-      const int g = group_before(scan.tile, p.list.groups, rt);
-      const int64_t row0 = scan.start[g] + 128 * (rt - scan.tile[g]);
-      QuantMxParams q = p.x;
-      q.src += row0 * q.ld;
-      q.q += row0 * q.kp;
-      q.scales += static_cast<size_t>(rt) * q.sf_chunks * 512;
-      q.rows = min(128, scan.start[g + 1] - static_cast<int>(row0));
-      quant_mxfp8_rows_tile(q, ct, tile_scales);
-    } else {
-      const int64_t u = t - x_tiles;
-      const int64_t e = u / w_tiles;
-      QuantMxParams q = p.w;
-      q.src += e * q.rows * q.ld;
-      q.q += e * q.rows * q.kp;
-      q.scales += static_cast<size_t>(e) * w_row_tiles * q.sf_chunks * 512;
-      quant_mxfp8_rows_tile(q, static_cast<int>(u - e * w_tiles), tile_scales);
+// 32 values of a row (zero from `valid` on).  align: 2 = 32-byte, 1 = 16-byte aligned rows, 0 = neither
+__device__ __forceinline__ void load_block32(const __nv_bfloat16* src, int valid, int align, uint32_t (&w)[16]) {
+  if (valid >= 32 && align == 2) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      asm("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+          : "=r"(w[8 * h]), "=r"(w[8 * h + 1]), "=r"(w[8 * h + 2]), "=r"(w[8 * h + 3]), "=r"(w[8 * h + 4]),
+            "=r"(w[8 * h + 5]), "=r"(w[8 * h + 6]), "=r"(w[8 * h + 7])
+          : "l"(src + 16 * h));
+  } else if (valid >= 32 && align == 1) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint4 v = __ldg(reinterpret_cast<const uint4*>(src) + j);
+      w[4 * j] = v.x; w[4 * j + 1] = v.y; w[4 * j + 2] = v.z; w[4 * j + 3] = v.w;
     }
+  } else {
+    const uint16_t* bits = reinterpret_cast<const uint16_t*>(src);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const uint32_t a = 2 * e < valid ? bits[2 * e] : 0u, b = 2 * e + 1 < valid ? bits[2 * e + 1] : 0u;
+      w[e] = a | (b << 16);
+    }
+  }
+}
+
+// one unit of a warp: rows r, r + 32, r + 64, r + 96 (r = this lane's) of a 128-row tile with `rows` live rows, block b
+__device__ __forceinline__ void quant_mxfp8_rows_unit(const RowsOperand& o, const RowsParams& p, const __nv_bfloat16* src,
+                                                      uint8_t* q, uint8_t* scales, int rows, int r, int b, int align) {
+  const int lane = threadIdx.x & 31;
+  const int valid = p.k - 32 * b;            // values of this block inside the row; <= 0: padding of the scale tile
+  const bool in_row = 32 * b < p.kp;
+  uint32_t word = 0;                         // scale bytes of the four rows
+#pragma unroll
+  for (int pair = 0; pair < 2; ++pair) {
+    uint32_t w[2][16];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int row = r + 32 * (2 * pair + i);
+      if (row < rows && in_row) {
+        load_block32(src + row * o.ld + 32 * b, valid, align, w[i]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) w[i][e] = 0;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int row = r + 32 * (2 * pair + i);
+      uint32_t m2 = 0;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) m2 = absmax_bf16x2(m2, w[i][e]);
+      const uint32_t code = e8m0_from_amax(fmax_nan(bf16_lo(m2), bf16_hi(m2)), p.round_to_infinity != 0);
+      const f32x2 recip = both(e8m0_reciprocal(code));
+      if (row < rows && in_row) {
+        uint32_t c[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) c[e] = cvt_e4m3x4_bf16(w[i][2 * e], w[i][2 * e + 1], recip);
+        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(q + static_cast<int64_t>(row) * p.kp + 32 * b),
+                     "r"(c[0]), "r"(c[1]), "r"(c[2]), "r"(c[3]), "r"(c[4]), "r"(c[5]), "r"(c[6]), "r"(c[7])
+                     : "memory");
+        word |= code << (8 * (2 * pair + i));
+      }
+    }
+  }
+  // four lanes with the blocks of one scale tile: lane j collects the bytes of row group j
+  const int j = lane & 3;
+  uint32_t seg = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) seg |= ((__shfl_sync(0xffffffffu, word, (lane & ~3) | i) >> (8 * j)) & 0xFFu) << (8 * i);
+  if ((b >> 2) < p.chunks) *reinterpret_cast<uint32_t*>(scales + static_cast<size_t>(b >> 2) * 512 + r * 16 + j * 4) = seg;
+}
+
+__global__ void __launch_bounds__(kQuantThreads, kRowsOccupancy) quant_mxfp8_rows_units_kernel(const RowsParams p) {
+  __shared__ GroupScan scan;
+  griddep_launch_dependents();
+  const bool grouped = p.list.offsets != nullptr;
+  if (grouped) {
+    scan_groups(p.list, scan, p.status);
+    if (blockIdx.x == 0) {
+      __shared__ int wide[kMaxGroups + 1];
+      write_group_plan(p.list, scan, p.plan, wide);
+    }
+    zero_rows_of_no_group(p.list, scan, p.out, p.out_cols, p.ldo);
+  }
+  const int lane = threadIdx.x & 31;
+  const int segs = (4 * p.chunks + p.lanes - 1) / p.lanes;   // units side by side along a row
+  const int stacked = 32 / p.lanes;                          // row numbers r that share a warp
+  const int per_tile = p.lanes * segs;                       // units of one 128-row tile: 32 / stacked row numbers x segs
+  const int64_t x_units = static_cast<int64_t>(grouped ? scan.tile[p.list.groups] : (p.x.rows + 127) / 128) * per_tile;
+  const int w_row_tiles = (p.w.rows + 127) / 128;
+  const int64_t units = x_units + (p.w.src ? static_cast<int64_t>(p.batches) * w_row_tiles * per_tile : 0);
+  auto alignment = [](const RowsOperand& o) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(o.src) | static_cast<uintptr_t>(o.ld * 2);
+    return a % 32 == 0 ? 2 : a % 16 == 0 ? 1 : 0;
+  };
+  const int align_x = alignment(p.x), align_w = alignment(p.w);
+  const int warps = gridDim.x * (kQuantThreads / 32);
+  for (int64_t u = blockIdx.x * (kQuantThreads / 32) + (threadIdx.x >> 5); u < units; u += warps) {
+    const bool is_x = u < x_units;
+    const int64_t v = is_x ? u : u - x_units;
+    const int64_t rt = v / per_tile;                         // 128-row tile (of all matrices)
+    const int in_tile = static_cast<int>(v - rt * per_tile);
+    const int r = in_tile / segs * stacked + lane / p.lanes;
+    const int b = in_tile % segs * p.lanes + lane % p.lanes;
+    int64_t row0;
+    int rows;
+    if (!is_x) {
+      const int64_t e = rt / w_row_tiles;
+      const int first = static_cast<int>(rt - e * w_row_tiles) * 128;
+      row0 = e * p.w.rows + first;
+      rows = min(128, p.w.rows - first);
+    } else if (grouped) {
+      const int g = group_before(scan.tile, p.list.groups, static_cast<int>(rt));
+      row0 = scan.start[g] + 128 * (rt - scan.tile[g]);
+      rows = min(128, scan.start[g + 1] - static_cast<int>(row0));
+    } else {
+      row0 = 128 * rt;
+      rows = static_cast<int>(min(int64_t(128), p.x.rows - row0));
+    }
+    if (in_tile / segs * stacked >= rows) continue;          // warp-uniform: no live row
+    const RowsOperand& o = is_x ? p.x : p.w;
+    quant_mxfp8_rows_unit(o, p, o.src + row0 * o.ld, o.q + row0 * p.kp, o.scales + static_cast<size_t>(rt) * p.chunks * 512,
+                          rows, r, b, is_x ? align_x : align_w);
   }
 }
 
