@@ -124,6 +124,7 @@ gemm_grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
   const int pair_id = blockIdx.x >> 1;
   const int num_pairs = gridDim.x >> 1;
 
+  griddep_launch_dependents();   // the second product of a backward sets up beside this one's tail
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
       mbar_init(&full_bar[s], 1);

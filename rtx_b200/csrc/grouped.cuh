@@ -391,6 +391,7 @@ quant_mxfp8_grouped_backward_kernel(const GroupedBackwardParams p) {
   __shared__ GroupScan scan;
   __shared__ __align__(16) uint8_t tile_scales[128][4];
   __shared__ __align__(16) uint8_t tile_scales_rows[128][4];
+  griddep_launch_dependents();
   scan_groups(p.list, scan, p.status);
   if (blockIdx.x == 0) write_group_plan(p.list, scan, p.plan, reinterpret_cast<int*>(qt_smem));
   if (p.dx) zero_rows_of_no_group(p.list, scan, p.dx, p.k, p.lddx);

@@ -13,21 +13,13 @@ from typing import Optional, Tuple
 
 import torch
 from torch import nn
+from torch.autograd.function import once_differentiable
 
 from . import fp8 as _fp8
 from . import ops
 from ._oplib import custom_op
 from .formats import (PACKED_OPERAND_SCHEMA_VERSION, SCALE_LAYOUT_CODES, MXFP8Tensor, make_mxfp8_tensor,
-                      mxfp8_matrix_shape, mxfp8_qdata_2d, mxfp8_scales_for_kernel, reject_packed_dtype_conversion)
-from .grouped import _rows_contiguous
-
-
-def _rows(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
-    return t if t is None else _rows_contiguous(t)
-
-
-def _vector(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
-    return t if t is None else t.contiguous()
+                      mxfp8_kernel_operands, mxfp8_matrix_shape, mxfp8_qdata_2d, mxfp8_scales_for_kernel, reject_packed_dtype_conversion)
 
 
 def _check(x, n, k, bias, residual, activation) -> None:
@@ -48,8 +40,7 @@ def _check(x, n, k, bias, residual, activation) -> None:
 def mxfp8_linear_epilogue_op(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor],
                              residual: Optional[torch.Tensor], activation: str) -> torch.Tensor:
     _check(x, *weight.shape, bias, residual, activation)
-    return ops.mxfp8_linear_epilogue_fwd(_rows(x), weight.contiguous(), _vector(bias), _rows(residual),
-                                         activation=activation)[0]
+    return ops.mxfp8_linear_epilogue_fwd(x, weight.contiguous(), bias, residual, activation=activation)[0]
 
 
 @mxfp8_linear_epilogue_op.register_fake
@@ -62,8 +53,7 @@ def mxfp8_linear_epilogue_prequant_w(x: torch.Tensor, weight_data: torch.Tensor,
                                      bias: Optional[torch.Tensor], residual: Optional[torch.Tensor], n: int, k: int,
                                      activation: str) -> torch.Tensor:
     _check(x, n, k, bias, residual, activation)
-    return ops.mxfp8_linear_epilogue_fwd_prequant_w(_rows(x), weight_data, weight_scales, n, _vector(bias), _rows(residual),
-                                                    activation=activation)
+    return ops.mxfp8_linear_epilogue_fwd_prequant_w(x, weight_data, weight_scales, n, bias, residual, activation=activation)
 
 
 @mxfp8_linear_epilogue_prequant_w.register_fake
@@ -71,20 +61,32 @@ def _(x, weight_data, weight_scales, bias, residual, n, k, activation):
     return x.new_empty((x.shape[0], n), dtype=torch.bfloat16)
 
 
-@custom_op("rtx::mxfp8_linear_epilogue_train", mutates_args=(), device_types="cuda")
-def mxfp8_linear_epilogue_train(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor],
-                                residual: Optional[torch.Tensor], activation: str) -> Tuple[torch.Tensor, torch.Tensor]:
+@custom_op("rtx::mxfp8_linear_epilogue_fwd", mutates_args=(), device_types="cuda")
+def mxfp8_linear_epilogue_fwd(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor],
+                              residual: Optional[torch.Tensor], activation: str) -> Tuple[torch.Tensor, torch.Tensor]:
     """(y, z): z is what the backward needs of the forward, empty for activation "none"."""
     _check(x, *weight.shape, bias, residual, activation)
-    y, z = ops.mxfp8_linear_epilogue_fwd(_rows(x), weight.contiguous(), _vector(bias), _rows(residual),
-                                         activation=activation, keep_z=activation != "none")
+    y, z = ops.mxfp8_linear_epilogue_fwd(x, weight.contiguous(), bias, residual, activation=activation,
+                                         keep_z=activation != "none")
     return y, (z if z is not None else y.new_empty(0))
 
 
-@mxfp8_linear_epilogue_train.register_fake
-def _(x, weight, bias, residual, activation):
+def _fake_fwd(x, weight, bias, residual, activation):
     y = x.new_empty((x.shape[0], weight.shape[0]), dtype=torch.bfloat16)
     return y, (torch.empty_like(y) if activation != "none" else y.new_empty(0))
+
+
+mxfp8_linear_epilogue_fwd.register_fake(_fake_fwd)
+
+
+@custom_op("rtx::mxfp8_linear_epilogue_train", mutates_args=(), device_types="cuda")
+def mxfp8_linear_epilogue_train(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor],
+                                residual: Optional[torch.Tensor], activation: str) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The differentiable op."""
+    return mxfp8_linear_epilogue_fwd.fn(x, weight, bias, residual, activation)
+
+
+mxfp8_linear_epilogue_train.register_fake(_fake_fwd)
 
 
 @custom_op("rtx::mxfp8_linear_epilogue_bwd", mutates_args=(), device_types="cuda")
@@ -96,8 +98,7 @@ def mxfp8_linear_epilogue_bwd(grad_output: torch.Tensor, z: torch.Tensor, x: tor
     _check(x, n, k, None, None, activation)
     if grad_output.dtype is not torch.bfloat16 or tuple(grad_output.shape) != (x.shape[0], n):
         raise ValueError(f"grad_output must be BF16 [{x.shape[0]}, {n}]")
-    grads = ops.mxfp8_linear_epilogue_bwd(_rows(grad_output), z if activation != "none" else None,
-                                          _rows(x) if need_dw else None, weight.contiguous() if need_dx else None, int(k),
+    grads = ops.mxfp8_linear_epilogue_bwd(grad_output, z, x, weight.contiguous() if need_dx else None, k,
                                           activation=activation, need_dx=need_dx, need_dw=need_dw, need_dbias=need_dbias)
     return tuple(g if g is not None else x.new_empty(0) for g in grads)
 
@@ -125,11 +126,27 @@ def _train_backward(ctx, grad_y, _grad_z):
     if not (need_dx or need_dw or need_db):
         return None, None, None, grad_y if need_dr else None, None
     x, weight, z = ctx.saved_tensors
-    dx, dw, db = torch.ops.rtx.mxfp8_linear_epilogue_bwd(grad_y, z, x, weight, ctx.activation, need_dx, need_dw, need_db)
+    dx, dw, db = mxfp8_linear_epilogue_bwd(grad_y, z, x, weight, ctx.activation, need_dx, need_dw, need_db)
     return (dx if need_dx else None, dw if need_dw else None, db if need_db else None, grad_y if need_dr else None, None)
 
 
 mxfp8_linear_epilogue_train.register_autograd(_train_backward, setup_context=_train_setup)
+
+
+class _LinearEpilogueFunction(torch.autograd.Function):
+    """The same graph node for eager calls, without the host time of an op's registered autograd formula."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, activation):
+        y, z = mxfp8_linear_epilogue_fwd(x, weight, bias, residual, activation)
+        ctx.save_for_backward(x, weight, z)
+        ctx.activation = activation
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_y):
+        return _train_backward(ctx, grad_y, None)
 
 
 def _needs_grad(*tensors) -> bool:
@@ -152,18 +169,21 @@ def mxfp8_linear_epilogue(x: torch.Tensor, weight, bias: Optional[torch.Tensor] 
     shape = (*x.shape[:-1], n)
     if residual is not None and tuple(residual.shape) != shape:
         raise ValueError(f"residual must have the result's shape {shape}, got {tuple(residual.shape)}")
-    x2d = x.reshape(-1, k)
-    r2d = residual.reshape(-1, n) if residual is not None else None
+    if x.ndim != 2:
+        x = x.reshape(-1, k)
+    if residual is not None and residual.ndim != 2:
+        residual = residual.reshape(-1, n)
     if isinstance(weight, MXFP8Tensor):
         if _needs_grad(x, bias, residual):
             raise RuntimeError("a prequantized MXFP8 weight is inference-only; keep the BF16 master weight to train")
-        y = torch.ops.rtx.mxfp8_linear_epilogue_prequant_w(x2d, mxfp8_qdata_2d(weight), mxfp8_scales_for_kernel(weight), bias,
-                                                           r2d, n, k, activation)
-    elif _needs_grad(x, weight, bias, residual):
-        y = torch.ops.rtx.mxfp8_linear_epilogue_train(x2d, weight, bias, r2d, activation)[0]
+        y = mxfp8_linear_epilogue_prequant_w(x, *mxfp8_kernel_operands(weight), bias, residual, n, k, activation)
+    elif not _needs_grad(x, weight, bias, residual):
+        y = mxfp8_linear_epilogue_op(x, weight, bias, residual, activation)
+    elif torch.compiler.is_compiling():
+        y = mxfp8_linear_epilogue_train(x, weight, bias, residual, activation)[0]
     else:
-        y = torch.ops.rtx.mxfp8_linear_epilogue(x2d, weight, bias, r2d, activation)
-    return y.reshape(shape)
+        y = _LinearEpilogueFunction.apply(x, weight, bias, residual, activation)
+    return y if len(shape) == 2 else y.reshape(shape)
 
 
 def mxfp8_linear_epilogue_backward(grad_output: torch.Tensor, z: Optional[torch.Tensor], x: torch.Tensor,
@@ -175,8 +195,8 @@ def mxfp8_linear_epilogue_backward(grad_output: torch.Tensor, z: Optional[torch.
     if activation != "none" and z is None:
         raise ValueError("an activation's backward needs the pre-activation z")
     z2d = z.reshape(-1, n).contiguous() if z is not None and activation != "none" else grad_output.new_empty(0)
-    dx, dw, db = torch.ops.rtx.mxfp8_linear_epilogue_bwd(grad_output.reshape(-1, n), z2d, x.reshape(-1, k), weight, activation,
-                                                         True, True, bias)
+    dx, dw, db = mxfp8_linear_epilogue_bwd(grad_output.reshape(-1, n), z2d, x.reshape(-1, k), weight, activation, True, True,
+                                           bias)
     return dx.reshape(x.shape), dw, db if bias else None
 
 

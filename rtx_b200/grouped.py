@@ -17,19 +17,13 @@ from typing import Tuple
 
 import torch
 from torch import nn
+from torch.autograd.function import once_differentiable
 
 from . import fp8 as _fp8
 from . import ops
 from ._oplib import custom_op
-from .formats import (PACKED_OPERAND_SCHEMA_VERSION, SCALE_LAYOUT_CODES, MXFP8Tensor, make_mxfp8_tensor, mxfp8_qdata_2d,
-                      mxfp8_scales_for_kernel, reject_packed_dtype_conversion)
-
-
-def _rows_contiguous(t: torch.Tensor) -> torch.Tensor:
-    """`t` itself if its rows are contiguous (any pitch), else a copy."""
-    if (t.shape[1] <= 1 or t.stride(1) == 1) and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1]):
-        return t
-    return t.contiguous()
+from .formats import (PACKED_OPERAND_SCHEMA_VERSION, SCALE_LAYOUT_CODES, MXFP8Tensor, make_mxfp8_tensor,
+                      mxfp8_kernel_operands, mxfp8_qdata_2d, mxfp8_scales_for_kernel, reject_packed_dtype_conversion)
 
 
 def _check_grouped(x: torch.Tensor, weight: torch.Tensor) -> None:
@@ -48,7 +42,7 @@ def _check_grouped(x: torch.Tensor, weight: torch.Tensor) -> None:
 @custom_op("rtx::mxfp8_grouped_linear", mutates_args=(), device_types="cuda")
 def mxfp8_grouped_linear_op(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor) -> torch.Tensor:
     _check_grouped(x, weight)
-    return ops.mxfp8_grouped_linear_fwd(_rows_contiguous(x), weight.contiguous(), offsets)
+    return ops.mxfp8_grouped_linear_fwd(x, weight, offsets)
 
 
 @mxfp8_grouped_linear_op.register_fake
@@ -59,9 +53,7 @@ def _(x, weight, offsets):
 @custom_op("rtx::mxfp8_grouped_linear_prequant_w", mutates_args=(), device_types="cuda")
 def mxfp8_grouped_linear_prequant_w(x: torch.Tensor, weight_data: torch.Tensor, weight_scales: torch.Tensor,
                                     offsets: torch.Tensor, n: int) -> torch.Tensor:
-    if x.dtype is not torch.bfloat16 or x.ndim != 2:
-        raise TypeError("x must be BF16 [rows, K]")
-    return ops.mxfp8_grouped_linear_fwd_prequant_w(_rows_contiguous(x), weight_data, weight_scales, offsets, n)
+    return ops.mxfp8_grouped_linear_fwd_prequant_w(x, weight_data, weight_scales, offsets, n)
 
 
 @mxfp8_grouped_linear_prequant_w.register_fake
@@ -71,9 +63,7 @@ def _(x, weight_data, weight_scales, offsets, n):
 
 def _bwd(grad_output, x, weight, offsets, need_dx, need_dw):
     groups, _, k = (int(v) for v in weight.shape)
-    return ops.mxfp8_grouped_linear_bwd(_rows_contiguous(grad_output), _rows_contiguous(x) if need_dw else None,
-                                        weight.contiguous() if need_dx else None, offsets, groups, k, need_dx=need_dx,
-                                        need_dw=need_dw)
+    return ops.mxfp8_grouped_linear_bwd(grad_output, x, weight, offsets, groups, k, need_dx=need_dx, need_dw=need_dw)
 
 
 def _check_grad(grad_output, x, weight) -> None:
@@ -122,6 +112,17 @@ def _(grad_output, x, weight, offsets):
     return weight.new_empty(weight.shape)
 
 
+@custom_op("rtx::mxfp8_grouped_linear_train", mutates_args=(), device_types="cuda")
+def mxfp8_grouped_linear_train(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor) -> torch.Tensor:
+    """Forward of the differentiable op; saves its inputs."""
+    return mxfp8_grouped_linear_op.fn(x, weight, offsets)
+
+
+@mxfp8_grouped_linear_train.register_fake
+def _(x, weight, offsets):
+    return x.new_empty((x.shape[0], weight.shape[1]), dtype=torch.bfloat16)
+
+
 def _train_setup(ctx, inputs, output):
     ctx.save_for_backward(*inputs)
 
@@ -130,15 +131,27 @@ def _train_backward(ctx, grad_output):
     x, weight, offsets = ctx.saved_tensors
     need_dx, need_dw = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
     if need_dx and need_dw:
-        return (*torch.ops.rtx.mxfp8_grouped_linear_bwd(grad_output, x, weight, offsets), None)
+        return (*mxfp8_grouped_linear_bwd(grad_output, x, weight, offsets), None)
     if need_dx:
-        return torch.ops.rtx.mxfp8_grouped_linear_dx(grad_output, x, weight, offsets), None, None
+        return mxfp8_grouped_linear_dx(grad_output, x, weight, offsets), None, None
     if need_dw:
-        return None, torch.ops.rtx.mxfp8_grouped_linear_dw(grad_output, x, weight, offsets), None
+        return None, mxfp8_grouped_linear_dw(grad_output, x, weight, offsets), None
     return None, None, None
 
 
-mxfp8_grouped_linear_op.register_autograd(_train_backward, setup_context=_train_setup)
+mxfp8_grouped_linear_train.register_autograd(_train_backward, setup_context=_train_setup)
+
+
+class _GroupedLinearFunction(torch.autograd.Function):
+    """The same graph node for eager calls: an op's registered autograd formula costs some 40 microseconds of host time
+    per call more than this, longer than a small layer takes on the device."""
+
+    @staticmethod
+    def forward(ctx, x, weight, offsets):
+        ctx.save_for_backward(x, weight, offsets)
+        return mxfp8_grouped_linear_op(x, weight, offsets)
+
+    backward = staticmethod(once_differentiable(_train_backward))
 
 
 def _packed_group_shape(weight) -> Tuple[int, int, int]:
@@ -161,22 +174,29 @@ def mxfp8_grouped_linear(x: torch.Tensor, weight, offsets: torch.Tensor) -> torc
     """
     if isinstance(weight, MXFP8Tensor):
         groups, n, k = _packed_group_shape(weight)
-        if x.shape[-1] != k:
+        if x.ndim != 2 or x.shape[1] != k:
             raise ValueError(f"K mismatch: x has {x.shape[-1]}, weight has {k}")
-        if offsets.numel() != groups + 1:
+        if offsets.shape != (groups + 1,):
             raise ValueError(f"offsets must be a contiguous vector of groups + 1 = {groups + 1} row numbers")
         if x.requires_grad and torch.is_grad_enabled():
             raise RuntimeError("a prequantized MXFP8 weight is inference-only; keep the BF16 master weight to train")
-        return torch.ops.rtx.mxfp8_grouped_linear_prequant_w(x, mxfp8_qdata_2d(weight), mxfp8_scales_for_kernel(weight),
-                                                             offsets, n)
-    return torch.ops.rtx.mxfp8_grouped_linear(x, weight, offsets)
+        return mxfp8_grouped_linear_prequant_w(x, *mxfp8_kernel_operands(weight), offsets, n)
+    return _dynamic(x, weight, offsets)
+
+
+def _dynamic(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor) -> torch.Tensor:
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
+        if torch.compiler.is_compiling():
+            return mxfp8_grouped_linear_train(x, weight, offsets)
+        return _GroupedLinearFunction.apply(x, weight, offsets)
+    return mxfp8_grouped_linear_op(x, weight, offsets)
 
 
 def mxfp8_grouped_linear_backward(grad_output: torch.Tensor, x: torch.Tensor, weight: torch.Tensor,
                                   offsets: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """BF16 dX [rows, K] and dW [groups, N, K] of `mxfp8_grouped_linear`, from independently quantized MXFP8 products
     (blocks along N for dX, along each group's rows for dW)."""
-    return torch.ops.rtx.mxfp8_grouped_linear_bwd(grad_output, x, weight, offsets)
+    return mxfp8_grouped_linear_bwd(grad_output, x, weight, offsets)
 
 
 class MXFP8GroupedLinear(nn.Module):
@@ -241,9 +261,8 @@ class MXFP8GroupedLinear(nn.Module):
         if self.weight_mode == "prequantized":
             if x.requires_grad and torch.is_grad_enabled():
                 raise RuntimeError("a prequantized MXFP8 weight is inference-only; keep the BF16 master weight to train")
-            return torch.ops.rtx.mxfp8_grouped_linear_prequant_w(x, self.weight_data, self.weight_scales, offsets,
-                                                                 self.out_features)
-        return torch.ops.rtx.mxfp8_grouped_linear(x, self.weight, offsets)
+            return mxfp8_grouped_linear_prequant_w(x, self.weight_data, self.weight_scales, offsets, self.out_features)
+        return _dynamic(x, self.weight, offsets)
 
 
 __all__ = ["MXFP8GroupedLinear", "mxfp8_grouped_linear", "mxfp8_grouped_linear_backward"]

@@ -319,48 +319,100 @@ def activation_code(name: str) -> int:
         raise ValueError(f"unknown activation {name!r}; built: {', '.join(ACTIVATIONS)}") from None
 
 
-def _require_vector(t: torch.Tensor, n: int, device: torch.device, name: str) -> None:
+@functools.lru_cache(maxsize=4096)
+def _bytes(query: str, *sizes: int) -> int:
+    """A workspace size: a function of the sizes alone, asked for once."""
+    return N.query(query, *sizes)
+
+
+def _new(like: torch.Tensor, *shape: int) -> torch.Tensor:
+    """Uninitialised BF16 tensor on `like`'s device and its current stream (`like` is BF16: the cheapest spelling)."""
+    return like.new_empty(shape)
+
+
+def _scratch(like: torch.Tensor, nbytes: int) -> torch.Tensor:
+    """Workspace of one call: a fresh allocation of the calling stream, so that calls on several streams and captured
+    graphs share nothing."""
+    return like.new_empty((nbytes + 1) // 2)
+
+
+def _status_ptr(device: torch.device) -> int:
+    return status_word(device).data_ptr()
+
+
+def _rows_of(t: torch.Tensor, cols: Optional[int], name: str) -> Tuple[torch.Tensor, int]:
+    """A BF16 CUDA matrix and its row pitch in elements; a matrix whose rows are not contiguous, or overlap, is copied."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor")
+    if t.dtype is not torch.bfloat16:
+        raise TypeError(f"{name} must have dtype {torch.bfloat16}, got {t.dtype}")
+    if t.dim() != 2 or (cols is not None and t.shape[1] != cols):
+        raise ValueError(f"{name} must be two-dimensional" + (f" with {cols} columns" if cols is not None else ""))
+    rows, width = t.shape
+    pitch, inner = t.stride()
+    if (inner == 1 or width <= 1) and (pitch >= width or rows <= 1):
+        return t, (pitch if rows > 1 else max(width, 1))     # a single row's stride says nothing
+    return t.contiguous(), width
+
+
+def _vector_of(t: torch.Tensor, n: int, device: torch.device, name: str) -> torch.Tensor:
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
     if t.dtype is not torch.bfloat16:
         raise TypeError(f"{name} must have dtype {torch.bfloat16}, got {t.dtype}")
-    if t.dim() != 1 or t.numel() != n or not t.is_contiguous() or t.device != device:
-        raise ValueError(f"{name} must be a contiguous vector of {n} values on the operands' device")
+    if t.dim() != 1 or t.shape[0] != n or t.device != device:
+        raise ValueError(f"{name} must be a vector of {n} values on the operands' device")
+    return t if t.is_contiguous() else t.contiguous()
 
 
-def _epilogue_operands(x, n, k, bias, residual):
-    _require_rows(x, k, "x")
+def _packed(qw: torch.Tensor, sw: torch.Tensor, rows: int, k: int, device: torch.device) -> None:
+    if qw.device != device or sw.device != device:
+        raise ValueError("x and the packed weight must share one device")
+    if qw.element_size() != 1 or qw.numel() != rows * mx_storage_k(k) or not qw.is_contiguous():
+        raise ValueError(f"packed weight must hold {rows} rows of {mx_storage_k(k)} values")
+    if (sw.element_size() != 1 or sw.numel() != _bytes("rtxb_mxfp8_scale_bytes", rows, k, N.SCALE_MMA128)
+            or not sw.is_contiguous()):
+        raise ValueError("packed weight scales must be mma128 tiles")
+
+
+def _bias_and_residual(x, m, n, bias, residual):
+    """(bias, residual, its pitch) checked; the tensors are returned because a copy may have been made."""
     if bias is not None:
-        _require_vector(bias, n, x.device, "bias")
+        bias = _vector_of(bias, n, x.device, "bias")
+    pitch = n
     if residual is not None:
-        _require_rows(residual, n, "residual")
-        if residual.shape[0] != x.shape[0] or residual.device != x.device:
+        residual, pitch = _rows_of(residual, n, "residual")
+        if residual.shape[0] != m or residual.device != x.device:
             raise ValueError("residual must have the result's shape and device")
-    return int(x.shape[0])
+    return bias, residual, pitch
 
 
 def mxfp8_linear_epilogue_fwd(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None,
                               residual: Optional[torch.Tensor] = None, *, activation: str = "none", keep_z: bool = False,
                               rounding: int = N.ROUND_INFINITY):
     """x bf16 [M, K] (any row pitch), w bf16 [N, K] -> (out, z): z = q(x) q(w)^T + bias, out = bf16(act(z) + residual);
-    z in BF16 with `keep_z`, else None.  The scratch is a fresh allocation of the calling stream."""
+    z in BF16 with `keep_z`, else None."""
     _require(w, torch.bfloat16, "weight")
-    n, k = (int(v) for v in w.shape)
-    m = _epilogue_operands(x, n, k, bias, residual)
-    if w.device != x.device:
+    n, k = w.shape
+    x, ldx = _rows_of(x, k, "x")
+    device = x.device
+    if w.device != device:
         raise ValueError("x and weight must share one device")
+    m = x.shape[0]
+    bias, residual, ldr = _bias_and_residual(x, m, n, bias, residual)
     code = activation_code(activation)
-    out = torch.empty(m, n, dtype=torch.bfloat16, device=x.device)
-    z = torch.empty_like(out) if keep_z else None
-    if out.numel() == 0:
-        return out, z
-    nbytes = N.query("rtxb_mxfp8_linear_epilogue_workspace_bytes", m, n, k, 1)
-    with _on(x.device):
-        buf = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-        N.call("rtxb_mxfp8_linear_epilogue_fwd", x.data_ptr(), _pitch(x), w.data_ptr(),
-               bias.data_ptr() if bias is not None else None, residual.data_ptr() if residual is not None else None,
-               _pitch(residual) if residual is not None else n, out.data_ptr(), z.data_ptr() if keep_z else None, m, n, k,
-               code, rounding, buf.data_ptr(), nbytes, _stream_ptr(), status_word(x.device).data_ptr())
+    with _on(device):
+        out = _new(x, m, n)
+        z = _new(x, m, n) if keep_z else None
+        if m and n:
+            nbytes = _bytes("rtxb_mxfp8_linear_epilogue_workspace_bytes", m, n, k, 1)
+            buf = _scratch(x, nbytes)
+            N.call("rtxb_mxfp8_linear_epilogue_fwd", x.data_ptr(), ldx, w.data_ptr(),
+                   None if bias is None else bias.data_ptr(), None if residual is None else residual.data_ptr(), ldr,
+                   out.data_ptr(), z.data_ptr() if keep_z else None, m, n, k, code, rounding, buf.data_ptr(), nbytes,
+                   _stream_ptr(), _status_ptr(device))
     return out, z
 
 
@@ -368,25 +420,20 @@ def mxfp8_linear_epilogue_fwd_prequant_w(x: torch.Tensor, qw: torch.Tensor, sw: 
                                          bias: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None, *,
                                          activation: str = "none", rounding: int = N.ROUND_INFINITY) -> torch.Tensor:
     """The same with a packed weight (qw u8 [N, Kp], mma128 scale tiles)."""
-    k = int(x.shape[1]) if x.dim() == 2 else 0
-    m = _epilogue_operands(x, n, k, bias, residual)
-    if qw.device != x.device or sw.device != x.device:
-        raise ValueError("x and the packed weight must share one device")
-    if qw.element_size() != 1 or qw.numel() != n * mx_storage_k(k) or not qw.is_contiguous():
-        raise ValueError(f"packed weight must hold {n} rows of {mx_storage_k(k)} values")
-    if sw.element_size() != 1 or sw.numel() != mxfp8_scale_numel(n, k, N.SCALE_MMA128) or not sw.is_contiguous():
-        raise ValueError("packed weight scales must be mma128 tiles")
+    x, ldx = _rows_of(x, None, "x")
+    m, k = x.shape
+    device = x.device
+    _packed(qw, sw, n, k, device)
+    bias, residual, ldr = _bias_and_residual(x, m, n, bias, residual)
     code = activation_code(activation)
-    out = torch.empty(m, n, dtype=torch.bfloat16, device=x.device)
-    if out.numel() == 0:
-        return out
-    nbytes = N.query("rtxb_mxfp8_linear_epilogue_workspace_bytes", m, n, k, 0)
-    with _on(x.device):
-        buf = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-        N.call("rtxb_mxfp8_linear_epilogue_fwd_prequant_w", x.data_ptr(), _pitch(x), qw.data_ptr(), sw.data_ptr(),
-               bias.data_ptr() if bias is not None else None, residual.data_ptr() if residual is not None else None,
-               _pitch(residual) if residual is not None else n, out.data_ptr(), m, n, k, code, rounding, buf.data_ptr(),
-               nbytes, _stream_ptr(), status_word(x.device).data_ptr())
+    with _on(device):
+        out = _new(x, m, n)
+        if m and n:
+            nbytes = _bytes("rtxb_mxfp8_linear_epilogue_workspace_bytes", m, n, k, 0)
+            buf = _scratch(x, nbytes)
+            N.call("rtxb_mxfp8_linear_epilogue_fwd_prequant_w", x.data_ptr(), ldx, qw.data_ptr(), sw.data_ptr(),
+                   None if bias is None else bias.data_ptr(), None if residual is None else residual.data_ptr(), ldr,
+                   out.data_ptr(), m, n, k, code, rounding, buf.data_ptr(), nbytes, _stream_ptr(), _status_ptr(device))
     return out
 
 
@@ -396,61 +443,42 @@ def mxfp8_linear_epilogue_bwd(dy: torch.Tensor, z: Optional[torch.Tensor], x: Op
     """(dY [M, N], z [M, N] of the forward, X [M, K], W [N, K]) -> (dX | None, dW | None, dbias [N] | None); z is read
     unless activation is none, X for dW only, W for dX only."""
     code = activation_code(activation)
-    _require_rows(dy, None, "grad_output")
-    m, n = (int(v) for v in dy.shape)
+    dy, lddy = _rows_of(dy, None, "grad_output")
+    m, n = dy.shape
+    device = dy.device
     if code:
         _require(z, torch.bfloat16, "z")
-        if z.shape != dy.shape or z.device != dy.device:
+        if z.shape != dy.shape or z.device != device:
             raise ValueError("z must have grad_output's shape and device")
+    ldx = k
     if need_dw:
-        _require_rows(x, k, "x")
-        if x.shape[0] != m or x.device != dy.device:
+        x, ldx = _rows_of(x, k, "x")
+        if x.shape[0] != m or x.device != device:
             raise ValueError("grad_output and x disagree on the rows or the device")
     if need_dx:
         _require(w, torch.bfloat16, "weight")
-        if tuple(w.shape) != (n, k) or w.device != dy.device:
+        if w.shape[0] != n or w.shape[1] != k or w.device != device:
             raise ValueError("weight must be [N, K] on grad_output's device")
-    new = functools.partial(torch.empty, dtype=torch.bfloat16, device=dy.device)
-    dx = new(m, k) if need_dx else None
-    dw = new(n, k) if need_dw else None
-    db = new(n) if need_dbias else None
-    outs = (dx, dw, db)
-    if all(t is None for t in outs):
-        return outs
-    if min(m, n, k) == 0:                 # an empty sum is zero
-        return tuple(None if t is None else t.zero_() for t in outs)
-    nbytes = N.query("rtxb_mxfp8_linear_epilogue_backward_workspace_bytes", m, n, k, int(need_dx), int(need_dw),
-                     int(need_dbias))
-    with _on(dy.device):
-        buf = torch.empty(nbytes, dtype=torch.uint8, device=dy.device)
-        N.call("rtxb_mxfp8_linear_epilogue_bwd", dy.data_ptr(), _pitch(dy), z.data_ptr() if code else None,
-               x.data_ptr() if need_dw else None, _pitch(x) if need_dw else k, w.data_ptr() if need_dx else None,
+    if not (need_dx or need_dw or need_dbias):
+        return None, None, None
+    with _on(device):
+        dx = _new(dy, m, k) if need_dx else None
+        dw = _new(dy, n, k) if need_dw else None
+        db = _new(dy, n) if need_dbias else None
+        if min(m, n, k) == 0:             # an empty sum is zero
+            return tuple(None if t is None else t.zero_() for t in (dx, dw, db))
+        nbytes = _bytes("rtxb_mxfp8_linear_epilogue_backward_workspace_bytes", m, n, k, int(need_dx), int(need_dw),
+                        int(need_dbias))
+        buf = _scratch(dy, nbytes)
+        N.call("rtxb_mxfp8_linear_epilogue_bwd", dy.data_ptr(), lddy, z.data_ptr() if code else None,
+               x.data_ptr() if need_dw else None, ldx, w.data_ptr() if need_dx else None,
                dx.data_ptr() if need_dx else None, dw.data_ptr() if need_dw else None,
                db.data_ptr() if need_dbias else None, m, n, k, code, buf.data_ptr(), nbytes, _stream_ptr(),
-               status_word(dy.device).data_ptr())
-    return outs
+               _status_ptr(device))
+    return dx, dw, db
 
 
 MAX_GROUPS = 512
-
-
-def _require_rows(t: torch.Tensor, cols: Optional[int], name: str) -> None:
-    """A BF16 CUDA matrix whose rows are contiguous (any row pitch)."""
-    if not isinstance(t, torch.Tensor):
-        raise TypeError(f"{name} must be a torch.Tensor")
-    if t.device.type != "cuda":
-        raise ValueError(f"{name} must be a CUDA tensor")
-    if t.dtype != torch.bfloat16:
-        raise TypeError(f"{name} must have dtype {torch.bfloat16}, got {t.dtype}")
-    if t.dim() != 2 or (cols is not None and t.shape[1] != cols):
-        raise ValueError(f"{name} must be two-dimensional" + (f" with {cols} columns" if cols is not None else ""))
-    if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
-        raise ValueError(f"{name} must have contiguous rows that do not overlap")
-
-
-def _pitch(t: torch.Tensor) -> int:
-    """Row pitch in elements; a single row's stride says nothing and is replaced by its width."""
-    return t.stride(0) if t.shape[0] > 1 else max(int(t.shape[1]), 1)
 
 
 def _require_offsets(offsets: torch.Tensor, groups: int, device: torch.device) -> None:
@@ -460,43 +488,50 @@ def _require_offsets(offsets: torch.Tensor, groups: int, device: torch.device) -
         raise TypeError(f"offsets must have dtype torch.int32, got {offsets.dtype}")
     if offsets.device != device:
         raise ValueError("offsets must be on the operands' device")
-    if offsets.dim() != 1 or offsets.numel() != groups + 1 or not offsets.is_contiguous():
+    if offsets.dim() != 1 or offsets.shape[0] != groups + 1 or not offsets.is_contiguous():
         raise ValueError(f"offsets must be a contiguous vector of groups + 1 = {groups + 1} row numbers")
-    if groups > MAX_GROUPS:
-        raise ValueError(f"at most {MAX_GROUPS} groups, got {groups}")
+    if not 1 <= groups <= MAX_GROUPS:
+        raise ValueError(f"between 1 and {MAX_GROUPS} groups, got {groups}")
+
+
+def _group_weight(w: torch.Tensor, device: torch.device) -> torch.Tensor:
+    if not isinstance(w, torch.Tensor):
+        raise TypeError("weight must be a torch.Tensor")
+    if w.dim() != 3 or w.dtype is not torch.bfloat16:
+        raise ValueError("weight must be a BF16 tensor [groups, N, K]")
+    if w.device != device:
+        raise ValueError("x and weight must share one device")
+    return w if w.is_contiguous() else w.contiguous()
+
+
+def _grouped_out(out: Optional[torch.Tensor], x: torch.Tensor, n: int) -> Tuple[torch.Tensor, int]:
+    if out is None:
+        return _new(x, x.shape[0], n), n
+    held, ldo = _rows_of(out, n, "out")
+    if held is not out or out.shape[0] != x.shape[0] or out.device != x.device:
+        raise ValueError(f"out must be [{x.shape[0]}, {n}] with contiguous rows on the operands' device")
+    return out, ldo
 
 
 def mxfp8_grouped_linear_fwd(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, *,
                              rounding: int = N.ROUND_INFINITY, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """x bf16 [T, K] (any row pitch), w bf16 [E, N, K], offsets int32 [E + 1] -> out bf16 [T, N]: row r of group g is
-    q(x[r]) q(w[g])^T, rows of no group are zero.  The scratch is a fresh allocation of the calling stream, so calls on
-    several streams and captured graphs share nothing."""
-    if w.dim() != 3 or w.dtype is not torch.bfloat16 or not w.is_contiguous():
-        raise ValueError("weight must be a contiguous BF16 tensor [groups, N, K]")
-    groups, n, k = (int(v) for v in w.shape)
-    _require_rows(x, k, "x")
-    if w.device != x.device:
-        raise ValueError("x and weight must share one device")
-    _require_offsets(offsets, groups, x.device)
-    rows = int(x.shape[0])
-    out = _grouped_out(out, rows, n, x.device)
-    if out.numel() == 0:
-        return out
-    nbytes = N.query("rtxb_mxfp8_grouped_linear_workspace_bytes", rows, n, k, groups, 1)
-    with _on(x.device):
-        buf = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-        N.call("rtxb_mxfp8_grouped_linear_fwd", x.data_ptr(), _pitch(x), w.data_ptr(), offsets.data_ptr(), groups,
-               out.data_ptr(), _pitch(out), rows, n, k, rounding, buf.data_ptr(), nbytes, _stream_ptr(),
-               status_word(x.device).data_ptr())
-    return out
-
-
-def _grouped_out(out: Optional[torch.Tensor], rows: int, n: int, device: torch.device) -> torch.Tensor:
-    if out is None:
-        return torch.empty(rows, n, dtype=torch.bfloat16, device=device)
-    _require_rows(out, n, "out")
-    if out.shape[0] != rows or out.device != device:
-        raise ValueError(f"out must be [{rows}, {n}] on the operands' device")
+    q(x[r]) q(w[g])^T, rows of no group are zero."""
+    x, ldx = _rows_of(x, None, "x")
+    device = x.device
+    w = _group_weight(w, device)
+    groups, n, k = w.shape
+    rows = x.shape[0]
+    if x.shape[1] != k:
+        raise ValueError(f"K mismatch: x has {x.shape[1]}, weight has {k}")
+    _require_offsets(offsets, groups, device)
+    with _on(device):
+        out, ldo = _grouped_out(out, x, n)
+        if rows and n:
+            nbytes = _bytes("rtxb_mxfp8_grouped_linear_workspace_bytes", rows, n, k, groups, 1)
+            buf = _scratch(x, nbytes)
+            N.call("rtxb_mxfp8_grouped_linear_fwd", x.data_ptr(), ldx, w.data_ptr(), offsets.data_ptr(), groups,
+                   out.data_ptr(), ldo, rows, n, k, rounding, buf.data_ptr(), nbytes, _stream_ptr(), _status_ptr(device))
     return out
 
 
@@ -504,25 +539,20 @@ def mxfp8_grouped_linear_fwd_prequant_w(x: torch.Tensor, qw: torch.Tensor, sw: t
                                         *, rounding: int = N.ROUND_INFINITY,
                                         out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The same with packed weights: qw u8 [E * N, Kp] and mma128 scale tiles, N a multiple of 128 when E > 1."""
-    _require_rows(x, None, "x")
-    rows, k = (int(v) for v in x.shape)
-    groups = int(offsets.numel()) - 1
-    _require_offsets(offsets, groups, x.device)
-    if qw.device != x.device or sw.device != x.device:
-        raise ValueError("x and the packed weight must share one device")
-    if qw.element_size() != 1 or qw.numel() != groups * n * mx_storage_k(k) or not qw.is_contiguous():
-        raise ValueError(f"packed weight must hold {groups} x {n} rows of {mx_storage_k(k)} values")
-    if sw.element_size() != 1 or sw.numel() != mxfp8_scale_numel(groups * n, k, N.SCALE_MMA128) or not sw.is_contiguous():
-        raise ValueError("packed weight scales must be mma128 tiles")
-    out = _grouped_out(out, rows, n, x.device)
-    if out.numel() == 0:
-        return out
-    nbytes = N.query("rtxb_mxfp8_grouped_linear_workspace_bytes", rows, n, k, groups, 0)
-    with _on(x.device):
-        buf = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-        N.call("rtxb_mxfp8_grouped_linear_fwd_prequant_w", x.data_ptr(), _pitch(x), qw.data_ptr(), sw.data_ptr(),
-               offsets.data_ptr(), groups, out.data_ptr(), _pitch(out), rows, n, k, rounding, buf.data_ptr(), nbytes,
-               _stream_ptr(), status_word(x.device).data_ptr())
+    x, ldx = _rows_of(x, None, "x")
+    rows, k = x.shape
+    device = x.device
+    groups = offsets.shape[0] - 1 if isinstance(offsets, torch.Tensor) and offsets.dim() == 1 else 0
+    _require_offsets(offsets, groups, device)
+    _packed(qw, sw, groups * n, k, device)
+    with _on(device):
+        out, ldo = _grouped_out(out, x, n)
+        if rows and n:
+            nbytes = _bytes("rtxb_mxfp8_grouped_linear_workspace_bytes", rows, n, k, groups, 0)
+            buf = _scratch(x, nbytes)
+            N.call("rtxb_mxfp8_grouped_linear_fwd_prequant_w", x.data_ptr(), ldx, qw.data_ptr(), sw.data_ptr(),
+                   offsets.data_ptr(), groups, out.data_ptr(), ldo, rows, n, k, rounding, buf.data_ptr(), nbytes,
+                   _stream_ptr(), _status_ptr(device))
     return out
 
 
@@ -530,29 +560,31 @@ def mxfp8_grouped_linear_bwd(dy: torch.Tensor, x: Optional[torch.Tensor], w: Opt
                              groups: int, k: int, *, need_dx: bool = True, need_dw: bool = True):
     """(dY [T, N], X [T, K], W [E, N, K]) -> (dX bf16 [T, K] | None, dW bf16 [E, N, K] | None); X is read for dW only,
     W for dX only."""
-    _require_rows(dy, None, "grad_output")
-    rows, n = (int(v) for v in dy.shape)
-    _require_offsets(offsets, groups, dy.device)
+    dy, lddy = _rows_of(dy, None, "grad_output")
+    rows, n = dy.shape
+    device = dy.device
+    _require_offsets(offsets, groups, device)
+    ldx = k
     if need_dw:
-        _require_rows(x, k, "x")
-        if x.shape[0] != rows or x.device != dy.device:
+        x, ldx = _rows_of(x, k, "x")
+        if x.shape[0] != rows or x.device != device:
             raise ValueError("grad_output and x disagree on the rows or the device")
-    if need_dx and (tuple(w.shape) != (groups, n, k) or w.dtype is not torch.bfloat16 or not w.is_contiguous()
-                    or w.device != dy.device):
-        raise ValueError("weight must be a contiguous BF16 tensor [groups, N, K] on grad_output's device")
-    dx = torch.empty(rows, k, dtype=torch.bfloat16, device=dy.device) if need_dx else None
-    dw = torch.empty(groups, n, k, dtype=torch.bfloat16, device=dy.device) if need_dw else None
+    if need_dx:
+        w = _group_weight(w, device)
+        if tuple(w.shape) != (groups, n, k):
+            raise ValueError(f"weight must be [{groups}, {n}, {k}]")
     if not (need_dx or need_dw):
-        return dx, dw
-    if min(rows, n, k, groups) == 0:      # an empty sum is zero
-        return (dx.zero_() if need_dx else None), (dw.zero_() if need_dw else None)
-    nbytes = N.query("rtxb_mxfp8_grouped_backward_workspace_bytes", rows, n, k, groups, int(need_dx), int(need_dw))
-    with _on(dy.device):
-        buf = torch.empty(nbytes, dtype=torch.uint8, device=dy.device)
-        N.call("rtxb_mxfp8_grouped_linear_bwd", dy.data_ptr(), _pitch(dy), x.data_ptr() if need_dw else None,
-               _pitch(x) if need_dw else k, w.data_ptr() if need_dx else None, offsets.data_ptr(), groups,
-               dx.data_ptr() if need_dx else None, dw.data_ptr() if need_dw else None, rows, n, k, buf.data_ptr(), nbytes,
-               _stream_ptr(), status_word(dy.device).data_ptr())
+        return None, None
+    with _on(device):
+        dx = _new(dy, rows, k) if need_dx else None
+        dw = _new(dy, groups, n, k) if need_dw else None
+        if min(rows, n, k) == 0:          # an empty sum is zero
+            return (dx.zero_() if need_dx else None), (dw.zero_() if need_dw else None)
+        nbytes = _bytes("rtxb_mxfp8_grouped_backward_workspace_bytes", rows, n, k, groups, int(need_dx), int(need_dw))
+        buf = _scratch(dy, nbytes)
+        N.call("rtxb_mxfp8_grouped_linear_bwd", dy.data_ptr(), lddy, x.data_ptr() if need_dw else None, ldx,
+               w.data_ptr() if need_dx else None, offsets.data_ptr(), groups, dx.data_ptr() if need_dx else None,
+               dw.data_ptr() if need_dw else None, rows, n, k, buf.data_ptr(), nbytes, _stream_ptr(), _status_ptr(device))
     return dx, dw
 
 

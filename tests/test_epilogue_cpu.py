@@ -74,11 +74,11 @@ def test_python_refusals():
     with pytest.raises(TypeError, match="BF16"):
         MXFP8LinearEpilogue(64, 128, dtype=torch.float16)
     with pytest.raises(ValueError, match="CUDA"):
-        ops._require_rows(x, 64, "x")
+        ops._rows_of(x, 64, "x")
     for bad, error in ((torch.zeros(128), TypeError), (torch.zeros(64, dtype=torch.bfloat16), ValueError),
-                       (torch.zeros(256, dtype=torch.bfloat16)[::2], ValueError), (1.0, TypeError)):
+                       (torch.zeros(1, 128, dtype=torch.bfloat16), ValueError), (1.0, TypeError)):
         with pytest.raises(error, match="bias"):
-            ops._require_vector(bad, 128, torch.device("cpu"), "bias")
+            ops._vector_of(bad, 128, torch.device("cpu"), "bias")
     packed = make_mxfp8_tensor(torch.zeros(128, 64, dtype=torch.uint8), torch.zeros(512, dtype=torch.uint8), (128, 64), "mma128")
     with pytest.raises(RuntimeError, match="inference-only"):
         mxfp8_linear_epilogue(x.clone().requires_grad_(True), packed)

@@ -58,7 +58,7 @@ def test_python_refusals():
     with pytest.raises(ValueError, match="CUDA"):
         ops.mxfp8_grouped_linear_fwd(x, w, o)
     with pytest.raises(ValueError, match="groups, N, K"):
-        ops.mxfp8_grouped_linear_fwd(x, w[0], o)
+        ops._group_weight(w[0], torch.device("cpu"))
     for bad, error in ((torch.zeros(3, dtype=torch.int64), TypeError), (torch.zeros(4, dtype=torch.int32), ValueError),
                        (torch.zeros(1, 3, dtype=torch.int32), ValueError), (torch.zeros(6, dtype=torch.int32)[::2], ValueError),
                        ([0, 1, 2], TypeError)):
