@@ -31,6 +31,14 @@ class OpHandle:
     def __call__(self, *args, **kwargs):
         return self.overload(*args, **kwargs)
 
+    def direct(self, *args):
+        """The op called from this package's own eager code: its implementation itself where that is what the dispatcher
+        would run (plain tensors, no tracing), the op otherwise.  Saves a dispatch of a few microseconds per call."""
+        kind = type(args[0])
+        if (kind is torch.Tensor or kind is torch.nn.Parameter) and args[0].is_cuda and not torch.compiler.is_compiling():
+            return self.fn(*args)
+        return self.overload(*args)
+
     def register_fake(self, fn: Callable) -> Callable:
         torch.library.register_fake(self.qualname, fn, lib=_LIB)
         return fn

@@ -99,7 +99,12 @@ __device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, const void*
                : "memory");
 }
 
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
+// Eight epilogue warps, two per TMEM lane quadrant, take the 32-column chunks in turn: where a pair has only one or two
+// tiles the epilogue is not hidden behind MMAs, and half of it is half of that time.
+constexpr int kGroupedEpiWarps = 8;
+constexpr int kGroupedThreads = 64 + 32 * kGroupedEpiWarps;
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGroupedThreads, 1)
 gemm_grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ GroupedMapsB maps_b,
                          const __grid_constant__ CUtensorMap map_sfa, const __grid_constant__ CUtensorMap map_sfb,
                          const __grid_constant__ CUtensorMap map_out, const GroupedGemmParams p) {
@@ -114,7 +119,7 @@ gemm_grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
   uint64_t* full_bar = bars;              // [GROUPS] used in the rank-0 CTA: both CTAs' loads land
   uint64_t* empty_bar = bars + S;         // [GROUPS] in each CTA
   uint64_t* acc_full_bar = bars + 2 * S;  // in each CTA: tile accumulated
-  uint64_t* acc_overlap_bar = acc_full_bar + 1;  // rank 0: shared columns drained by all 8 epilogue warps
+  uint64_t* acc_overlap_bar = acc_full_bar + 1;  // rank 0: shared columns drained (one arrival per epilogue warp)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_overlap_bar + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -131,7 +136,7 @@ gemm_grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
       mbar_init(&empty_bar[s], 1);
     }
     mbar_init(acc_full_bar, 1);
-    mbar_init(acc_overlap_bar, 8);
+    mbar_init(acc_overlap_bar, 2 * kGroupedEpiWarps);
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -268,11 +273,11 @@ gemm_grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
     __syncwarp();
   } else {
     // ------------------------------ epilogue (both CTAs) ------------------------------
-    const int quad = warp & 3;
+    const int quad = warp & 3, turn = (warp - 2) >> 2;   // this warp's lane quadrant; chunks turn, turn + 2, ...
     const uint32_t lane_base = static_cast<uint32_t>(quad * 32) << 16;
     const uint32_t overlap_addr = mapa_shared(smem_u32(acc_overlap_bar), 0);
-    uint8_t* stage = smem + T::kOffStage + quad * 2 * kEpiStageBufBytes;
-    uint32_t local_tile = 0, staged = 0;
+    uint8_t* buf = smem + T::kOffStage + (warp - 2) * kEpiStageBufBytes;
+    uint32_t local_tile = 0;
     for (int tile = pair_id; tile < total_tiles; tile += num_pairs) {
       const GroupedTile t = grouped_tile(p, tile);
       const int mma_n = grouped_mma_n(t.live);
@@ -283,9 +288,7 @@ gemm_grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
       auto emit = [&](const int c, const uint32_t (&r)[32]) {
         if (col0 >= p.out_cols) return;   // warp-uniform: nothing of this warp's columns exists
         if (p.tma_out && c + 32 <= t.live) {
-          uint8_t* buf = stage + (staged & 1) * kEpiStageBufBytes;
-          ++staged;
-          if (lane == 0) tma_store_wait_read<1>();   // the store that read this buffer two chunks ago is done
+          if (lane == 0) tma_store_wait_read<0>();   // the last store has read the buffer
           __syncwarp();
 #pragma unroll
           for (int j = 0; j < 32; ++j)
@@ -308,7 +311,7 @@ gemm_grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
 #pragma unroll
         for (int j = 0; j < 32; ++j) zero[j] = 0;
 #pragma unroll 1
-        for (int c = 0; c < mma_n; c += 32) emit(c, zero);
+        for (int c = 32 * turn; c < mma_n; c += 64) emit(c, zero);
         continue;
       }
       const bool odd = (local_tile & 1) != 0;
@@ -320,22 +323,24 @@ gemm_grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
       }
       ++local_tile;
       tc_fence_after_sync();
-      // the 32 columns both windows share first: with them in registers the next tile's MMAs may start
+      // The 32 columns both windows share (the last of an even window, the first of an odd one) are read first by the
+      // warps whose turn they are; with them in registers the next tile's MMAs may start.  All warps signal, and only
+      // after they have seen this tile accumulated, so that no signal can count for the tile before it.
       static_assert(TP::kOverlapChunks == 1, "one shared chunk");
       const int shared0 = odd ? 0 : TP::kAccWindow1;
-      uint32_t held[32];
-      if (shared0 < mma_n) {
-        tmem_ld_32x32(tacc + shared0, held);
+      const bool holder = turn == (odd ? 0 : 1) && shared0 < mma_n;
+      uint32_t r[32];
+      if (holder) {
+        tmem_ld_32x32(tacc + shared0, r);
         tmem_ld_wait();
+        tc_fence_before_sync();
+        __syncwarp();
       }
-      tc_fence_before_sync();
-      __syncwarp();
       if (lane == 0) mbar_arrive_cluster(overlap_addr);
-      if (shared0 < mma_n) emit(shared0, held);
+      if (holder) emit(shared0, r);
 #pragma unroll 1
-      for (int c = 0; c < mma_n; c += 32) {
+      for (int c = 32 * turn; c < mma_n; c += 64) {
         if (c == shared0) continue;
-        uint32_t r[32];
         tmem_ld_32x32(tacc + c, r);
         tmem_ld_wait();
         emit(c, r);

@@ -79,7 +79,7 @@ int launch_grouped(GroupedGemmParams p, const Operand& a, const Operand& b, int6
   if (e != cudaSuccess) return fail_cuda(e, "cudaFuncSetAttribute(grouped gemm)");
   const int64_t max_pairs = sm_count() / 2;
   const int pairs = static_cast<int>(most < max_pairs ? most : max_pairs);
-  e = launch_dependent(gemm_grouped_pair_kernel, 2 * pairs, kGemmThreads, P::kSmemBytes, stream, true, map_a, maps_b, map_sfa,
+  e = launch_dependent(gemm_grouped_pair_kernel, 2 * pairs, kGroupedThreads, P::kSmemBytes, stream, true, map_a, maps_b, map_sfa,
                        map_sfb, map_out, p);
   if (e != cudaSuccess) return fail_cuda(e, "gemm_grouped_pair_kernel launch");
   return RTXB_OK;

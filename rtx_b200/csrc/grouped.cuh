@@ -176,10 +176,10 @@ __device__ __forceinline__ void load_block32(const __nv_bfloat16* src, int valid
           : "=r"(w[8 * h]), "=r"(w[8 * h + 1]), "=r"(w[8 * h + 2]), "=r"(w[8 * h + 3]), "=r"(w[8 * h + 4]),
             "=r"(w[8 * h + 5]), "=r"(w[8 * h + 6]), "=r"(w[8 * h + 7])
           : "l"(src + 16 * h));
-  } else if (valid >= 32 && align == 1) {
+  } else if (align != 0 && (valid >= 32 || valid % 8 == 0)) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const uint4 v = __ldg(reinterpret_cast<const uint4*>(src) + j);
+      const uint4 v = 8 * j < valid ? __ldg(reinterpret_cast<const uint4*>(src) + j) : make_uint4(0, 0, 0, 0);
       w[4 * j] = v.x; w[4 * j + 1] = v.y; w[4 * j + 2] = v.z; w[4 * j + 3] = v.w;
     }
   } else {

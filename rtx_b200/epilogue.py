@@ -126,7 +126,7 @@ def _train_backward(ctx, grad_y, _grad_z):
     if not (need_dx or need_dw or need_db):
         return None, None, None, grad_y if need_dr else None, None
     x, weight, z = ctx.saved_tensors
-    dx, dw, db = mxfp8_linear_epilogue_bwd(grad_y, z, x, weight, ctx.activation, need_dx, need_dw, need_db)
+    dx, dw, db = mxfp8_linear_epilogue_bwd.direct(grad_y, z, x, weight, ctx.activation, need_dx, need_dw, need_db)
     return (dx if need_dx else None, dw if need_dw else None, db if need_db else None, grad_y if need_dr else None, None)
 
 
@@ -138,7 +138,7 @@ class _LinearEpilogueFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, residual, activation):
-        y, z = mxfp8_linear_epilogue_fwd(x, weight, bias, residual, activation)
+        y, z = mxfp8_linear_epilogue_fwd.direct(x, weight, bias, residual, activation)
         ctx.save_for_backward(x, weight, z)
         ctx.activation = activation
         return y
@@ -176,9 +176,9 @@ def mxfp8_linear_epilogue(x: torch.Tensor, weight, bias: Optional[torch.Tensor] 
     if isinstance(weight, MXFP8Tensor):
         if _needs_grad(x, bias, residual):
             raise RuntimeError("a prequantized MXFP8 weight is inference-only; keep the BF16 master weight to train")
-        y = mxfp8_linear_epilogue_prequant_w(x, *mxfp8_kernel_operands(weight), bias, residual, n, k, activation)
+        y = mxfp8_linear_epilogue_prequant_w.direct(x, *mxfp8_kernel_operands(weight), bias, residual, n, k, activation)
     elif not _needs_grad(x, weight, bias, residual):
-        y = mxfp8_linear_epilogue_op(x, weight, bias, residual, activation)
+        y = mxfp8_linear_epilogue_op.direct(x, weight, bias, residual, activation)
     elif torch.compiler.is_compiling():
         y = mxfp8_linear_epilogue_train(x, weight, bias, residual, activation)[0]
     else:
@@ -195,8 +195,8 @@ def mxfp8_linear_epilogue_backward(grad_output: torch.Tensor, z: Optional[torch.
     if activation != "none" and z is None:
         raise ValueError("an activation's backward needs the pre-activation z")
     z2d = z.reshape(-1, n).contiguous() if z is not None and activation != "none" else grad_output.new_empty(0)
-    dx, dw, db = mxfp8_linear_epilogue_bwd(grad_output.reshape(-1, n), z2d, x.reshape(-1, k), weight, activation, True, True,
-                                           bias)
+    dx, dw, db = mxfp8_linear_epilogue_bwd.direct(grad_output.reshape(-1, n), z2d, x.reshape(-1, k), weight, activation,
+                                                  True, True, bias)
     return dx.reshape(x.shape), dw, db if bias else None
 
 

@@ -131,11 +131,11 @@ def _train_backward(ctx, grad_output):
     x, weight, offsets = ctx.saved_tensors
     need_dx, need_dw = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
     if need_dx and need_dw:
-        return (*mxfp8_grouped_linear_bwd(grad_output, x, weight, offsets), None)
+        return (*mxfp8_grouped_linear_bwd.direct(grad_output, x, weight, offsets), None)
     if need_dx:
-        return mxfp8_grouped_linear_dx(grad_output, x, weight, offsets), None, None
+        return mxfp8_grouped_linear_dx.direct(grad_output, x, weight, offsets), None, None
     if need_dw:
-        return None, mxfp8_grouped_linear_dw(grad_output, x, weight, offsets), None
+        return None, mxfp8_grouped_linear_dw.direct(grad_output, x, weight, offsets), None
     return None, None, None
 
 
@@ -149,7 +149,7 @@ class _GroupedLinearFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, offsets):
         ctx.save_for_backward(x, weight, offsets)
-        return mxfp8_grouped_linear_op(x, weight, offsets)
+        return mxfp8_grouped_linear_op.direct(x, weight, offsets)
 
     backward = staticmethod(once_differentiable(_train_backward))
 
@@ -180,7 +180,7 @@ def mxfp8_grouped_linear(x: torch.Tensor, weight, offsets: torch.Tensor) -> torc
             raise ValueError(f"offsets must be a contiguous vector of groups + 1 = {groups + 1} row numbers")
         if x.requires_grad and torch.is_grad_enabled():
             raise RuntimeError("a prequantized MXFP8 weight is inference-only; keep the BF16 master weight to train")
-        return mxfp8_grouped_linear_prequant_w(x, *mxfp8_kernel_operands(weight), offsets, n)
+        return mxfp8_grouped_linear_prequant_w.direct(x, *mxfp8_kernel_operands(weight), offsets, n)
     return _dynamic(x, weight, offsets)
 
 
@@ -189,14 +189,14 @@ def _dynamic(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor) -> to
         if torch.compiler.is_compiling():
             return mxfp8_grouped_linear_train(x, weight, offsets)
         return _GroupedLinearFunction.apply(x, weight, offsets)
-    return mxfp8_grouped_linear_op(x, weight, offsets)
+    return mxfp8_grouped_linear_op.direct(x, weight, offsets)
 
 
 def mxfp8_grouped_linear_backward(grad_output: torch.Tensor, x: torch.Tensor, weight: torch.Tensor,
                                   offsets: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """BF16 dX [rows, K] and dW [groups, N, K] of `mxfp8_grouped_linear`, from independently quantized MXFP8 products
     (blocks along N for dX, along each group's rows for dW)."""
-    return mxfp8_grouped_linear_bwd(grad_output, x, weight, offsets)
+    return mxfp8_grouped_linear_bwd.direct(grad_output, x, weight, offsets)
 
 
 class MXFP8GroupedLinear(nn.Module):
@@ -261,7 +261,7 @@ class MXFP8GroupedLinear(nn.Module):
         if self.weight_mode == "prequantized":
             if x.requires_grad and torch.is_grad_enabled():
                 raise RuntimeError("a prequantized MXFP8 weight is inference-only; keep the BF16 master weight to train")
-            return mxfp8_grouped_linear_prequant_w(x, self.weight_data, self.weight_scales, offsets, self.out_features)
+            return mxfp8_grouped_linear_prequant_w.direct(x, self.weight_data, self.weight_scales, offsets, self.out_features)
         return _dynamic(x, self.weight, offsets)
 
 
