@@ -14,8 +14,17 @@ int launch_quantize_rows(RowsParams& p, int64_t x_tiles, int64_t k, int rounding
   p.lanes = 4;
   while (p.lanes < 32 && p.lanes < p.kp / 32) p.lanes *= 2;
   p.round_to_infinity = rounding != RTXB_ROUND_FLOOR;
-  const int64_t w_tiles = p.w.src ? static_cast<int64_t>(p.batches) * ((p.w.rows + 127) / 128) : 0;
-  const int64_t units = (x_tiles + w_tiles) * p.lanes * ((4 * p.chunks + p.lanes - 1) / p.lanes);
+  p.stacked = 32 / p.lanes;
+  p.segs = (4 * p.chunks + p.lanes - 1) / p.lanes;
+  p.per_tile = p.lanes * p.segs;
+  p.w_row_tiles = (p.w.rows + 127) / 128;
+  for (RowsOperand* o : {&p.x, &p.w}) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(o->src) | static_cast<uintptr_t>(o->ld * 2);
+    o->align = a % 32 == 0 ? 2 : a % 16 == 0 ? 1 : 0;
+  }
+  const int64_t w_tiles = p.w.src ? static_cast<int64_t>(p.batches) * p.w_row_tiles : 0;
+  const int64_t units = (x_tiles + w_tiles) * p.per_tile;
+  if (units > INT32_MAX) return fail_msg(RTXB_E_UNSUPPORTED, "operand exceeds the 32-bit unit count of the quantizer");
   quant_mxfp8_rows_units_kernel<<<quant_grid((units + 7) / 8, kRowsOccupancy), kQuantThreads, 0, stream>>>(p);
   RTXB_CHECK_LAUNCH("quant_mxfp8_rows_units_kernel");
   return RTXB_OK;

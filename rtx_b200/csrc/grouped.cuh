@@ -252,44 +252,36 @@ __global__ void __launch_bounds__(kQuantThreads, kRowsOccupancy) quant_mxfp8_row
     zero_rows_of_no_group(p.list, scan, p.out, p.out_cols, p.ldo);
   }
   const int lane = threadIdx.x & 31;
-  const int segs = (4 * p.chunks + p.lanes - 1) / p.lanes;   // units side by side along a row
-  const int stacked = 32 / p.lanes;                          // row numbers r that share a warp
-  const int per_tile = p.lanes * segs;                       // units of one 128-row tile: 32 / stacked row numbers x segs
-  const int64_t x_units = static_cast<int64_t>(grouped ? scan.tile[p.list.groups] : (p.x.rows + 127) / 128) * per_tile;
-  const int w_row_tiles = (p.w.rows + 127) / 128;
-  const int64_t units = x_units + (p.w.src ? static_cast<int64_t>(p.batches) * w_row_tiles * per_tile : 0);
-  auto alignment = [](const RowsOperand& o) {
-    const uintptr_t a = reinterpret_cast<uintptr_t>(o.src) | static_cast<uintptr_t>(o.ld * 2);
-    return a % 32 == 0 ? 2 : a % 16 == 0 ? 1 : 0;
-  };
-  const int align_x = alignment(p.x), align_w = alignment(p.w);
-  const int warps = gridDim.x * (kQuantThreads / 32);
-  for (int64_t u = blockIdx.x * (kQuantThreads / 32) + (threadIdx.x >> 5); u < units; u += warps) {
+  const uint32_t x_units = (grouped ? scan.tile[p.list.groups] : (p.x.rows + 127) / 128) * p.per_tile;
+  const uint32_t units = x_units + (p.w.src ? p.batches * p.w_row_tiles * p.per_tile : 0u);   // < 2^31, checked by the host
+  const uint32_t warps = gridDim.x * (kQuantThreads / 32);
+  for (uint32_t u = blockIdx.x * (kQuantThreads / 32) + (threadIdx.x >> 5); u < units; u += warps) {
     const bool is_x = u < x_units;
-    const int64_t v = is_x ? u : u - x_units;
-    const int64_t rt = v / per_tile;                         // 128-row tile (of all matrices)
-    const int in_tile = static_cast<int>(v - rt * per_tile);
-    const int r = in_tile / segs * stacked + lane / p.lanes;
-    const int b = in_tile % segs * p.lanes + lane % p.lanes;
+    const uint32_t v = is_x ? u : u - x_units;
+    const uint32_t rt = v / p.per_tile;                      // 128-row tile (of all matrices)
+    const uint32_t in_tile = v - rt * p.per_tile;
+    const uint32_t first_r = in_tile / p.segs * p.stacked;
+    const int r = first_r + lane / p.lanes;
+    const int b = in_tile % p.segs * p.lanes + lane % p.lanes;
     int64_t row0;
     int rows;
     if (!is_x) {
-      const int64_t e = rt / w_row_tiles;
-      const int first = static_cast<int>(rt - e * w_row_tiles) * 128;
-      row0 = e * p.w.rows + first;
+      const uint32_t e = rt / p.w_row_tiles;
+      const int first = (rt - e * p.w_row_tiles) * 128;
+      row0 = static_cast<int64_t>(e) * p.w.rows + first;
       rows = min(128, p.w.rows - first);
     } else if (grouped) {
-      const int g = group_before(scan.tile, p.list.groups, static_cast<int>(rt));
-      row0 = scan.start[g] + 128 * (rt - scan.tile[g]);
+      const int g = group_before(scan.tile, p.list.groups, rt);
+      row0 = scan.start[g] + 128ll * (rt - scan.tile[g]);
       rows = min(128, scan.start[g + 1] - static_cast<int>(row0));
     } else {
-      row0 = 128 * rt;
-      rows = static_cast<int>(min(int64_t(128), p.x.rows - row0));
+      row0 = 128ll * rt;
+      rows = min(128, p.x.rows - static_cast<int>(row0));
     }
-    if (in_tile / segs * stacked >= rows) continue;          // warp-uniform: no live row
+    if (static_cast<int>(first_r) >= rows) continue;         // warp-uniform: no live row
     const RowsOperand& o = is_x ? p.x : p.w;
     quant_mxfp8_rows_unit(o, p, o.src + row0 * o.ld, o.q + row0 * p.kp, o.scales + static_cast<size_t>(rt) * p.chunks * 512,
-                          rows, r, b, is_x ? align_x : align_w);
+                          rows, r, b, o.align);
   }
 }
 
@@ -400,27 +392,32 @@ quant_mxfp8_grouped_backward_kernel(const GroupedBackwardParams p) {
   const int x_tiles = p.x.src ? row_tiles * ((p.x.cols + 127) / 128) : 0;
   const int w_tiles = p.w ? (p.n + 127) / 128 * ((p.k + 127) / 128) : 0;   // per matrix
   const int64_t total = static_cast<int64_t>(dy_tiles) + x_tiles + static_cast<int64_t>(p.batches) * w_tiles;
+  // One thread works out where a tile lies (divisions, the search for its group), a step ahead of the fetch; everybody
+  // else reads it: worked out by all 256 it was a fifth of the kernel's instructions.
+  __shared__ BackwardTile place[2];
+  auto locate = [&](int64_t t) {
+    if (t < total) place[(t / gridDim.x) & 1] = backward_tile(p, scan, t, dy_tiles, x_tiles, w_tiles);
+  };
   int buf = 0;
-  BackwardTile b;
   auto fetch = [&](const BackwardTile& f, uint16_t (*dst)[kQtPitch]) {
     const bool vec_ok = (f.f.ld % 8 == 0) && ((reinterpret_cast<uintptr_t>(f.f.src) & 15) == 0);
     quant_mxfp8_t_fetch(f.f, dst, f.row0, 0, vec_ok);
   };
-  if (blockIdx.x < total) {
-    b = backward_tile(p, scan, blockIdx.x, dy_tiles, x_tiles, w_tiles);
-    fetch(b, tiles[0]);
-  }
+  if (threadIdx.x == 0) locate(blockIdx.x);
+  if (threadIdx.x == 32) locate(static_cast<int64_t>(blockIdx.x) + gridDim.x);
+  __syncthreads();
+  if (blockIdx.x < total) fetch(place[0], tiles[0]);
   for (int64_t t = blockIdx.x; t < total; t += gridDim.x) {
     const int64_t tn = t + gridDim.x;
-    BackwardTile next = b;
+    const BackwardTile b = place[buf];
     if (tn < total) {
-      next = backward_tile(p, scan, tn, dy_tiles, x_tiles, w_tiles);
-      fetch(next, tiles[buf ^ 1]);
+      fetch(place[buf ^ 1], tiles[buf ^ 1]);
       cp_async_wait<1>();   // everything but the newest group (the next tile) has landed
     } else {
       cp_async_wait<0>();
     }
-    __syncthreads();
+    __syncthreads();        // (also: everybody has read place[buf])
+    if (threadIdx.x == kQuantThreads - 1) locate(tn + gridDim.x);   // into place[buf], used after this tile's barriers
     uint32_t o[2][8];
     if (b.q_t)
       quant_mxfp8_tile_columns(tiles[buf], tile_scales, o, static_cast<int>(min(b.pitch_t, int64_t(INT32_MAX))), b.f.rows,
@@ -439,7 +436,6 @@ quant_mxfp8_grouped_backward_kernel(const GroupedBackwardParams p) {
                           ((b.f.rows + 31) / 32 + 3) / 4);
     __syncthreads();   // the scale tiles and this buffer are free again
     buf ^= 1;
-    b = next;
   }
 }
 

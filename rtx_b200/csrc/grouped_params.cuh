@@ -25,13 +25,18 @@ struct RowsOperand {
   uint8_t* q;                 // [.., kp], 32-byte aligned
   uint8_t* scales;            // 128-row tiles
   int rows;                   // per matrix (x: all groups)
+  int align;                  // of src and its pitch: 2 = 32 bytes, 1 = 16 bytes, 0 = neither
 };
 struct RowsParams {
   RowsOperand x, w;
   GroupList list;             // offsets nullptr: x is one group of all its rows, no plan, no rows to zero
   int batches;                // matrices of w
   int k, kp, chunks;          // chunks = 512-byte scale tiles per 128 rows
-  int lanes;                  // lanes that share a row: 4, 8, 16 or 32
+  int lanes;                  // lanes that share a row: 4, 8, 16 or 32; then 32 / lanes rows share a warp
+  int stacked;
+  int segs;                   // units side by side along a row
+  int per_tile;               // units of one 128-row tile
+  int w_row_tiles;            // 128-row tiles of one matrix of w
   int round_to_infinity;
   GroupPlan plan;
   __nv_bfloat16* out;         // result whose rows of no group become zero

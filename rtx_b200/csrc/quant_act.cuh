@@ -96,9 +96,12 @@ __global__ void __launch_bounds__(kQuantThreads, kActOccupancy) quant_mxfp8_act_
   const bool vec_z = (p.n % 8 == 0) && ((reinterpret_cast<uintptr_t>(p.z) & 15) == 0);   // true without z
   const int c8 = (threadIdx.x & 15) * 8, r0 = threadIdx.x >> 4;
   const int64_t total = static_cast<int64_t>(row_tiles) * col_tiles;
-  for (int64_t t = blockIdx.x; t < total; t += gridDim.x) {
-    const int rt = static_cast<int>(t / col_tiles);
-    const int row0 = rt * 128, col0 = static_cast<int>(t - static_cast<int64_t>(rt) * col_tiles) * 128;
+  // tile (rt, ct); the grid's stride in both, so that no tile costs a division
+  int rt = blockIdx.x / col_tiles, ct = blockIdx.x - rt * col_tiles;
+  const int step_r = gridDim.x / col_tiles, step_c = gridDim.x - step_r * col_tiles;
+  for (int64_t t = blockIdx.x; t < total; t += gridDim.x, rt += step_r, ct += step_c) {
+    if (ct >= col_tiles) { ct -= col_tiles; ++rt; }
+    const int row0 = rt * 128, col0 = ct * 128;
     const int col = col0 + c8;
     f32x2 sum[4];
 #pragma unroll
