@@ -1003,33 +1003,20 @@ int rtxb_mxfp8_linear_epilogue_bwd(const void* dy, int64_t lddy, const void* z, 
   if (e != cudaSuccess) return fail_cuda(e, "cudaFuncSetAttribute(activation backward quantizer)");
   kernel<<<quant_grid(tiles, kActOccupancy), kQuantThreads, kActSmemBytes, s>>>(q);
   RTXB_CHECK_LAUNCH("quant_mxfp8_act_backward_kernel");
-  TransposedPairParams t = {};
-  auto transposed = [](const void* src, int64_t rows, int64_t k_, int64_t ld, uint8_t* q_, uint8_t* scales) {
-    QuantMxTParams p = {};
-    p.src = static_cast<const __nv_bfloat16*>(src);
-    p.q = q_;
-    p.scales = scales;
-    p.rows = static_cast<int>(rows);
-    p.k = static_cast<int>(k_);
-    p.kp = static_cast<int>(round_up(k_, 32));
-    p.ld = ld;
-    p.nb = p.kp / 32;
-    p.sf_chunks = (p.nb + 3) / 4;
-    return p;
-  };
-  if (dx) t.w = transposed(w, k, n, k, mem.q_wt, mem.s_wt);
-  if (dw) t.x = transposed(x, k, m, ldx, mem.q_xt, mem.s_xt);
+  TransposedParams t = {};
+  if (dw)
+    t.x = TransposedOperand{static_cast<const __nv_bfloat16*>(x), ldx, static_cast<int>(m), static_cast<int>(k), mem.q_xt,
+                            round_up(m, 32), mem.s_xt, static_cast<int>(row_tiles)};
+  if (dx) {
+    t.w = TransposedOperand{static_cast<const __nv_bfloat16*>(w), k, static_cast<int>(n), static_cast<int>(k), mem.q_wt,
+                            round_up(n, 32), mem.s_wt, static_cast<int>((n + 127) / 128)};
+    t.batches = 1;
+  }
   t.partial = mem.partial;
   t.row_tiles = static_cast<int>(row_tiles);
   t.n = static_cast<int>(n);
   t.dbias = static_cast<__nv_bfloat16*>(dbias);
-  const int64_t kt = (k + 127) / 128;
-  int64_t work = (dx ? kt * ((n + 127) / 128) : 0) + (dw ? kt * row_tiles : 0);
-  if (dbias && work < (n + 31) / 32) work = (n + 31) / 32;
-  e = ensure_dynamic_smem(reinterpret_cast<const void*>(quant_mxfp8_transposed_pair_kernel), kQtSmemBytes);
-  if (e != cudaSuccess) return fail_cuda(e, "cudaFuncSetAttribute(transposed pair)");
-  e = launch_dependent(quant_mxfp8_transposed_pair_kernel, quant_grid(work, kQtOccupancy), kQuantThreads, kQtSmemBytes, s, true, t);
-  if (e != cudaSuccess) return fail_cuda(e, "quant_mxfp8_transposed_pair_kernel launch");
+  if ((rc = launch_quantize_transposed(t, row_tiles, s))) return rc;
   if (dx && (rc = mxfp8_gemm_impl(mem.q_dz, mem.s_dz, mem.q_wt, mem.s_wt, dx, m, k, n, k, RTXB_OUT_BF16, stream, status, true)))
     return rc;
   if (dw && (rc = mxfp8_gemm_impl(mem.q_dzt, mem.s_dzt, mem.q_xt, mem.s_xt, dw, n, k, m, k, RTXB_OUT_BF16, stream, status, true)))

@@ -30,6 +30,21 @@ int launch_quantize_rows(RowsParams& p, int64_t x_tiles, int64_t k, int rounding
   return RTXB_OK;
 }
 
+int launch_quantize_transposed(TransposedParams& p, int64_t x_tiles, cudaStream_t stream) {
+  p.x_col_units = (p.x.cols + 63) / 64;
+  p.w_col_units = (p.w.cols + 63) / 64;
+  p.w_row_tiles = (p.w.rows + 127) / 128;
+  const int64_t units = (p.x.src ? x_tiles * p.x_col_units : 0) +
+                        (p.w.src ? static_cast<int64_t>(p.batches) * p.w_row_tiles * p.w_col_units : 0);
+  if (units > INT32_MAX) return fail_msg(RTXB_E_UNSUPPORTED, "operand exceeds the 32-bit unit count of the quantizer");
+  int64_t blocks = (units + 7) / 8;
+  if (p.partial && blocks < (p.n + 31) / 32) blocks = (p.n + 31) / 32;
+  const cudaError_t e = launch_dependent(quant_mxfp8_transposed_units_kernel, quant_grid(blocks, kTransposedOccupancy),
+                                         kQuantThreads, 0, stream, true, p);
+  if (e != cudaSuccess) return fail_cuda(e, "quant_mxfp8_transposed_units_kernel launch");
+  return RTXB_OK;
+}
+
 }  // namespace rtxb
 
 namespace {
@@ -266,29 +281,36 @@ int rtxb_mxfp8_grouped_linear_bwd(const void* dy, int64_t lddy, const void* x, i
   if (!aligned(workspace, 256)) return fail_msg(RTXB_E_ALIGNMENT, "workspace must be 256-byte aligned");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int64_t tiles128 = most_tiles(rows, groups, 128), nt = (n + 127) / 128, kt = (k + 127) / 128;
-  GroupedBackwardParams q = {};
-  q.list = GroupList{offsets, static_cast<int>(groups), static_cast<int>(rows)};
-  q.dy = GroupedSource{static_cast<const __nv_bfloat16*>(dy), static_cast<int>(n), lddy, mem.q_dy, mem.s_dy, mem.q_dyt, mem.s_dyt};
-  if (dw) q.x = GroupedSource{static_cast<const __nv_bfloat16*>(x), static_cast<int>(k), ldx, nullptr, nullptr, mem.q_xt, mem.s_xt};
+  GroupedGradientParams q = {};
+  q.src = static_cast<const __nv_bfloat16*>(dy);
+  q.cols = static_cast<int>(n);
+  q.ld = lddy;
+  q.q_rows = mem.q_dy;
+  q.s_rows = mem.s_dy;
+  q.q_t = mem.q_dyt;
+  q.s_t = mem.s_dyt;
   q.pitch_t = tiles128 * 128;
   q.chunks_t = static_cast<int>(tiles128);
-  q.n = static_cast<int>(n);
-  q.k = static_cast<int>(k);
-  if (dx) {
-    q.w = static_cast<const __nv_bfloat16*>(w);
-    q.q_wt = mem.q_wt;
-    q.s_wt = mem.s_wt;
-    q.batches = static_cast<int>(groups);
-    q.dx = static_cast<__nv_bfloat16*>(dx);
-    q.lddx = k;
-  }
+  q.list = GroupList{offsets, static_cast<int>(groups), static_cast<int>(rows)};
   q.plan = mem.plan.plan;
+  q.dx = static_cast<__nv_bfloat16*>(dx);
+  q.dx_cols = static_cast<int>(k);
   q.status = status;
-  const int64_t tiles = tiles128 * nt + (dw ? tiles128 * kt : 0) + (dx ? groups * nt * kt : 0);
-  cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(quant_mxfp8_grouped_backward_kernel), kQtSmemBytes);
-  if (e != cudaSuccess) return fail_cuda(e, "cudaFuncSetAttribute(grouped backward quantizer)");
-  quant_mxfp8_grouped_backward_kernel<<<quant_grid(tiles, kQtOccupancy), kQuantThreads, kQtSmemBytes, s>>>(q);
-  RTXB_CHECK_LAUNCH("quant_mxfp8_grouped_backward_kernel");
+  cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(quant_mxfp8_grouped_gradient_kernel), kQtSmemBytes);
+  if (e != cudaSuccess) return fail_cuda(e, "cudaFuncSetAttribute(grouped gradient quantizer)");
+  quant_mxfp8_grouped_gradient_kernel<<<quant_grid(tiles128 * nt, kQtOccupancy), kQuantThreads, kQtSmemBytes, s>>>(q);
+  RTXB_CHECK_LAUNCH("quant_mxfp8_grouped_gradient_kernel");
+  TransposedParams t = {};
+  t.list = q.list;
+  if (dw)
+    t.x = TransposedOperand{static_cast<const __nv_bfloat16*>(x), ldx, static_cast<int>(rows), static_cast<int>(k), mem.q_xt,
+                            q.pitch_t, mem.s_xt, q.chunks_t};
+  if (dx) {
+    t.w = TransposedOperand{static_cast<const __nv_bfloat16*>(w), k, static_cast<int>(n), static_cast<int>(k), mem.q_wt,
+                            round_up(n, 32), mem.s_wt, static_cast<int>(nt)};
+    t.batches = static_cast<int>(groups);
+  }
+  if ((rc = launch_quantize_transposed(t, tiles128, s))) return rc;
   if (dx && (rc = launch_rows_form(mem.plan.plan, mem.q_dy, mem.s_dy, rows, mem.q_wt, mem.s_wt, k, n, groups, dx, k, status, s)))
     return rc;
   if (dw) {

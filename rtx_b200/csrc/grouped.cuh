@@ -286,97 +286,154 @@ __global__ void __launch_bounds__(kQuantThreads, kRowsOccupancy) quant_mxfp8_row
 }
 
 // ---------------------------------------------------------------------------
-// Backward operands in one launch, all walked as 128 x 128 tiles of their source:
-//   dy   by group: rows (blocks along n, for dX) and transposed (blocks along the tokens, for dW), one read;
-//   x    by group: transposed (for dW);
-//   w    `batches` matrices [n, k]: transposed (blocks along n, for dX), each with scale tiles of its own.
-// A null destination leaves that product out.
+// Transposed quantizer of the backward's operands that are quantized one way only: x (by group, for dW) and the weight
+// matrices (for dX).  One lane owns two neighbouring columns and walks down 32 rows at a time: the block is in its
+// registers, so there is no staging, no exchange and no barrier.  A warp reads 128-byte row segments, 32 of them in
+// flight, and writes 32-byte sectors, four next to one another per column (128 rows = one K step of the GEMM).
 // ---------------------------------------------------------------------------
-struct GroupedSource {
-  const __nv_bfloat16* src;   // nullptr = absent
+constexpr int kTransposedOccupancy = 3;
+
+// 64 columns from `col0` of a 128-row tile with `live` rows; payload bytes [k0, k0 + 128) of each column
+__device__ __forceinline__ void quant_mxfp8_transposed_unit(const TransposedOperand& o, const __nv_bfloat16* src, int live,
+                                                            uint8_t* q, uint8_t* scales, int64_t k0, int chunk, int col0) {
+  const int lane = threadIdx.x & 31;
+  const int c = col0 + 2 * lane;
+  const bool ok0 = c < o.cols, ok1 = c + 1 < o.cols;
+  const bool pairs = (o.ld & 1) == 0 && (reinterpret_cast<uintptr_t>(o.src) & 3) == 0;   // both columns in one load
+  const uint16_t* at = reinterpret_cast<const uint16_t*>(src) + c;
+  uint32_t word0 = 0, word1 = 0;   // the four scale bytes of either column
+#pragma unroll 1
+  for (int j = 0; j < 4; ++j) {
+    if (k0 + 32 * j >= o.pitch) break;
+    uint32_t w[32];
+    if (pairs && 32 * j + 32 <= live && ok1) {
+#pragma unroll
+      for (int e = 0; e < 32; ++e) w[e] = __ldg(reinterpret_cast<const uint32_t*>(at + e * o.ld));
+    } else {
+#pragma unroll
+      for (int e = 0; e < 32; ++e) {
+        const bool row = 32 * j + e < live;
+        const uint32_t a = row && ok0 ? at[e * o.ld] : 0u, b = row && ok1 ? at[e * o.ld + 1] : 0u;
+        w[e] = a | (b << 16);
+      }
+    }
+    at += 32 * o.ld;
+    uint32_t m2 = 0;
+#pragma unroll
+    for (int e = 0; e < 32; ++e) m2 = absmax_bf16x2(m2, w[e]);
+    const uint32_t code0 = e8m0_from_amax(bf16_lo(m2), true), code1 = e8m0_from_amax(bf16_hi(m2), true);
+    const f32x2 recip = pack2(e8m0_reciprocal(code0), e8m0_reciprocal(code1));
+    word0 |= code0 << (8 * j);
+    word1 |= code1 << (8 * j);
+    uint32_t o0[8], o1[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      f32x2 v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = mul2(unpack_bf16x2(w[4 * e + i]), recip);
+      o0[e] = cvt_e4m3x2(lo(v[0]), lo(v[1])) | (cvt_e4m3x2(lo(v[2]), lo(v[3])) << 16);
+      o1[e] = cvt_e4m3x2(hi(v[0]), hi(v[1])) | (cvt_e4m3x2(hi(v[2]), hi(v[3])) << 16);
+    }
+    uint8_t* dst = q + c * o.pitch + k0 + 32 * j;
+    if (ok0)
+      asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(o0[0]), "r"(o0[1]), "r"(o0[2]),
+                   "r"(o0[3]), "r"(o0[4]), "r"(o0[5]), "r"(o0[6]), "r"(o0[7])
+                   : "memory");
+    if (ok1)
+      asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst + o.pitch), "r"(o1[0]), "r"(o1[1]),
+                   "r"(o1[2]), "r"(o1[3]), "r"(o1[4]), "r"(o1[5]), "r"(o1[6]), "r"(o1[7])
+                   : "memory");
+  }
+  uint8_t* tile = scales + (static_cast<size_t>(c >> 7) * o.chunks + chunk) * 512;   // c is even: both columns in one tile
+  if (ok0) *reinterpret_cast<uint32_t*>(tile + (c & 31) * 16 + ((c >> 5) & 3) * 4) = word0;
+  if (ok1) *reinterpret_cast<uint32_t*>(tile + ((c + 1) & 31) * 16 + ((c >> 5) & 3) * 4) = word1;
+}
+
+__global__ void __launch_bounds__(kQuantThreads, kTransposedOccupancy)
+quant_mxfp8_transposed_units_kernel(const TransposedParams p) {
+  __shared__ GroupScan scan;
+  __shared__ float part[8][33];
+  griddep_launch_dependents();
+  const bool grouped = p.list.offsets != nullptr;
+  if (grouped && p.x.src) scan_groups(p.list, scan, nullptr);
+  const uint32_t x_tiles = !p.x.src ? 0 : grouped ? scan.tile[p.list.groups] : (p.x.rows + 127) / 128;
+  const uint32_t x_units = x_tiles * p.x_col_units;
+  const uint32_t units = x_units + (p.w.src ? p.batches * p.w_row_tiles * p.w_col_units : 0u);   // < 2^31 (host)
+  for (uint32_t u = blockIdx.x * (kQuantThreads / 32) + (threadIdx.x >> 5); u < units;
+       u += gridDim.x * (kQuantThreads / 32)) {
+    if (u < x_units) {
+      const uint32_t rt = u / p.x_col_units;
+      int64_t row0 = 128ll * rt;
+      int live = p.x.rows - static_cast<int>(row0);
+      if (grouped) {
+        const int g = group_before(scan.tile, p.list.groups, rt);
+        row0 = scan.start[g] + 128ll * (rt - scan.tile[g]);
+        live = scan.start[g + 1] - static_cast<int>(row0);
+      }
+      quant_mxfp8_transposed_unit(p.x, p.x.src + row0 * p.x.ld, min(128, live), p.x.q, p.x.scales, 128ll * rt, rt,
+                                  (u - rt * p.x_col_units) * 64);
+    } else {
+      const uint32_t v = u - x_units;
+      const uint32_t rt = v / p.w_col_units;
+      const uint32_t e = rt / p.w_row_tiles;
+      const uint32_t nt = rt - e * p.w_row_tiles;
+      const TransposedOperand& o = p.w;
+      quant_mxfp8_transposed_unit(o, o.src + (static_cast<int64_t>(e) * o.rows + 128 * nt) * o.ld,
+                                  min(128, o.rows - static_cast<int>(128 * nt)), o.q + e * (o.cols * o.pitch),
+                                  o.scales + static_cast<size_t>(e) * ((o.cols + 127) / 128) * o.chunks * 512, 128ll * nt, nt,
+                                  (v - rt * p.w_col_units) * 64);
+    }
+  }
+  griddep_wait();   // the launch before this one is complete: whoever waits for this grid has waited for that one too
+  if (p.partial == nullptr) return;
+  // dbias[c] = bf16( sum over the row tiles of partial[t][c] ): eight threads per column add every eighth tile, the eight
+  // sums are added in a fixed order
+  const int lane = threadIdx.x & 31, k = threadIdx.x >> 5;
+  for (int c = blockIdx.x; c < (p.n + 31) / 32; c += gridDim.x) {
+    const int col = c * 32 + lane;
+    float s = 0.0f;
+    if (col < p.n)
+      for (int t = k; t < p.row_tiles; t += 8) s += __ldcg(p.partial + static_cast<int64_t>(t) * p.n + col);
+    part[k][lane] = s;
+    __syncthreads();
+    if (k == 0 && col < p.n) {
+#pragma unroll
+      for (int i = 1; i < 8; ++i) s += part[i][lane];
+      p.dbias[col] = __float2bfloat16_rn(s);
+    }
+    __syncthreads();
+  }
+}
+
+// ---------------------------------------------------------------------------
+// The gradient operand dy by group, walked as 128 x 128 tiles: rows (blocks along n, for dX) and transposed (blocks along
+// the tokens, for dW) from one staged read.  A null destination leaves that product out.
+// ---------------------------------------------------------------------------
+struct GroupedGradientParams {
+  const __nv_bfloat16* src;
   int cols;
   int64_t ld;
   uint8_t* q_rows;            // [rows, round_up(cols, 32)]
-  uint8_t* s_rows;
+  uint8_t* s_rows;            // 128-row tiles counted per group
   uint8_t* q_t;               // [cols, pitch_t]
   uint8_t* s_t;               // [ceil(cols / 128)][chunks_t][512]
-};
-struct GroupedBackwardParams {
-  GroupedSource dy, x;
-  GroupList list;
   int64_t pitch_t;            // 128 * (most tiles the list can have)
   int chunks_t;               // pitch_t / 128
-  const __nv_bfloat16* w;     // nullptr = absent
-  uint8_t* q_wt;              // [batches][k, round_up(n, 32)]
-  uint8_t* s_wt;
-  int batches, n, k;
+  GroupList list;
   GroupPlan plan;
   __nv_bfloat16* dx;          // result whose rows of no group become zero; nullptr = none
-  int64_t lddx;
+  int dx_cols;
   int* status;
 };
 
-// one tile: where it is read and where its two quantizations go
-struct BackwardTile {
-  QuantMxTParams f;           // what the fetch needs (src, rows = source columns, k = live source rows, ld)
-  int row0;                   // first source column
-  uint8_t* q_t;
-  uint8_t* s_t;
-  int64_t pitch_t;            // payload pitch and limit of q_t
-  int k0, chunks_t, blk0;
-  uint8_t* q_rows;
-  uint8_t* s_rows;
+// where a tile lies: first row and live rows, first column, its 128-row tile number
+struct GradientTile {
+  int64_t row0;
+  int live, col0, rt;
 };
 
-__device__ __forceinline__ BackwardTile backward_tile(const GroupedBackwardParams& p, const GroupScan& scan, int64_t t,
-                                                      int dy_tiles, int x_tiles, int w_tiles) {
-  BackwardTile b;
-  if (t < dy_tiles + static_cast<int64_t>(x_tiles)) {
-    const bool is_x = t >= dy_tiles;
-    const GroupedSource& s = is_x ? p.x : p.dy;
-    const int u = static_cast<int>(is_x ? t - dy_tiles : t);
-    const int ct = (s.cols + 127) / 128;
-    const int rt = u / ct;
-    const int g = group_before(scan.tile, p.list.groups, rt);
-    const int64_t first = scan.start[g] + 128 * (rt - scan.tile[g]);
-    const int chunks_rows = ((s.cols + 31) / 32 + 3) / 4, np = (s.cols + 31) / 32 * 32;
-    b.row0 = (u - rt * ct) * 128;
-    b.f.src = s.src + first * s.ld;
-    b.f.rows = s.cols;
-    b.f.k = min(128, scan.start[g + 1] - static_cast<int>(first));
-    b.f.ld = s.ld;
-    b.q_t = s.q_t ? s.q_t + static_cast<int64_t>(rt) * 128 : nullptr;
-    b.s_t = s.s_t;
-    b.pitch_t = p.pitch_t;
-    b.k0 = 0;
-    b.chunks_t = p.chunks_t;
-    b.blk0 = rt * 4;
-    b.q_rows = s.q_rows ? s.q_rows + first * np : nullptr;
-    b.s_rows = s.q_rows ? s.s_rows + static_cast<size_t>(rt) * chunks_rows * 512 : nullptr;
-  } else {
-    const int64_t u = t - dy_tiles - x_tiles;
-    const int64_t e = u / w_tiles;
-    const int v = static_cast<int>(u - e * w_tiles);
-    const int ct = (p.k + 127) / 128, np = (p.n + 31) / 32 * 32;
-    const int nt = v / ct;
-    b.row0 = (v - nt * ct) * 128;
-    b.f.src = p.w + (e * p.n + 128 * nt) * p.k;
-    b.f.rows = p.k;
-    b.f.k = min(128, p.n - 128 * nt);
-    b.f.ld = p.k;
-    b.q_t = p.q_wt + e * p.k * np;
-    b.pitch_t = np;
-    b.k0 = 128 * nt;
-    b.chunks_t = (np / 32 + 3) / 4;
-    b.s_t = p.s_wt + static_cast<size_t>(e) * ct * b.chunks_t * 512;
-    b.blk0 = nt * 4;
-    b.q_rows = b.s_rows = nullptr;
-  }
-  return b;
-}
-
 __global__ void __launch_bounds__(kQuantThreads, kQtOccupancy)
-quant_mxfp8_grouped_backward_kernel(const GroupedBackwardParams p) {
+quant_mxfp8_grouped_gradient_kernel(const GroupedGradientParams p) {
   extern __shared__ __align__(16) uint8_t qt_smem[];
   uint16_t (*tiles[2])[kQtPitch] = {reinterpret_cast<uint16_t (*)[kQtPitch]>(qt_smem),
                                     reinterpret_cast<uint16_t (*)[kQtPitch]>(qt_smem + kQtTileBytes)};
@@ -386,54 +443,57 @@ quant_mxfp8_grouped_backward_kernel(const GroupedBackwardParams p) {
   griddep_launch_dependents();
   scan_groups(p.list, scan, p.status);
   if (blockIdx.x == 0) write_group_plan(p.list, scan, p.plan, reinterpret_cast<int*>(qt_smem));
-  if (p.dx) zero_rows_of_no_group(p.list, scan, p.dx, p.k, p.lddx);
-  const int row_tiles = scan.tile[p.list.groups];
-  const int dy_tiles = row_tiles * ((p.dy.cols + 127) / 128);
-  const int x_tiles = p.x.src ? row_tiles * ((p.x.cols + 127) / 128) : 0;
-  const int w_tiles = p.w ? (p.n + 127) / 128 * ((p.k + 127) / 128) : 0;   // per matrix
-  const int64_t total = static_cast<int64_t>(dy_tiles) + x_tiles + static_cast<int64_t>(p.batches) * w_tiles;
-  // One thread works out where a tile lies (divisions, the search for its group), a step ahead of the fetch; everybody
-  // else reads it: worked out by all 256 it was a fifth of the kernel's instructions.
-  __shared__ BackwardTile place[2];
-  auto locate = [&](int64_t t) {
-    if (t < total) place[(t / gridDim.x) & 1] = backward_tile(p, scan, t, dy_tiles, x_tiles, w_tiles);
+  if (p.dx) zero_rows_of_no_group(p.list, scan, p.dx, p.dx_cols, p.dx_cols);
+  const int col_tiles = (p.cols + 127) / 128;
+  const int total = scan.tile[p.list.groups] * col_tiles;   // < 2^31 (host)
+  const int np = (p.cols + 31) / 32 * 32, chunks_rows = (np / 32 + 3) / 4;
+  const bool vec_ok = (p.ld % 8 == 0) && ((reinterpret_cast<uintptr_t>(p.src) & 15) == 0);
+  // One thread works out where a tile lies (a division, the search for its group), a step ahead of the fetch.
+  __shared__ GradientTile place[2];
+  auto locate = [&](int t, int slot) {
+    if (t >= total) return;
+    const int rt = t / col_tiles;
+    const int g = group_before(scan.tile, p.list.groups, rt);
+    const int row0 = scan.start[g] + 128 * (rt - scan.tile[g]);
+    place[slot] = GradientTile{row0, min(128, scan.start[g + 1] - row0), (t - rt * col_tiles) * 128, rt};
   };
-  int buf = 0;
-  auto fetch = [&](const BackwardTile& f, uint16_t (*dst)[kQtPitch]) {
-    const bool vec_ok = (f.f.ld % 8 == 0) && ((reinterpret_cast<uintptr_t>(f.f.src) & 15) == 0);
-    quant_mxfp8_t_fetch(f.f, dst, f.row0, 0, vec_ok);
+  auto fetch = [&](const GradientTile& f, uint16_t (*dst)[kQtPitch]) {
+    QuantMxTParams q;
+    q.src = p.src + f.row0 * p.ld;
+    q.rows = p.cols;
+    q.k = f.live;
+    q.ld = p.ld;
+    quant_mxfp8_t_fetch(q, dst, f.col0, 0, vec_ok);
   };
-  if (threadIdx.x == 0) locate(blockIdx.x);
-  if (threadIdx.x == 32) locate(static_cast<int64_t>(blockIdx.x) + gridDim.x);
+  if (threadIdx.x == 0) locate(blockIdx.x, 0);
+  if (threadIdx.x == 32) locate(blockIdx.x + gridDim.x, 1);
   __syncthreads();
-  if (blockIdx.x < total) fetch(place[0], tiles[0]);
-  for (int64_t t = blockIdx.x; t < total; t += gridDim.x) {
-    const int64_t tn = t + gridDim.x;
-    const BackwardTile b = place[buf];
-    if (tn < total) {
+  int buf = 0;
+  if (static_cast<int>(blockIdx.x) < total) fetch(place[0], tiles[0]);
+  for (int t = blockIdx.x; t < total; t += gridDim.x) {
+    const GradientTile b = place[buf];
+    if (t + static_cast<int>(gridDim.x) < total) {
       fetch(place[buf ^ 1], tiles[buf ^ 1]);
       cp_async_wait<1>();   // everything but the newest group (the next tile) has landed
     } else {
       cp_async_wait<0>();
     }
     __syncthreads();        // (also: everybody has read place[buf])
-    if (threadIdx.x == kQuantThreads - 1) locate(tn + gridDim.x);   // into place[buf], used after this tile's barriers
+    if (threadIdx.x == kQuantThreads - 1) locate(t + 2 * gridDim.x, buf);   // read after this tile's other barriers
     uint32_t o[2][8];
-    if (b.q_t)
-      quant_mxfp8_tile_columns(tiles[buf], tile_scales, o, static_cast<int>(min(b.pitch_t, int64_t(INT32_MAX))), b.f.rows,
-                               b.row0, b.k0, true);
-    if (b.q_rows)
-      quant_mxfp8_tile_rows(tiles[buf], tile_scales_rows, b.q_rows, (b.f.rows + 31) / 32 * 32, b.f.k, b.f.rows, 0, b.row0,
-                            true);
+    if (p.q_t)
+      quant_mxfp8_tile_columns(tiles[buf], tile_scales, o, 128, p.cols, b.col0, 0, true);
+    if (p.q_rows)
+      quant_mxfp8_tile_rows(tiles[buf], tile_scales_rows, p.q_rows + b.row0 * np, np, b.live, p.cols, 0, b.col0, true);
     __syncthreads();   // every thread has read the staged tile: its storage now collects the transposed payload
-    if (b.q_t) {
-      quant_mxfp8_tile_columns_store(reinterpret_cast<uint8_t*>(tiles[buf]), o, b.q_t, static_cast<int>(b.pitch_t), b.f.rows,
-                                     b.row0, b.k0);
-      store_scale_tile<4>(tile_scales, b.s_t, kScaleMma128, b.row0, b.blk0, b.f.rows, 0, b.chunks_t);
+    if (p.q_t) {
+      quant_mxfp8_tile_columns_store(reinterpret_cast<uint8_t*>(tiles[buf]), o, p.q_t + 128ll * b.rt,
+                                     static_cast<int>(p.pitch_t), p.cols, b.col0, 0);
+      store_scale_tile<4>(tile_scales, p.s_t, kScaleMma128, b.col0, b.rt * 4, p.cols, 0, p.chunks_t);
     }
-    if (b.q_rows)
-      store_scale_tile<4>(tile_scales_rows, b.s_rows, kScaleMma128, 0, b.row0 / 32, b.f.k, 0,
-                          ((b.f.rows + 31) / 32 + 3) / 4);
+    if (p.q_rows)
+      store_scale_tile<4>(tile_scales_rows, p.s_rows + static_cast<size_t>(b.rt) * chunks_rows * 512, kScaleMma128, 0,
+                          b.col0 / 32, b.live, 0, chunks_rows);
     __syncthreads();   // the scale tiles and this buffer are free again
     buf ^= 1;
   }

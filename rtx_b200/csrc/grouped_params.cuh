@@ -47,4 +47,28 @@ struct RowsParams {
 // fills in the fields that follow from k and enqueues the quantizer; x_tiles: the most 128-row tiles x can have
 int launch_quantize_rows(RowsParams& p, int64_t x_tiles, int64_t k, int rounding, cudaStream_t stream);   // grouped.cu
 
+// Operand of the transposed quantizer: matrices [rows, cols] quantized in blocks of 32 along their rows, the payload
+// [cols, pitch] K-major per matrix.
+struct TransposedOperand {
+  const __nv_bfloat16* src;   // nullptr = absent
+  int64_t ld;
+  int rows, cols;             // per matrix (x: all groups)
+  uint8_t* q;                 // per matrix [cols, pitch], 32-byte aligned
+  int64_t pitch;              // bytes; also where the payload ends
+  uint8_t* scales;            // per matrix [ceil(cols / 128)][chunks][512]
+  int chunks;
+};
+struct TransposedParams {
+  TransposedOperand x, w;
+  GroupList list;             // offsets nullptr: x is one group of all its rows
+  int batches;                // matrices of w
+  int x_col_units, w_col_units, w_row_tiles;
+  const float* partial;       // column sums [row_tiles][n] left by the launch before this one; nullptr = none
+  int row_tiles, n;
+  __nv_bfloat16* dbias;       // their sum over the row tiles
+};
+// enqueues the transposed quantizer as a programmatic dependent that may run beside the launch before it (none of whose
+// results it reads but `partial`) and ends after that launch has; x_tiles: the most 128-row tiles x can have
+int launch_quantize_transposed(TransposedParams& p, int64_t x_tiles, cudaStream_t stream);   // grouped.cu
+
 }  // namespace rtxb

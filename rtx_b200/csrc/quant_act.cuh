@@ -2,7 +2,7 @@
 //   dz = dy act'(z)                          [m, n], FP32, rounded once to BF16 (the gradient autograd would carry)
 //   q_rows  MXFP8 of dz, blocks along n      (A operand of dX = dz W)
 //   q_t     MXFP8 of dz^T, blocks along m    (A operand of dW = dz^T X)
-//   partial[m / 128][n] = sum of 128 rows of dz in FP32, before the rounding   (dbias, finished by the kernel below)
+//   partial[m / 128][n] = sum of 128 rows of dz in FP32, before the rounding   (dbias, finished by quant_mxfp8_transposed_units_kernel)
 // dy and z are read once (4 bytes per value), 2 bytes of payload leave: without the fusion dz is written and read again
 // (4 more).  One 128 x 128 tile per block step, three blocks per SM
 // overlap one another's loads, arithmetic and stores.
@@ -173,80 +173,6 @@ __global__ void __launch_bounds__(kQuantThreads, kActOccupancy) quant_mxfp8_act_
     if (p.q_rows)
       store_scale_tile<4>(scales_rows, p.s_rows, kScaleMma128, row0, col0 / 32, p.m, np / 32, (np / 32 + 3) / 4);
     __syncthreads();   // the staged tile, the sums and the scale tiles are free again
-  }
-}
-
-// What the two GEMMs of the backward still need, in one launch that may start beside the pass above: W^T and X^T
-// quantized (operands of the caller, nothing of that pass), then, once that pass is complete,
-//   dbias[c] = bf16( sum over the row tiles of partial[t][c] )
-// with eight threads per column that add every eighth tile, the eight sums added in a fixed order.
-struct TransposedPairParams {
-  QuantMxTParams w, x;        // src nullptr = absent
-  const float* partial;       // nullptr = no dbias
-  int row_tiles, n;
-  __nv_bfloat16* dbias;
-};
-
-__global__ void __launch_bounds__(kQuantThreads, kQtOccupancy) quant_mxfp8_transposed_pair_kernel(const TransposedPairParams p) {
-  extern __shared__ __align__(16) uint8_t qt_smem[];
-  uint16_t (*tiles[2])[kQtPitch] = {reinterpret_cast<uint16_t (*)[kQtPitch]>(qt_smem),
-                                    reinterpret_cast<uint16_t (*)[kQtPitch]>(qt_smem + kQtTileBytes)};
-  __shared__ __align__(16) uint8_t tile_scales[128][4];
-  __shared__ float part[8][33];
-  griddep_launch_dependents();
-  const int64_t w_tiles = p.w.src ? static_cast<int64_t>((p.w.rows + 127) / 128) * ((p.w.kp + 127) / 128) : 0;
-  const int64_t total = w_tiles + (p.x.src ? static_cast<int64_t>((p.x.rows + 127) / 128) * ((p.x.kp + 127) / 128) : 0);
-  auto operand = [&](int64_t t) -> const QuantMxTParams& { return t < w_tiles ? p.w : p.x; };
-  auto place = [&](int64_t t, int& row0, int& k0) {
-    const QuantMxTParams& q = operand(t);
-    const int64_t u = t < w_tiles ? t : t - w_tiles;
-    const int row_tiles = (q.rows + 127) / 128;
-    k0 = static_cast<int>(u / row_tiles) * 128;
-    row0 = static_cast<int>(u % row_tiles) * 128;
-  };
-  auto fetch = [&](int64_t t, uint16_t (*dst)[kQtPitch]) {
-    const QuantMxTParams& q = operand(t);
-    int row0, k0;
-    place(t, row0, k0);
-    quant_mxfp8_t_fetch(q, dst, row0, k0, (q.ld % 8 == 0) && ((reinterpret_cast<uintptr_t>(q.src) & 15) == 0));
-  };
-  int buf = 0;
-  if (blockIdx.x < total) fetch(blockIdx.x, tiles[0]);
-  for (int64_t t = blockIdx.x; t < total; t += gridDim.x) {
-    const QuantMxTParams& q = operand(t);
-    int row0, k0;
-    place(t, row0, k0);
-    if (t + gridDim.x < total) {
-      fetch(t + gridDim.x, tiles[buf ^ 1]);
-      cp_async_wait<1>();   // everything but the newest group (the next tile) has landed
-    } else {
-      cp_async_wait<0>();
-    }
-    __syncthreads();
-    uint32_t o[2][8];
-    quant_mxfp8_tile_columns(tiles[buf], tile_scales, o, q.kp, q.rows, row0, k0, true);
-    __syncthreads();   // every thread has read the staged tile: its storage now collects the transposed payload
-    quant_mxfp8_tile_columns_store(reinterpret_cast<uint8_t*>(tiles[buf]), o, q.q, q.kp, q.rows, row0, k0);
-    store_scale_tile<4>(tile_scales, q.scales, kScaleMma128, row0, k0 / 32, q.rows, q.nb, q.sf_chunks);
-    __syncthreads();   // the scale tile and this buffer are free again
-    buf ^= 1;
-  }
-  griddep_wait();   // the pass that leaves dz and the partial sums; whoever waits for this grid has waited for that one too
-  if (p.partial == nullptr) return;
-  const int lane = threadIdx.x & 31, k = threadIdx.x >> 5;
-  for (int c = blockIdx.x; c < (p.n + 31) / 32; c += gridDim.x) {
-    const int col = c * 32 + lane;
-    float s = 0.0f;
-    if (col < p.n)
-      for (int t = k; t < p.row_tiles; t += 8) s += __ldcg(p.partial + static_cast<int64_t>(t) * p.n + col);
-    part[k][lane] = s;
-    __syncthreads();
-    if (k == 0 && col < p.n) {
-#pragma unroll
-      for (int i = 1; i < 8; ++i) s += part[i][lane];
-      p.dbias[col] = __float2bfloat16_rn(s);
-    }
-    __syncthreads();
   }
 }
 
