@@ -72,14 +72,20 @@ struct MapSlot {
   bool valid;
 };
 
-constexpr int kMapSlots = 64;
+constexpr int kMapSlots = 256;
 inline thread_local MapSlot t_map_cache[kMapSlots];
 
 inline int encode_map(CUtensorMap* out, const MapKey& key, const char* what) {
-  uint64_t h = reinterpret_cast<uintptr_t>(key.base) >> 4;
-  h = h * 0x9E3779B97F4A7C15ull + key.dim[1] * 31 + key.dim[2] * 7 + key.box[1] * 131 + key.box[2] * 17 + key.rank +
-      key.words * 3 + key.stride[1];
-  MapSlot& slot = t_map_cache[(h >> 17) % kMapSlots];
+  // every word of the key (blank_key cleared its padding) enters the slot number: the maps of one launch differ in the
+  // box height or the base alone, and two of them in one slot would be encoded anew at every call
+  static_assert(sizeof(MapKey) % 8 == 0, "the key is hashed in 64-bit words");
+  uint64_t words[sizeof(MapKey) / 8], h = 0;
+  memcpy(words, &key, sizeof(MapKey));
+  for (uint64_t w : words) {
+    h = (h ^ w) * 0x9E3779B97F4A7C15ull;
+    h ^= h >> 29;
+  }
+  MapSlot& slot = t_map_cache[(h >> 32) % kMapSlots];
   if (slot.valid && memcmp(&slot.key, &key, sizeof(MapKey)) == 0) {
     *out = slot.map;
     return RTXB_OK;

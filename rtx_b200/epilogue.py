@@ -163,26 +163,40 @@ def mxfp8_linear_epilogue(x: torch.Tensor, weight, bias: Optional[torch.Tensor] 
     residual    BF16 [..., N], the shape of the result, or None
     activation  "none", "relu", "relu2" (max(z, 0)^2), "silu", "gelu" (erf) or "gelu_tanh"
     """
-    n, k = mxfp8_matrix_shape(weight) if isinstance(weight, MXFP8Tensor) else (int(v) for v in weight.shape)
-    if x.shape[-1] != k:
-        raise ValueError(f"K mismatch: x has {x.shape[-1]}, weight has {k}")
-    shape = (*x.shape[:-1], n)
-    if residual is not None and tuple(residual.shape) != shape:
-        raise ValueError(f"residual must have the result's shape {shape}, got {tuple(residual.shape)}")
-    if x.ndim != 2:
-        x = x.reshape(-1, k)
-    if residual is not None and residual.ndim != 2:
-        residual = residual.reshape(-1, n)
     if isinstance(weight, MXFP8Tensor):
-        if _needs_grad(x, bias, residual):
-            raise RuntimeError("a prequantized MXFP8 weight is inference-only; keep the BF16 master weight to train")
-        y = mxfp8_linear_epilogue_prequant_w.direct(x, *mxfp8_kernel_operands(weight), bias, residual, n, k, activation)
-    elif not _needs_grad(x, weight, bias, residual):
+        n, k = mxfp8_matrix_shape(weight)
+        return _apply_packed(x, weight, n, k, bias, residual, activation)
+    n, k = weight.shape
+    shape, x, residual = _matrices(x, residual, n, k)
+    if not _needs_grad(x, weight, bias, residual):
         y = mxfp8_linear_epilogue_op.direct(x, weight, bias, residual, activation)
     elif torch.compiler.is_compiling():
         y = mxfp8_linear_epilogue_train(x, weight, bias, residual, activation)[0]
     else:
         y = _LinearEpilogueFunction.apply(x, weight, bias, residual, activation)
+    return y if len(shape) == 2 else y.reshape(shape)
+
+
+def _matrices(x, residual, n, k):
+    """(shape of the result, x and residual as matrices)"""
+    if x.ndim < 1 or x.shape[-1] != k:
+        raise ValueError(f"K mismatch: x has {x.shape[-1] if x.ndim else 'no dimension'}, weight has {k}")
+    shape = (*x.shape[:-1], n)
+    if residual is not None:
+        if tuple(residual.shape) != shape:
+            raise ValueError(f"residual must have the result's shape {shape}, got {tuple(residual.shape)}")
+        if residual.ndim != 2:
+            residual = residual.reshape(-1, n)
+    return shape, (x if x.ndim == 2 else x.reshape(-1, k)), residual
+
+
+def _apply_packed(x, packed, n, k, bias, residual, activation):
+    """`packed`: an MXFP8Tensor, or its (payload, scales) as the kernels take them"""
+    shape, x, residual = _matrices(x, residual, n, k)
+    if _needs_grad(x, bias, residual):
+        raise RuntimeError("a prequantized MXFP8 weight is inference-only; keep the BF16 master weight to train")
+    data, scales = packed if isinstance(packed, tuple) else mxfp8_kernel_operands(packed)
+    y = mxfp8_linear_epilogue_prequant_w.direct(x, data, scales, bias, residual, n, k, activation)
     return y if len(shape) == 2 else y.reshape(shape)
 
 
@@ -275,8 +289,10 @@ class MXFP8LinearEpilogue(nn.Module):
                 f"activation={self.activation}, weight_mode={self.weight_mode}")
 
     def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
-        weight = self.weight if self.weight_mode == "dynamic" else self.packed_weight()
-        return mxfp8_linear_epilogue(x, weight, self.bias, residual, activation=self.activation)
+        if self.weight_mode == "prequantized":
+            return _apply_packed(x, (self.weight_data, self.weight_scales), self.out_features, self.in_features, self.bias,
+                                 residual, self.activation)
+        return mxfp8_linear_epilogue(x, self.weight, self.bias, residual, activation=self.activation)
 
 
 __all__ = ["MXFP8LinearEpilogue", "mxfp8_linear_epilogue", "mxfp8_linear_epilogue_backward"]

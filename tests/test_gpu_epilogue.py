@@ -464,3 +464,52 @@ def test_experts_and_epilogue_as_used_together(dev):
     want, bound = first["dx"]
     total = want + dy.double()
     within(xd.grad, total, 2.0 ** -8 * total.abs() + (1 + 2.0 ** -8) * bound)
+
+
+def test_second_derivatives_are_refused(dev):
+    import rtx_b200
+
+    x, w, b, r, dy = (t.to(dev) for t in inputs(20, 32, 32, seed=14))
+    x.requires_grad_(True)
+    g = torch.autograd.grad(rtx_b200.mxfp8_linear_epilogue(x, w, b, activation="silu"), x, dy.requires_grad_(True),
+                            create_graph=True)[0]
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        g.sum().backward()
+
+
+def test_packed_module_under_compile_and_with_leading_dimensions(dev):
+    import rtx_b200
+
+    torch.manual_seed(1)
+    m = rtx_b200.MXFP8LinearEpilogue(96, 72, activation="gelu", device=dev).to_quantized_weight()
+    x = torch.randn(2, 3, 96, device=dev).bfloat16()
+    r = torch.randn(2, 3, 72, device=dev).bfloat16()
+    y = m(x, r)
+    assert y.shape == (2, 3, 72)
+    assert torch.equal(torch.compile(lambda a, c: m(a, c), fullgraph=True)(x, r), y)
+    assert torch.equal(rtx_b200.mxfp8_linear_epilogue(x, m.packed_weight(), m.bias, r, activation="gelu"), y)
+    one = rtx_b200.mxfp8_linear_epilogue(x[0, 0], m.packed_weight(), m.bias, activation="gelu")
+    assert one.shape == (72,) and torch.equal(one, m(x[0, 0]))
+
+
+def test_row_major_packed_scales(dev):
+    """A packed weight whose scales are stored row-major is re-tiled on the way in."""
+    import rtx_b200
+    from rtx_b200.formats import convert_mxfp8_scale_layout
+
+    x, w, b, _, _ = (t.to(dev) for t in inputs(20, 200, 96, seed=15))
+    packed = rtx_b200.quantize_mxfp8(w)
+    rows = convert_mxfp8_scale_layout(packed, "row_major")
+    want = rtx_b200.mxfp8_linear_epilogue(x, packed, b)
+    assert torch.equal(rtx_b200.mxfp8_linear_epilogue(x, rows, b), want)
+    assert torch.equal(rtx_b200.mxfp8_linear_epilogue(x, rows, b), want)
+
+
+def test_replaced_packed_storage_is_noticed(dev):
+    import rtx_b200
+
+    x, w, _, _, _ = (t.to(dev) for t in inputs(20, 128, 96, seed=16))
+    packed, other = rtx_b200.quantize_mxfp8(w), rtx_b200.quantize_mxfp8(-w)
+    rtx_b200.mxfp8_linear_epilogue(x, packed)
+    packed.qdata, packed.scale = other.qdata, other.scale
+    assert torch.equal(rtx_b200.mxfp8_linear_epilogue(x, packed), rtx_b200.mxfp8_linear_epilogue(x, other))

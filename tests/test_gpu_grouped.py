@@ -397,3 +397,37 @@ def test_compiled_graph_gives_the_same_bits(dev):
     assert torch.equal(y, rtx_b200.mxfp8_grouped_linear(xd, wd, od) * 2)
     got = torch.autograd.grad(y, wd, dy.to(dev))[0]
     assert torch.equal(got, torch.autograd.grad(rtx_b200.mxfp8_grouped_linear(xd, wd, od) * 2, wd, dy.to(dev))[0])
+
+
+def test_packed_weight_under_compile(dev):
+    import rtx_b200
+
+    x, w, _ = inputs(60, 2, 128, 64, seed=15)
+    xd, od = x.to(dev), on(dev, offs(20, 30))
+    m = rtx_b200.MXFP8GroupedLinear(2, 64, 128, packed_weight=rtx_b200.quantize_mxfp8(w.to(dev)))
+    y = m(xd, od)
+    assert torch.equal(torch.compile(lambda a, o: m(a, o), fullgraph=True)(xd, od), y)
+    close(y, *forward(x, w, offs(20, 30)), 64)
+
+
+def test_second_derivatives_are_refused(dev):
+    import rtx_b200
+
+    x, w, dy = inputs(40, 2, 64, 64, seed=16)
+    xd = x.to(dev).requires_grad_(True)
+    y = rtx_b200.mxfp8_grouped_linear(xd, w.to(dev), on(dev, offs(10, 30)))
+    g = torch.autograd.grad(y, xd, dy.to(dev).requires_grad_(True), create_graph=True)[0]
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        g.sum().backward()
+
+
+def test_offsets_changed_between_forward_and_backward_are_refused(dev):
+    """The backward needs the forward's offsets: writing into them in between is caught by autograd's version count."""
+    import rtx_b200
+
+    x, w, dy = inputs(40, 2, 64, 64, seed=17)
+    xd, od = x.to(dev).requires_grad_(True), on(dev, offs(10, 30))
+    y = rtx_b200.mxfp8_grouped_linear(xd, w.to(dev), od)
+    od.copy_(on(dev, offs(20, 20)))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward(dy.to(dev))
