@@ -17,6 +17,12 @@ import torch
 _LIB = torch.library.Library("rtx", "FRAGMENT")
 
 
+def eager(t: torch.Tensor) -> bool:
+    """Whether an op on `t` would only be dispatched back into this package's CUDA implementation (a plain CUDA tensor, no
+    tracing): the package's own functions then call the launcher itself and save a dispatch of a few microseconds."""
+    return (type(t) is torch.Tensor or type(t) is torch.nn.Parameter) and t.is_cuda and not torch.compiler.is_compiling()
+
+
 class OpHandle:
     """Callable handle of one registered op (`torch.ops.rtx.<name>.default`)."""
 
@@ -30,14 +36,6 @@ class OpHandle:
 
     def __call__(self, *args, **kwargs):
         return self.overload(*args, **kwargs)
-
-    def direct(self, *args):
-        """The op called from this package's own eager code: its implementation itself where that is what the dispatcher
-        would run (plain tensors, no tracing), the op otherwise.  Saves a dispatch of a few microseconds per call."""
-        kind = type(args[0])
-        if (kind is torch.Tensor or kind is torch.nn.Parameter) and args[0].is_cuda and not torch.compiler.is_compiling():
-            return self.fn(*args)
-        return self.overload(*args)
 
     def register_fake(self, fn: Callable) -> Callable:
         torch.library.register_fake(self.qualname, fn, lib=_LIB)

@@ -17,7 +17,7 @@ from torch.autograd.function import once_differentiable
 
 from . import fp8 as _fp8
 from . import ops
-from ._oplib import custom_op
+from ._oplib import custom_op, eager
 from .formats import (PACKED_OPERAND_SCHEMA_VERSION, SCALE_LAYOUT_CODES, MXFP8Tensor, make_mxfp8_tensor,
                       mxfp8_kernel_operands, mxfp8_matrix_shape, mxfp8_qdata_2d, mxfp8_scales_for_kernel, reject_packed_dtype_conversion)
 
@@ -126,7 +126,12 @@ def _train_backward(ctx, grad_y, _grad_z):
     if not (need_dx or need_dw or need_db):
         return None, None, None, grad_y if need_dr else None, None
     x, weight, z = ctx.saved_tensors
-    dx, dw, db = mxfp8_linear_epilogue_bwd.direct(grad_y, z, x, weight, ctx.activation, need_dx, need_dw, need_db)
+    if eager(grad_y):
+        weight = weight.contiguous() if need_dx else weight
+        return (*ops.mxfp8_linear_epilogue_bwd(grad_y, z, x, weight, weight.shape[1], activation=ctx.activation,
+                                               need_dx=need_dx, need_dw=need_dw, need_dbias=need_db),
+                grad_y if need_dr else None, None)
+    dx, dw, db = mxfp8_linear_epilogue_bwd(grad_y, z, x, weight, ctx.activation, need_dx, need_dw, need_db)
     return (dx if need_dx else None, dw if need_dw else None, db if need_db else None, grad_y if need_dr else None, None)
 
 
@@ -138,7 +143,8 @@ class _LinearEpilogueFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, residual, activation):
-        y, z = mxfp8_linear_epilogue_fwd.direct(x, weight, bias, residual, activation)
+        forward = mxfp8_linear_epilogue_fwd.fn if eager(x) else mxfp8_linear_epilogue_fwd
+        y, z = forward(x, weight, bias, residual, activation)
         ctx.save_for_backward(x, weight, z)
         ctx.activation = activation
         return y
@@ -169,7 +175,8 @@ def mxfp8_linear_epilogue(x: torch.Tensor, weight, bias: Optional[torch.Tensor] 
     n, k = weight.shape
     shape, x, residual = _matrices(x, residual, n, k)
     if not _needs_grad(x, weight, bias, residual):
-        y = mxfp8_linear_epilogue_op.direct(x, weight, bias, residual, activation)
+        forward = mxfp8_linear_epilogue_op.fn if eager(x) else mxfp8_linear_epilogue_op
+        y = forward(x, weight, bias, residual, activation)
     elif torch.compiler.is_compiling():
         y = mxfp8_linear_epilogue_train(x, weight, bias, residual, activation)[0]
     else:
@@ -196,7 +203,10 @@ def _apply_packed(x, packed, n, k, bias, residual, activation):
     if _needs_grad(x, bias, residual):
         raise RuntimeError("a prequantized MXFP8 weight is inference-only; keep the BF16 master weight to train")
     data, scales = packed if isinstance(packed, tuple) else mxfp8_kernel_operands(packed)
-    y = mxfp8_linear_epilogue_prequant_w.direct(x, data, scales, bias, residual, n, k, activation)
+    if eager(x):
+        y = ops.mxfp8_linear_epilogue_fwd_prequant_w(x, data, scales, n, bias, residual, activation=activation)
+    else:
+        y = mxfp8_linear_epilogue_prequant_w(x, data, scales, bias, residual, n, k, activation)
     return y if len(shape) == 2 else y.reshape(shape)
 
 
@@ -209,8 +219,8 @@ def mxfp8_linear_epilogue_backward(grad_output: torch.Tensor, z: Optional[torch.
     if activation != "none" and z is None:
         raise ValueError("an activation's backward needs the pre-activation z")
     z2d = z.reshape(-1, n).contiguous() if z is not None and activation != "none" else grad_output.new_empty(0)
-    dx, dw, db = mxfp8_linear_epilogue_bwd.direct(grad_output.reshape(-1, n), z2d, x.reshape(-1, k), weight, activation,
-                                                  True, True, bias)
+    backward = mxfp8_linear_epilogue_bwd.fn if eager(x) else mxfp8_linear_epilogue_bwd
+    dx, dw, db = backward(grad_output.reshape(-1, n), z2d, x.reshape(-1, k), weight, activation, True, True, bias)
     return dx.reshape(x.shape), dw, db if bias else None
 
 

@@ -21,7 +21,7 @@ from torch.autograd.function import once_differentiable
 
 from . import fp8 as _fp8
 from . import ops
-from ._oplib import custom_op
+from ._oplib import custom_op, eager
 from .formats import (PACKED_OPERAND_SCHEMA_VERSION, SCALE_LAYOUT_CODES, MXFP8Tensor, make_mxfp8_tensor,
                       mxfp8_kernel_operands, mxfp8_qdata_2d, mxfp8_scales_for_kernel, reject_packed_dtype_conversion)
 
@@ -130,12 +130,14 @@ def _train_setup(ctx, inputs, output):
 def _train_backward(ctx, grad_output):
     x, weight, offsets = ctx.saved_tensors
     need_dx, need_dw = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
+    if eager(grad_output):
+        return (*_bwd(grad_output, x, weight, offsets, need_dx, need_dw), None)
     if need_dx and need_dw:
-        return (*mxfp8_grouped_linear_bwd.direct(grad_output, x, weight, offsets), None)
+        return (*mxfp8_grouped_linear_bwd(grad_output, x, weight, offsets), None)
     if need_dx:
-        return mxfp8_grouped_linear_dx.direct(grad_output, x, weight, offsets), None, None
+        return mxfp8_grouped_linear_dx(grad_output, x, weight, offsets), None, None
     if need_dw:
-        return None, mxfp8_grouped_linear_dw.direct(grad_output, x, weight, offsets), None
+        return None, mxfp8_grouped_linear_dw(grad_output, x, weight, offsets), None
     return None, None, None
 
 
@@ -149,7 +151,7 @@ class _GroupedLinearFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, offsets):
         ctx.save_for_backward(x, weight, offsets)
-        return mxfp8_grouped_linear_op.direct(x, weight, offsets)
+        return _forward(x, weight, offsets)
 
     backward = staticmethod(once_differentiable(_train_backward))
 
@@ -180,8 +182,20 @@ def mxfp8_grouped_linear(x: torch.Tensor, weight, offsets: torch.Tensor) -> torc
             raise ValueError(f"offsets must be a contiguous vector of groups + 1 = {groups + 1} row numbers")
         if x.requires_grad and torch.is_grad_enabled():
             raise RuntimeError("a prequantized MXFP8 weight is inference-only; keep the BF16 master weight to train")
-        return mxfp8_grouped_linear_prequant_w.direct(x, *mxfp8_kernel_operands(weight), offsets, n)
+        return _packed(x, *mxfp8_kernel_operands(weight), offsets, n)
     return _dynamic(x, weight, offsets)
+
+
+def _packed(x, weight_data, weight_scales, offsets, n) -> torch.Tensor:
+    if eager(x):
+        return ops.mxfp8_grouped_linear_fwd_prequant_w(x, weight_data, weight_scales, offsets, n)
+    return mxfp8_grouped_linear_prequant_w(x, weight_data, weight_scales, offsets, n)
+
+
+def _forward(x, weight, offsets) -> torch.Tensor:
+    if eager(x):
+        return mxfp8_grouped_linear_op.fn(x, weight, offsets)
+    return mxfp8_grouped_linear_op(x, weight, offsets)
 
 
 def _dynamic(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor) -> torch.Tensor:
@@ -189,14 +203,16 @@ def _dynamic(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor) -> to
         if torch.compiler.is_compiling():
             return mxfp8_grouped_linear_train(x, weight, offsets)
         return _GroupedLinearFunction.apply(x, weight, offsets)
-    return mxfp8_grouped_linear_op.direct(x, weight, offsets)
+    return _forward(x, weight, offsets)
 
 
 def mxfp8_grouped_linear_backward(grad_output: torch.Tensor, x: torch.Tensor, weight: torch.Tensor,
                                   offsets: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """BF16 dX [rows, K] and dW [groups, N, K] of `mxfp8_grouped_linear`, from independently quantized MXFP8 products
     (blocks along N for dX, along each group's rows for dW)."""
-    return mxfp8_grouped_linear_bwd.direct(grad_output, x, weight, offsets)
+    if eager(x):
+        return mxfp8_grouped_linear_bwd.fn(grad_output, x, weight, offsets)
+    return mxfp8_grouped_linear_bwd(grad_output, x, weight, offsets)
 
 
 class MXFP8GroupedLinear(nn.Module):
@@ -261,7 +277,7 @@ class MXFP8GroupedLinear(nn.Module):
         if self.weight_mode == "prequantized":
             if x.requires_grad and torch.is_grad_enabled():
                 raise RuntimeError("a prequantized MXFP8 weight is inference-only; keep the BF16 master weight to train")
-            return mxfp8_grouped_linear_prequant_w.direct(x, self.weight_data, self.weight_scales, offsets, self.out_features)
+            return _packed(x, self.weight_data, self.weight_scales, offsets, self.out_features)
         return _dynamic(x, self.weight, offsets)
 
 

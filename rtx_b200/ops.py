@@ -325,19 +325,27 @@ def _bytes(query: str, *sizes: int) -> int:
     return N.query(query, *sizes)
 
 
-def _new(like: torch.Tensor, *shape: int) -> torch.Tensor:
-    """Uninitialised BF16 tensor on `like`'s device and its current stream (`like` is BF16: the cheapest spelling)."""
-    return like.new_empty(shape)
+def _new(device: torch.device, *shape: int) -> torch.Tensor:
+    return torch.empty(shape, dtype=torch.bfloat16, device=device)
 
 
-def _scratch(like: torch.Tensor, nbytes: int) -> torch.Tensor:
+def _scratch(device: torch.device, nbytes: int) -> torch.Tensor:
     """Workspace of one call: a fresh allocation of the calling stream, so that calls on several streams and captured
     graphs share nothing."""
-    return like.new_empty((nbytes + 1) // 2)
+    return torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+
+_status_ptrs: dict[int, int] = {}
 
 
 def _status_ptr(device: torch.device) -> int:
-    return status_word(device).data_ptr()
+    """Address of the device's status word, which lives as long as the process."""
+    ptr = _status_ptrs.get(device.index)
+    if ptr is None:
+        ptr = status_word(device).data_ptr()
+        if device.index is not None:
+            _status_ptrs[device.index] = ptr
+    return ptr
 
 
 def _rows_of(t: torch.Tensor, cols: Optional[int], name: str) -> Tuple[torch.Tensor, int]:
@@ -404,11 +412,11 @@ def mxfp8_linear_epilogue_fwd(x: torch.Tensor, w: torch.Tensor, bias: Optional[t
     bias, residual, ldr = _bias_and_residual(x, m, n, bias, residual)
     code = activation_code(activation)
     with _on(device):
-        out = _new(x, m, n)
-        z = _new(x, m, n) if keep_z else None
+        out = _new(device, m, n)
+        z = _new(device, m, n) if keep_z else None
         if m and n:
             nbytes = _bytes("rtxb_mxfp8_linear_epilogue_workspace_bytes", m, n, k, 1)
-            buf = _scratch(x, nbytes)
+            buf = _scratch(device, nbytes)
             N.call("rtxb_mxfp8_linear_epilogue_fwd", x.data_ptr(), ldx, w.data_ptr(),
                    None if bias is None else bias.data_ptr(), None if residual is None else residual.data_ptr(), ldr,
                    out.data_ptr(), z.data_ptr() if keep_z else None, m, n, k, code, rounding, buf.data_ptr(), nbytes,
@@ -427,10 +435,10 @@ def mxfp8_linear_epilogue_fwd_prequant_w(x: torch.Tensor, qw: torch.Tensor, sw: 
     bias, residual, ldr = _bias_and_residual(x, m, n, bias, residual)
     code = activation_code(activation)
     with _on(device):
-        out = _new(x, m, n)
+        out = _new(device, m, n)
         if m and n:
             nbytes = _bytes("rtxb_mxfp8_linear_epilogue_workspace_bytes", m, n, k, 0)
-            buf = _scratch(x, nbytes)
+            buf = _scratch(device, nbytes)
             N.call("rtxb_mxfp8_linear_epilogue_fwd_prequant_w", x.data_ptr(), ldx, qw.data_ptr(), sw.data_ptr(),
                    None if bias is None else bias.data_ptr(), None if residual is None else residual.data_ptr(), ldr,
                    out.data_ptr(), m, n, k, code, rounding, buf.data_ptr(), nbytes, _stream_ptr(), _status_ptr(device))
@@ -462,14 +470,14 @@ def mxfp8_linear_epilogue_bwd(dy: torch.Tensor, z: Optional[torch.Tensor], x: Op
     if not (need_dx or need_dw or need_dbias):
         return None, None, None
     with _on(device):
-        dx = _new(dy, m, k) if need_dx else None
-        dw = _new(dy, n, k) if need_dw else None
-        db = _new(dy, n) if need_dbias else None
+        dx = _new(device, m, k) if need_dx else None
+        dw = _new(device, n, k) if need_dw else None
+        db = _new(device, n) if need_dbias else None
         if min(m, n, k) == 0:             # an empty sum is zero
             return tuple(None if t is None else t.zero_() for t in (dx, dw, db))
         nbytes = _bytes("rtxb_mxfp8_linear_epilogue_backward_workspace_bytes", m, n, k, int(need_dx), int(need_dw),
                         int(need_dbias))
-        buf = _scratch(dy, nbytes)
+        buf = _scratch(device, nbytes)
         N.call("rtxb_mxfp8_linear_epilogue_bwd", dy.data_ptr(), lddy, z.data_ptr() if code else None,
                x.data_ptr() if need_dw else None, ldx, w.data_ptr() if need_dx else None,
                dx.data_ptr() if need_dx else None, dw.data_ptr() if need_dw else None,
@@ -506,7 +514,7 @@ def _group_weight(w: torch.Tensor, device: torch.device) -> torch.Tensor:
 
 def _grouped_out(out: Optional[torch.Tensor], x: torch.Tensor, n: int) -> Tuple[torch.Tensor, int]:
     if out is None:
-        return _new(x, x.shape[0], n), n
+        return _new(x.device, x.shape[0], n), n
     held, ldo = _rows_of(out, n, "out")
     if held is not out or out.shape[0] != x.shape[0] or out.device != x.device:
         raise ValueError(f"out must be [{x.shape[0]}, {n}] with contiguous rows on the operands' device")
@@ -529,7 +537,7 @@ def mxfp8_grouped_linear_fwd(x: torch.Tensor, w: torch.Tensor, offsets: torch.Te
         out, ldo = _grouped_out(out, x, n)
         if rows and n:
             nbytes = _bytes("rtxb_mxfp8_grouped_linear_workspace_bytes", rows, n, k, groups, 1)
-            buf = _scratch(x, nbytes)
+            buf = _scratch(device, nbytes)
             N.call("rtxb_mxfp8_grouped_linear_fwd", x.data_ptr(), ldx, w.data_ptr(), offsets.data_ptr(), groups,
                    out.data_ptr(), ldo, rows, n, k, rounding, buf.data_ptr(), nbytes, _stream_ptr(), _status_ptr(device))
     return out
@@ -549,7 +557,7 @@ def mxfp8_grouped_linear_fwd_prequant_w(x: torch.Tensor, qw: torch.Tensor, sw: t
         out, ldo = _grouped_out(out, x, n)
         if rows and n:
             nbytes = _bytes("rtxb_mxfp8_grouped_linear_workspace_bytes", rows, n, k, groups, 0)
-            buf = _scratch(x, nbytes)
+            buf = _scratch(device, nbytes)
             N.call("rtxb_mxfp8_grouped_linear_fwd_prequant_w", x.data_ptr(), ldx, qw.data_ptr(), sw.data_ptr(),
                    offsets.data_ptr(), groups, out.data_ptr(), ldo, rows, n, k, rounding, buf.data_ptr(), nbytes,
                    _stream_ptr(), _status_ptr(device))
@@ -576,12 +584,12 @@ def mxfp8_grouped_linear_bwd(dy: torch.Tensor, x: Optional[torch.Tensor], w: Opt
     if not (need_dx or need_dw):
         return None, None
     with _on(device):
-        dx = _new(dy, rows, k) if need_dx else None
-        dw = _new(dy, groups, n, k) if need_dw else None
+        dx = _new(device, rows, k) if need_dx else None
+        dw = _new(device, groups, n, k) if need_dw else None
         if min(rows, n, k) == 0:          # an empty sum is zero
             return (dx.zero_() if need_dx else None), (dw.zero_() if need_dw else None)
         nbytes = _bytes("rtxb_mxfp8_grouped_backward_workspace_bytes", rows, n, k, groups, int(need_dx), int(need_dw))
-        buf = _scratch(dy, nbytes)
+        buf = _scratch(device, nbytes)
         N.call("rtxb_mxfp8_grouped_linear_bwd", dy.data_ptr(), lddy, x.data_ptr() if need_dw else None, ldx,
                w.data_ptr() if need_dx else None, offsets.data_ptr(), groups, dx.data_ptr() if need_dx else None,
                dw.data_ptr() if need_dw else None, rows, n, k, buf.data_ptr(), nbytes, _stream_ptr(), _status_ptr(device))
