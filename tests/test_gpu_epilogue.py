@@ -513,3 +513,46 @@ def test_replaced_packed_storage_is_noticed(dev):
     rtx_b200.mxfp8_linear_epilogue(x, packed)
     packed.qdata, packed.scale = other.qdata, other.scale
     assert torch.equal(rtx_b200.mxfp8_linear_epilogue(x, packed), rtx_b200.mxfp8_linear_epilogue(x, other))
+
+
+@pytest.mark.parametrize("m,n,k", [(140_000, 64, 16_384), (70_000, 32_768, 32)])
+def test_operands_beyond_32_bit_offsets(dev, m, n, k):
+    """More than 2^31 values in x, respectively in the result: the last rows have the bits of a call on those rows alone."""
+    import rtx_b200
+
+    tail = slice(m - 200, m)
+    x = torch.randn(m, k, device=dev, dtype=torch.bfloat16)
+    w = torch.randn(n, k, device=dev, dtype=torch.bfloat16)
+    b = torch.randn(n, device=dev, dtype=torch.bfloat16)
+    r = torch.randn(m, n, device=dev, dtype=torch.bfloat16)
+    y = rtx_b200.mxfp8_linear_epilogue(x, w, b, r, activation="silu")
+    assert torch.equal(y[tail], rtx_b200.mxfp8_linear_epilogue(x[tail], w, b, r[tail], activation="silu"))
+    dx = rtx_b200.mxfp8_linear_epilogue_backward(r, y, x, w, activation="silu", bias=False)[0]
+    assert torch.equal(dx[tail], rtx_b200.mxfp8_linear_epilogue_backward(r[tail], y[tail].contiguous(), x[tail], w,
+                                                                         activation="silu", bias=False)[0])
+
+
+def test_two_threads_at_once(dev):
+    """Two threads on two streams: launch state is per thread, scratch per call."""
+    import threading
+
+    import rtx_b200
+
+    cases = [tuple(t.to(dev) for t in inputs(300, 256, 128, seed=s)[:4]) for s in (20, 21)]
+    want = [rtx_b200.mxfp8_linear_epilogue(*c, activation="silu") for c in cases]
+    torch.cuda.synchronize()
+    got = [[], []]
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(50):
+                got[i].append(rtx_b200.mxfp8_linear_epilogue(*cases[i], activation="silu"))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert len(got[i]) == 50 and all(torch.equal(y, want[i]) for y in got[i])

@@ -431,3 +431,51 @@ def test_offsets_changed_between_forward_and_backward_are_refused(dev):
     od.copy_(on(dev, offs(20, 20)))
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.backward(dy.to(dev))
+
+
+def test_empty_batch(dev):
+    import rtx_b200
+
+    w = torch.randn(2, 64, 32, device=dev).bfloat16().requires_grad_(True)
+    x = torch.empty(0, 32, dtype=torch.bfloat16, device=dev, requires_grad=True)
+    y = rtx_b200.mxfp8_grouped_linear(x, w, on(dev, offs(0, 0)))
+    assert y.shape == (0, 64)
+    y.sum().backward()
+    assert x.grad.shape == (0, 32) and (w.grad == 0).all()
+
+
+def test_shared_weights_and_expanded_inputs(dev):
+    """One weight expanded over the groups, one row expanded over the batch: copied on the way in, gradients summed."""
+    import rtx_b200
+
+    gen = torch.Generator().manual_seed(18)
+    w1 = torch.randint(-1, 2, (1, 32, 32), generator=gen).bfloat16().to(dev).requires_grad_(True)
+    row = torch.randint(-1, 2, (1, 32), generator=gen).bfloat16().to(dev).requires_grad_(True)
+    od = on(dev, offs(3, 2))
+    y = rtx_b200.mxfp8_grouped_linear(row.expand(5, 32), w1.expand(2, 32, 32), od)
+    want = row.detach().double() @ w1.detach()[0].double().T
+    assert torch.equal(y.double(), want.expand(5, 32))        # small whole numbers: exact throughout
+    y.sum().backward()
+    assert torch.equal(row.grad.double(), 5 * w1.detach()[0].double().sum(0, keepdim=True))
+    assert torch.equal(w1.grad[0].double(), 5 * row.detach().double().expand(32, 32))
+
+
+@pytest.mark.parametrize("rows,n,k", [(140_000, 64, 16_384), (70_000, 32_768, 32)])
+def test_operands_beyond_32_bit_offsets(dev, rows, n, k):
+    """More than 2^31 values in x, respectively in the result: the last group's rows, and its gradients, have the bits of
+    a call on those rows alone."""
+    import rtx_b200
+
+    last = 300
+    x = torch.randn(rows, k, device=dev, dtype=torch.bfloat16)
+    w = torch.randn(2, n, k, device=dev, dtype=torch.bfloat16)
+    od, alone = on(dev, offs(rows - last - 5, last)), on(dev, offs(last))
+    assert max(rows * k, rows * n) > 2 ** 31
+    y = rtx_b200.mxfp8_grouped_linear(x, w, od)
+    tail = slice(rows - last - 5, rows - 5)
+    assert torch.equal(y[tail], rtx_b200.mxfp8_grouped_linear(x[tail], w[1:], alone))
+    assert (y[-5:] == 0).all()
+    dy = y.mul_(2.0 ** -8)
+    dx, dw = rtx_b200.mxfp8_grouped_linear_backward(dy, x, w, od)
+    want_dx, want_dw = rtx_b200.mxfp8_grouped_linear_backward(dy[tail], x[tail], w[1:], alone)
+    assert torch.equal(dx[tail], want_dx) and torch.equal(dw[1], want_dw[0]) and (dx[-5:] == 0).all()
