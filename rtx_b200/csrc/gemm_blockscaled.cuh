@@ -611,11 +611,11 @@ __device__ __forceinline__ void issue_scale_copy(uint32_t tmem_base, uint32_t ss
 // the four MMAs (32 bytes of K each) of one K step
 template <int KIND, bool PAIR>
 __device__ __forceinline__ void issue_k_step(uint32_t tmem_base, uint32_t acc_col, uint32_t sa, uint32_t sb, int set,
-                                             uint32_t idesc, bool first_step) {
+                                             uint32_t idesc, bool first_step, uint32_t sfb_shift = 0) {
   using TP = TmemPlan<KIND>;
   const uint64_t da = umma_desc_sw128(sa);
   const uint64_t db = umma_desc_sw128(sb);
-  const uint32_t ta = tmem_base + TP::sfa_col(set), tb = tmem_base + TP::sfb_col(set);
+  const uint32_t ta = tmem_base + TP::sfa_col(set), tb = tmem_base + TP::sfb_col(set) + sfb_shift;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const uint32_t acc = (!first_step || j > 0) ? 1u : 0u;

@@ -8,7 +8,7 @@
 // ragged extent is then the MMA's N, which may be any multiple of 32 up to 256: the last tile of a group costs what its
 // rows cost (a tile of 40 tokens runs N = 64, a quarter of a full one), and one decode step streams its weights through
 // the 256-row operand while a handful of tokens sits on the 32-wide side.  With the ragged extent on the MMA's rows
-// every started tile costs 256 rows.
+// every started tile costs 256 rows.  Small batches take tiles of 128 or 64 rows (rows_per_tile in grouped.cu).
 //
 // Roles, TMEM plan and ring as in gemm_blockscaled_pair_kernel; what differs: tiles come from the plan the quantizer
 // left, N and the number of K steps are per tile, and the epilogue holds one output column per lane, so a chunk of 32
@@ -25,7 +25,8 @@ struct GroupedGemmParams {
   int a_rows;              // rows of operand A per group (= output columns)
   int a_tiles;             // 256-row tiles of A per group
   int a_sf_tiles;          // 128-row scale tiles of A per group (rows form)
-  int b_rows, b_tiles;     // contraction form: output rows per group and their 256-row tiles
+  int b_rows, b_tiles;     // contraction form: output rows per group and their tiles
+  int tile_rows;           // most rows of B per tile (64, 128 or 256)
   int groups;
   int k_tiles;             // rows form: K steps; contraction form: read per group from plan_k
   int sf_chunks_a, sf_chunks_b;   // 512-byte scale tiles per 128 rows
@@ -49,6 +50,7 @@ struct GroupedMapsB {
 struct GroupedTile {
   int a_row, a_sf;         // first row of operand A (in its tensor map) and its first 128-row scale tile
   int b_row, b_sf, live;   // the same of operand B; rows of it that belong to the tile
+  int sf_shift;            // 32-row groups of that scale tile before b_row (the scales of 32 rows are one TMEM column)
   int kt0, k_steps;
   int out_row, out_col, out_g;
 };
@@ -67,9 +69,10 @@ __device__ __forceinline__ GroupedTile grouped_tile(const GroupedGemmParams& p, 
     t.k_steps = __ldcg(p.plan_k + g + 1) - t.kt0;
     t.a_row = at * 256;
     t.a_sf = at * 2;
-    t.b_row = bt * 256;
-    t.b_sf = bt * 2;
-    t.live = min(256, p.b_rows - t.b_row);
+    t.b_row = bt * p.tile_rows;
+    t.b_sf = t.b_row >> 7;
+    t.sf_shift = (t.b_row & 127) >> 5;
+    t.live = min(p.tile_rows, p.b_rows - t.b_row);
     t.out_row = t.b_row;
     t.out_col = at * 256;
     t.out_g = g;
@@ -78,8 +81,10 @@ __device__ __forceinline__ GroupedTile grouped_tile(const GroupedGemmParams& p, 
     const int4 e = __ldcg(p.plan_tiles + m);
     t.kt0 = 0;
     t.k_steps = p.k_tiles;
-    t.a_row = e.w * p.a_rows + at * 256;
-    t.a_sf = e.w * p.a_sf_tiles + at * 2;
+    const int g = e.w & 0xFFFF;
+    t.a_row = g * p.a_rows + at * 256;
+    t.a_sf = g * p.a_sf_tiles + at * 2;
+    t.sf_shift = e.w >> 16;
     t.b_row = e.x;
     t.b_sf = e.z;
     t.live = e.y;
@@ -257,7 +262,7 @@ gemm_grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
                                                  ssfb + KS * T::kSfaBytes, set);
               issue_k_step<kKindMxfp8, true>(tmem_base, acc_col, smem_base + slot * T::kABytes,
                                              smem_base + T::kOffB + group * KS * T::kBBytes + sub * b_bytes, set, idesc,
-                                             kg == 0 && sub == 0);
+                                             kg == 0 && sub == 0, t.sf_shift);
             }
             tc_commit_pair(&empty_bar[group], 3);
           }

@@ -116,7 +116,7 @@ __device__ __forceinline__ void write_group_plan(const GroupList& l, GroupScan& 
   int n[kPer], sum = 0;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    n[i] = first + i < l.groups ? (s.start[first + i + 1] - s.start[first + i] + 255) >> 8 : 0;
+    n[i] = first + i < l.groups ? (s.start[first + i + 1] - s.start[first + i] + plan.tile_rows - 1) / plan.tile_rows : 0;
     sum += n[i];
   }
   int before = block_scan_sum(sum, s.warp_part) - sum;
@@ -133,8 +133,9 @@ __device__ __forceinline__ void write_group_plan(const GroupList& l, GroupScan& 
   if (threadIdx.x == 0) plan.row_tiles[0] = total;
   for (int t = threadIdx.x; t < total; t += kQuantThreads) {
     const int g = group_before(wide, l.groups, t);
-    const int j = t - wide[g], row = s.start[g] + 256 * j;
-    plan.tiles[t] = make_int4(row, min(256, s.start[g + 1] - row), s.tile[g] + 2 * j, g);
+    const int off = (t - wide[g]) * plan.tile_rows, row = s.start[g] + off;
+    plan.tiles[t] = make_int4(row, min(plan.tile_rows, s.start[g + 1] - row), s.tile[g] + (off >> 7),
+                              g | ((off & 127) >> 5) << 16);
   }
   __syncthreads();
 }

@@ -14,9 +14,10 @@ struct GroupList {
 
 // What the quantizer leaves for the GEMM behind it (global memory, written by block 0).
 struct GroupPlan {
-  int* row_tiles;    // [0] = number of 256-row tiles over all groups
-  int4* tiles;       // per 256-row tile: {first row, live rows, first scale tile, group}
+  int* row_tiles;    // [0] = number of row tiles over all groups
+  int4* tiles;       // per row tile: {first row, live rows, first 128-row scale tile, group | (32-row offset in it) << 16}
   int* k_tiles;      // [groups + 1] = GroupScan::tile
+  int tile_rows;     // 64, 128 or 256
 };
 
 struct RowsOperand {
