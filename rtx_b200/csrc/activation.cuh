@@ -2,9 +2,10 @@
 //
 // The epilogue evaluates one activation per output element beside the MMAs of the next tile, the backward quantizer one
 // slope per gradient element at memory speed, so an evaluation may cost two special-function operations and some twenty
-// multiply-adds; the library's erff / tanhf / expf cost two to four times that (8192 x 4096 x 8192, gelu with z kept:
-// the GEMM ran 315 us against 168 for the plain one, the slope pass 210 us at 30 % of the copy rate).  Forms without
-// cancellation:
+// multiply-adds; the library's erff / tanhf / expf cost two to four times that.  Measured, gelu, 8192 x 8192: slope pass
+// 210 us with erff and expf, 178 with the forms below a value at a time, 148 with them on packed pairs (and 110 with its
+// table, quant_act.cuh); GEMM of 8192 x 4096 x 8192 with residual and z 265 us a value at a time, 217 on pairs.  Forms
+// without cancellation:
 //   silu       z s(z), s(z) = 1 / (1 + e^-z)
 //   gelu_tanh  z s(2 a (z + b z^3)), since (1 + tanh u) / 2 = s(2 u)
 //   gelu       z Phi(z), Phi(-|z|) = erfc(|z| / sqrt 2) / 2 with erfc(x) = e^(-x^2) (c1 t + .. + c5 t^5), t = 1 / (1 + p x)

@@ -463,9 +463,13 @@ __device__ __forceinline__ void epilogue_drain(const GemmParams& p, uint32_t tac
 }
 
 // kEpiAct in the pair kernel: one tile of this warp's 32 rows, columns [128 half, 128 half + 128) of the accumulator.
-// Eight warps drain a tile (two per lane quadrant): an activation costs some thirty instructions per value and every
-// chunk waits for TMEM, for the residual and for its staging buffer, more than four warps can hide behind the next
-// tile's MMAs (8192 x 4096 x 8192 with gelu, residual and z: 304 us with four warps).  A chunk is 32 rows x 32 columns:
+// Eight warps drain a tile (two per lane quadrant): a value costs some twenty instructions and every chunk waits for
+// TMEM, for the residual and for its staging buffer, more than four warps can hide behind the next tile's MMAs.  Measured,
+// 8192 x 4096 x 8192 with bias, gelu, residual and z kept: 304 us with four warps, 265 with eight, 217 to 222 with
+// activations on packed pairs too (activation.cuh; tensor pipe 73 % of active cycles); the plain GEMM takes 168, and z and
+// the residual are 268 MB more (41 us at the copy rate).  8192 x 4096 x 14336 with bias and gelu: 328 us, 2.93 PFLOP/s.
+// Fetching a chunk's accumulators a chunk ahead (the loop unrolled for it) was slower, 245 us: the code no longer fits the
+// instruction cache.  A chunk is 32 rows x 32 columns:
 //   z = acc + bias, staged and stored while act(z) is computed (training only; rounded to BF16 for the backward, the
 //   activation takes the FP32 value), then act(z) + residual through the same 2 KB buffer.
 // The residual of the next chunk is fetched before the current one is finished.
@@ -1060,21 +1064,21 @@ gemm_blockscaled_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __
           *abort_flag = 1;
           break;
         }
-        continue;
+      } else {
+        if (!mbar_wait(acc_full_bar, local_tile & 1, abort_flag)) {
+          if (p.status && lane == 0) atomicCAS(p.status, 0, kStatusWaitEpilogue);
+          *abort_flag = 1;
+          break;
+        }
+        tc_fence_after_sync();
+        const float row_scale = (EPI == kEpiRegionBf16 && row_ok) ? __ldg(p.x_region_scales + row / p.x_region_rows)
+                                                                  : out_scale;
+        // the output block this 256-row pair tile belongs to (whole tiles never straddle blocks)
+        const int out_blk = p.out_block_rows > 0 ? (mp_idx * 256) / p.out_block_rows : 0;
+        epilogue_drain<KIND, EPI>(p, tmem_base + lane_base + acc_col, row, row_ok, n_idx, (local_tile & 1) != 0,
+                                  overlap_addr, row_scale, lane, &maps_out.m[out_blk],
+                                  smem + T::kOffStage + quad * 2 * kEpiStageBufBytes, out_blk * p.out_block_rows);
       }
-      if (!mbar_wait(acc_full_bar, local_tile & 1, abort_flag)) {
-        if (p.status && lane == 0) atomicCAS(p.status, 0, kStatusWaitEpilogue);
-        *abort_flag = 1;
-        break;
-      }
-      tc_fence_after_sync();
-      const float row_scale = (EPI == kEpiRegionBf16 && row_ok) ? __ldg(p.x_region_scales + row / p.x_region_rows)
-                                                                : out_scale;
-      // the output block this 256-row pair tile belongs to (whole tiles never straddle blocks)
-      const int out_blk = p.out_block_rows > 0 ? (mp_idx * 256) / p.out_block_rows : 0;
-      epilogue_drain<KIND, EPI>(p, tmem_base + lane_base + acc_col, row, row_ok, n_idx, (local_tile & 1) != 0,
-                                overlap_addr, row_scale, lane, &maps_out.m[out_blk],
-                                smem + T::kOffStage + quad * 2 * kEpiStageBufBytes, out_blk * p.out_block_rows);
     }
     if (p.tma_out && lane == 0) tma_store_wait_all<0>();   // shared memory outlives the last store's reads
     __syncwarp();

@@ -10,6 +10,15 @@
 // the 256-row operand while a handful of tokens sits on the 32-wide side.  With the ragged extent on the MMA's rows
 // every started tile costs 256 rows.  Small batches take tiles of 128 or 64 rows (rows_per_tile in grouped.cu).
 //
+// What bounds it.  Large batches: the tensor pipe, 81 to 83 % of active cycles (8192 rows, 4 groups, 4096 x 4096: 93 us,
+// 2.95 PFLOP/s in a burst; in a longer run the 1 kW power cap, at 1.43 GHz).  The rest of the cycles is the hand-over
+// between tiles: 2 x 256 accumulator columns and the scale sets do not fit TMEM, so a tile's MMAs wait for the shared
+// chunk of the tile before.  Decode: HBM, every weight read once (128 rows, 32 groups of 4096 x 4096: 84 us, 6.6 TB/s).
+// In between, the weights of groups with one partial tile each: 8192 rows in 32 uneven groups of 2048 x 4096 take 79 us
+// where weights and rows are 51 us of HBM and the MMAs 46: pairs are 88 to 120 k cycles busy, since tiles of unlike size
+// are dealt out in turn.  Dealing the full tiles first and the partial ones by size was no faster (86 us): groups of
+// several tiles lose their weights from L2 in between, 413 MB read instead of 312.
+//
 // Roles, TMEM plan and ring as in gemm_blockscaled_pair_kernel; what differs: tiles come from the plan the quantizer
 // left, N and the number of K steps are per tile, and the epilogue holds one output column per lane, so a chunk of 32
 // accumulator columns is 32 output rows of 64 bytes, staged and stored as one TMA box where all 32 rows belong to the

@@ -4,8 +4,9 @@
 //   q_t     MXFP8 of dz^T, blocks along m    (A operand of dW = dz^T X)
 //   partial[m / 128][n] = sum of 128 rows of dz in FP32, before the rounding   (dbias, finished by quant_mxfp8_transposed_units_kernel)
 // dy and z are read once (4 bytes per value), 2 bytes of payload leave: without the fusion dz is written and read again
-// (4 more).  One 128 x 128 tile per block step, three blocks per SM
-// overlap one another's loads, arithmetic and stores.
+// (4 more).  One 128 x 128 tile per block step; three blocks per SM overlap one another's loads, arithmetic and stores.
+// Measured, gelu, 8192 x 8192: 108 to 112 us, 3.7 TB/s, 0.56 of the copy rate, bound by instructions (63 % issue): 29 a
+// value, 17 of them before the quantization.  With slopes evaluated instead of looked up 148 us.
 #pragma once
 
 #include "activation.cuh"

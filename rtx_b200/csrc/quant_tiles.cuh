@@ -27,17 +27,6 @@ struct QuantMxParams {
   int round_to_infinity; // 1 = default, 0 = OCP floor ablation
 };
 
-__device__ __forceinline__ void load8_bf16(const __nv_bfloat16* row_ptr, int col, int k, bool vec_ok, float (&v)[8]) {
-  if (vec_ok && col + 8 <= k) {
-    uint4 raw = __ldg(reinterpret_cast<const uint4*>(row_ptr + col));
-    v[0] = bf16_lo(raw.x); v[1] = bf16_hi(raw.x); v[2] = bf16_lo(raw.y); v[3] = bf16_hi(raw.y);
-    v[4] = bf16_lo(raw.z); v[5] = bf16_hi(raw.z); v[6] = bf16_lo(raw.w); v[7] = bf16_hi(raw.w);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = (col + e < k) ? __bfloat162float(row_ptr[col + e]) : 0.0f;
-  }
-}
-
 __device__ __forceinline__ float amax8(const float (&v)[8]) {
   float a = fabsf(v[0]);
 #pragma unroll
