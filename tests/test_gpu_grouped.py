@@ -157,6 +157,37 @@ def test_many_groups_and_larger_operands(dev, groups):
     close(dw, want_dw, dw_mag, max(sizes))
 
 
+@pytest.mark.parametrize("groups", [30, 31, 32, 33])
+def test_list_lengths_around_a_warp(dev, groups):
+    """Lists shorter and longer than a warp are read by different code: same results, and the same for a bad list."""
+    import rtx_b200
+    from rtx_b200 import ops
+
+    gen = torch.Generator().manual_seed(groups)
+    sizes = torch.randint(0, 20, (groups,), generator=gen).tolist()
+    sizes[0], sizes[-1] = 300, 130
+    offsets = offs(*sizes, head=3)
+    n, k = 64, 96
+    x, w, dy = inputs(offsets[-1] + 5, groups, n, k, seed=4)
+    xd, wd, dyd = x.to(dev), w.to(dev), dy.to(dev)
+    close(rtx_b200.mxfp8_grouped_linear(xd, wd, on(dev, offsets)), *forward(x, w, offsets), k)
+    dx, dw = rtx_b200.mxfp8_grouped_linear_backward(dyd, xd, wd, on(dev, offsets))
+    want_dx, want_dw, dx_mag, dw_mag = backward(dy, x, w, offsets)
+    close(dx, want_dx, dx_mag, n)
+    close(dw, want_dw, dw_mag, max(sizes))
+
+    bad = list(offsets)
+    bad[groups // 2], bad[-1] = -7, 2 ** 31 - 1
+    held = [0] * len(bad)
+    for i, v in enumerate(bad):
+        held[i] = max(min(max(v, 0), x.shape[0]), held[i - 1] if i else 0)
+    y = rtx_b200.mxfp8_grouped_linear(xd, wd, on(dev, bad))
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="offsets"):
+        ops.check_device_status(dev)
+    close(y, *forward(x, w, held), k)
+
+
 @pytest.mark.parametrize("rows", [1, 4, 48, 400])
 def test_packed_weight_gives_the_same_bits_as_the_bf16_weight(dev, rows):
     import rtx_b200
