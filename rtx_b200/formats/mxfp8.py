@@ -149,15 +149,13 @@ def mxfp8_scales_for_kernel(value) -> torch.Tensor:
 
 
 def mxfp8_kernel_operands(value) -> tuple[torch.Tensor, torch.Tensor]:
-    """(payload u8 [rows, storage_k], mma128 scale codes u8) as the kernels take them.  For mma128 storage both are views,
-    made once per packed tensor (a decode step is shorter than making them anew); replaced storage is noticed."""
-    kept = getattr(value, "_rtx_kernel_operands", None)
-    if kept is not None and kept[0] is value.qdata and kept[1] is value.scale:
-        return kept[2], kept[3]
-    q, s = mxfp8_qdata_2d(value).view(torch.uint8), mxfp8_scales_for_kernel(value)
-    if mxfp8_scale_layout(value) == "mma128":
-        value._rtx_kernel_operands = (value.qdata, value.scale, q, s)
-    return q, s
+    """(payload, mma128 scale codes) for the launchers that take packed operands of any shape and check their sizes: the
+    stored tensors themselves where they are laid out so (making views costs a decode step's host time)."""
+    validate_mxfp8_tensor(value)
+    q, s = value.qdata, value.scale
+    if getattr(value, "_rtx_scale_layout", None) != "mma128":
+        s = mxfp8_scales_for_kernel(value)
+    return q.contiguous(), s.contiguous()
 
 
 def convert_mxfp8_scale_layout(value, scale_layout: ScaleLayout):

@@ -466,6 +466,19 @@ def test_experts_and_epilogue_as_used_together(dev):
     within(xd.grad, total, 2.0 ** -8 * total.abs() + (1 + 2.0 ** -8) * bound)
 
 
+def test_replaced_packed_storage_is_used(dev):
+    """A packed weight whose storage is exchanged (a reload in place) is read where it now is."""
+    import rtx_b200
+
+    x, w, b, r, _ = (t.to(dev) for t in inputs(20, 64, 96, seed=18))
+    packed, other = rtx_b200.quantize_mxfp8(w), rtx_b200.quantize_mxfp8(2 * w.flip(0))
+    first = rtx_b200.mxfp8_linear_epilogue(x, packed, b, r)
+    want = rtx_b200.mxfp8_linear_epilogue(x, other, b, r)
+    packed.qdata.data, packed.scale.data = other.qdata.data, other.scale.data
+    got = rtx_b200.mxfp8_linear_epilogue(x, packed, b, r)
+    assert torch.equal(got, want) and not torch.equal(got, first)
+
+
 def test_second_derivatives_are_refused(dev):
     import rtx_b200
 

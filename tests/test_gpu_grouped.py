@@ -441,6 +441,19 @@ def test_packed_weight_under_compile(dev):
     close(y, *forward(x, w, offs(20, 30)), 64)
 
 
+def test_replaced_packed_storage_is_used(dev):
+    """A packed weight whose storage is exchanged (a reload in place) is read where it now is."""
+    import rtx_b200
+
+    x, w, _ = inputs(60, 2, 128, 64, seed=17)
+    xd, wd, od = x.to(dev), w.to(dev), on(dev, offs(20, 30))
+    packed, other = rtx_b200.quantize_mxfp8(wd), rtx_b200.quantize_mxfp8(2 * wd.flip(1))
+    first, want = rtx_b200.mxfp8_grouped_linear(xd, packed, od), rtx_b200.mxfp8_grouped_linear(xd, other, od)
+    packed.qdata.data, packed.scale.data = other.qdata.data, other.scale.data
+    got = rtx_b200.mxfp8_grouped_linear(xd, packed, od)
+    assert torch.equal(got, want) and not torch.equal(got, first)
+
+
 def test_second_derivatives_are_refused(dev):
     import rtx_b200
 
