@@ -13,14 +13,24 @@ from __future__ import annotations
 from typing import Callable, Optional
 
 import torch
+from torch.autograd import forward_ad
 
 _LIB = torch.library.Library("rtx", "FRAGMENT")
 
 
 def eager(t: torch.Tensor) -> bool:
     """Whether an op on `t` would only be dispatched back into this package's CUDA implementation (a plain CUDA tensor, no
-    tracing): the package's own functions then call the launcher itself and save a dispatch of a few microseconds."""
-    return (type(t) is torch.Tensor or type(t) is torch.nn.Parameter) and t.is_cuda and not torch.compiler.is_compiling()
+    tracing, no `torch.func` transform): the package's own functions then call the launcher itself and save a dispatch of a
+    few microseconds."""
+    return ((type(t) is torch.Tensor or type(t) is torch.nn.Parameter) and t.is_cuda
+            and not torch.compiler.is_compiling() and not torch._C._are_functorch_transforms_active())
+
+
+def refuse_tangents(name: str, *tensors) -> None:
+    """Forward-mode differentiation of an op without a formula for it would drop the tangents: refuse it."""
+    if forward_ad._current_level >= 0 and not torch.compiler.is_compiling():
+        if any(isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+            raise NotImplementedError(f"{name} has no forward-mode derivative")
 
 
 class OpHandle:

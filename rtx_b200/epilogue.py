@@ -17,7 +17,7 @@ from torch.autograd.function import once_differentiable
 
 from . import fp8 as _fp8
 from . import ops
-from ._oplib import custom_op, eager
+from ._oplib import custom_op, eager, refuse_tangents
 from .formats import (PACKED_OPERAND_SCHEMA_VERSION, SCALE_LAYOUT_CODES, MXFP8Tensor, make_mxfp8_tensor,
                       mxfp8_kernel_operands, mxfp8_matrix_shape, mxfp8_qdata_2d, mxfp8_scales_for_kernel, reject_packed_dtype_conversion)
 
@@ -172,6 +172,7 @@ def mxfp8_linear_epilogue(x: torch.Tensor, weight, bias: Optional[torch.Tensor] 
     if isinstance(weight, MXFP8Tensor):
         n, k = mxfp8_matrix_shape(weight)
         return _apply_packed(x, weight, n, k, bias, residual, activation)
+    refuse_tangents("mxfp8_linear_epilogue", x, weight, bias, residual)
     n, k = weight.shape
     shape, x, residual = _matrices(x, residual, n, k)
     if not _needs_grad(x, weight, bias, residual):
@@ -199,6 +200,7 @@ def _matrices(x, residual, n, k):
 
 def _apply_packed(x, packed, n, k, bias, residual, activation):
     """`packed`: an MXFP8Tensor, or its (payload, scales) as the kernels take them"""
+    refuse_tangents("mxfp8_linear_epilogue", x, bias, residual)
     shape, x, residual = _matrices(x, residual, n, k)
     if _needs_grad(x, bias, residual):
         raise RuntimeError("a prequantized MXFP8 weight is inference-only; keep the BF16 master weight to train")

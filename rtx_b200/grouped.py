@@ -21,7 +21,7 @@ from torch.autograd.function import once_differentiable
 
 from . import fp8 as _fp8
 from . import ops
-from ._oplib import custom_op, eager
+from ._oplib import custom_op, eager, refuse_tangents
 from .formats import (PACKED_OPERAND_SCHEMA_VERSION, SCALE_LAYOUT_CODES, MXFP8Tensor, make_mxfp8_tensor,
                       mxfp8_kernel_operands, mxfp8_qdata_2d, mxfp8_scales_for_kernel, reject_packed_dtype_conversion)
 
@@ -187,6 +187,7 @@ def mxfp8_grouped_linear(x: torch.Tensor, weight, offsets: torch.Tensor) -> torc
 
 
 def _packed(x, weight_data, weight_scales, offsets, n) -> torch.Tensor:
+    refuse_tangents("mxfp8_grouped_linear", x)
     if eager(x):
         return ops.mxfp8_grouped_linear_fwd_prequant_w(x, weight_data, weight_scales, offsets, n)
     return mxfp8_grouped_linear_prequant_w(x, weight_data, weight_scales, offsets, n)
@@ -199,6 +200,7 @@ def _forward(x, weight, offsets) -> torch.Tensor:
 
 
 def _dynamic(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor) -> torch.Tensor:
+    refuse_tangents("mxfp8_grouped_linear", x, weight)
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
         if torch.compiler.is_compiling():
             return mxfp8_grouped_linear_train(x, weight, offsets)

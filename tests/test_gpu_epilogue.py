@@ -479,6 +479,34 @@ def test_replaced_packed_storage_is_used(dev):
     assert torch.equal(got, want) and not torch.equal(got, first)
 
 
+def test_forward_mode_is_refused(dev):
+    import rtx_b200
+    from torch.autograd import forward_ad
+
+    x, w, b, r, _ = (t.to(dev) for t in inputs(20, 32, 32, seed=19))
+    with forward_ad.dual_level():
+        rtx_b200.mxfp8_linear_epilogue(x, w, b, r)                      # no tangents: nothing to drop
+        for i in range(4):
+            args = [x, w, b, r]
+            args[i] = forward_ad.make_dual(args[i], torch.ones_like(args[i]))
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                rtx_b200.mxfp8_linear_epilogue(*args)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            rtx_b200.mxfp8_linear_epilogue(forward_ad.make_dual(x, torch.ones_like(x)), rtx_b200.quantize_mxfp8(w), b, r)
+    with pytest.raises(NotImplementedError, match="forward-mode"):
+        torch.func.jvp(lambda t: rtx_b200.mxfp8_linear_epilogue(t, w, b, r), (x,), (torch.ones_like(x),))
+
+
+def test_vmap_runs_one_call_after_the_other(dev):
+    import rtx_b200
+
+    x, w, b, r, _ = (t.to(dev) for t in inputs(40, 32, 48, seed=20))
+    got = torch.func.vmap(lambda a, c: rtx_b200.mxfp8_linear_epilogue(a, w, b, c, activation="silu"))(
+        x.view(2, 20, 48), r.view(2, 20, 32))
+    want = [rtx_b200.mxfp8_linear_epilogue(x[i:i + 20], w, b, r[i:i + 20], activation="silu") for i in (0, 20)]
+    assert torch.equal(got, torch.stack(want))
+
+
 def test_second_derivatives_are_refused(dev):
     import rtx_b200
 

@@ -454,6 +454,30 @@ def test_replaced_packed_storage_is_used(dev):
     assert torch.equal(got, want) and not torch.equal(got, first)
 
 
+def test_forward_mode_is_refused(dev):
+    import rtx_b200
+    from torch.autograd import forward_ad
+
+    x, w, _ = inputs(60, 2, 128, 64, seed=18)
+    xd, wd, od = x.to(dev), w.to(dev), on(dev, offs(20, 30))
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(xd, torch.ones_like(xd))
+        for args in ((dual, wd), (xd, forward_ad.make_dual(wd, torch.ones_like(wd))), (dual, rtx_b200.quantize_mxfp8(wd))):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                rtx_b200.mxfp8_grouped_linear(*args, od)
+    with pytest.raises(NotImplementedError, match="forward-mode"):
+        torch.func.jvp(lambda t: rtx_b200.mxfp8_grouped_linear(t, wd, od), (xd,), (torch.ones_like(xd),))
+
+
+def test_vmap_runs_one_call_after_the_other(dev):
+    import rtx_b200
+
+    x, w, _ = inputs(60, 2, 128, 64, seed=19)
+    xd, wd, od = x.to(dev), w.to(dev), on(dev, offs(10, 15, head=2))
+    got = torch.func.vmap(lambda t: rtx_b200.mxfp8_grouped_linear(t, wd, od))(xd.view(2, 30, 64))
+    assert torch.equal(got, torch.stack([rtx_b200.mxfp8_grouped_linear(t, wd, od) for t in xd.view(2, 30, 64)]))
+
+
 def test_second_derivatives_are_refused(dev):
     import rtx_b200
 
