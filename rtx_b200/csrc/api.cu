@@ -998,10 +998,11 @@ int rtxb_mxfp8_linear_epilogue_bwd(const void* dy, int64_t lddy, const void* z, 
   q.s_t = mem.s_dzt;
   q.partial = mem.partial;
   const int64_t row_tiles = (m + 127) / 128, tiles = row_tiles * ((n + 127) / 128);
-  auto kernel = activation >= RTXB_ACT_SILU ? quant_mxfp8_act_backward_kernel<true> : quant_mxfp8_act_backward_kernel<false>;
-  cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), kActSmemBytes);
+  const bool lookup = activation >= RTXB_ACT_SILU;
+  auto kernel = lookup ? quant_mxfp8_act_backward_kernel<true> : quant_mxfp8_act_backward_kernel<false>;
+  cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), act_smem_bytes(lookup));
   if (e != cudaSuccess) return fail_cuda(e, "cudaFuncSetAttribute(activation backward quantizer)");
-  kernel<<<quant_grid(tiles, kActOccupancy), kQuantThreads, kActSmemBytes, s>>>(q);
+  kernel<<<quant_grid(tiles, kActOccupancy), kQuantThreads, act_smem_bytes(lookup), s>>>(q);
   RTXB_CHECK_LAUNCH("quant_mxfp8_act_backward_kernel");
   TransposedParams t = {};
   if (dw)

@@ -29,13 +29,15 @@ struct QuantActParams {
 constexpr int kActOccupancy = 3;                  // resident blocks per SM (registers)
 constexpr int kActSumRows = kQuantThreads / 32;   // partial column sums per tile before the last step, one per warp
 
-// z has eight significant bits, so between 2^-21 and 32 it takes 26 x 128 magnitudes: the slopes of silu and the gelus
-// are looked up.  Each of them is 1/2 plus an odd function (f(z) - f(-z) = z), so the table holds act'(|z|) - 1/2 and the
-// sign of z is put on it.  Below 2^-21 the slope is within 4e-7 of 1/2, from 32 on it is 1.  That is a third of the
-// instructions of an evaluation, and instructions are what bounds the pass.
-constexpr int kSlopeLow = 106 << 7, kSlopeHigh = 132 << 7;     // BF16 magnitudes of 2^-21 and 32
+// z has eight significant bits, so between 2^-21 and 128 it takes 28 x 128 magnitudes: the slopes of silu and the gelus are
+// looked up.  For each of them act'(z) = 1 - act'(-z) (f(z) - f(-z) = z), so the table holds the slopes of negative z, which
+// keep their relative accuracy however small, and a positive z takes 1 less its entry.  Below 2^-21 the slope is within
+// 8e-7 of 1/2, beyond +-128 it is 1 or 0.  That is a third of the instructions of an evaluation, and instructions are what
+// bounds the pass.  A second table for positive z saves three instructions a pair and is slower (98 -> 122 us at the size
+// above; relu, which reads no table, 88 -> 110): three blocks with 31 KB of tables each leave L1 too little.
+constexpr int kSlopeLow = 106 << 7, kSlopeHigh = 134 << 7;     // BF16 magnitudes of 2^-21 and 128
 constexpr int kSlopeEntries = kSlopeHigh - kSlopeLow + 1;
-constexpr int kActSmemBytes = kQtTileBytes + (kSlopeEntries * 4 + 15) / 16 * 16;
+constexpr int act_smem_bytes(bool lookup) { return kQtTileBytes + (lookup ? (kSlopeEntries * 4 + 15) / 16 * 16 : 0); }
 
 // Eight gradients dy act'(z) as four pairs.  LOOKUP: from the table; else relu, relu2 or none by `act`.
 template <bool LOOKUP>
@@ -48,9 +50,10 @@ __device__ __forceinline__ void act_gradient8(const float* table, int act, const
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const uint32_t mag = __vminu2(__vmaxu2(w[e] & 0x7FFF7FFFu, kSlopeLow * 0x10001u), kSlopeHigh * 0x10001u);
-      const uint32_t u0 = __float_as_uint(table[mag & 0xFFFFu]) ^ ((w[e] << 16) & 0x80000000u);
-      const uint32_t u1 = __float_as_uint(table[mag >> 16]) ^ (w[e] & 0x80000000u);
-      v[e] = mul2(v[e], add2(pack2(__uint_as_float(u0), __uint_as_float(u1)), both(0.5f)));
+      // t for z < 0, 1 - t for z >= 0: sign t + (1 - sign) / 2 with sign = -1 for z >= 0
+      const f32x2 sign = pack2(__uint_as_float((~(w[e] << 16) & 0x80000000u) | 0x3F800000u),
+                               __uint_as_float((~w[e] & 0x80000000u) | 0x3F800000u));
+      v[e] = mul2(v[e], fma2(pack2(table[mag & 0xFFFFu], table[mag >> 16]), sign, fma2(sign, both(-0.5f), both(0.5f))));
       m2 = absmax_bf16x2(m2, w[e]);
     }
     if (bf16_lo(m2) != bf16_lo(m2) || bf16_hi(m2) != bf16_hi(m2)) {   // a NaN among them: it goes on to dz
@@ -85,8 +88,8 @@ __global__ void __launch_bounds__(kQuantThreads, kActOccupancy) quant_mxfp8_act_
       for (int i = kSlopeLow + threadIdx.x; i <= kSlopeHigh; i += kQuantThreads) {
         const float z = __uint_as_float(static_cast<uint32_t>(i) << 16);
         float a = 1.0f, b = 0.0f;
-        act_slope2<decltype(tag)::value>(a, b, z, 0.0f);
-        slopes[i] = a - 0.5f;
+        act_slope2<decltype(tag)::value>(a, b, -z, 0.0f);
+        slopes[i] = a;
       }
     });
     __syncthreads();
@@ -94,7 +97,7 @@ __global__ void __launch_bounds__(kQuantThreads, kActOccupancy) quant_mxfp8_act_
   const int col_tiles = (p.n + 127) / 128, row_tiles = (p.m + 127) / 128;
   const int np = (p.n + 31) / 32 * 32, mp = (p.m + 31) / 32 * 32;
   const bool vec_dy = (p.lddy % 8 == 0) && ((reinterpret_cast<uintptr_t>(p.dy) & 15) == 0);
-  const bool vec_z = (p.n % 8 == 0) && ((reinterpret_cast<uintptr_t>(p.z) & 15) == 0);   // true without z
+  const bool vec_z = p.z == nullptr || ((p.n % 8 == 0) && ((reinterpret_cast<uintptr_t>(p.z) & 15) == 0));
   const int c8 = (threadIdx.x & 15) * 8, r0 = threadIdx.x >> 4;
   const int64_t total = static_cast<int64_t>(row_tiles) * col_tiles;
   // tile (rt, ct); the grid's stride in both, so that no tile costs a division

@@ -466,6 +466,29 @@ def test_experts_and_epilogue_as_used_together(dev):
     within(xd.grad, total, 2.0 ** -8 * total.abs() + (1 + 2.0 ** -8) * bound)
 
 
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh"])
+def test_small_slopes_keep_their_relative_accuracy(dev, act):
+    """One row, so that dbias is dz: every BF16 z in [-64, -2], where the slopes fall from 0.1 to nothing.
+
+    Beside the BF16 rounding: the exponent (up to z^2 / 2 = 90 where a slope above 1e-30 is left) is off by a rounding or
+    two, 90 * 2^-22 = 2^-15 of the slope, a dozen other roundings less than that; gelu's Phi(z) is off by at most 0.08 of
+    itself and 1 / z^2 of the slope there, at most 3e-4 over this range (at z = -12: 0.032 / 144).  2^-11 covers both."""
+    import rtx_b200
+
+    bits = torch.arange(0xC000, 0xC281, dtype=torch.int32)              # -2 ... -64
+    z = (bits - 65536).to(torch.int16).view(torch.bfloat16)[None]
+    assert z[0, 0] == -2 and z[0, -1] == -64
+    n = z.shape[1]
+    x, w = torch.zeros(1, 32, dtype=torch.bfloat16), torch.zeros(n, 32, dtype=torch.bfloat16)
+    db = rtx_b200.mxfp8_linear_epilogue_backward(torch.ones(1, n, device=dev).bfloat16(), z.to(dev), x.to(dev), w.to(dev),
+                                                 activation=act)[2].double().cpu()
+    want = slope64(z[0].double(), act)
+    live = want.abs() > 1e-30
+    off = (db - want).abs()[live] / want.abs()[live]
+    assert live.sum() > 150 and (off <= 2.0 ** -8 + 2.0 ** -11).all(), off.max().item()
+    assert (db.abs() <= 2 * want.abs() + 1e-36).all()
+
+
 def test_replaced_packed_storage_is_used(dev):
     """A packed weight whose storage is exchanged (a reload in place) is read where it now is."""
     import rtx_b200
