@@ -347,9 +347,9 @@ gemm_grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
       if (holder) {
         tmem_ld_32x32(tacc + shared0, r);
         tmem_ld_wait();
-        tc_fence_before_sync();
-        __syncwarp();
       }
+      tc_fence_before_sync();
+      __syncwarp();
       if (lane == 0) mbar_arrive_cluster(overlap_addr);
       if (holder) emit(shared0, r);
 #pragma unroll 1
