@@ -523,7 +523,11 @@ __device__ __forceinline__ bool act_epilogue_tile(const GemmParams& p, uint32_t 
   if (res_ahead) act_load_residual(p, res, row, row_ok && col_base + 32 * first < p.out_cols, col_base + 32 * first);
   if (!mbar_wait(acc_full_bar, parity, abort_flag)) return false;
   tc_fence_after_sync();
-  if (!holder && lane == 0) mbar_arrive_cluster(overlap_bar_addr);
+  if (!holder) {
+    tc_fence_before_sync();   // the reads of the tile before
+    __syncwarp();
+    if (lane == 0) mbar_arrive_cluster(overlap_bar_addr);
+  }
 #pragma unroll 1
   for (int i = 0; i < 4; ++i) {
     const int c = 32 * ((first + i) & 3), col = col_base + c;
