@@ -217,6 +217,7 @@ def mxfp8_linear_epilogue_backward(grad_output: torch.Tensor, z: Optional[torch.
                                    bias: bool = True) -> Tuple[torch.Tensor, torch.Tensor, Optional[torch.Tensor]]:
     """BF16 (dX, dW, dbias) of `mxfp8_linear_epilogue`; `z` is the pre-activation in BF16 (None for activation "none"),
     `bias=False` leaves dbias out (None).  The residual's gradient is grad_output."""
+    refuse_tangents("mxfp8_linear_epilogue_backward", grad_output, z, x, weight)
     n, k = weight.shape
     if activation != "none" and z is None:
         raise ValueError("an activation's backward needs the pre-activation z")

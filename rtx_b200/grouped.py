@@ -212,6 +212,7 @@ def mxfp8_grouped_linear_backward(grad_output: torch.Tensor, x: torch.Tensor, we
                                   offsets: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """BF16 dX [rows, K] and dW [groups, N, K] of `mxfp8_grouped_linear`, from independently quantized MXFP8 products
     (blocks along N for dX, along each group's rows for dW)."""
+    refuse_tangents("mxfp8_grouped_linear_backward", grad_output, x, weight)
     if eager(x):
         return mxfp8_grouped_linear_bwd.fn(grad_output, x, weight, offsets)
     return mxfp8_grouped_linear_bwd(grad_output, x, weight, offsets)

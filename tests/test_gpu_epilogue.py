@@ -516,6 +516,8 @@ def test_forward_mode_is_refused(dev):
                 rtx_b200.mxfp8_linear_epilogue(*args)
         with pytest.raises(NotImplementedError, match="forward-mode"):
             rtx_b200.mxfp8_linear_epilogue(forward_ad.make_dual(x, torch.ones_like(x)), rtx_b200.quantize_mxfp8(w), b, r)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            rtx_b200.mxfp8_linear_epilogue_backward(forward_ad.make_dual(r, torch.ones_like(r)), None, x, w)
     with pytest.raises(NotImplementedError, match="forward-mode"):
         torch.func.jvp(lambda t: rtx_b200.mxfp8_linear_epilogue(t, w, b, r), (x,), (torch.ones_like(x),))
 

@@ -465,6 +465,8 @@ def test_forward_mode_is_refused(dev):
         for args in ((dual, wd), (xd, forward_ad.make_dual(wd, torch.ones_like(wd))), (dual, rtx_b200.quantize_mxfp8(wd))):
             with pytest.raises(NotImplementedError, match="forward-mode"):
                 rtx_b200.mxfp8_grouped_linear(*args, od)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            rtx_b200.mxfp8_grouped_linear_backward(torch.ones(60, 128, device=dev).bfloat16(), dual, wd, od)
     with pytest.raises(NotImplementedError, match="forward-mode"):
         torch.func.jvp(lambda t: rtx_b200.mxfp8_grouped_linear(t, wd, od), (xd,), (torch.ones_like(xd),))
 
