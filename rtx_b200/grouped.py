@@ -157,7 +157,7 @@ class _GroupedLinearFunction(torch.autograd.Function):
 
 
 def _packed_group_shape(weight) -> Tuple[int, int, int]:
-    shape = tuple(int(v) for v in weight._rtx_logical_shape)
+    shape = weight._rtx_logical_shape
     if len(shape) != 3:
         raise ValueError(f"a packed group weight has the logical shape (groups, N, K), got {shape}")
     if shape[0] > 1 and shape[1] % 128:

@@ -325,10 +325,6 @@ def _bytes(query: str, *sizes: int) -> int:
     return N.query(query, *sizes)
 
 
-def _new(device: torch.device, *shape: int) -> torch.Tensor:
-    return torch.empty(shape, dtype=torch.bfloat16, device=device)
-
-
 def _scratch(device: torch.device, nbytes: int) -> torch.Tensor:
     """Workspace of one call: a fresh allocation of the calling stream, so that calls on several streams and captured
     graphs share nothing."""
@@ -412,8 +408,8 @@ def mxfp8_linear_epilogue_fwd(x: torch.Tensor, w: torch.Tensor, bias: Optional[t
     bias, residual, ldr = _bias_and_residual(x, m, n, bias, residual)
     code = activation_code(activation)
     with _on(device):
-        out = _new(device, m, n)
-        z = _new(device, m, n) if keep_z else None
+        out = x.new_empty(m, n)
+        z = x.new_empty(m, n) if keep_z else None
         if m and n:
             nbytes = _bytes("rtxb_mxfp8_linear_epilogue_workspace_bytes", m, n, k, 1)
             buf = _scratch(device, nbytes)
@@ -435,7 +431,7 @@ def mxfp8_linear_epilogue_fwd_prequant_w(x: torch.Tensor, qw: torch.Tensor, sw: 
     bias, residual, ldr = _bias_and_residual(x, m, n, bias, residual)
     code = activation_code(activation)
     with _on(device):
-        out = _new(device, m, n)
+        out = x.new_empty(m, n)
         if m and n:
             nbytes = _bytes("rtxb_mxfp8_linear_epilogue_workspace_bytes", m, n, k, 0)
             buf = _scratch(device, nbytes)
@@ -470,9 +466,9 @@ def mxfp8_linear_epilogue_bwd(dy: torch.Tensor, z: Optional[torch.Tensor], x: Op
     if not (need_dx or need_dw or need_dbias):
         return None, None, None
     with _on(device):
-        dx = _new(device, m, k) if need_dx else None
-        dw = _new(device, n, k) if need_dw else None
-        db = _new(device, n) if need_dbias else None
+        dx = dy.new_empty(m, k) if need_dx else None
+        dw = dy.new_empty(n, k) if need_dw else None
+        db = dy.new_empty(n) if need_dbias else None
         if min(m, n, k) == 0:             # an empty sum is zero
             return tuple(None if t is None else t.zero_() for t in (dx, dw, db))
         nbytes = _bytes("rtxb_mxfp8_linear_epilogue_backward_workspace_bytes", m, n, k, int(need_dx), int(need_dw),
@@ -514,7 +510,7 @@ def _group_weight(w: torch.Tensor, device: torch.device) -> torch.Tensor:
 
 def _grouped_out(out: Optional[torch.Tensor], x: torch.Tensor, n: int) -> Tuple[torch.Tensor, int]:
     if out is None:
-        return _new(x.device, x.shape[0], n), n
+        return x.new_empty(x.shape[0], n), n
     held, ldo = _rows_of(out, n, "out")
     if held is not out or out.shape[0] != x.shape[0] or out.device != x.device:
         raise ValueError(f"out must be [{x.shape[0]}, {n}] with contiguous rows on the operands' device")
@@ -584,8 +580,8 @@ def mxfp8_grouped_linear_bwd(dy: torch.Tensor, x: Optional[torch.Tensor], w: Opt
     if not (need_dx or need_dw):
         return None, None
     with _on(device):
-        dx = _new(device, rows, k) if need_dx else None
-        dw = _new(device, groups, n, k) if need_dw else None
+        dx = dy.new_empty(rows, k) if need_dx else None
+        dw = dy.new_empty(groups, n, k) if need_dw else None
         if min(rows, n, k) == 0:          # an empty sum is zero
             return (dx.zero_() if need_dx else None), (dw.zero_() if need_dw else None)
         nbytes = _bytes("rtxb_mxfp8_grouped_backward_workspace_bytes", rows, n, k, groups, int(need_dx), int(need_dw))
