@@ -17,7 +17,9 @@
 // In between, the weights of groups with one partial tile each: 8192 rows in 32 uneven groups of 2048 x 4096 take 79 us
 // where weights and rows are 51 us of HBM and the MMAs 46: pairs are 88 to 120 k cycles busy, since tiles of unlike size
 // are dealt out in turn.  Dealing the full tiles first and the partial ones by size was no faster (86 us): groups of
-// several tiles lose their weights from L2 in between, 413 MB read instead of 312.
+// several tiles lose their weights from L2 in between, 413 MB read instead of 312.  Handing tiles out as pairs come free (a
+// counter in memory, drawn ahead by an idle warp and passed on through shared memory) was slower everywhere: whole forward
+// 96.6 -> 98.9 us, backward with its short dW tiles 476 -> 529, however many tiles were drawn ahead.
 //
 // Roles, TMEM plan and ring as in gemm_blockscaled_pair_kernel; what differs: tiles come from the plan the quantizer
 // left, N and the number of K steps are per tile, and the epilogue holds one output column per lane, so a chunk of 32
