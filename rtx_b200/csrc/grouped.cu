@@ -39,8 +39,10 @@ int launch_quantize_transposed(TransposedParams& p, int64_t x_tiles, cudaStream_
   if (units > INT32_MAX) return fail_msg(RTXB_E_UNSUPPORTED, "operand exceeds the 32-bit unit count of the quantizer");
   int64_t blocks = (units + 7) / 8;
   if (p.partial && blocks < (p.n + 31) / 32) blocks = (p.n + 31) / 32;
-  const cudaError_t e = launch_dependent(quant_mxfp8_transposed_units_kernel, quant_grid(blocks, kTransposedOccupancy),
-                                         kQuantThreads, 0, stream, true, p);
+  cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(quant_mxfp8_transposed_units_kernel), kTransposedSmemBytes);
+  if (e != cudaSuccess) return fail_cuda(e, "cudaFuncSetAttribute(transposed quantizer)");
+  e = launch_dependent(quant_mxfp8_transposed_units_kernel, quant_grid(blocks, kTransposedOccupancy), kQuantThreads,
+                       kTransposedSmemBytes, stream, true, p);
   if (e != cudaSuccess) return fail_cuda(e, "quant_mxfp8_transposed_units_kernel launch");
   return RTXB_OK;
 }

@@ -345,19 +345,23 @@ __global__ void __launch_bounds__(kQuantThreads, kRowsOccupancy) quant_mxfp8_row
 // 776 x 520: 37.6 -> 31.0 us), because the two passes run side by side and a warp's unit is a quarter of a tile's work.
 // ---------------------------------------------------------------------------
 constexpr int kTransposedOccupancy = 3;
+constexpr int kTransposedStageBytes = 64 * 128;   // of one warp
+constexpr int kTransposedSmemBytes = kQuantThreads / 32 * kTransposedStageBytes;
 
-// 64 columns from `col0` of a 128-row tile with `live` rows; payload bytes [k0, k0 + 128) of each column
+// 64 columns from `col0` of a 128-row tile with `live` rows; payload bytes [k0, k0 + 128) of each column, through `stage`
+// (8 KB of this warp's): a lane holds 32 bytes of a column, a line of the payload is 128
 __device__ __forceinline__ void quant_mxfp8_transposed_unit(const TransposedOperand& o, const __nv_bfloat16* src, int live,
-                                                            uint8_t* q, uint8_t* scales, int64_t k0, int chunk, int col0) {
+                                                            uint8_t* q, uint8_t* scales, int64_t k0, int chunk, int col0,
+                                                            uint8_t* stage) {
   const int lane = threadIdx.x & 31;
   const int c = col0 + 2 * lane;
   const bool ok0 = c < o.cols, ok1 = c + 1 < o.cols;
   const bool pairs = (o.ld & 1) == 0 && (reinterpret_cast<uintptr_t>(o.src) & 3) == 0;   // both columns in one load
   const uint16_t* at = reinterpret_cast<const uint16_t*>(src) + c;
+  const int bytes = static_cast<int>(min(static_cast<int64_t>(128), o.pitch - k0));       // a multiple of 32
   uint32_t word0 = 0, word1 = 0;   // the four scale bytes of either column
 #pragma unroll 1
-  for (int j = 0; j < 4; ++j) {
-    if (k0 + 32 * j >= o.pitch) break;
+  for (int j = 0; 32 * j < bytes; ++j) {
     uint32_t w[32];
     if (pairs && 32 * j + 32 <= live && ok1) {
 #pragma unroll
@@ -378,25 +382,32 @@ __device__ __forceinline__ void quant_mxfp8_transposed_unit(const TransposedOper
     const f32x2 recip = pack2(e8m0_reciprocal(code0), e8m0_reciprocal(code1));
     word0 |= code0 << (8 * j);
     word1 |= code1 << (8 * j);
-    uint32_t o0[8], o1[8];
+    // 16-byte chunk i of column c at chunk i ^ (c / 2 % 8): no two of eight lanes meet in a bank, here or below
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      f32x2 v[4];
+    for (int h = 0; h < 2; ++h) {
+      uint32_t o0[4], o1[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = mul2(unpack_bf16x2(w[4 * e + i]), recip);
-      o0[e] = cvt_e4m3x2(lo(v[0]), lo(v[1])) | (cvt_e4m3x2(lo(v[2]), lo(v[3])) << 16);
-      o1[e] = cvt_e4m3x2(hi(v[0]), hi(v[1])) | (cvt_e4m3x2(hi(v[2]), hi(v[3])) << 16);
+      for (int e = 0; e < 4; ++e) {
+        f32x2 v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = mul2(unpack_bf16x2(w[16 * h + 4 * e + i]), recip);
+        o0[e] = cvt_e4m3x2(lo(v[0]), lo(v[1])) | (cvt_e4m3x2(lo(v[2]), lo(v[3])) << 16);
+        o1[e] = cvt_e4m3x2(hi(v[0]), hi(v[1])) | (cvt_e4m3x2(hi(v[2]), hi(v[3])) << 16);
+      }
+      uint8_t* chunk_at = stage + lane * 256 + (((2 * j + h) ^ (lane & 7)) << 4);
+      *reinterpret_cast<uint4*>(chunk_at) = make_uint4(o0[0], o0[1], o0[2], o0[3]);
+      *reinterpret_cast<uint4*>(chunk_at + 128) = make_uint4(o1[0], o1[1], o1[2], o1[3]);
     }
-    uint8_t* dst = q + c * o.pitch + k0 + 32 * j;
-    if (ok0)
-      asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(o0[0]), "r"(o0[1]), "r"(o0[2]),
-                   "r"(o0[3]), "r"(o0[4]), "r"(o0[5]), "r"(o0[6]), "r"(o0[7])
-                   : "memory");
-    if (ok1)
-      asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst + o.pitch), "r"(o1[0]), "r"(o1[1]),
-                   "r"(o1[2]), "r"(o1[3]), "r"(o1[4]), "r"(o1[5]), "r"(o1[6]), "r"(o1[7])
-                   : "memory");
   }
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int col = 4 * i + (lane >> 3), part = lane & 7;
+    if (col0 + col < o.cols && part * 16 < bytes)
+      *reinterpret_cast<uint4*>(q + (col0 + col) * o.pitch + k0 + part * 16) =
+          *reinterpret_cast<const uint4*>(stage + col * 128 + ((part ^ ((col >> 1) & 7)) << 4));
+  }
+  __syncwarp();   // the stage is free again
   uint8_t* tile = scales + (static_cast<size_t>(c >> 7) * o.chunks + chunk) * 512;   // c is even: both columns in one tile
   if (ok0) *reinterpret_cast<uint32_t*>(tile + (c & 31) * 16 + ((c >> 5) & 3) * 4) = word0;
   if (ok1) *reinterpret_cast<uint32_t*>(tile + ((c + 1) & 31) * 16 + ((c >> 5) & 3) * 4) = word1;
@@ -404,6 +415,8 @@ __device__ __forceinline__ void quant_mxfp8_transposed_unit(const TransposedOper
 
 __global__ void __launch_bounds__(kQuantThreads, kTransposedOccupancy)
 quant_mxfp8_transposed_units_kernel(const TransposedParams p) {
+  extern __shared__ __align__(16) uint8_t qt_smem[];
+  uint8_t* stage = qt_smem + (threadIdx.x >> 5) * kTransposedStageBytes;
   __shared__ GroupScan scan;
   __shared__ float part[8][33];
   griddep_launch_dependents();
@@ -424,7 +437,7 @@ quant_mxfp8_transposed_units_kernel(const TransposedParams p) {
         live = scan.start[g + 1] - static_cast<int>(row0);
       }
       quant_mxfp8_transposed_unit(p.x, p.x.src + row0 * p.x.ld, min(128, live), p.x.q, p.x.scales, 128ll * rt, rt,
-                                  (u - rt * p.x_col_units) * 64);
+                                  (u - rt * p.x_col_units) * 64, stage);
     } else {
       const uint32_t v = u - x_units;
       const uint32_t rt = v / p.w_col_units;
@@ -434,7 +447,7 @@ quant_mxfp8_transposed_units_kernel(const TransposedParams p) {
       quant_mxfp8_transposed_unit(o, o.src + (static_cast<int64_t>(e) * o.rows + 128 * nt) * o.ld,
                                   min(128, o.rows - static_cast<int>(128 * nt)), o.q + e * (o.cols * o.pitch),
                                   o.scales + static_cast<size_t>(e) * ((o.cols + 127) / 128) * o.chunks * 512, 128ll * nt, nt,
-                                  (v - rt * p.w_col_units) * 64);
+                                  (v - rt * p.w_col_units) * 64, stage);
     }
   }
   griddep_wait();   // the launch before this one is complete: whoever waits for this grid has waited for that one too
