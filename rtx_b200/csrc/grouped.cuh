@@ -336,87 +336,58 @@ __global__ void __launch_bounds__(kQuantThreads, kRowsOccupancy) quant_mxfp8_row
 
 // ---------------------------------------------------------------------------
 // Transposed quantizer of the backward's operands that are quantized one way only: x (by group, for dW) and the weight
-// matrices (for dX).  One lane owns two neighbouring columns and walks down 32 rows at a time: the block is in its
-// registers, so there is no staging, no exchange and no barrier.  A warp reads 128-byte row segments, 32 of them in
-// flight, and writes 32-byte sectors, four next to one another per column (128 rows = one K step of the GEMM).
-// HBM bound with a sector-sized write pattern: 8192 x 4096 rows and 4 weights of 4096 x 4096 (201 MB read, 104 MB written)
-// in 59 us, 5.2 TB/s, 0.79 of the copy rate.  Against the staged 128 x 128 tiles of the gradient's pass for these operands
-// too: the same for large ones (the step is power bound), but a small backward ends sooner (777 rows, 12 groups,
-// 776 x 520: 37.6 -> 31.0 us), because the two passes run side by side and a warp's unit is a quarter of a tile's work.
+// matrices (for dX).  A warp takes 64 columns of a 128-row tile; one lane owns two neighbouring columns and walks down 32
+// rows at a time, so that a block is in its registers and its maximum needs no exchange.  The blocks come through shared
+// memory, two ahead of the one at work (with loads into the registers themselves 96 KB are in flight per SM only while
+// nothing is computed), and the payload leaves through it, because a lane holds 32 bytes of a column whose K step is 128.
+// No barrier but the warp's own.  Both quantizers of the backward together, 8192 rows, 32 groups, 2048 x 4096 (604 MB read,
+// 336 MB written): 253 us with direct loads and stores, 225 with staged stores, 195 with blocks fetched ahead too, 4.8 TB/s.
 // ---------------------------------------------------------------------------
-constexpr int kTransposedOccupancy = 3;
-constexpr int kTransposedStageBytes = 64 * 128;   // of one warp
-constexpr int kTransposedSmemBytes = kQuantThreads / 32 * kTransposedStageBytes;
+constexpr int kTransposedOccupancy = 2;
+constexpr int kTransposedFetchBytes = 32 * 128;   // a block of 64 columns
+constexpr int kTransposedStageBytes = 64 * 64;    // 64 bytes of each column's payload
+constexpr int kTransposedWarpBytes = 2 * kTransposedFetchBytes + kTransposedStageBytes;
+constexpr int kTransposedSmemBytes = kQuantThreads / 32 * kTransposedWarpBytes;
 
-// 64 columns from `col0` of a 128-row tile with `live` rows; payload bytes [k0, k0 + 128) of each column, through `stage`
-// (8 KB of this warp's): a lane holds 32 bytes of a column, a line of the payload is 128
-__device__ __forceinline__ void quant_mxfp8_transposed_unit(const TransposedOperand& o, const __nv_bfloat16* src, int live,
-                                                            uint8_t* q, uint8_t* scales, int64_t k0, int chunk, int col0,
-                                                            uint8_t* stage) {
+// what one warp does at a time: 64 columns of a 128-row tile, four blocks of 32 rows
+struct TransposedUnit {
+  const uint16_t* src;   // first row, first column
+  uint8_t* q;            // payload of the first column, at the tile's K step
+  uint8_t* scales;       // 512-byte scale tile of the first column's 128 columns
+  int live, cols, bytes; // rows, columns (from the first one on) and payload bytes of a column
+  int col0;
+  int is_x;
+};
+
+// block j of the unit into `buf` [32 rows][64 columns]; what lies outside the operand is zero
+__device__ __forceinline__ void quant_mxfp8_transposed_fetch(const TransposedUnit& f, int64_t ld, bool vec, int j, uint8_t* buf) {
   const int lane = threadIdx.x & 31;
-  const int c = col0 + 2 * lane;
-  const bool ok0 = c < o.cols, ok1 = c + 1 < o.cols;
-  const bool pairs = (o.ld & 1) == 0 && (reinterpret_cast<uintptr_t>(o.src) & 3) == 0;   // both columns in one load
-  const uint16_t* at = reinterpret_cast<const uint16_t*>(src) + c;
-  const int bytes = static_cast<int>(min(static_cast<int64_t>(128), o.pitch - k0));       // a multiple of 32
-  uint32_t word0 = 0, word1 = 0;   // the four scale bytes of either column
-#pragma unroll 1
-  for (int j = 0; 32 * j < bytes; ++j) {
-    uint32_t w[32];
-    if (pairs && 32 * j + 32 <= live && ok1) {
+  if (vec) {
+    const int c8 = (lane & 7) * 8, r0 = 32 * j + (lane >> 3);
+    const uint16_t* at = f.src + r0 * ld + c8;
 #pragma unroll
-      for (int e = 0; e < 32; ++e) w[e] = __ldg(reinterpret_cast<const uint32_t*>(at + e * o.ld));
-    } else {
-#pragma unroll
-      for (int e = 0; e < 32; ++e) {
-        const bool row = 32 * j + e < live;
-        const uint32_t a = row && ok0 ? at[e * o.ld] : 0u, b = row && ok1 ? at[e * o.ld + 1] : 0u;
-        w[e] = a | (b << 16);
-      }
+    for (int i = 0; i < 8; ++i) {
+      const bool valid = r0 + 4 * i < f.live && c8 < f.cols;   // cols is a multiple of 8 here
+      cp_async_16(buf + (4 * i + (lane >> 3)) * 128 + c8 * 2, valid ? at + 4 * i * ld : f.src, valid);
     }
-    at += 32 * o.ld;
-    uint32_t m2 = 0;
-#pragma unroll
-    for (int e = 0; e < 32; ++e) m2 = absmax_bf16x2(m2, w[e]);
-    const uint32_t code0 = e8m0_from_amax(bf16_lo(m2), true), code1 = e8m0_from_amax(bf16_hi(m2), true);
-    const f32x2 recip = pack2(e8m0_reciprocal(code0), e8m0_reciprocal(code1));
-    word0 |= code0 << (8 * j);
-    word1 |= code1 << (8 * j);
-    // 16-byte chunk i of column c at chunk i ^ (c / 2 % 8): no two of eight lanes meet in a bank, here or below
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      uint32_t o0[4], o1[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        f32x2 v[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = mul2(unpack_bf16x2(w[16 * h + 4 * e + i]), recip);
-        o0[e] = cvt_e4m3x2(lo(v[0]), lo(v[1])) | (cvt_e4m3x2(lo(v[2]), lo(v[3])) << 16);
-        o1[e] = cvt_e4m3x2(hi(v[0]), hi(v[1])) | (cvt_e4m3x2(hi(v[2]), hi(v[3])) << 16);
-      }
-      uint8_t* chunk_at = stage + lane * 256 + (((2 * j + h) ^ (lane & 7)) << 4);
-      *reinterpret_cast<uint4*>(chunk_at) = make_uint4(o0[0], o0[1], o0[2], o0[3]);
-      *reinterpret_cast<uint4*>(chunk_at + 128) = make_uint4(o1[0], o1[1], o1[2], o1[3]);
+  } else {
+    const int c = 2 * lane;
+    const uint16_t* at = f.src + 32 * j * ld + c;
+#pragma unroll 8
+    for (int e = 0; e < 32; ++e) {
+      const bool row = 32 * j + e < f.live;
+      const uint32_t a = row && c < f.cols ? at[e * ld] : 0u, b = row && c + 1 < f.cols ? at[e * ld + 1] : 0u;
+      *reinterpret_cast<uint32_t*>(buf + e * 128 + 4 * lane) = a | (b << 16);
     }
   }
-  __syncwarp();
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int col = 4 * i + (lane >> 3), part = lane & 7;
-    if (col0 + col < o.cols && part * 16 < bytes)
-      *reinterpret_cast<uint4*>(q + (col0 + col) * o.pitch + k0 + part * 16) =
-          *reinterpret_cast<const uint4*>(stage + col * 128 + ((part ^ ((col >> 1) & 7)) << 4));
-  }
-  __syncwarp();   // the stage is free again
-  uint8_t* tile = scales + (static_cast<size_t>(c >> 7) * o.chunks + chunk) * 512;   // c is even: both columns in one tile
-  if (ok0) *reinterpret_cast<uint32_t*>(tile + (c & 31) * 16 + ((c >> 5) & 3) * 4) = word0;
-  if (ok1) *reinterpret_cast<uint32_t*>(tile + ((c + 1) & 31) * 16 + ((c >> 5) & 3) * 4) = word1;
+  cp_async_commit();
 }
 
 __global__ void __launch_bounds__(kQuantThreads, kTransposedOccupancy)
 quant_mxfp8_transposed_units_kernel(const TransposedParams p) {
   extern __shared__ __align__(16) uint8_t qt_smem[];
-  uint8_t* stage = qt_smem + (threadIdx.x >> 5) * kTransposedStageBytes;
+  uint8_t* buf = qt_smem + (threadIdx.x >> 5) * kTransposedWarpBytes;
+  uint8_t* stage = buf + 2 * kTransposedFetchBytes;
   __shared__ GroupScan scan;
   __shared__ float part[8][33];
   griddep_launch_dependents();
@@ -425,36 +396,118 @@ quant_mxfp8_transposed_units_kernel(const TransposedParams p) {
   const uint32_t x_tiles = !p.x.src ? 0 : grouped ? scan.tile[p.list.groups] : (p.x.rows + 127) / 128;
   const uint32_t x_units = x_tiles * p.x_col_units;
   const uint32_t units = x_units + (p.w.src ? p.batches * p.w_row_tiles * p.w_col_units : 0u);   // < 2^31 (host)
-  for (uint32_t u = blockIdx.x * (kQuantThreads / 32) + (threadIdx.x >> 5); u < units;
-       u += gridDim.x * (kQuantThreads / 32)) {
-    if (u < x_units) {
-      const uint32_t rt = u / p.x_col_units;
-      int64_t row0 = 128ll * rt;
-      int live = p.x.rows - static_cast<int>(row0);
-      if (grouped) {
-        const int g = group_before(scan.tile, p.list.groups, rt);
-        row0 = scan.start[g] + 128ll * (rt - scan.tile[g]);
-        live = scan.start[g + 1] - static_cast<int>(row0);
-      }
-      quant_mxfp8_transposed_unit(p.x, p.x.src + row0 * p.x.ld, min(128, live), p.x.q, p.x.scales, 128ll * rt, rt,
-                                  (u - rt * p.x_col_units) * 64, stage);
+  auto locate = [&](uint32_t u) {
+    TransposedUnit f;
+    f.is_x = u < x_units;
+    const TransposedOperand& o = f.is_x ? p.x : p.w;
+    const uint32_t v = f.is_x ? u : u - x_units;
+    const uint32_t col_units = f.is_x ? p.x_col_units : p.w_col_units;
+    uint32_t rt = v / col_units, e = 0;
+    f.col0 = (v - rt * col_units) * 64;
+    int64_t row0;
+    if (!f.is_x) {
+      e = rt / p.w_row_tiles;
+      rt -= e * p.w_row_tiles;
+      row0 = static_cast<int64_t>(e) * o.rows + 128 * rt;
+      f.live = o.rows - static_cast<int>(128 * rt);
+    } else if (grouped) {
+      const int g = group_before(scan.tile, p.list.groups, rt);
+      row0 = scan.start[g] + 128ll * (rt - scan.tile[g]);
+      f.live = scan.start[g + 1] - static_cast<int>(row0);
     } else {
-      const uint32_t v = u - x_units;
-      const uint32_t rt = v / p.w_col_units;
-      const uint32_t e = rt / p.w_row_tiles;
-      const uint32_t nt = rt - e * p.w_row_tiles;
-      const TransposedOperand& o = p.w;
-      quant_mxfp8_transposed_unit(o, o.src + (static_cast<int64_t>(e) * o.rows + 128 * nt) * o.ld,
-                                  min(128, o.rows - static_cast<int>(128 * nt)), o.q + e * (o.cols * o.pitch),
-                                  o.scales + static_cast<size_t>(e) * ((o.cols + 127) / 128) * o.chunks * 512, 128ll * nt, nt,
-                                  (v - rt * p.w_col_units) * 64, stage);
+      row0 = 128ll * rt;
+      f.live = o.rows - static_cast<int>(row0);
     }
+    f.live = min(128, f.live);
+    f.src = reinterpret_cast<const uint16_t*>(o.src) + row0 * o.ld + f.col0;
+    f.cols = o.cols - f.col0;
+    f.bytes = static_cast<int>(min(static_cast<int64_t>(128), o.pitch - static_cast<int64_t>(128 * rt)));   // a multiple of 32
+    f.q = o.q + (static_cast<int64_t>(e) * o.cols + f.col0) * o.pitch + 128ll * rt;
+    f.scales = o.scales + ((static_cast<size_t>(e) * ((o.cols + 127) / 128) + (f.col0 >> 7)) * o.chunks + rt) * 512;
+    return f;
+  };
+  auto vec_of = [](const TransposedOperand& o) {
+    return o.ld % 8 == 0 && o.cols % 8 == 0 && (reinterpret_cast<uintptr_t>(o.src) & 15) == 0;
+  };
+  const bool vec_x = vec_of(p.x), vec_w = vec_of(p.w);
+  auto fetch = [&](const TransposedUnit& f, int j) {
+    quant_mxfp8_transposed_fetch(f, f.is_x ? p.x.ld : p.w.ld, f.is_x ? vec_x : vec_w, j, buf + (j & 1) * kTransposedFetchBytes);
+  };
+  const int lane = threadIdx.x & 31;
+  const uint32_t stride = gridDim.x * (kQuantThreads / 32);
+  uint32_t u = blockIdx.x * (kQuantThreads / 32) + (threadIdx.x >> 5);
+  TransposedUnit f, ahead;
+  if (u < units) {
+    f = ahead = locate(u);
+    fetch(f, 0);
+    fetch(f, 1);
   }
+  for (; u < units; u += stride, f = ahead) {
+    const int64_t pitch = f.is_x ? p.x.pitch : p.w.pitch;
+    uint32_t word0 = 0, word1 = 0;   // the four scale bytes of either column
+#pragma unroll 1
+    for (int j = 0; j < 4; ++j) {
+      cp_async_wait<1>();            // everything but the newest group: block j is here
+      __syncwarp();
+      const uint8_t* rows = buf + (j & 1) * kTransposedFetchBytes + 4 * lane;
+      uint32_t w[32];
+#pragma unroll
+      for (int e = 0; e < 32; ++e) w[e] = *reinterpret_cast<const uint32_t*>(rows + e * 128);
+      __syncwarp();
+      // the buffer takes the block after the next one
+      if (j == 2 && u + stride < units) ahead = locate(u + stride);
+      if (j < 2) fetch(f, j + 2);
+      else if (u + stride < units) fetch(ahead, j - 2);
+      else cp_async_commit();
+      if (32 * j >= f.bytes) continue;
+      uint32_t m2 = 0;
+#pragma unroll
+      for (int e = 0; e < 32; ++e) m2 = absmax_bf16x2(m2, w[e]);
+      const uint32_t code0 = e8m0_from_amax(bf16_lo(m2), true), code1 = e8m0_from_amax(bf16_hi(m2), true);
+      const f32x2 recip = pack2(e8m0_reciprocal(code0), e8m0_reciprocal(code1));
+      word0 |= code0 << (8 * j);
+      word1 |= code1 << (8 * j);
+      // the stage holds 64 bytes of each column as four 16-byte chunks: chunk i of column c at chunk i ^ (c / 2 % 4) of row
+      // c ^ (c / 8 % 2): no two of eight lanes meet in a bank, here or below
+      uint8_t* at0 = stage + ((2 * lane) ^ ((lane >> 2) & 1)) * 64;
+      uint8_t* at1 = stage + ((2 * lane + 1) ^ ((lane >> 2) & 1)) * 64;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t o0[4], o1[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          f32x2 v[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[i] = mul2(unpack_bf16x2(w[16 * h + 4 * e + i]), recip);
+          o0[e] = cvt_e4m3x2(lo(v[0]), lo(v[1])) | (cvt_e4m3x2(lo(v[2]), lo(v[3])) << 16);
+          o1[e] = cvt_e4m3x2(hi(v[0]), hi(v[1])) | (cvt_e4m3x2(hi(v[2]), hi(v[3])) << 16);
+        }
+        const int chunk = ((2 * (j & 1) + h) ^ (lane & 3)) << 4;
+        *reinterpret_cast<uint4*>(at0 + chunk) = make_uint4(o0[0], o0[1], o0[2], o0[3]);
+        *reinterpret_cast<uint4*>(at1 + chunk) = make_uint4(o1[0], o1[1], o1[2], o1[3]);
+      }
+      if ((j & 1) == 0 && 32 * j + 32 < f.bytes) continue;
+      __syncwarp();
+      const int first = 64 * (j >> 1), part = lane & 3;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int col = 8 * i + (lane >> 2);
+        if (col < f.cols && first + 16 * part < f.bytes)
+          *reinterpret_cast<uint4*>(f.q + col * pitch + first + 16 * part) = *reinterpret_cast<const uint4*>(
+              stage + (col ^ ((col >> 3) & 1)) * 64 + ((part ^ ((col >> 1) & 3)) << 4));
+      }
+      __syncwarp();   // the stage is free again
+    }
+    const int c = (f.col0 & 127) + 2 * lane;   // within its 128 columns; even: both columns in one scale tile
+    if (2 * lane < f.cols) *reinterpret_cast<uint32_t*>(f.scales + (c & 31) * 16 + (c >> 5) * 4) = word0;
+    if (2 * lane + 1 < f.cols) *reinterpret_cast<uint32_t*>(f.scales + ((c + 1) & 31) * 16 + (c >> 5) * 4) = word1;
+  }
+  cp_async_wait<0>();
   griddep_wait();   // the launch before this one is complete: whoever waits for this grid has waited for that one too
   if (p.partial == nullptr) return;
   // dbias[c] = bf16( sum over the row tiles of partial[t][c] ): eight threads per column add every eighth tile, the eight
   // sums are added in a fixed order
-  const int lane = threadIdx.x & 31, k = threadIdx.x >> 5;
+  const int k = threadIdx.x >> 5;
   for (int c = blockIdx.x; c < (p.n + 31) / 32; c += gridDim.x) {
     const int col = c * 32 + lane;
     float s = 0.0f;
