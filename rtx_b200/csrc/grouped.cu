@@ -34,15 +34,17 @@ int launch_quantize_transposed(TransposedParams& p, int64_t x_tiles, cudaStream_
   p.x_col_units = (p.x.cols + 63) / 64;
   p.w_col_units = (p.w.cols + 63) / 64;
   p.w_row_tiles = (p.w.rows + 127) / 128;
-  const int64_t units = (p.x.src ? x_tiles * p.x_col_units : 0) +
+  const bool gradient = p.dy.src != nullptr;
+  p.dy_col_units = (p.dy.cols + 63) / 64;
+  const int64_t units = (gradient ? x_tiles * p.dy_col_units : 0) + (p.x.src ? x_tiles * p.x_col_units : 0) +
                         (p.w.src ? static_cast<int64_t>(p.batches) * p.w_row_tiles * p.w_col_units : 0);
   if (units > INT32_MAX) return fail_msg(RTXB_E_UNSUPPORTED, "operand exceeds the 32-bit unit count of the quantizer");
   int64_t blocks = (units + 7) / 8;
   if (p.partial && blocks < (p.n + 31) / 32) blocks = (p.n + 31) / 32;
-  cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(quant_mxfp8_transposed_units_kernel), kTransposedSmemBytes);
+  auto kernel = gradient ? quant_mxfp8_transposed_units_kernel<true> : quant_mxfp8_transposed_units_kernel<false>;
+  cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), kTransposedSmemBytes);
   if (e != cudaSuccess) return fail_cuda(e, "cudaFuncSetAttribute(transposed quantizer)");
-  e = launch_dependent(quant_mxfp8_transposed_units_kernel, quant_grid(blocks, kTransposedOccupancy), kQuantThreads,
-                       kTransposedSmemBytes, stream, true, p);
+  e = launch_dependent(kernel, quant_grid(blocks, kTransposedOccupancy), kQuantThreads, kTransposedSmemBytes, stream, !gradient, p);
   if (e != cudaSuccess) return fail_cuda(e, "quant_mxfp8_transposed_units_kernel launch");
   return RTXB_OK;
 }
@@ -300,31 +302,20 @@ int rtxb_mxfp8_grouped_linear_bwd(const void* dy, int64_t lddy, const void* x, i
   if (!aligned(workspace, 256)) return fail_msg(RTXB_E_ALIGNMENT, "workspace must be 256-byte aligned");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int64_t tiles128 = most_tiles(rows, groups, 128), nt = (n + 127) / 128, kt = (k + 127) / 128;
-  GroupedGradientParams q = {};
-  q.src = static_cast<const __nv_bfloat16*>(dy);
-  q.cols = static_cast<int>(n);
-  q.ld = lddy;
-  q.q_rows = mem.q_dy;
-  q.s_rows = mem.s_dy;
-  q.q_t = mem.q_dyt;
-  q.s_t = mem.s_dyt;
-  q.pitch_t = tiles128 * 128;
-  q.chunks_t = static_cast<int>(tiles128);
-  q.list = GroupList{offsets, static_cast<int>(groups), static_cast<int>(rows)};
-  mem.plan.plan.tile_rows = rows_per_tile(rows, groups, k);
-  q.plan = mem.plan.plan;
-  q.dx = static_cast<__nv_bfloat16*>(dx);
-  q.dx_cols = static_cast<int>(k);
-  q.status = status;
-  cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(quant_mxfp8_grouped_gradient_kernel), kQtSmemBytes);
-  if (e != cudaSuccess) return fail_cuda(e, "cudaFuncSetAttribute(grouped gradient quantizer)");
-  quant_mxfp8_grouped_gradient_kernel<<<quant_grid(tiles128 * nt, kQtOccupancy), kQuantThreads, kQtSmemBytes, s>>>(q);
-  RTXB_CHECK_LAUNCH("quant_mxfp8_grouped_gradient_kernel");
   TransposedParams t = {};
-  t.list = q.list;
+  t.dy = TransposedOperand{static_cast<const __nv_bfloat16*>(dy), lddy, static_cast<int>(rows), static_cast<int>(n), mem.q_dyt,
+                           tiles128 * 128, mem.s_dyt, static_cast<int>(tiles128)};
+  t.dy_rows = mem.q_dy;
+  t.dy_row_scales = mem.s_dy;
+  t.list = GroupList{offsets, static_cast<int>(groups), static_cast<int>(rows)};
+  mem.plan.plan.tile_rows = rows_per_tile(rows, groups, k);
+  t.plan = mem.plan.plan;
+  t.dx = static_cast<__nv_bfloat16*>(dx);
+  t.dx_cols = static_cast<int>(k);
+  t.status = status;
   if (dw)
     t.x = TransposedOperand{static_cast<const __nv_bfloat16*>(x), ldx, static_cast<int>(rows), static_cast<int>(k), mem.q_xt,
-                            q.pitch_t, mem.s_xt, q.chunks_t};
+                            tiles128 * 128, mem.s_xt, static_cast<int>(tiles128)};
   if (dx) {
     t.w = TransposedOperand{static_cast<const __nv_bfloat16*>(w), k, static_cast<int>(n), static_cast<int>(k), mem.q_wt,
                             round_up(n, 32), mem.s_wt, static_cast<int>(nt)};

@@ -356,10 +356,13 @@ struct TransposedUnit {
   uint8_t* scales;       // 512-byte scale tile of the first column's 128 columns
   int live, cols, bytes; // rows, columns (from the first one on) and payload bytes of a column
   int col0;
-  int is_x;
+  uint8_t* q_rows;       // gradient: payload of the first row from the first column on, and the rows' scale tile
+  uint8_t* row_scales;
+  int operand;           // 0 = w, 1 = x, 2 = gradient
 };
 
-// block j of the unit into `buf` [32 rows][64 columns]; what lies outside the operand is zero
+// Block j of the unit into `buf` [32 rows][64 columns]; what lies outside the operand is zero.  16-byte chunk i of row r
+// lies at chunk i ^ (r % 8): eight lanes that read one chunk of eight rows meet in no bank, nor do 32 that read a row.
 __device__ __forceinline__ void quant_mxfp8_transposed_fetch(const TransposedUnit& f, int64_t ld, bool vec, int j, uint8_t* buf) {
   const int lane = threadIdx.x & 31;
   if (vec) {
@@ -368,7 +371,8 @@ __device__ __forceinline__ void quant_mxfp8_transposed_fetch(const TransposedUni
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const bool valid = r0 + 4 * i < f.live && c8 < f.cols;   // cols is a multiple of 8 here
-      cp_async_16(buf + (4 * i + (lane >> 3)) * 128 + c8 * 2, valid ? at + 4 * i * ld : f.src, valid);
+      const int r = 4 * i + (lane >> 3);
+      cp_async_16(buf + r * 128 + (((lane & 7) ^ (r & 7)) << 4), valid ? at + 4 * i * ld : f.src, valid);
     }
   } else {
     const int c = 2 * lane;
@@ -377,35 +381,80 @@ __device__ __forceinline__ void quant_mxfp8_transposed_fetch(const TransposedUni
     for (int e = 0; e < 32; ++e) {
       const bool row = 32 * j + e < f.live;
       const uint32_t a = row && c < f.cols ? at[e * ld] : 0u, b = row && c + 1 < f.cols ? at[e * ld + 1] : 0u;
-      *reinterpret_cast<uint32_t*>(buf + e * 128 + 4 * lane) = a | (b << 16);
+      *reinterpret_cast<uint32_t*>(buf + e * 128 + (((lane >> 2) ^ (e & 7)) << 4) + 4 * (lane & 3)) = a | (b << 16);
     }
   }
   cp_async_commit();
 }
 
+// The rows of a gradient block in `buf`, a lane each: two blocks of 32 values along the columns
+__device__ __forceinline__ void quant_mxfp8_gradient_rows(const TransposedUnit& f, int np, int j, const uint8_t* buf) {
+  const int lane = threadIdx.x & 31, row = 32 * j + lane;
+  uint32_t codes = 0;
+#pragma unroll
+  for (int blk = 0; blk < 2; ++blk) {
+    if (f.col0 + 32 * blk >= np) break;   // warp-uniform
+    uint32_t w[16];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint4 v = *reinterpret_cast<const uint4*>(buf + lane * 128 + (((4 * blk + i) ^ (lane & 7)) << 4));
+      w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+    }
+    uint32_t m2 = 0;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) m2 = absmax_bf16x2(m2, w[e]);
+    const uint32_t code = e8m0_from_amax(fmax_nan(bf16_lo(m2), bf16_hi(m2)), true);
+    const f32x2 recip = both(e8m0_reciprocal(code));
+    codes |= code << (8 * blk);
+    if (row < f.live) {
+      uint32_t c[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) c[e] = cvt_e4m3x4_bf16(w[2 * e], w[2 * e + 1], recip);
+      asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(f.q_rows + static_cast<int64_t>(row) * np + 32 * blk),
+                   "r"(c[0]), "r"(c[1]), "r"(c[2]), "r"(c[3]), "r"(c[4]), "r"(c[5]), "r"(c[6]), "r"(c[7])
+                   : "memory");
+    }
+  }
+  if (row < f.live) {
+    // 64 columns are half a word of a row's four codes; the last ones fill theirs with zeros
+    uint8_t* at = f.row_scales + lane * 16 + j * 4 + ((f.col0 >> 5) & 3);
+    if ((f.col0 & 64) == 0 && f.col0 + 64 >= np) *reinterpret_cast<uint32_t*>(at) = codes;
+    else *reinterpret_cast<uint16_t*>(at) = static_cast<uint16_t>(codes);
+  }
+}
+
+// GRADIENT: the gradient's units come first, in both orientations from one read, and the kernel is the first of its chain
+// (it leaves the plan and sets the result's rows of no group to zero)
+template <bool GRADIENT>
 __global__ void __launch_bounds__(kQuantThreads, kTransposedOccupancy)
 quant_mxfp8_transposed_units_kernel(const TransposedParams p) {
-  extern __shared__ __align__(16) uint8_t qt_smem[];
+  extern __shared__ __align__(128) uint8_t qt_smem[];
   uint8_t* buf = qt_smem + (threadIdx.x >> 5) * kTransposedWarpBytes;
   uint8_t* stage = buf + 2 * kTransposedFetchBytes;
   __shared__ GroupScan scan;
-  __shared__ float part[8][33];
   griddep_launch_dependents();
-  const bool grouped = p.list.offsets != nullptr;
-  if (grouped && p.x.src) scan_groups(p.list, scan, nullptr);
-  const uint32_t x_tiles = !p.x.src ? 0 : grouped ? scan.tile[p.list.groups] : (p.x.rows + 127) / 128;
-  const uint32_t x_units = x_tiles * p.x_col_units;
-  const uint32_t units = x_units + (p.w.src ? p.batches * p.w_row_tiles * p.w_col_units : 0u);   // < 2^31 (host)
+  const bool grouped = GRADIENT || p.list.offsets != nullptr;
+  if (grouped && (GRADIENT || p.x.src)) scan_groups(p.list, scan, GRADIENT ? p.status : nullptr);
+  if (GRADIENT) {
+    if (blockIdx.x == 0) write_group_plan(p.list, scan, p.plan, reinterpret_cast<int*>(qt_smem));
+    if (p.dx) zero_rows_of_no_group(p.list, scan, p.dx, p.dx_cols, p.dx_cols);
+  }
+  const uint32_t x_tiles = grouped ? (GRADIENT || p.x.src ? scan.tile[p.list.groups] : 0) : p.x.src ? (p.x.rows + 127) / 128 : 0;
+  const uint32_t dy_units = GRADIENT ? x_tiles * p.dy_col_units : 0;
+  const uint32_t x_end = dy_units + (p.x.src ? x_tiles * p.x_col_units : 0);
+  const uint32_t units = x_end + (p.w.src ? p.batches * p.w_row_tiles * p.w_col_units : 0u);   // < 2^31 (host)
+  const int np = GRADIENT ? (p.dy.cols + 31) / 32 * 32 : 0, row_chunks = (np / 32 + 3) / 4;
+  auto operand = [&](int i) -> const TransposedOperand& { return GRADIENT && i == 2 ? p.dy : i ? p.x : p.w; };
   auto locate = [&](uint32_t u) {
     TransposedUnit f;
-    f.is_x = u < x_units;
-    const TransposedOperand& o = f.is_x ? p.x : p.w;
-    const uint32_t v = f.is_x ? u : u - x_units;
-    const uint32_t col_units = f.is_x ? p.x_col_units : p.w_col_units;
+    f.operand = GRADIENT && u < dy_units ? 2 : u < x_end ? 1 : 0;
+    const TransposedOperand& o = operand(f.operand);
+    const uint32_t v = u - (f.operand == 2 ? 0 : f.operand ? dy_units : x_end);
+    const uint32_t col_units = f.operand == 2 ? p.dy_col_units : f.operand ? p.x_col_units : p.w_col_units;
     uint32_t rt = v / col_units, e = 0;
     f.col0 = (v - rt * col_units) * 64;
     int64_t row0;
-    if (!f.is_x) {
+    if (f.operand == 0) {
       e = rt / p.w_row_tiles;
       rt -= e * p.w_row_tiles;
       row0 = static_cast<int64_t>(e) * o.rows + 128 * rt;
@@ -424,14 +473,18 @@ quant_mxfp8_transposed_units_kernel(const TransposedParams p) {
     f.bytes = static_cast<int>(min(static_cast<int64_t>(128), o.pitch - static_cast<int64_t>(128 * rt)));   // a multiple of 32
     f.q = o.q + (static_cast<int64_t>(e) * o.cols + f.col0) * o.pitch + 128ll * rt;
     f.scales = o.scales + ((static_cast<size_t>(e) * ((o.cols + 127) / 128) + (f.col0 >> 7)) * o.chunks + rt) * 512;
+    if (GRADIENT && f.operand == 2) {
+      f.q_rows = p.dy_rows + row0 * np + f.col0;
+      f.row_scales = p.dy_row_scales + (static_cast<size_t>(rt) * row_chunks + (f.col0 >> 7)) * 512;
+    }
     return f;
   };
   auto vec_of = [](const TransposedOperand& o) {
     return o.ld % 8 == 0 && o.cols % 8 == 0 && (reinterpret_cast<uintptr_t>(o.src) & 15) == 0;
   };
-  const bool vec_x = vec_of(p.x), vec_w = vec_of(p.w);
+  const int vec = (vec_of(p.w) ? 1 : 0) | (vec_of(p.x) ? 2 : 0) | (GRADIENT && vec_of(p.dy) ? 4 : 0);
   auto fetch = [&](const TransposedUnit& f, int j) {
-    quant_mxfp8_transposed_fetch(f, f.is_x ? p.x.ld : p.w.ld, f.is_x ? vec_x : vec_w, j, buf + (j & 1) * kTransposedFetchBytes);
+    quant_mxfp8_transposed_fetch(f, operand(f.operand).ld, vec >> f.operand & 1, j, buf + (j & 1) * kTransposedFetchBytes);
   };
   const int lane = threadIdx.x & 31;
   const uint32_t stride = gridDim.x * (kQuantThreads / 32);
@@ -443,23 +496,26 @@ quant_mxfp8_transposed_units_kernel(const TransposedParams p) {
     fetch(f, 1);
   }
   for (; u < units; u += stride, f = ahead) {
-    const int64_t pitch = f.is_x ? p.x.pitch : p.w.pitch;
+    const int64_t pitch = operand(f.operand).pitch;
+    const bool columns = !GRADIENT || f.operand != 2 || p.dy.q != nullptr;
     uint32_t word0 = 0, word1 = 0;   // the four scale bytes of either column
 #pragma unroll 1
     for (int j = 0; j < 4; ++j) {
       cp_async_wait<1>();            // everything but the newest group: block j is here
       __syncwarp();
-      const uint8_t* rows = buf + (j & 1) * kTransposedFetchBytes + 4 * lane;
+      const uint8_t* rows = buf + (j & 1) * kTransposedFetchBytes;
+      if (GRADIENT && f.operand == 2 && p.dy_rows && 32 * j < f.live) quant_mxfp8_gradient_rows(f, np, j, rows);
       uint32_t w[32];
 #pragma unroll
-      for (int e = 0; e < 32; ++e) w[e] = *reinterpret_cast<const uint32_t*>(rows + e * 128);
+      for (int e = 0; e < 32; ++e)
+        w[e] = *reinterpret_cast<const uint32_t*>(rows + e * 128 + (((lane >> 2) ^ (e & 7)) << 4) + 4 * (lane & 3));
       __syncwarp();
       // the buffer takes the block after the next one
       if (j == 2 && u + stride < units) ahead = locate(u + stride);
       if (j < 2) fetch(f, j + 2);
       else if (u + stride < units) fetch(ahead, j - 2);
       else cp_async_commit();
-      if (32 * j >= f.bytes) continue;
+      if (!columns || 32 * j >= f.bytes) continue;
       uint32_t m2 = 0;
 #pragma unroll
       for (int e = 0; e < 32; ++e) m2 = absmax_bf16x2(m2, w[e]);
@@ -498,13 +554,17 @@ quant_mxfp8_transposed_units_kernel(const TransposedParams p) {
       }
       __syncwarp();   // the stage is free again
     }
-    const int c = (f.col0 & 127) + 2 * lane;   // within its 128 columns; even: both columns in one scale tile
-    if (2 * lane < f.cols) *reinterpret_cast<uint32_t*>(f.scales + (c & 31) * 16 + (c >> 5) * 4) = word0;
-    if (2 * lane + 1 < f.cols) *reinterpret_cast<uint32_t*>(f.scales + ((c + 1) & 31) * 16 + (c >> 5) * 4) = word1;
+    if (columns) {
+      const int c = (f.col0 & 127) + 2 * lane;   // within its 128 columns; even: both columns in one scale tile
+      if (2 * lane < f.cols) *reinterpret_cast<uint32_t*>(f.scales + (c & 31) * 16 + (c >> 5) * 4) = word0;
+      if (2 * lane + 1 < f.cols) *reinterpret_cast<uint32_t*>(f.scales + ((c + 1) & 31) * 16 + (c >> 5) * 4) = word1;
+    }
   }
   cp_async_wait<0>();
+  if (GRADIENT) return;
   griddep_wait();   // the launch before this one is complete: whoever waits for this grid has waited for that one too
   if (p.partial == nullptr) return;
+  __shared__ float part[8][33];
   // dbias[c] = bf16( sum over the row tiles of partial[t][c] ): eight threads per column add every eighth tile, the eight
   // sums are added in a fixed order
   const int k = threadIdx.x >> 5;
@@ -521,102 +581,6 @@ quant_mxfp8_transposed_units_kernel(const TransposedParams p) {
       p.dbias[col] = __float2bfloat16_rn(s);
     }
     __syncthreads();
-  }
-}
-
-// ---------------------------------------------------------------------------
-// The gradient operand dy by group, walked as 128 x 128 tiles: rows (blocks along n, for dX) and transposed (blocks along
-// the tokens, for dW) from one staged read.  A null destination leaves that product out.  Bound by instructions and
-// barriers (52 % issue, a quarter of the stalls at barriers): 8192 x 4096 in 33 us, 4.1 TB/s, 0.62 of the copy rate; two
-// separate passes would read the gradient twice.
-// ---------------------------------------------------------------------------
-struct GroupedGradientParams {
-  const __nv_bfloat16* src;
-  int cols;
-  int64_t ld;
-  uint8_t* q_rows;            // [rows, round_up(cols, 32)]
-  uint8_t* s_rows;            // 128-row tiles counted per group
-  uint8_t* q_t;               // [cols, pitch_t]
-  uint8_t* s_t;               // [ceil(cols / 128)][chunks_t][512]
-  int64_t pitch_t;            // 128 * (most tiles the list can have)
-  int chunks_t;               // pitch_t / 128
-  GroupList list;
-  GroupPlan plan;
-  __nv_bfloat16* dx;          // result whose rows of no group become zero; nullptr = none
-  int dx_cols;
-  int* status;
-};
-
-// where a tile lies: first row and live rows, first column, its 128-row tile number
-struct GradientTile {
-  int64_t row0;
-  int live, col0, rt;
-};
-
-__global__ void __launch_bounds__(kQuantThreads, kQtOccupancy)
-quant_mxfp8_grouped_gradient_kernel(const GroupedGradientParams p) {
-  extern __shared__ __align__(16) uint8_t qt_smem[];
-  uint16_t (*tiles[2])[kQtPitch] = {reinterpret_cast<uint16_t (*)[kQtPitch]>(qt_smem),
-                                    reinterpret_cast<uint16_t (*)[kQtPitch]>(qt_smem + kQtTileBytes)};
-  __shared__ GroupScan scan;
-  __shared__ __align__(16) uint8_t tile_scales[128][4];
-  __shared__ __align__(16) uint8_t tile_scales_rows[128][4];
-  griddep_launch_dependents();
-  scan_groups(p.list, scan, p.status);
-  if (blockIdx.x == 0) write_group_plan(p.list, scan, p.plan, reinterpret_cast<int*>(qt_smem));
-  if (p.dx) zero_rows_of_no_group(p.list, scan, p.dx, p.dx_cols, p.dx_cols);
-  const int col_tiles = (p.cols + 127) / 128;
-  const int total = scan.tile[p.list.groups] * col_tiles;   // < 2^31 (host)
-  const int np = (p.cols + 31) / 32 * 32, chunks_rows = (np / 32 + 3) / 4;
-  const bool vec_ok = (p.ld % 8 == 0) && ((reinterpret_cast<uintptr_t>(p.src) & 15) == 0);
-  // One thread works out where a tile lies (a division, the search for its group), a step ahead of the fetch.
-  __shared__ GradientTile place[2];
-  auto locate = [&](int t, int slot) {
-    if (t >= total) return;
-    const int rt = t / col_tiles;
-    const int g = group_before(scan.tile, p.list.groups, rt);
-    const int row0 = scan.start[g] + 128 * (rt - scan.tile[g]);
-    place[slot] = GradientTile{row0, min(128, scan.start[g + 1] - row0), (t - rt * col_tiles) * 128, rt};
-  };
-  auto fetch = [&](const GradientTile& f, uint16_t (*dst)[kQtPitch]) {
-    QuantMxTParams q;
-    q.src = p.src + f.row0 * p.ld;
-    q.rows = p.cols;
-    q.k = f.live;
-    q.ld = p.ld;
-    quant_mxfp8_t_fetch(q, dst, f.col0, 0, vec_ok);
-  };
-  if (threadIdx.x == 0) locate(blockIdx.x, 0);
-  if (threadIdx.x == 32) locate(blockIdx.x + gridDim.x, 1);
-  __syncthreads();
-  int buf = 0;
-  if (static_cast<int>(blockIdx.x) < total) fetch(place[0], tiles[0]);
-  for (int t = blockIdx.x; t < total; t += gridDim.x) {
-    const GradientTile b = place[buf];
-    if (t + static_cast<int>(gridDim.x) < total) {
-      fetch(place[buf ^ 1], tiles[buf ^ 1]);
-      cp_async_wait<1>();   // everything but the newest group (the next tile) has landed
-    } else {
-      cp_async_wait<0>();
-    }
-    __syncthreads();        // (also: everybody has read place[buf])
-    if (threadIdx.x == kQuantThreads - 1) locate(t + 2 * gridDim.x, buf);   // read after this tile's other barriers
-    uint32_t o[2][8];
-    if (p.q_t)
-      quant_mxfp8_tile_columns(tiles[buf], tile_scales, o, 128, p.cols, b.col0, 0, true);
-    if (p.q_rows)
-      quant_mxfp8_tile_rows(tiles[buf], tile_scales_rows, p.q_rows + b.row0 * np, np, b.live, p.cols, 0, b.col0, true);
-    __syncthreads();   // every thread has read the staged tile: its storage now collects the transposed payload
-    if (p.q_t) {
-      quant_mxfp8_tile_columns_store(reinterpret_cast<uint8_t*>(tiles[buf]), o, p.q_t + 128ll * b.rt,
-                                     static_cast<int>(p.pitch_t), p.cols, b.col0, 0);
-      store_scale_tile<4>(tile_scales, p.s_t, kScaleMma128, b.col0, b.rt * 4, p.cols, 0, p.chunks_t);
-    }
-    if (p.q_rows)
-      store_scale_tile<4>(tile_scales_rows, p.s_rows + static_cast<size_t>(b.rt) * chunks_rows * 512, kScaleMma128, 0,
-                          b.col0 / 32, b.live, 0, chunks_rows);
-    __syncthreads();   // the scale tiles and this buffer are free again
-    buf ^= 1;
   }
 }
 

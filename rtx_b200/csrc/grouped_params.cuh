@@ -67,9 +67,19 @@ struct TransposedParams {
   const float* partial;       // column sums [row_tiles][n] left by the launch before this one; nullptr = none
   int row_tiles, n;
   __nv_bfloat16* dbias;       // their sum over the row tiles
+  // with the gradient, whose groups are those of x: q null = no columns (dW), dy_rows null = no rows (dX)
+  TransposedOperand dy;
+  int dy_col_units;
+  uint8_t* dy_rows;           // [rows, round_up(cols, 32)]
+  uint8_t* dy_row_scales;     // 128-row tiles counted per group
+  GroupPlan plan;
+  __nv_bfloat16* dx;          // result whose rows of no group become zero; nullptr = none
+  int dx_cols;
+  int* status;
 };
 // enqueues the transposed quantizer as a programmatic dependent that may run beside the launch before it (none of whose
-// results it reads but `partial`) and ends after that launch has; x_tiles: the most 128-row tiles x can have
+// results it reads but `partial`) and ends after that launch has, or, with a gradient, as the first launch of its chain;
+// x_tiles: the most 128-row tiles x can have
 int launch_quantize_transposed(TransposedParams& p, int64_t x_tiles, cudaStream_t stream);   // grouped.cu
 
 }  // namespace rtxb
