@@ -335,13 +335,17 @@ __global__ void __launch_bounds__(kQuantThreads, kRowsOccupancy) quant_mxfp8_row
 }
 
 // ---------------------------------------------------------------------------
-// Transposed quantizer of the backward's operands that are quantized one way only: x (by group, for dW) and the weight
-// matrices (for dX).  A warp takes 64 columns of a 128-row tile; one lane owns two neighbouring columns and walks down 32
-// rows at a time, so that a block is in its registers and its maximum needs no exchange.  The blocks come through shared
-// memory, two ahead of the one at work (with loads into the registers themselves 96 KB are in flight per SM only while
-// nothing is computed), and the payload leaves through it, because a lane holds 32 bytes of a column whose K step is 128.
-// No barrier but the warp's own.  Both quantizers of the backward together, 8192 rows, 32 groups, 2048 x 4096 (604 MB read,
-// 336 MB written): 253 us with direct loads and stores, 225 with staged stores, 195 with blocks fetched ahead too, 4.8 TB/s.
+// Quantizer of the backward's operands, in one launch: the gradient (by group; blocks along the columns for dX and along
+// the rows for dW, from one read), x (by group, along the rows, for dW) and the weight matrices (along the rows, for dX).
+// A warp takes 64 columns of a 128-row tile.  Along the rows, one lane owns two neighbouring columns and walks down 32 rows
+// at a time, so that a block is in its registers and its maximum needs no exchange; along the columns a lane owns a row.
+// The blocks come through shared memory, two ahead of the one at work (with loads into the registers themselves 96 KB are
+// in flight per SM only while nothing is computed), and the columns' payload leaves through it, because a lane holds 32
+// bytes of a column whose K step is 128.  No barrier but the warp's own.
+// Bound by memory and, with 16 warps per SM, by instruction latency (56 % issue): 8192 x 4096 gradient and x, 4 weights of
+// 4096 x 4096 (268 MB read, 168 MB written) in 78 us, 5.6 TB/s, 0.85 of the copy rate.  On the way, 8192 rows, 32 groups,
+// 2048 x 4096 (a launch for the gradient on staged 128 x 128 tiles and one for the rest, together): 253 us with direct loads
+// and stores, 225 with staged stores, 195 with blocks fetched ahead too; one launch 196, without register spills 187.
 // ---------------------------------------------------------------------------
 constexpr int kTransposedOccupancy = 2;
 constexpr int kTransposedFetchBytes = 32 * 128;   // a block of 64 columns
@@ -349,38 +353,38 @@ constexpr int kTransposedStageBytes = 64 * 64;    // 64 bytes of each column's p
 constexpr int kTransposedWarpBytes = 2 * kTransposedFetchBytes + kTransposedStageBytes;
 constexpr int kTransposedSmemBytes = kQuantThreads / 32 * kTransposedWarpBytes;
 
-// what one warp does at a time: 64 columns of a 128-row tile, four blocks of 32 rows
+// What one warp does at a time: 64 columns of a 128-row tile, four blocks of 32 rows.  Two of these live in registers, and
+// pointers are formed where they are used: a register too many is a load from L2 where shared memory leaves L1 nothing.
 struct TransposedUnit {
-  const uint16_t* src;   // first row, first column
-  uint8_t* q;            // payload of the first column, at the tile's K step
-  uint8_t* scales;       // 512-byte scale tile of the first column's 128 columns
-  int live, cols, bytes; // rows, columns (from the first one on) and payload bytes of a column
+  int operand;      // 0 = w, 1 = x, 2 = gradient
+  int row0, live;   // first row (over all matrices) and rows
+  int rt, matrix;   // 128-row tile, of its matrix
   int col0;
-  uint8_t* q_rows;       // gradient: payload of the first row from the first column on, and the rows' scale tile
-  uint8_t* row_scales;
-  int operand;           // 0 = w, 1 = x, 2 = gradient
 };
 
 // Block j of the unit into `buf` [32 rows][64 columns]; what lies outside the operand is zero.  16-byte chunk i of row r
 // lies at chunk i ^ (r % 8): eight lanes that read one chunk of eight rows meet in no bank, nor do 32 that read a row.
-__device__ __forceinline__ void quant_mxfp8_transposed_fetch(const TransposedUnit& f, int64_t ld, bool vec, int j, uint8_t* buf) {
+__device__ __forceinline__ void quant_mxfp8_transposed_fetch(const TransposedUnit& f, const TransposedOperand& o, bool vec, int j,
+                                                             uint8_t* buf) {
   const int lane = threadIdx.x & 31;
+  const uint16_t* src = reinterpret_cast<const uint16_t*>(o.src) + static_cast<int64_t>(f.row0) * o.ld + f.col0;
+  const int cols = o.cols - f.col0;
   if (vec) {
     const int c8 = (lane & 7) * 8, r0 = 32 * j + (lane >> 3);
-    const uint16_t* at = f.src + r0 * ld + c8;
+    const uint16_t* at = src + r0 * o.ld + c8;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const bool valid = r0 + 4 * i < f.live && c8 < f.cols;   // cols is a multiple of 8 here
+      const bool valid = r0 + 4 * i < f.live && c8 < cols;   // cols is a multiple of 8 here
       const int r = 4 * i + (lane >> 3);
-      cp_async_16(buf + r * 128 + (((lane & 7) ^ (r & 7)) << 4), valid ? at + 4 * i * ld : f.src, valid);
+      cp_async_16(buf + r * 128 + (((lane & 7) ^ (r & 7)) << 4), valid ? at + 4 * i * o.ld : src, valid);
     }
   } else {
     const int c = 2 * lane;
-    const uint16_t* at = f.src + 32 * j * ld + c;
+    const uint16_t* at = src + 32 * j * o.ld + c;
 #pragma unroll 8
     for (int e = 0; e < 32; ++e) {
       const bool row = 32 * j + e < f.live;
-      const uint32_t a = row && c < f.cols ? at[e * ld] : 0u, b = row && c + 1 < f.cols ? at[e * ld + 1] : 0u;
+      const uint32_t a = row && c < cols ? at[e * o.ld] : 0u, b = row && c + 1 < cols ? at[e * o.ld + 1] : 0u;
       *reinterpret_cast<uint32_t*>(buf + e * 128 + (((lane >> 2) ^ (e & 7)) << 4) + 4 * (lane & 3)) = a | (b << 16);
     }
   }
@@ -388,8 +392,10 @@ __device__ __forceinline__ void quant_mxfp8_transposed_fetch(const TransposedUni
 }
 
 // The rows of a gradient block in `buf`, a lane each: two blocks of 32 values along the columns
-__device__ __forceinline__ void quant_mxfp8_gradient_rows(const TransposedUnit& f, int np, int j, const uint8_t* buf) {
+__device__ __forceinline__ void quant_mxfp8_gradient_rows(const TransposedUnit& f, const TransposedParams& p, int j,
+                                                          const uint8_t* buf) {
   const int lane = threadIdx.x & 31, row = 32 * j + lane;
+  const int np = (p.dy.cols + 31) / 32 * 32;
   uint32_t codes = 0;
 #pragma unroll
   for (int blk = 0; blk < 2; ++blk) {
@@ -410,14 +416,15 @@ __device__ __forceinline__ void quant_mxfp8_gradient_rows(const TransposedUnit& 
       uint32_t c[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) c[e] = cvt_e4m3x4_bf16(w[2 * e], w[2 * e + 1], recip);
-      asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(f.q_rows + static_cast<int64_t>(row) * np + 32 * blk),
+      asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p.dy_rows + static_cast<int64_t>(f.row0 + row) * np + f.col0 + 32 * blk),
                    "r"(c[0]), "r"(c[1]), "r"(c[2]), "r"(c[3]), "r"(c[4]), "r"(c[5]), "r"(c[6]), "r"(c[7])
                    : "memory");
     }
   }
   if (row < f.live) {
     // 64 columns are half a word of a row's four codes; the last ones fill theirs with zeros
-    uint8_t* at = f.row_scales + lane * 16 + j * 4 + ((f.col0 >> 5) & 3);
+    uint8_t* at = p.dy_row_scales + (static_cast<size_t>(f.rt) * ((np + 127) / 128) + (f.col0 >> 7)) * 512 + lane * 16 + j * 4 +
+                  ((f.col0 >> 5) & 3);
     if ((f.col0 & 64) == 0 && f.col0 + 64 >= np) *reinterpret_cast<uint32_t*>(at) = codes;
     else *reinterpret_cast<uint16_t*>(at) = static_cast<uint16_t>(codes);
   }
@@ -443,7 +450,6 @@ quant_mxfp8_transposed_units_kernel(const TransposedParams p) {
   const uint32_t dy_units = GRADIENT ? x_tiles * p.dy_col_units : 0;
   const uint32_t x_end = dy_units + (p.x.src ? x_tiles * p.x_col_units : 0);
   const uint32_t units = x_end + (p.w.src ? p.batches * p.w_row_tiles * p.w_col_units : 0u);   // < 2^31 (host)
-  const int np = GRADIENT ? (p.dy.cols + 31) / 32 * 32 : 0, row_chunks = (np / 32 + 3) / 4;
   auto operand = [&](int i) -> const TransposedOperand& { return GRADIENT && i == 2 ? p.dy : i ? p.x : p.w; };
   auto locate = [&](uint32_t u) {
     TransposedUnit f;
@@ -451,32 +457,23 @@ quant_mxfp8_transposed_units_kernel(const TransposedParams p) {
     const TransposedOperand& o = operand(f.operand);
     const uint32_t v = u - (f.operand == 2 ? 0 : f.operand ? dy_units : x_end);
     const uint32_t col_units = f.operand == 2 ? p.dy_col_units : f.operand ? p.x_col_units : p.w_col_units;
-    uint32_t rt = v / col_units, e = 0;
-    f.col0 = (v - rt * col_units) * 64;
-    int64_t row0;
+    f.rt = v / col_units;
+    f.matrix = 0;
+    f.col0 = (v - f.rt * col_units) * 64;
     if (f.operand == 0) {
-      e = rt / p.w_row_tiles;
-      rt -= e * p.w_row_tiles;
-      row0 = static_cast<int64_t>(e) * o.rows + 128 * rt;
-      f.live = o.rows - static_cast<int>(128 * rt);
+      f.matrix = f.rt / p.w_row_tiles;
+      f.rt -= f.matrix * p.w_row_tiles;
+      f.row0 = f.matrix * o.rows + 128 * f.rt;
+      f.live = o.rows - 128 * f.rt;
     } else if (grouped) {
-      const int g = group_before(scan.tile, p.list.groups, rt);
-      row0 = scan.start[g] + 128ll * (rt - scan.tile[g]);
-      f.live = scan.start[g + 1] - static_cast<int>(row0);
+      const int g = group_before(scan.tile, p.list.groups, f.rt);
+      f.row0 = scan.start[g] + 128 * (f.rt - scan.tile[g]);
+      f.live = scan.start[g + 1] - f.row0;
     } else {
-      row0 = 128ll * rt;
-      f.live = o.rows - static_cast<int>(row0);
+      f.row0 = 128 * f.rt;
+      f.live = o.rows - f.row0;
     }
     f.live = min(128, f.live);
-    f.src = reinterpret_cast<const uint16_t*>(o.src) + row0 * o.ld + f.col0;
-    f.cols = o.cols - f.col0;
-    f.bytes = static_cast<int>(min(static_cast<int64_t>(128), o.pitch - static_cast<int64_t>(128 * rt)));   // a multiple of 32
-    f.q = o.q + (static_cast<int64_t>(e) * o.cols + f.col0) * o.pitch + 128ll * rt;
-    f.scales = o.scales + ((static_cast<size_t>(e) * ((o.cols + 127) / 128) + (f.col0 >> 7)) * o.chunks + rt) * 512;
-    if (GRADIENT && f.operand == 2) {
-      f.q_rows = p.dy_rows + row0 * np + f.col0;
-      f.row_scales = p.dy_row_scales + (static_cast<size_t>(rt) * row_chunks + (f.col0 >> 7)) * 512;
-    }
     return f;
   };
   auto vec_of = [](const TransposedOperand& o) {
@@ -484,7 +481,7 @@ quant_mxfp8_transposed_units_kernel(const TransposedParams p) {
   };
   const int vec = (vec_of(p.w) ? 1 : 0) | (vec_of(p.x) ? 2 : 0) | (GRADIENT && vec_of(p.dy) ? 4 : 0);
   auto fetch = [&](const TransposedUnit& f, int j) {
-    quant_mxfp8_transposed_fetch(f, operand(f.operand).ld, vec >> f.operand & 1, j, buf + (j & 1) * kTransposedFetchBytes);
+    quant_mxfp8_transposed_fetch(f, operand(f.operand), vec >> f.operand & 1, j, buf + (j & 1) * kTransposedFetchBytes);
   };
   const int lane = threadIdx.x & 31;
   const uint32_t stride = gridDim.x * (kQuantThreads / 32);
@@ -496,7 +493,8 @@ quant_mxfp8_transposed_units_kernel(const TransposedParams p) {
     fetch(f, 1);
   }
   for (; u < units; u += stride, f = ahead) {
-    const int64_t pitch = operand(f.operand).pitch;
+    const TransposedOperand& o = operand(f.operand);
+    const int bytes = static_cast<int>(min(static_cast<int64_t>(128), o.pitch - static_cast<int64_t>(128 * f.rt)));   // of a column
     const bool columns = !GRADIENT || f.operand != 2 || p.dy.q != nullptr;
     uint32_t word0 = 0, word1 = 0;   // the four scale bytes of either column
 #pragma unroll 1
@@ -504,7 +502,7 @@ quant_mxfp8_transposed_units_kernel(const TransposedParams p) {
       cp_async_wait<1>();            // everything but the newest group: block j is here
       __syncwarp();
       const uint8_t* rows = buf + (j & 1) * kTransposedFetchBytes;
-      if (GRADIENT && f.operand == 2 && p.dy_rows && 32 * j < f.live) quant_mxfp8_gradient_rows(f, np, j, rows);
+      if (GRADIENT && f.operand == 2 && p.dy_rows && 32 * j < f.live) quant_mxfp8_gradient_rows(f, p, j, rows);
       uint32_t w[32];
 #pragma unroll
       for (int e = 0; e < 32; ++e)
@@ -515,7 +513,7 @@ quant_mxfp8_transposed_units_kernel(const TransposedParams p) {
       if (j < 2) fetch(f, j + 2);
       else if (u + stride < units) fetch(ahead, j - 2);
       else cp_async_commit();
-      if (!columns || 32 * j >= f.bytes) continue;
+      if (!columns || 32 * j >= bytes) continue;
       uint32_t m2 = 0;
 #pragma unroll
       for (int e = 0; e < 32; ++e) m2 = absmax_bf16x2(m2, w[e]);
@@ -542,22 +540,24 @@ quant_mxfp8_transposed_units_kernel(const TransposedParams p) {
         *reinterpret_cast<uint4*>(at0 + chunk) = make_uint4(o0[0], o0[1], o0[2], o0[3]);
         *reinterpret_cast<uint4*>(at1 + chunk) = make_uint4(o1[0], o1[1], o1[2], o1[3]);
       }
-      if ((j & 1) == 0 && 32 * j + 32 < f.bytes) continue;
+      if ((j & 1) == 0 && 32 * j + 32 < bytes) continue;
       __syncwarp();
       const int first = 64 * (j >> 1), part = lane & 3;
+      uint8_t* q = o.q + (static_cast<int64_t>(f.matrix) * o.cols + f.col0) * o.pitch + 128ll * f.rt + first + 16 * part;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int col = 8 * i + (lane >> 2);
-        if (col < f.cols && first + 16 * part < f.bytes)
-          *reinterpret_cast<uint4*>(f.q + col * pitch + first + 16 * part) = *reinterpret_cast<const uint4*>(
+        if (f.col0 + col < o.cols && first + 16 * part < bytes)
+          *reinterpret_cast<uint4*>(q + col * o.pitch) = *reinterpret_cast<const uint4*>(
               stage + (col ^ ((col >> 3) & 1)) * 64 + ((part ^ ((col >> 1) & 3)) << 4));
       }
       __syncwarp();   // the stage is free again
     }
     if (columns) {
       const int c = (f.col0 & 127) + 2 * lane;   // within its 128 columns; even: both columns in one scale tile
-      if (2 * lane < f.cols) *reinterpret_cast<uint32_t*>(f.scales + (c & 31) * 16 + (c >> 5) * 4) = word0;
-      if (2 * lane + 1 < f.cols) *reinterpret_cast<uint32_t*>(f.scales + ((c + 1) & 31) * 16 + (c >> 5) * 4) = word1;
+      uint8_t* at = o.scales + ((static_cast<size_t>(f.matrix) * ((o.cols + 127) / 128) + (f.col0 >> 7)) * o.chunks + f.rt) * 512;
+      if (f.col0 + 2 * lane < o.cols) *reinterpret_cast<uint32_t*>(at + (c & 31) * 16 + (c >> 5) * 4) = word0;
+      if (f.col0 + 2 * lane + 1 < o.cols) *reinterpret_cast<uint32_t*>(at + ((c + 1) & 31) * 16 + (c >> 5) * 4) = word1;
     }
   }
   cp_async_wait<0>();
