@@ -244,6 +244,75 @@ __device__ __forceinline__ void stage_bf16x32(uint8_t* buf, int lane, const uint
         make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
 }
 
+// 32 rows x 32 columns between a staging buffer (64-byte swizzle) and rows of any alignment.  Half a warp takes a row, a word
+// a lane: two values that share a word of memory, or, where the row starts between two words, one lane its two ends.  Rows
+// r and r + 2 start alike, so what a lane takes is the same for all of its rows.
+struct RowWords {
+  int e, other;       // the lane's values within the row; other = e + 1, or 0 when it has the two ends
+  bool split;
+  __device__ __forceinline__ RowWords(const __nv_bfloat16* first, int64_t ld, int lane) {
+    e = 2 * (lane & 15) + static_cast<int>((reinterpret_cast<uintptr_t>(first + (lane >> 4) * ld) >> 1) & 1);
+    split = e == 31;
+    other = (e + 1) & 31;
+  }
+  // byte of value i of row 2 j + lane / 16 in the buffer
+  static __device__ __forceinline__ int at(int i, int j, int lane) {
+    return (2 * j + (lane >> 4)) * 64 + (((i >> 3) ^ (j & 3)) << 4) + (i & 7) * 2;
+  }
+};
+
+// Direct stores of a row per lane touch 32 rows each: 3666 x 3860 results summed over 222 values took 171 us, and 66 this way.
+__device__ __forceinline__ void store_rows_any(const uint8_t* buf, __nv_bfloat16* out, int64_t ldo, int row0, int rows, int col,
+                                               int cols, int lane) {
+  __nv_bfloat16* first = out + static_cast<int64_t>(row0) * ldo + col;
+  const RowWords w(first, ldo, lane);
+  uint16_t* dst = reinterpret_cast<uint16_t*>(first + (lane >> 4) * ldo);
+  const bool whole = col + 32 <= cols;
+#pragma unroll
+  for (int j = 0; j < 16; ++j, dst += 2 * ldo) {
+    if (row0 + 2 * j + (lane >> 4) >= rows) break;
+    const uint32_t a = *reinterpret_cast<const uint16_t*>(buf + w.at(w.e, j, lane));
+    const uint32_t b = *reinterpret_cast<const uint16_t*>(buf + w.at(w.other, j, lane));
+    if (!w.split && (whole || col + w.other < cols)) {
+      *reinterpret_cast<uint32_t*>(dst + w.e) = a | (b << 16);
+    } else {
+      if (col + w.e < cols) dst[w.e] = static_cast<uint16_t>(a);
+      if (w.split) dst[0] = static_cast<uint16_t>(b);   // col < cols: the caller's
+    }
+  }
+}
+// the reverse: into one row per lane, packed two values per word; zero outside
+__device__ __forceinline__ void load_rows_any(uint8_t* buf, const __nv_bfloat16* src, int64_t ld, int row0, int rows, int col,
+                                              int cols, int lane, uint32_t (&w)[16]) {
+  const __nv_bfloat16* first = src + static_cast<int64_t>(row0) * ld + col;
+  const RowWords words(first, ld, lane);
+  const uint16_t* at = reinterpret_cast<const uint16_t*>(first + (lane >> 4) * ld);
+#pragma unroll
+  for (int j = 0; j < 16; ++j, at += 2 * ld) {
+    w[j] = 0;
+    if (row0 + 2 * j + (lane >> 4) < rows) {
+      if (!words.split && col + words.other < cols) {
+        w[j] = __ldg(reinterpret_cast<const uint32_t*>(at + words.e));
+      } else {
+        if (col + words.e < cols) w[j] = at[words.e];
+        if (words.split) w[j] |= static_cast<uint32_t>(at[0]) << 16;
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    *reinterpret_cast<uint16_t*>(buf + words.at(words.e, j, lane)) = static_cast<uint16_t>(w[j]);
+    *reinterpret_cast<uint16_t*>(buf + words.at(words.other, j, lane)) = static_cast<uint16_t>(w[j] >> 16);
+  }
+  __syncwarp();
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint4 v = *reinterpret_cast<const uint4*>(buf + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4));
+    w[4 * j] = v.x; w[4 * j + 1] = v.y; w[4 * j + 2] = v.z; w[4 * j + 3] = v.w;
+  }
+  __syncwarp();
+}
+
 // Drains one 128 x 256 accumulator window of this warp's 32 TMEM lanes.  `tacc` already holds the
 // lane quadrant and the window's first column.  The columns the two windows share are at the top of
 // the even window and at the bottom of the odd one; they are read first and `overlap_bar_addr` is
@@ -343,8 +412,10 @@ __device__ __forceinline__ void epilogue_drain(const GemmParams& p, uint32_t tac
     const int last_region = EPI == kEpiRegionBf16 ? (p.out_cols - 1) / p.w_region_rows : 0;
     // converts and stores one 32-column group `r` (local column c, i-th group visited)
     auto emit = [&](const int c, const int i, const uint32_t (&r)[32]) {
-      if (!staged && !row_ok) return;
       const int col = col_base + c;
+      // an output that neither TMA nor vectors can store goes through the staging buffer by rows; all lanes take part
+      const bool by_rows = !staged && stage != nullptr && !p.out_vec_ok && (EPI == kEpiBf16 || EPI == kEpiRegionBf16);
+      if (!staged && (by_rows ? col >= p.out_cols : !row_ok)) return;
       // per-column factors: the launch-wide (or this row's) scale, times the column's region scale for the
       // NVFP4 row-region policy (the product of the two outer scales is formed first, then applied:
       // rtx/kernels/mxfp8_gemm.py:1720-1760; column scales are warp-uniform loads)
@@ -438,6 +509,11 @@ __device__ __forceinline__ void epilogue_drain(const GemmParams& p, uint32_t tac
             tma_store_2d(map_out, buf, col, row - lane - out_row0);
             tma_store_commit();
           }
+        } else if (by_rows) {
+          stage_bf16x32(stage, lane, w);
+          __syncwarp();
+          store_rows_any(stage, reinterpret_cast<__nv_bfloat16*>(p.out), p.ldo, row - lane, p.m, col, p.out_cols, lane);
+          __syncwarp();
         } else {
           __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(p.out) + static_cast<int64_t>(row) * p.ldo;
 #pragma unroll
@@ -478,33 +554,6 @@ __device__ __forceinline__ void epilogue_drain(const GemmParams& p, uint32_t tac
 // accumulated, so that no signal can be counted for the tile before it.
 constexpr int kActEpiWarps = 8;
 constexpr int kActGemmThreads = 64 + 32 * kActEpiWarps;
-
-// 32 rows x 32 columns from the staging buffer (64-byte swizzle) to rows of any alignment: 64-byte segments
-__device__ __forceinline__ void act_store_rows(const uint8_t* buf, __nv_bfloat16* out, int64_t ldo, int row0, int rows,
-                                               int col, int cols, int lane) {
-  if (col + lane >= cols) return;
-  __nv_bfloat16* dst = out + static_cast<int64_t>(row0) * ldo + col + lane;
-#pragma unroll 8
-  for (int j = 0; j < 32; ++j)
-    if (row0 + j < rows)
-      dst[j * ldo] = *reinterpret_cast<const __nv_bfloat16*>(buf + j * 64 + (((lane >> 3) ^ ((j >> 1) & 3)) << 4) + (lane & 7) * 2);
-}
-// the reverse for a residual of any alignment: through the buffer into one row per lane
-__device__ __forceinline__ void act_load_rows(const GemmParams& p, uint8_t* buf, uint32_t (&w)[16], int row0, int col, int lane) {
-  const uint16_t* src = reinterpret_cast<const uint16_t*>(p.residual) + static_cast<int64_t>(row0) * p.ldr + col + lane;
-  const bool col_ok = col + lane < p.out_cols;
-#pragma unroll 8
-  for (int j = 0; j < 32; ++j)
-    *reinterpret_cast<uint16_t*>(buf + j * 64 + (((lane >> 3) ^ ((j >> 1) & 3)) << 4) + (lane & 7) * 2) =
-        col_ok && row0 + j < p.m ? src[j * p.ldr] : static_cast<uint16_t>(0);
-  __syncwarp();
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const uint4 v = *reinterpret_cast<const uint4*>(buf + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4));
-    w[4 * j] = v.x; w[4 * j + 1] = v.y; w[4 * j + 2] = v.z; w[4 * j + 3] = v.w;
-  }
-  __syncwarp();
-}
 
 template <int KIND>
 __device__ __forceinline__ bool act_epilogue_tile(const GemmParams& p, uint32_t tacc, int row0, int n_idx, bool odd, int half,
@@ -563,13 +612,13 @@ __device__ __forceinline__ bool act_epilogue_tile(const GemmParams& p, uint32_t 
           }
         } else {
           __syncwarp();
-          act_store_rows(buf, p.z_out, p.ldo, row0, p.m, col, p.out_cols, lane);
+          store_rows_any(buf, p.z_out, p.ldo, row0, p.m, col, p.out_cols, lane);
         }
       }
       act_apply(p.act, v);
       if (p.tma_out && lane == 0) tma_store_wait_read<0>();
       __syncwarp();
-      if (p.residual != nullptr && !p.residual_vec_ok) act_load_rows(p, buf, res, row0, col, lane);
+      if (p.residual != nullptr && !p.residual_vec_ok) load_rows_any(buf, p.residual, p.ldr, row0, p.m, col, p.out_cols, lane, res);
       act_add_residual(p, v, res);
       pack_bf16x32(v, w);
       stage_bf16x32(buf, lane, w);
@@ -582,7 +631,7 @@ __device__ __forceinline__ bool act_epilogue_tile(const GemmParams& p, uint32_t 
         }
       } else {
         __syncwarp();
-        act_store_rows(buf, reinterpret_cast<__nv_bfloat16*>(p.out), p.ldo, row0, p.m, col, p.out_cols, lane);
+        store_rows_any(buf, reinterpret_cast<__nv_bfloat16*>(p.out), p.ldo, row0, p.m, col, p.out_cols, lane);
         __syncwarp();
       }
     }
