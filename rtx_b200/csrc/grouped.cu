@@ -21,6 +21,8 @@ int launch_quantize_rows(RowsParams& p, int64_t x_tiles, int64_t k, int rounding
   for (RowsOperand* o : {&p.x, &p.w}) {
     const uintptr_t a = reinterpret_cast<uintptr_t>(o->src) | static_cast<uintptr_t>(o->ld * 2);
     o->align = a % 32 == 0 ? 2 : a % 16 == 0 ? 1 : 0;
+    const int64_t rows = o == &p.w ? static_cast<int64_t>(p.batches) * o->rows : o->rows;
+    o->end = o->src ? o->src + (rows - 1) * o->ld + k : nullptr;
   }
   const int64_t w_tiles = p.w.src ? static_cast<int64_t>(p.batches) * p.w_row_tiles : 0;
   const int64_t units = (x_tiles + w_tiles) * p.per_tile;

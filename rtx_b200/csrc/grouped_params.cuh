@@ -27,6 +27,7 @@ struct RowsOperand {
   uint8_t* scales;            // 128-row tiles
   int rows;                   // per matrix (x: all groups)
   int align;                  // of src and its pitch: 2 = 32 bytes, 1 = 16 bytes, 0 = neither
+  const __nv_bfloat16* end;   // behind the last value of all matrices
 };
 struct RowsParams {
   RowsOperand x, w;

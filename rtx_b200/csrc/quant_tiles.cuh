@@ -256,6 +256,10 @@ __device__ __forceinline__ void cp_async_16(void* smem_dst, const void* gmem_src
                "r"(valid ? 16 : 0)
                : "memory");
 }
+// the first `bytes` (0, 2 or 4) of a word, zeros behind them
+__device__ __forceinline__ void cp_async_4(void* smem_dst, const void* gmem_src, int bytes) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(smem_dst)), "l"(gmem_src), "r"(bytes) : "memory");
+}
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }

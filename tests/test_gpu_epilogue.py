@@ -466,6 +466,36 @@ def test_experts_and_epilogue_as_used_together(dev):
     within(xd.grad, total, 2.0 ** -8 * total.abs() + (1 + 2.0 ** -8) * bound)
 
 
+@pytest.mark.parametrize("m,n,k", [(300, 222, 386), (131, 255, 97), (257, 33, 520), (150, 129, 64)])
+def test_every_alignment_gives_the_same_bits(dev, m, n, k):
+    """Operands in wider tensors of NaN, at every two-byte place: the bits of the contiguous ones, which are right."""
+    import rtx_b200
+
+    x, w, b, r, dy = inputs(m, n, k, seed=22)
+    xd, wd, bd, rd, dyd = (t.to(dev) for t in (x, w, b, r, dy))
+    z = rtx_b200.mxfp8_linear_epilogue(xd, wd, bd)
+    y = rtx_b200.mxfp8_linear_epilogue(xd, wd, bd, rd, activation="gelu")
+    grads = rtx_b200.mxfp8_linear_epilogue_backward(dyd, z, xd, wd, activation="gelu")
+    within(y, *forward(x, w, b, r, "gelu")[:2])
+    for got, (want, bound) in zip(grads, backward(dy, z.cpu(), x, w, "gelu").values()):
+        within(got, want, bound)
+
+    def moved(t, pad, lead):
+        flat = torch.full((t.shape[0] * (t.shape[1] + pad) + lead + 8,), float("nan"), dtype=torch.bfloat16, device=dev)
+        view = flat.as_strided(t.shape, (t.shape[1] + pad, 1), lead)
+        view.copy_(t)
+        return view
+
+    for pad, lead in ((0, 1), (0, 2), (1, 0), (1, 4), (1, 3), (2, 0), (2, 6), (7, 5), (8, 8)):
+        xv, rv, dyv, wv = moved(xd, pad, lead), moved(rd, pad, lead), moved(dyd, pad, lead), moved(wd, 0, lead)
+        bv = moved(bd[None], 0, lead)[0]
+        zv = moved(z, 0, lead)
+        assert torch.equal(rtx_b200.mxfp8_linear_epilogue(xv, wv, bv, rv, activation="gelu"), y), (pad, lead)
+        got = rtx_b200.mxfp8_linear_epilogue_backward(dyv, zv, xv, wv, activation="gelu")
+        for a, c in zip(got, grads):
+            assert torch.equal(a, c), (pad, lead)
+
+
 @pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh"])
 def test_small_slopes_keep_their_relative_accuracy(dev, act):
     """One row, so that dbias is dz: every BF16 z in [-64, -2], where the slopes fall from 0.1 to nothing.

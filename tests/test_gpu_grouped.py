@@ -238,6 +238,38 @@ def test_pitches_views_and_unaligned_rows(dev):
           want, mag, 96)
 
 
+@pytest.mark.parametrize("n,k", [(64, 63), (65, 130), (191, 97), (136, 264), (33, 192)])
+def test_every_alignment_gives_the_same_bits(dev, n, k):
+    """Operands in wider tensors of NaN: pitches odd and even, starts at every two-byte place, groups that begin on odd rows.
+    All of them against the contiguous operands' bits, and those against the definition."""
+    import rtx_b200
+
+    offsets = offs(45, 1, 140, 66, head=3)
+    rows = offsets[-1] + 2
+    x, w, dy = inputs(rows, 4, n, k, seed=21)
+    xd, wd, dyd, od = x.to(dev), w.to(dev), dy.to(dev), on(dev, offsets)
+    y = rtx_b200.mxfp8_grouped_linear(xd, wd, od)
+    dx, dw = rtx_b200.mxfp8_grouped_linear_backward(dyd, xd, wd, od)
+    close(y, *forward(x, w, offsets), k)
+    want_dx, want_dw, dx_mag, dw_mag = backward(dy, x, w, offsets)
+    close(dx, want_dx, dx_mag, n)
+    close(dw, want_dw, dw_mag, 140)
+
+    def moved(t, pad, lead):
+        flat = torch.full((t.shape[0] * (t.shape[1] + pad) + lead + 8,), float("nan"), dtype=torch.bfloat16, device=dev)
+        view = flat.as_strided(t.shape, (t.shape[1] + pad, 1), lead)
+        view.copy_(t)
+        return view
+
+    for pad, lead in ((0, 1), (0, 2), (1, 0), (1, 4), (1, 3), (2, 0), (2, 6), (7, 5), (8, 8)):
+        xv, dyv = moved(xd, pad, lead), moved(dyd, pad, lead)
+        wv = moved(wd.view(-1, k), 0, lead).view(4, n, k)
+        assert wv.data_ptr() % 16 == 2 * lead % 16
+        assert torch.equal(rtx_b200.mxfp8_grouped_linear(xv, wv, od), y), (pad, lead)
+        got_dx, got_dw = rtx_b200.mxfp8_grouped_linear_backward(dyv, xv, wv, od)
+        assert torch.equal(got_dx, dx) and torch.equal(got_dw, dw), (pad, lead)
+
+
 def test_out_argument_with_a_pitch_keeps_what_is_beside_it(dev):
     from rtx_b200 import ops
 
