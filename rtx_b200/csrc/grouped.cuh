@@ -370,7 +370,7 @@ __global__ void __launch_bounds__(kQuantThreads, kRowsOccupancy) quant_mxfp8_row
 // in flight per SM only while nothing is computed), and the columns' payload leaves through it, because a lane holds 32
 // bytes of a column whose K step is 128.  No barrier but the warp's own.
 // Bound by memory and, with 16 warps per SM, by instruction latency (56 % issue): 8192 x 4096 gradient and x, 4 weights of
-// 4096 x 4096 (268 MB read, 168 MB written) in 78 us, 5.6 TB/s, 0.85 of the copy rate.  On the way, 8192 rows, 32 groups,
+// 4096 x 4096 (268 MB read, 168 MB written) in 79 us, 5.5 TB/s, 0.84 of the copy rate.  On the way, 8192 rows, 32 groups,
 // 2048 x 4096 (a launch for the gradient on staged 128 x 128 tiles and one for the rest, together): 253 us with direct loads
 // and stores, 225 with staged stores, 195 with blocks fetched ahead too; one launch 196, without register spills 187.
 // ---------------------------------------------------------------------------
@@ -389,6 +389,36 @@ struct TransposedUnit {
   int rt, matrix;   // 128-row tile, of its matrix
   int col0;
 };
+
+// the block at `src` value by value or by words, where rows or columns are no 16-byte pieces (quant_mxfp8_transposed_fetch); a
+// call, so that it costs the common path no registers
+__device__ __noinline__ void quant_mxfp8_transposed_fetch_words(const uint16_t* src, const void* none, int64_t ld, int row0, int live,
+                                                                int cols, int by, uint8_t* buf, uint8_t* last) {
+  const int lane = threadIdx.x & 31, left = cols - 2 * lane;   // columns from this lane's first one on
+  const uint16_t* at = src + 2 * lane;
+  auto slot = [&](int e) { return buf + e * 128 + (((lane >> 2) ^ (e & 7)) << 4) + 4 * (lane & 3); };
+  if (by == 1) {
+    // with an odd pitch every other row starts between two words: it comes one value early (shift_odd_rows puts it right)
+    const int odd = static_cast<int>(ld & 1);
+#pragma unroll 8
+    for (int e = 0; e < 32; ++e) {
+      const int early = odd & (row0 + e), have = e < live ? left + early : 0;
+      cp_async_4(slot(e), have > 0 ? static_cast<const void*>(at + e * ld - early) : none, have >= 2 ? 4 : have == 1 ? 2 : 0);
+    }
+    if (odd && lane < 16) {   // the last value of each of those rows
+      const int e = 2 * lane + (~row0 & 1);
+      const bool have = e < live && cols >= 64;
+      cp_async_4(last + 4 * lane, have ? static_cast<const void*>(src + e * ld + 63) : none, have ? 2 : 0);
+    }
+  } else {
+#pragma unroll 8
+    for (int e = 0; e < 32; ++e) {
+      const bool row = e < live;
+      const uint32_t a = row && left >= 1 ? at[e * ld] : 0u, b = row && left >= 2 ? at[e * ld + 1] : 0u;
+      *reinterpret_cast<uint32_t*>(slot(e)) = a | (b << 16);
+    }
+  }
+}
 
 // Block j of the unit into `buf` [32 rows][64 columns]; what lies outside the operand is zero.  16-byte chunk i of row r
 // lies at chunk i ^ (r % 8): eight lanes that read one chunk of eight rows meet in no bank, nor do 32 that read a row.
@@ -409,39 +439,16 @@ __device__ __forceinline__ void quant_mxfp8_transposed_fetch(const TransposedUni
       cp_async_16(buf + r * 128 + (((lane & 7) ^ (r & 7)) << 4), valid ? at + 4 * i * o.ld : src, valid);
     }
   } else {
-    const int left = cols - 2 * lane;   // columns from this lane's first one on
-    const uint16_t* at = src + 32 * j * o.ld + 2 * lane;
-    auto slot = [&](int e) { return buf + e * 128 + (((lane >> 2) ^ (e & 7)) << 4) + 4 * (lane & 3); };
-    if (by == 1) {
-      // with an odd pitch every other row starts between two words: it comes one value early (shift_odd_rows puts it right)
-      const int odd = static_cast<int>(o.ld & 1);
-#pragma unroll 4
-      for (int e = 0; e < 32; ++e) {
-        const int early = odd & (f.row0 + e), have = 32 * j + e < f.live ? left + early : 0;
-        cp_async_4(slot(e), have > 0 ? static_cast<const void*>(at + e * o.ld - early) : o.src, have >= 2 ? 4 : have == 1 ? 2 : 0);
-      }
-      if (odd && lane < 16) {   // the last value of each of those rows
-        const int e = 2 * lane + (~f.row0 & 1);
-        const bool have = 32 * j + e < f.live && cols >= 64;
-        cp_async_4(last + 4 * lane, have ? static_cast<const void*>(src + (32 * j + e) * o.ld + 63) : o.src, have ? 2 : 0);
-      }
-    } else {
-#pragma unroll 8
-      for (int e = 0; e < 32; ++e) {
-        const bool row = 32 * j + e < f.live;
-        const uint32_t a = row && left >= 1 ? at[e * o.ld] : 0u, b = row && left >= 2 ? at[e * o.ld + 1] : 0u;
-        *reinterpret_cast<uint32_t*>(slot(e)) = a | (b << 16);
-      }
-    }
+    quant_mxfp8_transposed_fetch_words(src + 32 * j * o.ld, o.src, o.ld, f.row0, f.live - 32 * j, cols, by, buf, last);
   }
   cp_async_commit();
 }
 
-__device__ __forceinline__ void shift_odd_rows(const TransposedUnit& f, uint8_t* buf, const uint8_t* last) {
+__device__ __noinline__ void shift_odd_rows(int row0, uint8_t* buf, const uint8_t* last) {
   const int lane = threadIdx.x & 31;
 #pragma unroll 8
   for (int i = 0; i < 16; ++i) {
-    const int e = 2 * i + (~f.row0 & 1);
+    const int e = 2 * i + (~row0 & 1);
     uint32_t* at = reinterpret_cast<uint32_t*>(buf + e * 128 + (((lane >> 2) ^ (e & 7)) << 4) + 4 * (lane & 3));
     const uint32_t word = *at;
     uint32_t next = __shfl_down_sync(0xffffffffu, word, 1);
@@ -559,13 +566,14 @@ quant_mxfp8_transposed_units_kernel(const TransposedParams p) {
     const TransposedOperand& o = operand(f.operand);
     const int bytes = static_cast<int>(min(static_cast<int64_t>(128), o.pitch - static_cast<int64_t>(128 * f.rt)));   // of a column
     const bool columns = !GRADIENT || f.operand != 2 || p.dy.q != nullptr;
+    const bool shifted = (o.ld & 1) && (by >> 2 * f.operand & 3) == 1;
     uint32_t word0 = 0, word1 = 0;   // the four scale bytes of either column
 #pragma unroll 1
     for (int j = 0; j < 4; ++j) {
       cp_async_wait<1>();            // everything but the newest group: block j is here
       __syncwarp();
       uint8_t* rows = buf + (j & 1) * kTransposedFetchBytes;
-      if ((o.ld & 1) && (by >> 2 * f.operand & 3) == 1) shift_odd_rows(f, rows, last + (j & 1) * kTransposedLastBytes);
+      if (shifted) shift_odd_rows(f.row0, rows, last + (j & 1) * kTransposedLastBytes);
       if (GRADIENT && f.operand == 2 && p.dy_rows && 32 * j < f.live) quant_mxfp8_gradient_rows(f, p, j, rows);
       uint32_t w[32];
 #pragma unroll
