@@ -497,8 +497,9 @@ __device__ __forceinline__ void quant_mxfp8_gradient_rows(const TransposedUnit& 
   }
 }
 
-// GRADIENT: the gradient's units come first, in both orientations from one read, and the kernel is the first of its chain
-// (it leaves the plan and sets the result's rows of no group to zero)
+// GRADIENT (the grouped backward): the gradient's units come first, in both orientations from one read, its rows and x's
+// are split into groups, and the kernel is the first of its chain (it leaves the plan and sets the result's rows of no
+// group to zero).  Else x is one group of all its rows.
 template <bool GRADIENT>
 __global__ void __launch_bounds__(kQuantThreads, kTransposedOccupancy)
 quant_mxfp8_transposed_units_kernel(const TransposedParams p) {
@@ -508,13 +509,12 @@ quant_mxfp8_transposed_units_kernel(const TransposedParams p) {
   uint8_t* last = stage + kTransposedStageBytes;
   __shared__ GroupScan scan;
   griddep_launch_dependents();
-  const bool grouped = GRADIENT || p.list.offsets != nullptr;
-  if (grouped && (GRADIENT || p.x.src)) scan_groups(p.list, scan, GRADIENT ? p.status : nullptr);
   if (GRADIENT) {
+    scan_groups(p.list, scan, p.status);
     if (blockIdx.x == 0) write_group_plan(p.list, scan, p.plan, reinterpret_cast<int*>(qt_smem));
     if (p.dx) zero_rows_of_no_group(p.list, scan, p.dx, p.dx_cols, p.dx_cols);
   }
-  const uint32_t x_tiles = grouped ? (GRADIENT || p.x.src ? scan.tile[p.list.groups] : 0) : p.x.src ? (p.x.rows + 127) / 128 : 0;
+  const uint32_t x_tiles = GRADIENT ? scan.tile[p.list.groups] : (p.x.rows + 127) / 128;
   const uint32_t dy_units = GRADIENT ? x_tiles * p.dy_col_units : 0;
   const uint32_t x_end = dy_units + (p.x.src ? x_tiles * p.x_col_units : 0);
   const uint32_t units = x_end + (p.w.src ? p.batches * p.w_row_tiles * p.w_col_units : 0u);   // < 2^31 (host)
@@ -533,7 +533,7 @@ quant_mxfp8_transposed_units_kernel(const TransposedParams p) {
       f.rt -= f.matrix * p.w_row_tiles;
       f.row0 = f.matrix * o.rows + 128 * f.rt;
       f.live = o.rows - 128 * f.rt;
-    } else if (grouped) {
+    } else if (GRADIENT) {
       const int g = group_before(scan.tile, p.list.groups, f.rt);
       f.row0 = scan.start[g] + 128 * (f.rt - scan.tile[g]);
       f.live = scan.start[g + 1] - f.row0;

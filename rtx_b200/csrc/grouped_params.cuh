@@ -62,7 +62,7 @@ struct TransposedOperand {
 };
 struct TransposedParams {
   TransposedOperand x, w;
-  GroupList list;             // offsets nullptr: x is one group of all its rows
+  GroupList list;             // with the gradient only; else x is one group of all its rows
   int batches;                // matrices of w
   int x_col_units, w_col_units, w_row_tiles;
   const float* partial;       // column sums [row_tiles][n] left by the launch before this one; nullptr = none
