@@ -18,12 +18,24 @@ from torch.autograd import forward_ad
 _LIB = torch.library.Library("rtx", "FRAGMENT")
 
 
-def eager(t: torch.Tensor) -> bool:
-    """Whether an op on `t` would only be dispatched back into this package's CUDA implementation (a plain CUDA tensor, no
-    tracing, no `torch.func` transform): the package's own functions then call the launcher itself and save a dispatch of a
-    few microseconds."""
-    return ((type(t) is torch.Tensor or type(t) is torch.nn.Parameter) and t.is_cuda
-            and not torch.compiler.is_compiling() and not torch._C._are_functorch_transforms_active())
+def interposed() -> bool:
+    """Whether something has to see an op's call before the CUDA implementation runs: `torch.compile`, a `torch.func`
+    transform, a dispatch mode (`make_fx`, a FLOP counter, a checkpointing policy, fake tensors) or `torch.jit.trace`.  A
+    launcher that is called past them writes through an address they know nothing of, and a graph they record lacks it."""
+    return (torch.compiler.is_compiling() or torch._C._are_functorch_transforms_active()
+            or torch._C._len_torch_dispatch_stack() > 0 or torch._C._is_tracing())
+
+
+def eager(t: torch.Tensor, *others: Optional[torch.Tensor]) -> bool:
+    """Whether an op on these operands would only be dispatched back into this package's CUDA implementation (plain CUDA
+    tensors, nothing interposed): the package's own functions then call the launcher itself and save a dispatch of a few
+    microseconds."""
+    if not t.is_cuda or interposed():
+        return False
+    for operand in (t, *others):
+        if operand is not None and type(operand) is not torch.Tensor and type(operand) is not torch.nn.Parameter:
+            return False
+    return True
 
 
 def refuse_tangents(name: str, *tensors) -> None:

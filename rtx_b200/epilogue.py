@@ -126,7 +126,7 @@ def _train_backward(ctx, grad_y, _grad_z):
     if not (need_dx or need_dw or need_db):
         return None, None, None, grad_y if need_dr else None, None
     x, weight, z = ctx.saved_tensors
-    if eager(grad_y):
+    if eager(grad_y, x, weight, z):
         weight = weight.contiguous() if need_dx else weight
         return (*ops.mxfp8_linear_epilogue_bwd(grad_y, z, x, weight, weight.shape[1], activation=ctx.activation,
                                                need_dx=need_dx, need_dw=need_dw, need_dbias=need_db),
@@ -143,8 +143,7 @@ class _LinearEpilogueFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, residual, activation):
-        forward = mxfp8_linear_epilogue_fwd.fn if eager(x) else mxfp8_linear_epilogue_fwd
-        y, z = forward(x, weight, bias, residual, activation)
+        y, z = mxfp8_linear_epilogue_fwd.fn(x, weight, bias, residual, activation)
         ctx.save_for_backward(x, weight, z)
         ctx.activation = activation
         return y
@@ -175,13 +174,13 @@ def mxfp8_linear_epilogue(x: torch.Tensor, weight, bias: Optional[torch.Tensor] 
     refuse_tangents("mxfp8_linear_epilogue", x, weight, bias, residual)
     n, k = weight.shape
     shape, x, residual = _matrices(x, residual, n, k)
+    direct = eager(x, weight, bias, residual)
     if not _needs_grad(x, weight, bias, residual):
-        forward = mxfp8_linear_epilogue_op.fn if eager(x) else mxfp8_linear_epilogue_op
-        y = forward(x, weight, bias, residual, activation)
-    elif torch.compiler.is_compiling():
-        y = mxfp8_linear_epilogue_train(x, weight, bias, residual, activation)[0]
-    else:
+        y = (mxfp8_linear_epilogue_op.fn if direct else mxfp8_linear_epilogue_op)(x, weight, bias, residual, activation)
+    elif direct:
         y = _LinearEpilogueFunction.apply(x, weight, bias, residual, activation)
+    else:
+        y = mxfp8_linear_epilogue_train(x, weight, bias, residual, activation)[0]
     return y if len(shape) == 2 else y.reshape(shape)
 
 
@@ -205,7 +204,7 @@ def _apply_packed(x, packed, n, k, bias, residual, activation):
     if _needs_grad(x, bias, residual):
         raise RuntimeError("a prequantized MXFP8 weight is inference-only; keep the BF16 master weight to train")
     data, scales = packed if isinstance(packed, tuple) else mxfp8_kernel_operands(packed)
-    if eager(x):
+    if eager(x, data, scales, bias, residual):
         y = ops.mxfp8_linear_epilogue_fwd_prequant_w(x, data, scales, n, bias, residual, activation=activation)
     else:
         y = mxfp8_linear_epilogue_prequant_w(x, data, scales, bias, residual, n, k, activation)
@@ -222,7 +221,7 @@ def mxfp8_linear_epilogue_backward(grad_output: torch.Tensor, z: Optional[torch.
     if activation != "none" and z is None:
         raise ValueError("an activation's backward needs the pre-activation z")
     z2d = z.reshape(-1, n).contiguous() if z is not None and activation != "none" else grad_output.new_empty(0)
-    backward = mxfp8_linear_epilogue_bwd.fn if eager(x) else mxfp8_linear_epilogue_bwd
+    backward = mxfp8_linear_epilogue_bwd.fn if eager(x, grad_output, z2d, weight) else mxfp8_linear_epilogue_bwd
     dx, dw, db = backward(grad_output.reshape(-1, n), z2d, x.reshape(-1, k), weight, activation, True, True, bias)
     return dx.reshape(x.shape), dw, db if bias else None
 

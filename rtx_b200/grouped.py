@@ -130,7 +130,7 @@ def _train_setup(ctx, inputs, output):
 def _train_backward(ctx, grad_output):
     x, weight, offsets = ctx.saved_tensors
     need_dx, need_dw = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
-    if eager(grad_output):
+    if eager(grad_output, x, weight, offsets):
         return (*_bwd(grad_output, x, weight, offsets, need_dx, need_dw), None)
     if need_dx and need_dw:
         return (*mxfp8_grouped_linear_bwd(grad_output, x, weight, offsets), None)
@@ -151,7 +151,7 @@ class _GroupedLinearFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, offsets):
         ctx.save_for_backward(x, weight, offsets)
-        return _forward(x, weight, offsets)
+        return mxfp8_grouped_linear_op.fn(x, weight, offsets)
 
     backward = staticmethod(once_differentiable(_train_backward))
 
@@ -188,24 +188,17 @@ def mxfp8_grouped_linear(x: torch.Tensor, weight, offsets: torch.Tensor) -> torc
 
 def _packed(x, weight_data, weight_scales, offsets, n) -> torch.Tensor:
     refuse_tangents("mxfp8_grouped_linear", x)
-    if eager(x):
+    if eager(x, weight_data, weight_scales, offsets):
         return ops.mxfp8_grouped_linear_fwd_prequant_w(x, weight_data, weight_scales, offsets, n)
     return mxfp8_grouped_linear_prequant_w(x, weight_data, weight_scales, offsets, n)
 
 
-def _forward(x, weight, offsets) -> torch.Tensor:
-    if eager(x):
-        return mxfp8_grouped_linear_op.fn(x, weight, offsets)
-    return mxfp8_grouped_linear_op(x, weight, offsets)
-
-
 def _dynamic(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor) -> torch.Tensor:
     refuse_tangents("mxfp8_grouped_linear", x, weight)
+    direct = eager(x, weight, offsets)
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
-        if torch.compiler.is_compiling():
-            return mxfp8_grouped_linear_train(x, weight, offsets)
-        return _GroupedLinearFunction.apply(x, weight, offsets)
-    return _forward(x, weight, offsets)
+        return (_GroupedLinearFunction.apply if direct else mxfp8_grouped_linear_train)(x, weight, offsets)
+    return (mxfp8_grouped_linear_op.fn if direct else mxfp8_grouped_linear_op)(x, weight, offsets)
 
 
 def mxfp8_grouped_linear_backward(grad_output: torch.Tensor, x: torch.Tensor, weight: torch.Tensor,
@@ -213,7 +206,7 @@ def mxfp8_grouped_linear_backward(grad_output: torch.Tensor, x: torch.Tensor, we
     """BF16 dX [rows, K] and dW [groups, N, K] of `mxfp8_grouped_linear`, from independently quantized MXFP8 products
     (blocks along N for dX, along each group's rows for dW)."""
     refuse_tangents("mxfp8_grouped_linear_backward", grad_output, x, weight)
-    if eager(x):
+    if eager(x, grad_output, weight, offsets):
         return mxfp8_grouped_linear_bwd.fn(grad_output, x, weight, offsets)
     return mxfp8_grouped_linear_bwd(grad_output, x, weight, offsets)
 

@@ -1,0 +1,134 @@
+"""The grouped linear and the linear with an epilogue where something else has to see their ops: `make_fx`,
+`torch.jit.trace`, a dispatch mode.  What they record is replayed on other inputs and has to give the eager call's bits."""
+import warnings
+
+import pytest
+import torch
+from torch.fx.experimental.proxy_tensor import make_fx
+from torch.utils._python_dispatch import TorchDispatchMode
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def dev(native_lib):
+    if not torch.cuda.is_available():
+        pytest.fail("these tests need a CUDA device")
+    torch.cuda.set_device(0)
+    return torch.device("cuda", 0)
+
+
+def calls(dev):
+    """{name: (function of tensors alone, its inputs, others of the same shapes, the op that a graph of it holds)}"""
+    import rtx_b200 as r
+
+    gen = torch.Generator(device=dev).manual_seed(5)
+
+    def normal(*shape):
+        return torch.randn(*shape, generator=gen, device=dev).bfloat16()
+
+    offsets = [torch.tensor(o, dtype=torch.int32, device=dev) for o in ((0, 20, 20, 66), (3, 5, 40, 70))]
+    wp, gp = r.quantize_mxfp8(normal(72, 96)), r.quantize_mxfp8(normal(3, 128, 96))
+
+    def two(make):
+        return make(0), make(1)
+
+    x2 = lambda i: (normal(70, 96),)
+    return {
+        "grouped": (r.mxfp8_grouped_linear, *two(lambda i: (*x2(i), normal(3, 72, 96), offsets[i])), "mxfp8_grouped_linear"),
+        "grouped packed": (lambda x, o: r.mxfp8_grouped_linear(x, gp, o), *two(lambda i: (*x2(i), offsets[i])),
+                           "mxfp8_grouped_linear_prequant_w"),
+        "grouped backward": (r.mxfp8_grouped_linear_backward,
+                             *two(lambda i: (normal(70, 72), *x2(i), normal(3, 72, 96), offsets[i])), "mxfp8_grouped_linear_bwd"),
+        "epilogue": (lambda x, w, b, res: r.mxfp8_linear_epilogue(x, w, b, res, activation="gelu"),
+                     *two(lambda i: (*x2(i), normal(72, 96), normal(72), normal(70, 72))), "mxfp8_linear_epilogue"),
+        "epilogue packed": (lambda x, b: r.mxfp8_linear_epilogue(x, wp, b, activation="silu"),
+                            *two(lambda i: (*x2(i), normal(72))), "mxfp8_linear_epilogue_prequant_w"),
+        "epilogue backward": (lambda dy, z, x, w: r.mxfp8_linear_epilogue_backward(dy, z, x, w, activation="gelu_tanh"),
+                              *two(lambda i: (normal(70, 72), normal(70, 72), *x2(i), normal(72, 96))), "mxfp8_linear_epilogue_bwd"),
+    }
+
+
+NAMES = ["grouped", "grouped packed", "grouped backward", "epilogue", "epilogue packed", "epilogue backward"]
+
+
+def same(got, want):
+    got, want = (v if isinstance(v, (tuple, list)) else [v] for v in (got, want))
+    assert len(got) == len(want)
+    for a, b in zip(got, want):
+        assert a.dtype is b.dtype and torch.equal(a, b)
+
+
+@pytest.mark.parametrize("name", NAMES)
+@pytest.mark.parametrize("mode", ["real", "fake"])
+def test_make_fx_graph(dev, name, mode):
+    f, first, other, op = calls(dev)[name]
+    graph = make_fx(f, tracing_mode=mode, _allow_non_fake_inputs=True)(*first)   # packed weights are the graph's own
+    assert [n for n in graph.graph.nodes if str(n.target) == f"rtx.{op}.default"], graph.graph
+    same(graph(*other), f(*other))
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_jit_trace_graph(dev, name):
+    f, first, other, op = calls(dev)[name]
+    with warnings.catch_warnings():
+        warnings.simplefilter("ignore")
+        graph = torch.jit.trace(f, first, check_trace=False)
+    assert f"rtx::{op}(" in str(graph.graph)
+    same(graph(*other), f(*other))
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_a_dispatch_mode_sees_the_op(dev, name):
+    f, first, _, op = calls(dev)[name]
+    seen = []
+
+    class Watch(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            seen.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    want = f(*first)
+    with Watch():
+        got = f(*first)
+    assert f"rtx.{op}.default" in seen
+    same(got, want)
+
+
+@pytest.mark.parametrize("name", ["grouped", "epilogue"])
+def test_traced_graphs_of_trainable_weights_are_differentiable(dev, name):
+    """The recorded op carries its gradient: a replayed graph's gradients are the eager call's."""
+    f, first, other, _ = calls(dev)[name]
+    leaves = [t.requires_grad_(True) for t in other if t.is_floating_point()]
+    traced = tuple(t.requires_grad_(True) if t.is_floating_point() else t for t in first)
+    y = f(*other)
+    dy = torch.randn_like(y)
+    want = torch.autograd.grad(y, leaves, dy)
+    with warnings.catch_warnings():
+        warnings.simplefilter("ignore")
+        graphs = [make_fx(f)(*traced), torch.jit.trace(f, traced, check_trace=False)]
+    for graph in graphs:
+        out = graph(*other)
+        same(out, y)
+        same(torch.autograd.grad(out, leaves, dy), want)
+
+    # a whole step, its backward inside the graph
+    def step(*args):
+        args = [a.detach().requires_grad_(a.is_floating_point()) for a in args]
+        return torch.autograd.grad(f(*args), [a for a in args if a.requires_grad], dy)
+
+    same(make_fx(step)(*first)(*other), want)
+
+
+@pytest.mark.parametrize("name", ["grouped", "epilogue"])
+def test_vmap_over_trainable_weights(dev, name):
+    """One call after the other, with the gradients of both in the shared operands."""
+    f, first, other, _ = calls(dev)[name]
+    rest = tuple(t.requires_grad_(True) if t.is_floating_point() else t for t in first[1:])
+    leaves = [t for t in rest if t.is_floating_point()]
+    x = torch.stack([first[0], other[0]]).requires_grad_(True)
+    y = torch.func.vmap(f, (0, *[None] * len(rest)))(x, *rest)
+    want = torch.stack([f(a, *rest) for a in x])
+    same(y, want)
+    dy = torch.randn_like(want)
+    same(torch.autograd.grad(y, [x, *leaves], dy, retain_graph=True), torch.autograd.grad(want, [x, *leaves], dy))
