@@ -38,6 +38,38 @@ def eager(t: torch.Tensor, *others: Optional[torch.Tensor]) -> bool:
     return True
 
 
+def transformed() -> bool:
+    """Whether a `torch.func` transform is active that differentiates or batches an `autograd.Function` with a
+    `setup_context`; a formula registered for an op cannot be differentiated there.  (`functionalize` is the other way
+    round: it takes ops and no such functions.)"""
+    if torch.compiler.is_compiling() or not torch._C._are_functorch_transforms_active():
+        return False
+    levels = torch._C._functorch.get_interpreter_stack() or ()
+    return all(level.key() != torch._C._functorch.TransformType.Functionalize for level in levels)
+
+
+class _Once(torch.autograd.Function):
+    generate_vmap_rule = True
+
+    @staticmethod
+    def forward(op, message, *args):
+        return op(*args)
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        ctx.message = inputs[1]
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise NotImplementedError(ctx.message)
+
+
+def call_without_derivative(op: "OpHandle", message: str, *args):
+    """An op that has no derivative: `torch.func` transforms that ask for one get the error `message`, where the bare op
+    would give zeros."""
+    return _Once.apply(op, message, *args) if transformed() else op(*args)
+
+
 def refuse_tangents(name: str, *tensors) -> None:
     """Forward-mode differentiation of an op without a formula for it would drop the tangents: refuse it."""
     if forward_ad._current_level >= 0 and not torch.compiler.is_compiling():
@@ -62,6 +94,13 @@ class OpHandle:
     def register_fake(self, fn: Callable) -> Callable:
         torch.library.register_fake(self.qualname, fn, lib=_LIB)
         return fn
+
+    def refuse_derivative(self, message: str) -> None:
+        """Differentiating the op raises, where an op without a formula would warn and give zeros."""
+        def backward(ctx, *grads):
+            raise NotImplementedError(message)
+
+        self.register_autograd(backward)
 
     def register_autograd(self, backward: Callable, *, setup_context: Optional[Callable] = None) -> None:
         torch.library.register_autograd(self.qualname, backward, setup_context=setup_context, lib=_LIB)

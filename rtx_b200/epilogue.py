@@ -17,9 +17,12 @@ from torch.autograd.function import once_differentiable
 
 from . import fp8 as _fp8
 from . import ops
-from ._oplib import custom_op, eager, refuse_tangents
+from ._oplib import call_without_derivative, custom_op, eager, refuse_tangents, transformed
 from .formats import (PACKED_OPERAND_SCHEMA_VERSION, SCALE_LAYOUT_CODES, MXFP8Tensor, make_mxfp8_tensor,
                       mxfp8_kernel_operands, mxfp8_matrix_shape, mxfp8_qdata_2d, mxfp8_scales_for_kernel, reject_packed_dtype_conversion)
+
+
+_FROZEN = "a prequantized MXFP8 weight is inference-only; keep the BF16 master weight to train"
 
 
 def _check(x, n, k, bias, residual, activation) -> None:
@@ -110,6 +113,10 @@ def _(grad_output, z, x, weight, activation, need_dx, need_dw, need_dbias):
             new((weight.shape[0],)) if need_dbias else new(0))
 
 
+_TWICE = "the backward of mxfp8_linear_epilogue has no derivative of its own"
+mxfp8_linear_epilogue_bwd.refuse_derivative(_TWICE)
+
+
 def _train_setup(ctx, inputs, output):
     x, weight, _bias, _residual, activation = inputs
     _y, z = output
@@ -121,17 +128,23 @@ def _train_setup(ctx, inputs, output):
 
 def _train_backward(ctx, grad_y, _grad_z):
     need_dx, need_dw, need_db, need_dr = ctx.needs_input_grad[:4]
-    if grad_y is None:
-        return (None,) * 5
-    if not (need_dx or need_dw or need_db):
+    if grad_y is None or not (need_dx or need_dw or need_db):
         return None, None, None, grad_y if need_dr else None, None
     x, weight, z = ctx.saved_tensors
-    if eager(grad_y, x, weight, z):
-        weight = weight.contiguous() if need_dx else weight
-        return (*ops.mxfp8_linear_epilogue_bwd(grad_y, z, x, weight, weight.shape[1], activation=ctx.activation,
-                                               need_dx=need_dx, need_dw=need_dw, need_dbias=need_db),
-                grad_y if need_dr else None, None)
-    dx, dw, db = mxfp8_linear_epilogue_bwd(grad_y, z, x, weight, ctx.activation, need_dx, need_dw, need_db)
+    if not eager(grad_y, x, weight, z):
+        return _dispatched_backward(ctx, grad_y, None)
+    weight = weight.contiguous() if need_dx else weight
+    return (*ops.mxfp8_linear_epilogue_bwd(grad_y, z, x, weight, weight.shape[1], activation=ctx.activation, need_dx=need_dx,
+                                           need_dw=need_dw, need_dbias=need_db), grad_y if need_dr else None, None)
+
+
+def _dispatched_backward(ctx, grad_y, _grad_z):
+    need_dx, need_dw, need_db, need_dr = ctx.needs_input_grad[:4]
+    if grad_y is None or not (need_dx or need_dw or need_db):
+        return None, None, None, grad_y if need_dr else None, None
+    x, weight, z = ctx.saved_tensors
+    dx, dw, db = call_without_derivative(mxfp8_linear_epilogue_bwd, _TWICE, grad_y, z, x, weight, ctx.activation, need_dx,
+                                         need_dw, need_db)
     return (dx if need_dx else None, dw if need_dw else None, db if need_db else None, grad_y if need_dr else None, None)
 
 
@@ -152,6 +165,19 @@ class _LinearEpilogueFunction(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, grad_y):
         return _train_backward(ctx, grad_y, None)
+
+
+class _TransformedLinearEpilogue(torch.autograd.Function):
+    """The same node in the form that `torch.func` transforms take."""
+
+    generate_vmap_rule = True
+
+    @staticmethod
+    def forward(x, weight, bias, residual, activation):
+        return mxfp8_linear_epilogue_fwd(x, weight, bias, residual, activation)
+
+    setup_context = staticmethod(_train_setup)
+    backward = staticmethod(_dispatched_backward)
 
 
 def _needs_grad(*tensors) -> bool:
@@ -175,7 +201,9 @@ def mxfp8_linear_epilogue(x: torch.Tensor, weight, bias: Optional[torch.Tensor] 
     n, k = weight.shape
     shape, x, residual = _matrices(x, residual, n, k)
     direct = eager(x, weight, bias, residual)
-    if not _needs_grad(x, weight, bias, residual):
+    if not direct and transformed():
+        y = _TransformedLinearEpilogue.apply(x, weight, bias, residual, activation)[0]
+    elif not _needs_grad(x, weight, bias, residual):
         y = (mxfp8_linear_epilogue_op.fn if direct else mxfp8_linear_epilogue_op)(x, weight, bias, residual, activation)
     elif direct:
         y = _LinearEpilogueFunction.apply(x, weight, bias, residual, activation)
@@ -202,12 +230,12 @@ def _apply_packed(x, packed, n, k, bias, residual, activation):
     refuse_tangents("mxfp8_linear_epilogue", x, bias, residual)
     shape, x, residual = _matrices(x, residual, n, k)
     if _needs_grad(x, bias, residual):
-        raise RuntimeError("a prequantized MXFP8 weight is inference-only; keep the BF16 master weight to train")
+        raise RuntimeError(_FROZEN)
     data, scales = packed if isinstance(packed, tuple) else mxfp8_kernel_operands(packed)
     if eager(x, data, scales, bias, residual):
         y = ops.mxfp8_linear_epilogue_fwd_prequant_w(x, data, scales, n, bias, residual, activation=activation)
     else:
-        y = mxfp8_linear_epilogue_prequant_w(x, data, scales, bias, residual, n, k, activation)
+        y = call_without_derivative(mxfp8_linear_epilogue_prequant_w, _FROZEN, x, data, scales, bias, residual, n, k, activation)
     return y if len(shape) == 2 else y.reshape(shape)
 
 
@@ -221,8 +249,11 @@ def mxfp8_linear_epilogue_backward(grad_output: torch.Tensor, z: Optional[torch.
     if activation != "none" and z is None:
         raise ValueError("an activation's backward needs the pre-activation z")
     z2d = z.reshape(-1, n).contiguous() if z is not None and activation != "none" else grad_output.new_empty(0)
-    backward = mxfp8_linear_epilogue_bwd.fn if eager(x, grad_output, z2d, weight) else mxfp8_linear_epilogue_bwd
-    dx, dw, db = backward(grad_output.reshape(-1, n), z2d, x.reshape(-1, k), weight, activation, True, True, bias)
+    args = (grad_output.reshape(-1, n), z2d, x.reshape(-1, k), weight, activation, True, True, bias)
+    if eager(x, grad_output, z2d, weight):
+        dx, dw, db = mxfp8_linear_epilogue_bwd.fn(*args)
+    else:
+        dx, dw, db = call_without_derivative(mxfp8_linear_epilogue_bwd, _TWICE, *args)
     return dx.reshape(x.shape), dw, db if bias else None
 
 

@@ -21,9 +21,12 @@ from torch.autograd.function import once_differentiable
 
 from . import fp8 as _fp8
 from . import ops
-from ._oplib import custom_op, eager, refuse_tangents
+from ._oplib import call_without_derivative, custom_op, eager, refuse_tangents, transformed
 from .formats import (PACKED_OPERAND_SCHEMA_VERSION, SCALE_LAYOUT_CODES, MXFP8Tensor, make_mxfp8_tensor,
                       mxfp8_kernel_operands, mxfp8_qdata_2d, mxfp8_scales_for_kernel, reject_packed_dtype_conversion)
+
+
+_FROZEN = "a prequantized MXFP8 weight is inference-only; keep the BF16 master weight to train"
 
 
 def _check_grouped(x: torch.Tensor, weight: torch.Tensor) -> None:
@@ -112,6 +115,12 @@ def _(grad_output, x, weight, offsets):
     return weight.new_empty(weight.shape)
 
 
+_TWICE = "the backward of mxfp8_grouped_linear has no derivative of its own"
+mxfp8_grouped_linear_bwd.refuse_derivative(_TWICE)
+mxfp8_grouped_linear_dx.refuse_derivative(_TWICE)
+mxfp8_grouped_linear_dw.refuse_derivative(_TWICE)
+
+
 @custom_op("rtx::mxfp8_grouped_linear_train", mutates_args=(), device_types="cuda")
 def mxfp8_grouped_linear_train(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor) -> torch.Tensor:
     """Forward of the differentiable op; saves its inputs."""
@@ -129,15 +138,20 @@ def _train_setup(ctx, inputs, output):
 
 def _train_backward(ctx, grad_output):
     x, weight, offsets = ctx.saved_tensors
-    need_dx, need_dw = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
     if eager(grad_output, x, weight, offsets):
-        return (*_bwd(grad_output, x, weight, offsets, need_dx, need_dw), None)
+        return (*_bwd(grad_output, x, weight, offsets, *ctx.needs_input_grad[:2]), None)
+    return _dispatched_backward(ctx, grad_output)
+
+
+def _dispatched_backward(ctx, grad_output):
+    need_dx, need_dw = ctx.needs_input_grad[:2]
+    args = (_TWICE, grad_output, *ctx.saved_tensors)
     if need_dx and need_dw:
-        return (*mxfp8_grouped_linear_bwd(grad_output, x, weight, offsets), None)
+        return (*call_without_derivative(mxfp8_grouped_linear_bwd, *args), None)
     if need_dx:
-        return mxfp8_grouped_linear_dx(grad_output, x, weight, offsets), None, None
+        return call_without_derivative(mxfp8_grouped_linear_dx, *args), None, None
     if need_dw:
-        return None, mxfp8_grouped_linear_dw(grad_output, x, weight, offsets), None
+        return None, call_without_derivative(mxfp8_grouped_linear_dw, *args), None
     return None, None, None
 
 
@@ -154,6 +168,20 @@ class _GroupedLinearFunction(torch.autograd.Function):
         return mxfp8_grouped_linear_op.fn(x, weight, offsets)
 
     backward = staticmethod(once_differentiable(_train_backward))
+
+
+class _TransformedGroupedLinear(torch.autograd.Function):
+    """The same node in the form that `torch.func` transforms take (30 microseconds of host time more than the one above).
+    A pullback may be called after its transform has ended, with saved tensors that only the dispatcher can unwrap."""
+
+    generate_vmap_rule = True
+
+    @staticmethod
+    def forward(x, weight, offsets):
+        return mxfp8_grouped_linear_op(x, weight, offsets)
+
+    setup_context = staticmethod(_train_setup)
+    backward = staticmethod(_dispatched_backward)
 
 
 def _packed_group_shape(weight) -> Tuple[int, int, int]:
@@ -181,7 +209,7 @@ def mxfp8_grouped_linear(x: torch.Tensor, weight, offsets: torch.Tensor) -> torc
         if offsets.shape != (groups + 1,):
             raise ValueError(f"offsets must be a contiguous vector of groups + 1 = {groups + 1} row numbers")
         if x.requires_grad and torch.is_grad_enabled():
-            raise RuntimeError("a prequantized MXFP8 weight is inference-only; keep the BF16 master weight to train")
+            raise RuntimeError(_FROZEN)
         return _packed(x, *mxfp8_kernel_operands(weight), offsets, n)
     return _dynamic(x, weight, offsets)
 
@@ -190,12 +218,14 @@ def _packed(x, weight_data, weight_scales, offsets, n) -> torch.Tensor:
     refuse_tangents("mxfp8_grouped_linear", x)
     if eager(x, weight_data, weight_scales, offsets):
         return ops.mxfp8_grouped_linear_fwd_prequant_w(x, weight_data, weight_scales, offsets, n)
-    return mxfp8_grouped_linear_prequant_w(x, weight_data, weight_scales, offsets, n)
+    return call_without_derivative(mxfp8_grouped_linear_prequant_w, _FROZEN, x, weight_data, weight_scales, offsets, n)
 
 
 def _dynamic(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor) -> torch.Tensor:
     refuse_tangents("mxfp8_grouped_linear", x, weight)
     direct = eager(x, weight, offsets)
+    if not direct and transformed():
+        return _TransformedGroupedLinear.apply(x, weight, offsets)
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
         return (_GroupedLinearFunction.apply if direct else mxfp8_grouped_linear_train)(x, weight, offsets)
     return (mxfp8_grouped_linear_op.fn if direct else mxfp8_grouped_linear_op)(x, weight, offsets)
@@ -208,7 +238,7 @@ def mxfp8_grouped_linear_backward(grad_output: torch.Tensor, x: torch.Tensor, we
     refuse_tangents("mxfp8_grouped_linear_backward", grad_output, x, weight)
     if eager(x, grad_output, weight, offsets):
         return mxfp8_grouped_linear_bwd.fn(grad_output, x, weight, offsets)
-    return mxfp8_grouped_linear_bwd(grad_output, x, weight, offsets)
+    return call_without_derivative(mxfp8_grouped_linear_bwd, _TWICE, grad_output, x, weight, offsets)
 
 
 class MXFP8GroupedLinear(nn.Module):
@@ -272,7 +302,7 @@ class MXFP8GroupedLinear(nn.Module):
             raise ValueError(f"K mismatch: x has {x.shape[-1]}, weight has {self.in_features}")
         if self.weight_mode == "prequantized":
             if x.requires_grad and torch.is_grad_enabled():
-                raise RuntimeError("a prequantized MXFP8 weight is inference-only; keep the BF16 master weight to train")
+                raise RuntimeError(_FROZEN)
             return _packed(x, self.weight_data, self.weight_scales, offsets, self.out_features)
         return _dynamic(x, self.weight, offsets)
 

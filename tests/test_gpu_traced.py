@@ -45,7 +45,8 @@ def calls(dev):
         "epilogue packed": (lambda x, b: r.mxfp8_linear_epilogue(x, wp, b, activation="silu"),
                             *two(lambda i: (*x2(i), normal(72))), "mxfp8_linear_epilogue_prequant_w"),
         "epilogue backward": (lambda dy, z, x, w: r.mxfp8_linear_epilogue_backward(dy, z, x, w, activation="gelu_tanh"),
-                              *two(lambda i: (normal(70, 72), normal(70, 72), *x2(i), normal(72, 96))), "mxfp8_linear_epilogue_bwd"),
+                              *two(lambda i: (normal(70, 72), normal(70, 72), *x2(i), normal(72, 96))),
+                              "mxfp8_linear_epilogue_bwd"),
     }
 
 
@@ -132,3 +133,75 @@ def test_vmap_over_trainable_weights(dev, name):
     same(y, want)
     dy = torch.randn_like(want)
     same(torch.autograd.grad(y, [x, *leaves], dy, retain_graph=True), torch.autograd.grad(want, [x, *leaves], dy))
+
+
+@pytest.mark.parametrize("name", ["grouped", "epilogue"])
+def test_func_transforms(dev, name):
+    """grad, vjp and jacrev, alone and around or inside vmap, give autograd's gradients."""
+    f, first, other, _ = calls(dev)[name]
+    rest = first[1:]
+    leaves = [t.requires_grad_(True) for t in first if t.is_floating_point()]
+    numbers = tuple(i for i, t in enumerate(first) if t.is_floating_point())
+    dy = torch.randn_like(f(*first))
+    want = torch.autograd.grad(f(*first), leaves, dy)
+    loss = lambda *args: (f(*args) * dy).sum()
+    same(torch.func.grad(loss, argnums=numbers)(*first), want)
+    same(torch.func.grad(loss, argnums=numbers)(*(t.detach() for t in first)), want)
+    y, pull = torch.func.vjp(lambda *args: f(*args, *first[len(numbers):]), *leaves)
+    same(y, f(*first))
+    same(pull(dy), want)
+    xs = torch.stack([first[0], other[0]]).detach()
+    each = [torch.autograd.grad(loss(x, *rest), leaves[1:]) for x in xs]
+    over = (0, *[None] * len(rest))
+    got = torch.func.vmap(torch.func.grad(loss, argnums=numbers[1:]), over)(xs, *rest)   # a gradient per sample
+    same(got, [torch.stack(g) for g in zip(*each)])
+    around = torch.func.grad(lambda *args: (torch.func.vmap(f, over)(xs, *args) * dy).sum(), argnums=tuple(range(len(leaves) - 1)))
+    same(around(*rest), [a + b for a, b in zip(*each)])
+    some = torch.func.jacrev(lambda x: f(x, *rest)[4, :3])(first[0])
+    for i in range(3):
+        pick = torch.zeros_like(dy)
+        pick[4, i] = 1
+        same(some[i], torch.autograd.grad(f(*first), first[0], pick)[0])
+    assert torch.equal(torch.func.functionalize(f)(*(t.detach() for t in first)), y)
+    scaled = torch.func.jvp(lambda s: f(*first) * s, (torch.ones((), device=dev),), (torch.ones((), device=dev),))
+    assert torch.equal(scaled[1].bfloat16(), y)                 # constants of a forward-mode call
+
+
+@pytest.mark.parametrize("name", ["grouped", "epilogue"])
+def test_no_form_drops_a_second_derivative(dev, name):
+    """Each path refuses it; none gives zeros."""
+    f, first, _, _ = calls(dev)[name]
+    x, *rest = first
+    x.requires_grad_(True)
+    loss = lambda x: f(x, *rest).square().sum()
+
+    class Pass(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    with Pass():                                                # the registered op
+        g = torch.autograd.grad(loss(x), x, create_graph=True)[0]
+        with pytest.raises(NotImplementedError, match="no derivative of its own"):
+            g.sum().backward()
+    with pytest.raises(NotImplementedError, match="no derivative of its own"):
+        torch.func.grad(lambda x: torch.func.grad(loss)(x).sum())(x)
+    g = torch.autograd.grad(loss(x), x, create_graph=True)[0]
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        g.sum().backward()
+
+
+@pytest.mark.parametrize("name", ["grouped packed", "grouped backward", "epilogue packed", "epilogue backward"])
+def test_transforms_of_what_has_no_derivative_are_refused(dev, name):
+    f, first, _, _ = calls(dev)[name]
+
+    def total(*args):
+        out = f(*args)
+        return sum(t.float().sum() for t in (out if isinstance(out, tuple) else (out,)))
+
+    with pytest.raises(RuntimeError, match="inference-only|no derivative of its own"):
+        torch.func.grad(total)(*first)
+    over = (None,) * (len(first) - 1)
+    with pytest.raises(RuntimeError, match="inference-only|no derivative of its own"):   # the batched operand hides the tracked one
+        torch.func.grad(lambda t: torch.func.vmap(total, (0, *over))(torch.stack([t, t]), *first[1:]).sum())(first[0])
+    batch = torch.func.vmap(f, (0, *over))(torch.stack([first[0]] * 2), *first[1:])
+    same([b[1] for b in batch] if isinstance(batch, tuple) else batch[1], f(*first))
