@@ -1,11 +1,9 @@
 // Activations of the linear with an epilogue, and their derivatives, in FP32.  Codes as RTXB_ACT_*.
 //
-// The epilogue evaluates one activation per output element beside the MMAs of the next tile, the backward quantizer one
-// slope per gradient element at memory speed, so an evaluation may cost two special-function operations and some twenty
-// multiply-adds; the library's erff / tanhf / expf cost two to four times that.  Measured, gelu, 8192 x 8192: slope pass
-// 210 us with erff and expf, 178 with the forms below a value at a time, 148 with them on packed pairs (and 110 with its
-// table, quant_act.cuh); GEMM of 8192 x 4096 x 8192 with residual and z 265 us a value at a time, 217 on pairs.  Forms
-// without cancellation:
+// The epilogue evaluates one activation per output element beside the MMAs of the next tile, so an evaluation may cost two
+// special-function operations and some twenty multiply-adds; the library's erff / tanhf / expf cost two to four times that.
+// Measured, gelu: GEMM of 8192 x 4096 x 8192 with residual and z 265 us a value at a time, 217 on pairs.  Forms without
+// cancellation:
 //   silu       z s(z), s(z) = 1 / (1 + e^-z)
 //   gelu_tanh  z s(2 a (z + b z^3)), since (1 + tanh u) / 2 = s(2 u)
 //   gelu       z Phi(z), Phi(-|z|) = erfc(|z| / sqrt 2) / 2 with erfc(x) = e^(-x^2) (c1 t + .. + c5 t^5), t = 1 / (1 + p x)
@@ -22,7 +20,6 @@ namespace rtxb {
 enum Activation : int { kActNone = 0, kActRelu = 1, kActRelu2 = 2, kActSilu = 3, kActGelu = 4, kActGeluTanh = 5 };
 
 constexpr float kSqrtHalf = 0.70710678118654752f;
-constexpr float kInvSqrt2Pi = 0.39894228040143268f;
 constexpr float kGeluTanhA = 0.79788456080286536f;   // sqrt(2 / pi)
 constexpr float kGeluTanhB = 0.044715f;
 
@@ -48,10 +45,10 @@ __device__ __forceinline__ f32x2 gelu_tanh_gate2(f32x2 z, f32x2 zz) {
   constexpr float k = -2.0f * kGeluTanhA * kLog2E;
   return rcp2(add2(exp2_2(mul2(z, fma2(zz, both(k * kGeluTanhB), both(k)))), both(1.0f)));
 }
-// -Phi(-a) for a >= 0; `e` receives e^(-a^2 / 2).  The 1/2 and the sign are in the coefficients.
-__device__ __forceinline__ f32x2 minus_tail2(f32x2 a, f32x2& e) {
+// -Phi(-a) for a >= 0.  The 1/2 and the sign are in the coefficients.
+__device__ __forceinline__ f32x2 minus_tail2(f32x2 a) {
   const f32x2 t = rcp2(fma2(a, both(0.3275911f * kSqrtHalf), both(1.0f)));
-  e = exp2_2(mul2(mul2(a, a), both(-0.5f * kLog2E)));
+  const f32x2 e = exp2_2(mul2(mul2(a, a), both(-0.5f * kLog2E)));
   f32x2 c = fma2(t, both(-0.5f * 1.061405429f), both(0.5f * 1.453152027f));
   c = fma2(c, t, both(-0.5f * 1.421413741f));
   c = fma2(c, t, both(0.5f * 0.284496736f));
@@ -74,9 +71,8 @@ __device__ __forceinline__ void act_value2(float& x, float& y) {
   f32x2 r;
   if (ACT == kActGelu) {
     // z Phi(z) = max(z, 0) - |z| Phi(-|z|)
-    f32x2 e;
     const f32x2 a = pack2(abs_upto_128(x), abs_upto_128(y));
-    r = fma2(a, minus_tail2(a, e), pack2(fmax_nan(x, 0.0f), fmax_nan(y, 0.0f)));
+    r = fma2(a, minus_tail2(a), pack2(fmax_nan(x, 0.0f), fmax_nan(y, 0.0f)));
   } else {
     const f32x2 z = pack2(fmax_nan(x, -128.0f), fmax_nan(y, -128.0f));
     r = mul2(z, ACT == kActSilu ? sigmoid2(z) : gelu_tanh_gate2(z, mul2(z, z)));
@@ -85,39 +81,47 @@ __device__ __forceinline__ void act_value2(float& x, float& y) {
   y = hi(r);
 }
 
-// g * act'(z) for a pair; relu has slope 0 at 0
+// g * act'(z) of relu and relu2 for a pair; relu has slope 0 at 0
 template <int ACT>
-__device__ __forceinline__ void act_slope2(float& gx, float& gy, float x, float y) {
-  if (ACT == kActRelu || ACT == kActRelu2) {
-    const float k = ACT == kActRelu ? 1.0f : 2.0f;
-    gx *= x > 0.0f ? (ACT == kActRelu ? k : k * x) : (x == x ? 0.0f : x);
-    gy *= y > 0.0f ? (ACT == kActRelu ? k : k * y) : (y == y ? 0.0f : y);
-    return;
+__device__ __forceinline__ void relu_slope2(float& gx, float& gy, float x, float y) {
+  static_assert(ACT == kActRelu || ACT == kActRelu2, "the others are looked up");
+  const float k = ACT == kActRelu ? 1.0f : 2.0f;
+  gx *= x > 0.0f ? (ACT == kActRelu ? k : k * x) : (x == x ? 0.0f : x);
+  gy *= y > 0.0f ? (ACT == kActRelu ? k : k * y) : (y == y ? 0.0f : y);
+}
+
+// act'(-a), 0 <= a <= 128, of silu and the two gelus: the entries of the backward's table, a few thousand per block, so they
+// are made to FP32 accuracy (a few 2^-24 of the slope, also beside its zero).  A slope that is off by 3 2^-24 of 1/2 moves
+// dz across a BF16 rounding, and now and then an E4M3 code behind it, for every gradient of an unlucky z: in the training
+// step of 8192 x 4096 x 8192 that was 2.1e-4 of dx (2-norm), where the MMAs' accumulation is 1.2e-4 and these entries are 0.
+//   silu, gelu_tanh  with s(-u) = q / (1 + q), q = e^-u:   q (1 - a u'(a) + q) / (1 + q)^2;  u = a,  or 2 A (a + B a^3)
+//   gelu             Phi(-a) - a phi(a) = e^(-a^2 / 2) (a0 - a) h(a): a0 its zero, in two parts, h a polynomial in
+//                    1 / (1 + 0.32 a), a minimax fit in relative error on 0 <= a <= 14 made for this file (4.6e-8)
+// The exponents are formed in FP64 and their rounding to FP32 is put back into the power.
+__device__ __forceinline__ float exp2_of(double x) {   // x <= 0
+  const float head = static_cast<float>(x);
+  float p;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p) : "f"(head));
+  return fmaf(p, static_cast<float>(x - head) * 0.693147181f, p);
+}
+__device__ __forceinline__ float slope_at_minus(int act, float a) {
+  constexpr double kLog2 = 1.4426950408889634, kA = 0.79788456080286536, kB = 0.044715;
+  const double d = a;
+  if (act == kActGelu) {
+    const float t = 1.0f / fmaf(a, 0.32f, 1.0f);
+    float h = fmaf(t, 0.0130718084f, -0.0584661273f);
+    h = fmaf(h, t, 0.0741537535f);
+    h = fmaf(h, t, -0.00356778049f);
+    h = fmaf(h, t, 0.0692133608f);
+    h = fmaf(h, t, 0.075452407f);
+    h = fmaf(h, t, 0.0962936944f);
+    h = fmaf(h, t, 0.398926866f);
+    return exp2_of(-0.5 * kLog2 * d * d) * ((0.751791537f - a) - 1.21144495e-08f) * h;
   }
-  const f32x2 one = both(1.0f);
-  const f32x2 z = pack2(fmin_nan(fmax_nan(x, -128.0f), 128.0f), fmin_nan(fmax_nan(y, -128.0f), 128.0f));
-  f32x2 d;
-  if (ACT == kActSilu) {
-    // s (1 + z (1 - s))
-    const f32x2 s = sigmoid2(z);
-    d = mul2(s, fma2(z, fma2(s, both(-1.0f), one), one));
-  } else if (ACT == kActGelu) {
-    // Phi(z) + z phi(z)
-    f32x2 e;
-    const f32x2 m = minus_tail2(pack2(fabsf(lo(z)), fabsf(hi(z))), e);
-    const f32x2 up = add2(m, one);
-    const f32x2 cdf = pack2(x < 0.0f ? -lo(m) : lo(up), y < 0.0f ? -hi(m) : hi(up));
-    d = fma2(mul2(z, both(kInvSqrt2Pi)), e, cdf);
-  } else {
-    // s + z s (1 - s) 2 a (1 + 3 b z^2)
-    const f32x2 zz = mul2(z, z);
-    const f32x2 s = gelu_tanh_gate2(z, zz);
-    const f32x2 w = mul2(mul2(z, s), fma2(zz, both(6.0f * kGeluTanhA * kGeluTanhB), both(2.0f * kGeluTanhA)));
-    d = fma2(w, fma2(s, both(-1.0f), one), s);
-  }
-  d = mul2(pack2(gx, gy), d);
-  gx = lo(d);
-  gy = hi(d);
+  const bool silu = act == kActSilu;
+  const double u = silu ? d : 2.0 * kA * d * (1.0 + kB * d * d), slope = silu ? 1.0 : 2.0 * kA * (1.0 + 3.0 * kB * d * d);
+  const float q = exp2_of(-kLog2 * u), r = 1.0f / (1.0f + q);
+  return q * (static_cast<float>(1.0 - d * slope) + q) * r * r;
 }
 
 template <int ACT>

@@ -67,8 +67,8 @@ __device__ __forceinline__ void act_gradient8(const float* table, int act, const
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       float a = lo(v[e]), b = hi(v[e]);
-      if (act == kActRelu) act_slope2<kActRelu>(a, b, bf16_lo(w[e]), bf16_hi(w[e]));
-      else act_slope2<kActRelu2>(a, b, bf16_lo(w[e]), bf16_hi(w[e]));
+      if (act == kActRelu) relu_slope2<kActRelu>(a, b, bf16_lo(w[e]), bf16_hi(w[e]));
+      else relu_slope2<kActRelu2>(a, b, bf16_lo(w[e]), bf16_hi(w[e]));
       v[e] = pack2(a, b);
     }
   }
@@ -84,14 +84,8 @@ __global__ void __launch_bounds__(kQuantThreads, kActOccupancy) quant_mxfp8_act_
   __shared__ float sums[kActSumRows][128];
   griddep_launch_dependents();
   if (LOOKUP) {
-    with_activation(p.act, [&](auto tag) {
-      for (int i = kSlopeLow + threadIdx.x; i <= kSlopeHigh; i += kQuantThreads) {
-        const float z = __uint_as_float(static_cast<uint32_t>(i) << 16);
-        float a = 1.0f, b = 0.0f;
-        act_slope2<decltype(tag)::value>(a, b, -z, 0.0f);
-        slopes[i] = a;
-      }
-    });
+    for (int i = kSlopeLow + threadIdx.x; i <= kSlopeHigh; i += kQuantThreads)
+      slopes[i] = slope_at_minus(p.act, __uint_as_float(static_cast<uint32_t>(i) << 16));
     __syncthreads();
   }
   const int col_tiles = (p.n + 127) / 128, row_tiles = (p.m + 127) / 128;
