@@ -2,15 +2,16 @@
 //
 // The epilogue evaluates one activation per output element beside the MMAs of the next tile, so an evaluation may cost two
 // special-function operations and some twenty multiply-adds; the library's erff / tanhf / expf cost two to four times that.
-// Measured, gelu: GEMM of 8192 x 4096 x 8192 with residual and z 265 us a value at a time, 217 on pairs.  Forms without
-// cancellation:
+// Forms without cancellation:
 //   silu       z s(z), s(z) = 1 / (1 + e^-z)
 //   gelu_tanh  z s(2 a (z + b z^3)), since (1 + tanh u) / 2 = s(2 u)
-//   gelu       z Phi(z), Phi(-|z|) = erfc(|z| / sqrt 2) / 2 with erfc(x) = e^(-x^2) (c1 t + .. + c5 t^5), t = 1 / (1 + p x)
-//              (Hastings' approximation, formula 7.1.26 of Abramowitz and Stegun, error below 1.5e-7), and
-//              Phi(|z|) = 1 - Phi(-|z|)
-// with the hardware exponential and reciprocal (relative errors of a few 2^-23 where the result is not negligible).
-// The BF16 result's half step is 2^-8.
+//   gelu       z Phi(z) = max(z, 0) - |z| Phi(-|z|), Phi(-a) = e^(-a^2 / 2) (c1 t + .. + c7 t^7), t = 1 / (1 + p a)
+// The polynomial is a minimax fit to Phi(-a) e^(a^2 / 2) on 0 <= a <= 14 in RELATIVE error, made for this file (8.1e-7 with
+// the coefficients rounded to FP32), so that the far tail keeps as many digits as the rest: a fit with an absolute bound of
+// 1e-7 is off by 1 % of gelu at z = -8.  Exponential and reciprocal are the hardware's (errors of a few 2^-23).  The
+// exponent's roundings are 2^-24 of it each, so the relative error grows to 2^-16 where the power leaves the normal range,
+// against the 2^-8 of the BF16 result's half step.  Results below 2^-119 in magnitude may come out as zero: s(z) or the
+// power is then below 2^-126, and |z| below 88 (silu), 11 (gelu_tanh) or 14 (gelu).
 #pragma once
 
 #include "common.cuh"
@@ -19,7 +20,6 @@ namespace rtxb {
 
 enum Activation : int { kActNone = 0, kActRelu = 1, kActRelu2 = 2, kActSilu = 3, kActGelu = 4, kActGeluTanh = 5 };
 
-constexpr float kSqrtHalf = 0.70710678118654752f;
 constexpr float kGeluTanhA = 0.79788456080286536f;   // sqrt(2 / pi)
 constexpr float kGeluTanhB = 0.044715f;
 
@@ -45,14 +45,16 @@ __device__ __forceinline__ f32x2 gelu_tanh_gate2(f32x2 z, f32x2 zz) {
   constexpr float k = -2.0f * kGeluTanhA * kLog2E;
   return rcp2(add2(exp2_2(mul2(z, fma2(zz, both(k * kGeluTanhB), both(k)))), both(1.0f)));
 }
-// -Phi(-a) for a >= 0.  The 1/2 and the sign are in the coefficients.
+// -Phi(-a) for a >= 0.  The sign is in the coefficients.
 __device__ __forceinline__ f32x2 minus_tail2(f32x2 a) {
-  const f32x2 t = rcp2(fma2(a, both(0.3275911f * kSqrtHalf), both(1.0f)));
+  const f32x2 t = rcp2(fma2(a, both(0.362f), both(1.0f)));
   const f32x2 e = exp2_2(mul2(mul2(a, a), both(-0.5f * kLog2E)));
-  f32x2 c = fma2(t, both(-0.5f * 1.061405429f), both(0.5f * 1.453152027f));
-  c = fma2(c, t, both(-0.5f * 1.421413741f));
-  c = fma2(c, t, both(0.5f * 0.284496736f));
-  c = fma2(c, t, both(-0.5f * 0.254829592f));
+  f32x2 c = fma2(t, both(-0.0479379926f), both(0.180008766f));
+  c = fma2(c, t, both(-0.176616161f));
+  c = fma2(c, t, both(-0.0288321568f));
+  c = fma2(c, t, both(-0.139429476f));
+  c = fma2(c, t, both(-0.142689345f));
+  c = fma2(c, t, both(-0.144503904f));
   return mul2(c, mul2(t, e));
 }
 __device__ __forceinline__ float abs_upto_128(float z) { return fmin_nan(fabsf(z), 128.0f); }
@@ -70,7 +72,6 @@ __device__ __forceinline__ void act_value2(float& x, float& y) {
   }
   f32x2 r;
   if (ACT == kActGelu) {
-    // z Phi(z) = max(z, 0) - |z| Phi(-|z|)
     const f32x2 a = pack2(abs_upto_128(x), abs_upto_128(y));
     r = fma2(a, minus_tail2(a), pack2(fmax_nan(x, 0.0f), fmax_nan(y, 0.0f)));
   } else {
@@ -96,7 +97,7 @@ __device__ __forceinline__ void relu_slope2(float& gx, float& gy, float x, float
 // step of 8192 x 4096 x 8192 that was 2.1e-4 of dx (2-norm), where the MMAs' accumulation is 1.2e-4 and these entries are 0.
 //   silu, gelu_tanh  with s(-u) = q / (1 + q), q = e^-u:   q (1 - a u'(a) + q) / (1 + q)^2;  u = a,  or 2 A (a + B a^3)
 //   gelu             Phi(-a) - a phi(a) = e^(-a^2 / 2) (a0 - a) h(a): a0 its zero, in two parts, h a polynomial in
-//                    1 / (1 + 0.32 a), a minimax fit in relative error on 0 <= a <= 14 made for this file (4.6e-8)
+//                    1 / (1 + 0.32 a) fitted as above on 0 <= a <= 14 (4.6e-8)
 // The exponents are formed in FP64 and their rounding to FP32 is put back into the power.
 __device__ __forceinline__ float exp2_of(double x) {   // x <= 0
   const float head = static_cast<float>(x);

@@ -1,6 +1,11 @@
-"""Slopes of the activations of the linear with an epilogue, for every BF16 pre-activation between 2^-20 and 128 in magnitude.
+"""Activations and slopes of the linear with an epilogue, for every BF16 pre-activation between 2^-20 and 128 in magnitude.
 
-Tolerances, derived before the first run (u = 2^-24, half an FP32 step; the hardware's 2^x is within 2^-22 of the value):
+Tolerances, derived before the first run (u = 2^-24, half an FP32 step; the hardware's 2^x is within 2^-22 of the value,
+its reciprocal within 2^-23):
+  value  The exponent of e^(..) has at most three roundings of magnitude up to 126 (below, the power has left the normal
+         range): 126 ln 2 * 3 u = 2^-16 of the result; the power, the reciprocal, the fit of gelu's tail (8.1e-7) and a dozen
+         roundings less than 2^-18 together.  2^-15 in all, beside the BF16 rounding (2^-8).  No form cancels.  Below 2^-119
+         a result may be zero: it is |z| times a power or reciprocal below 2^-126, and |z| < 88 < 2^7 there.
   slope  At z = -a.  gelu: the power 4 u and u for the exponent's put-back rounding, the fit 4.6e-8 < u, its evaluation
          2 u (the leading term is two thirds or more of the sum), 1 / (1 + 0.32 a) u, a0 - a 2 u, two products 2 u: 12 u of
          the slope with everything.  silu and gelu_tanh: q (g + q) / (1 + q)^2: q 5 u, which the sum g + q passes on in
@@ -36,6 +41,25 @@ def value64(z, act):
     if act == "gelu":
         return 0.5 * z * torch.erfc(-z / math.sqrt(2))
     return z * torch.sigmoid(2 * math.sqrt(2 / math.pi) * (z + 0.044715 * z ** 3))
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh"])
+@pytest.mark.parametrize("m", [3, 150])
+def test_values_keep_their_relative_accuracy(dev, act, m):
+    """Zero weights: z is the bias."""
+    import rtx_b200
+
+    z = every_z()
+    x, w = torch.zeros(m, 32).bfloat16().to(dev), torch.zeros(z.numel(), 32).bfloat16().to(dev)
+    y = rtx_b200.mxfp8_linear_epilogue(x, w, z.to(dev), activation=act).cpu()
+    assert torch.equal(y, y[:1].expand_as(y))
+    want = value64(z.double(), act)
+    off = (y[0].double() - want).abs()
+    live = want.abs() >= 2.0 ** -119
+    rel = off[live] / want[live].abs()
+    worst = rel.argmax()
+    assert (rel <= 2.0 ** -8 + 2.0 ** -15).all(), (z[live][worst].item(), rel[worst].item() * 2 ** 8)
+    assert (off[~live] <= 2.0 ** -119).all()
 
 
 @pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh"])
