@@ -12,10 +12,12 @@ rejected.
 from __future__ import annotations
 
 from math import ceil
+from typing import Optional
 
 import torch
 
-from .common import (ScaleLayout, flattened_matrix_shape, scales_mma128_to_row_major, scales_row_major_to_mma128)
+from .common import (PACKED_OPERAND_SCHEMA_VERSION, SCALE_LAYOUT_CODES, SCALE_LAYOUT_NAMES, ScaleLayout,
+                     flattened_matrix_shape, scales_mma128_to_row_major, scales_row_major_to_mma128)
 
 try:  # pragma: no cover - depends on the environment
     from torchao.prototype.mx_formats.mx_tensor import MXTensor as _AOMXTensor
@@ -156,6 +158,35 @@ def mxfp8_kernel_operands(value) -> tuple[torch.Tensor, torch.Tensor]:
     if getattr(value, "_rtx_scale_layout", None) != "mma128":
         s = mxfp8_scales_for_kernel(value)
     return q.contiguous(), s.contiguous()
+
+
+def mxfp8_state_for_kernel(state_dict: dict, prefix: str, rows: int, k: int) -> Optional[str]:
+    """Bring the packed weight of a module's state (`weight_data`, `weight_scales`, `weight_packing_meta`) to what the
+    kernels take: row-major scales become mma128 tiles, in place in `state_dict`.  Returns what keeps it from being loaded
+    as a [rows, k] weight, or None.  Both layouts often have the same size, so only the meta tells them apart."""
+    meta = state_dict.get(prefix + "weight_packing_meta")
+    if meta is None:
+        return None
+    storage_k = (k + 31) // 32 * 32
+    found = [int(v) for v in meta.reshape(-1)]
+    if len(found) != 4 or found[0] != PACKED_OPERAND_SCHEMA_VERSION:
+        return f"{prefix}weight_packing_meta {found} is not of packing schema {PACKED_OPERAND_SCHEMA_VERSION}"
+    if found[2:] != [k, storage_k]:
+        return f"{prefix}weight_data has K = {found[2]} in rows of {found[3]}, the module K = {k} in rows of {storage_k}"
+    layout = SCALE_LAYOUT_NAMES.get(found[1])
+    if layout == "row_major":
+        blocks = storage_k // 32
+        scales = state_dict.get(prefix + "weight_scales")
+        if scales is not None:
+            if scales.numel() != rows * blocks:
+                return f"{prefix}weight_scales has {scales.numel()} values, expected {rows * blocks} (row_major)"
+            state_dict[prefix + "weight_scales"] = scales_row_major_to_mma128(scales, rows, blocks, ceil(blocks / 4))
+        meta = meta.clone()
+        meta.reshape(-1)[1] = SCALE_LAYOUT_CODES["mma128"]
+        state_dict[prefix + "weight_packing_meta"] = meta
+    elif layout != "mma128":
+        return f"{prefix}weight_scales are in layout {layout or found[1]}, which the sm_100a kernels do not read; requantize"
+    return None
 
 
 def convert_mxfp8_scale_layout(value, scale_layout: ScaleLayout):

@@ -23,7 +23,8 @@ from . import fp8 as _fp8
 from . import ops
 from ._oplib import call_without_derivative, custom_op, eager, refuse_tangents, transformed
 from .formats import (PACKED_OPERAND_SCHEMA_VERSION, SCALE_LAYOUT_CODES, MXFP8Tensor, make_mxfp8_tensor,
-                      mxfp8_kernel_operands, mxfp8_qdata_2d, mxfp8_scales_for_kernel, reject_packed_dtype_conversion)
+                      mxfp8_kernel_operands, mxfp8_qdata_2d, mxfp8_scales_for_kernel, mxfp8_state_for_kernel,
+                      reject_packed_dtype_conversion)
 
 
 _FROZEN = "a prequantized MXFP8 weight is inference-only; keep the BF16 master weight to train"
@@ -287,6 +288,14 @@ class MXFP8GroupedLinear(nn.Module):
             raise RuntimeError("module holds a BF16 weight; call to_quantized_weight() first")
         return make_mxfp8_tensor(self.weight_data, self.weight_scales,
                                  (self.num_groups, self.out_features, self.in_features), "mma128")
+
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs):
+        if self.weight_mode == "prequantized":
+            problem = mxfp8_state_for_kernel(state_dict, prefix, self.num_groups * self.out_features, self.in_features)
+            if problem is not None:
+                error_msgs.append(problem)
+                return
+        super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs)
 
     def to(self, *args, **kwargs):
         if self.weight_mode == "prequantized":
