@@ -26,14 +26,15 @@ def interposed() -> bool:
             or torch._C._len_torch_dispatch_stack() > 0 or torch._C._is_tracing())
 
 
-def eager(t: torch.Tensor, *others: Optional[torch.Tensor]) -> bool:
+def eager(t: torch.Tensor, *others) -> bool:
     """Whether an op on these operands would only be dispatched back into this package's CUDA implementation (plain CUDA
     tensors, nothing interposed): the package's own functions then call the launcher itself and save a dispatch of a few
-    microseconds."""
+    microseconds.  What is no tensor is the launcher's to refuse."""
     if not t.is_cuda or interposed():
         return False
     for operand in (t, *others):
-        if operand is not None and type(operand) is not torch.Tensor and type(operand) is not torch.nn.Parameter:
+        kind = type(operand)
+        if kind is not torch.Tensor and kind is not torch.nn.Parameter and isinstance(operand, torch.Tensor):
             return False
     return True
 

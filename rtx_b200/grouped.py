@@ -207,7 +207,7 @@ def mxfp8_grouped_linear(x: torch.Tensor, weight, offsets: torch.Tensor) -> torc
         groups, n, k = _packed_group_shape(weight)
         if x.ndim != 2 or x.shape[1] != k:
             raise ValueError(f"K mismatch: x has {x.shape[-1]}, weight has {k}")
-        if offsets.shape != (groups + 1,):
+        if isinstance(offsets, torch.Tensor) and offsets.shape != (groups + 1,):
             raise ValueError(f"offsets must be a contiguous vector of groups + 1 = {groups + 1} row numbers")
         if x.requires_grad and torch.is_grad_enabled():
             raise RuntimeError(_FROZEN)

@@ -205,3 +205,12 @@ def test_transforms_of_what_has_no_derivative_are_refused(dev, name):
         torch.func.grad(lambda t: torch.func.vmap(total, (0, *over))(torch.stack([t, t]), *first[1:]).sum())(first[0])
     batch = torch.func.vmap(f, (0, *over))(torch.stack([first[0]] * 2), *first[1:])
     same([b[1] for b in batch] if isinstance(batch, tuple) else batch[1], f(*first))
+
+
+def test_offsets_that_are_no_tensor_are_named(dev):
+    import rtx_b200 as r
+
+    x, w = torch.zeros(8, 64, device=dev).bfloat16(), torch.zeros(2, 128, 64, device=dev).bfloat16()
+    for weight in (w, r.quantize_mxfp8(w)):
+        with pytest.raises(TypeError, match="offsets must be a torch.Tensor"):
+            r.mxfp8_grouped_linear(x, weight, [0, 4, 8])
