@@ -250,6 +250,9 @@ def mxfp8_linear_epilogue_backward(grad_output: torch.Tensor, z: Optional[torch.
     n, k = weight.shape
     if activation != "none" and z is None:
         raise ValueError("an activation's backward needs the pre-activation z")
+    for name, t, width in (("grad_output", grad_output, n), ("x", x, k), ("z", z if activation != "none" else None, n)):
+        if t is not None and (t.ndim < 1 or t.shape[-1] != width):
+            raise ValueError(f"{name} must have rows of {width} values, got shape {tuple(t.shape)}")
     z2d = z.reshape(-1, n).contiguous() if z is not None and activation != "none" else grad_output.new_empty(0)
     args = (grad_output.reshape(-1, n), z2d, x.reshape(-1, k), weight, activation, True, True, bias)
     if eager(x, grad_output, z2d, weight):

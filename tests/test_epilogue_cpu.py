@@ -105,3 +105,21 @@ def test_shapes_under_fake_tensors():
         assert tuple(y.shape) == (2, 4, 96) and y.dtype is torch.bfloat16 and y.requires_grad
         dx, dw, db = epilogue.mxfp8_linear_epilogue_backward(y.detach(), y.detach(), x.detach(), w, activation="silu")
         assert dx.shape == x.shape and dw.shape == w.shape and db.shape == b.shape
+
+
+def test_backward_takes_no_operand_by_its_number_of_values():
+    """Rows of another width whose values happen to fill whole rows of the right one are refused, not reshaped."""
+    from rtx_b200.epilogue import mxfp8_linear_epilogue_backward
+
+    def zeros(*shape):
+        return torch.zeros(*shape, dtype=torch.bfloat16)
+
+    w = zeros(16, 32)
+    for dy, z, x, name in ((zeros(4, 32), zeros(8, 16), zeros(8, 32), "grad_output"), (zeros(8, 16), zeros(8, 16), zeros(4, 64), "x"),
+                           (zeros(8, 16), zeros(16, 8), zeros(8, 32), "z"), (zeros(8, 16), zeros(8, 16), zeros(()), "x")):
+        with pytest.raises(ValueError, match=f"{name} must have rows of"):
+            mxfp8_linear_epilogue_backward(dy, z, x, w, activation="silu")
+    with pytest.raises(NotImplementedError):                    # the right widths reach the op (which needs a GPU)
+        mxfp8_linear_epilogue_backward(zeros(2, 4, 16), zeros(8, 16), zeros(8, 32), w, activation="silu")
+    with pytest.raises(NotImplementedError):                    # z is not looked at without an activation
+        mxfp8_linear_epilogue_backward(zeros(8, 16), zeros(3), zeros(8, 32), w)
