@@ -8,6 +8,7 @@ librtxb.  PyTorch is used only for device memory and the stream handle.
 
 from __future__ import annotations
 
+import ctypes
 import functools
 import threading
 from typing import Optional, Tuple
@@ -45,6 +46,35 @@ def _on(device: torch.device):
     return torch.cuda.device(idx)
 
 
+class _RelaxedCapture:
+    """While a stream is being captured, allocations and synchronisation of other streams are allowed in here."""
+
+    def __init__(self):
+        self.cuda = ctypes.CDLL("libcuda.so.1")
+
+    def __enter__(self):
+        self.mode = ctypes.c_int(2)                          # CU_STREAM_CAPTURE_MODE_RELAXED, of this thread
+        if self.cuda.cuThreadExchangeStreamCaptureMode(ctypes.byref(self.mode)):
+            raise RuntimeError("cuThreadExchangeStreamCaptureMode failed")
+
+    def __exit__(self, *exc):
+        self.cuda.cuThreadExchangeStreamCaptureMode(ctypes.byref(self.mode))
+        return False
+
+
+def _new_status_word(device: torch.device) -> torch.Tensor:
+    if not torch.cuda.is_current_stream_capturing():
+        return torch.zeros(1, dtype=torch.int32, device=device)
+    # A first call inside a capture: allocated and cleared on the captured stream, the word would be the graph's, unset until
+    # the first replay and cleared again, with what was reported since, by every later one.
+    with _RelaxedCapture():
+        side = torch.cuda.Stream(device)
+        with torch.cuda.stream(side):
+            word = torch.zeros(1, dtype=torch.int32, device=device)
+        side.synchronize()
+    return word
+
+
 def status_word(device: torch.device) -> torch.Tensor:
     """Per-device int32 the kernels set when a bounded wait runs out."""
     idx = device.index if device.index is not None else torch.cuda.current_device()
@@ -53,7 +83,9 @@ def status_word(device: torch.device) -> torch.Tensor:
         with _status_lock:
             word = _status_words.get(idx)
             if word is None:
-                word = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", idx))
+                device = torch.device("cuda", idx)
+                with _on(device):
+                    word = _new_status_word(device)
                 _status_words[idx] = word
     return word
 
