@@ -18,23 +18,31 @@ from torch.autograd import forward_ad
 _LIB = torch.library.Library("rtx", "FRAGMENT")
 
 
+# bound once: these stand on the launch path of calls that take 15 microseconds in all
+_is_compiling = torch.compiler.is_compiling
+_transforms_active = torch._C._are_functorch_transforms_active
+_dispatch_modes = torch._C._len_torch_dispatch_stack
+_is_tracing = torch._C._is_tracing
+_PLAIN = frozenset((torch.Tensor, torch.nn.Parameter, type(None)))
+
+
 def interposed() -> bool:
     """Whether something has to see an op's call before the CUDA implementation runs: `torch.compile`, a `torch.func`
     transform, a dispatch mode (`make_fx`, a FLOP counter, a checkpointing policy, fake tensors) or `torch.jit.trace`.  A
     launcher that is called past them writes through an address they know nothing of, and a graph they record lacks it."""
-    return (torch.compiler.is_compiling() or torch._C._are_functorch_transforms_active()
-            or torch._C._len_torch_dispatch_stack() > 0 or torch._C._is_tracing())
+    return bool(_is_compiling() or _dispatch_modes() or _transforms_active() or _is_tracing())
 
 
 def eager(t: torch.Tensor, *others) -> bool:
     """Whether an op on these operands would only be dispatched back into this package's CUDA implementation (plain CUDA
     tensors, nothing interposed): the package's own functions then call the launcher itself and save a dispatch of a few
     microseconds.  What is no tensor is the launcher's to refuse."""
-    if not t.is_cuda or interposed():
+    if not t.is_cuda or _is_compiling() or _dispatch_modes() or _transforms_active() or _is_tracing():
         return False
-    for operand in (t, *others):
-        kind = type(operand)
-        if kind is not torch.Tensor and kind is not torch.nn.Parameter and isinstance(operand, torch.Tensor):
+    if type(t) not in _PLAIN:
+        return False
+    for operand in others:
+        if type(operand) not in _PLAIN and isinstance(operand, torch.Tensor):
             return False
     return True
 
@@ -43,7 +51,7 @@ def transformed() -> bool:
     """Whether a `torch.func` transform is active that differentiates or batches an `autograd.Function` with a
     `setup_context`; a formula registered for an op cannot be differentiated there.  (`functionalize` is the other way
     round: it takes ops and no such functions.)"""
-    if torch.compiler.is_compiling() or not torch._C._are_functorch_transforms_active():
+    if _is_compiling() or not _transforms_active():
         return False
     levels = torch._C._functorch.get_interpreter_stack() or ()
     return all(level.key() != torch._C._functorch.TransformType.Functionalize for level in levels)
