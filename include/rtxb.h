@@ -272,7 +272,8 @@ int rtxb_mxfp8_linear_epilogue_fwd_prequant_w(const void* x_bf16, int64_t ldx, c
  *     dx    = dz w, dw = dz^T x                     as rtxb_mxfp8_linear_bwd of dz
  *     dbias = bf16( sum over the rows of dy act'(z) )   FP32 sums in a fixed order
  * (the residual's gradient is dy itself).  dx [m, k], dw [n, k], dbias [n], any of them NULL to leave it out; w is read
- * for dx only, x for dw only.  dz never reaches memory: one launch reads dy and z once and writes both quantizations. */
+ * for dx only, x for dw only.  dz never reaches memory: one launch reads dy and z once and writes both quantizations.
+ * dw is BF16 only: a sum of it over ranks adds rounded parts, where rtxb_mxfp8_linear_bwd can leave FP32 ones. */
 size_t rtxb_mxfp8_linear_epilogue_backward_workspace_bytes(int64_t m, int64_t n, int64_t k, int need_dx, int need_dw,
                                                            int need_dbias);
 int rtxb_mxfp8_linear_epilogue_bwd(const void* dy_bf16, int64_t lddy, const void* z_bf16, const void* x_bf16, int64_t ldx,
@@ -306,8 +307,8 @@ int rtxb_mxfp8_grouped_linear_fwd_prequant_w(const void* x_bf16, int64_t ldx, co
  *     dx[r] = dy[r] w[g]                    operands quantized in blocks of 32 along n
  *     dw[g] = dy_g^T x_g                    blocks of 32 along the group's rows, counted from its first row
  * dx BF16 [rows, k] (zero in rows of no group), dw BF16 [groups, n, k] (zero for a group without rows), contiguous;
- * either may be NULL to leave that product out (then w, respectively x, is not read).  One quantizer launch, one GEMM
- * per product. */
+ * either may be NULL to leave that product out (then w, respectively x, is not read).  dw is BF16 only, as in
+ * rtxb_mxfp8_linear_epilogue_bwd.  One quantizer launch, one GEMM per product. */
 size_t rtxb_mxfp8_grouped_backward_workspace_bytes(int64_t rows, int64_t n, int64_t k, int64_t groups, int need_dx,
                                                    int need_dw);
 int rtxb_mxfp8_grouped_linear_bwd(const void* dy_bf16, int64_t lddy, const void* x_bf16, int64_t ldx, const void* w_bf16,

@@ -5,8 +5,9 @@
 //   partial[m / 128][n] = sum of 128 rows of dz in FP32, before the rounding   (dbias, finished by quant_mxfp8_transposed_units_kernel)
 // dy and z are read once (4 bytes per value), 2 bytes of payload leave: without the fusion dz is written and read again
 // (4 more).  One 128 x 128 tile per block step; three blocks per SM overlap one another's loads, arithmetic and stores.
-// Measured, gelu, 8192 x 8192: 108 to 112 us, 3.7 TB/s, 0.56 of the copy rate, bound by instructions (63 % issue): 29 a
-// value, 17 of them before the quantization.  With slopes evaluated instead of looked up 148 us.
+// Measured, gelu, 8192 x 8192 (409 MB): 93 us at 1965 MHz (4.4 TB/s, 0.67 of the copy rate), 126 us at 1390 MHz, where the
+// GEMMs of a training step hold the power cap.  The time goes with the clock, because instructions bound it (63 % issue): 29
+// a value, 17 of them before the quantization.  Evaluating the slopes instead of looking them up takes a third longer.
 #pragma once
 
 #include "activation.cuh"
@@ -33,8 +34,8 @@ constexpr int kActSumRows = kQuantThreads / 32;   // partial column sums per til
 // looked up.  For each of them act'(z) = 1 - act'(-z) (f(z) - f(-z) = z), so the table holds the slopes of negative z, which
 // keep their relative accuracy however small, and a positive z takes 1 less its entry.  Below 2^-21 the slope is within
 // 8e-7 of 1/2, beyond +-128 it is 1 or 0.  That is a third of the instructions of an evaluation, and instructions are what
-// bounds the pass.  A second table for positive z saves three instructions a pair and is slower (98 -> 122 us at the size
-// above; relu, which reads no table, 88 -> 110): three blocks with 31 KB of tables each leave L1 too little.
+// bounds the pass.  A second table for positive z saves three instructions a pair and is a quarter slower (for relu too, which
+// reads no table): three blocks with 31 KB of tables each leave L1 too little.
 constexpr int kSlopeLow = 106 << 7, kSlopeHigh = 134 << 7;     // BF16 magnitudes of 2^-21 and 128
 constexpr int kSlopeEntries = kSlopeHigh - kSlopeLow + 1;
 constexpr int act_smem_bytes(bool lookup) { return kQtTileBytes + (lookup ? (kSlopeEntries * 4 + 15) / 16 * 16 : 0); }

@@ -245,7 +245,8 @@ def mxfp8_linear_epilogue_backward(grad_output: torch.Tensor, z: Optional[torch.
                                    weight: torch.Tensor, *, activation: str = "none",
                                    bias: bool = True) -> Tuple[torch.Tensor, torch.Tensor, Optional[torch.Tensor]]:
     """BF16 (dX, dW, dbias) of `mxfp8_linear_epilogue`; `z` is the pre-activation in BF16 (None for activation "none"),
-    `bias=False` leaves dbias out (None).  The residual's gradient is grad_output."""
+    `bias=False` leaves dbias out (None).  The residual's gradient is grad_output.  There is no FP32 dW for sums over ranks,
+    as the dense linear's backward has one."""
     refuse_tangents("mxfp8_linear_epilogue_backward", grad_output, z, x, weight)
     n, k = weight.shape
     if activation != "none" and z is None:

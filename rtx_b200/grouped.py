@@ -235,7 +235,8 @@ def _dynamic(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor) -> to
 def mxfp8_grouped_linear_backward(grad_output: torch.Tensor, x: torch.Tensor, weight: torch.Tensor,
                                   offsets: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """BF16 dX [rows, K] and dW [groups, N, K] of `mxfp8_grouped_linear`, from independently quantized MXFP8 products
-    (blocks along N for dX, along each group's rows for dW)."""
+    (blocks along N for dX, along each group's rows for dW).  There is no FP32 dW for sums over ranks, as the dense linear's
+    backward has one."""
     refuse_tangents("mxfp8_grouped_linear_backward", grad_output, x, weight)
     if eager(x, grad_output, weight, offsets):
         return mxfp8_grouped_linear_bwd.fn(grad_output, x, weight, offsets)
