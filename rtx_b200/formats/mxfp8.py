@@ -165,7 +165,7 @@ def mxfp8_state_for_kernel(state_dict: dict, prefix: str, rows: int, k: int) -> 
     kernels take: row-major scales become mma128 tiles, in place in `state_dict`.  Returns what keeps it from being loaded
     as a [rows, k] weight, or None.  Both layouts often have the same size, so only the meta tells them apart."""
     meta = state_dict.get(prefix + "weight_packing_meta")
-    if meta is None:
+    if meta is None or meta.is_meta:     # nothing to read
         return None
     storage_k = (k + 31) // 32 * 32
     found = [int(v) for v in meta.reshape(-1)]

@@ -36,6 +36,7 @@ def test_what_cannot_be_loaded_is_said():
                                (state("mma64", 128, 128)[0], 128, 128, "mma64")):
         assert why in mxfp8_state_for_kernel(held, "a.", rows, k)
     assert mxfp8_state_for_kernel({}, "a.", 128, 128) is None        # nothing to load: strict loading says what is missing
+    assert mxfp8_state_for_kernel({k: v.to("meta") for k, v in state("mma128", 128, 128)[0].items()}, "a.", 128, 128) is None
     held, _ = state("row_major", 128, 128)
     del held["a.weight_scales"]
     assert mxfp8_state_for_kernel(held, "a.", 128, 128) is None
