@@ -80,10 +80,21 @@ def call_without_derivative(op: "OpHandle", message: str, *args):
 
 
 def refuse_tangents(name: str, *tensors) -> None:
-    """Forward-mode differentiation of an op without a formula for it would drop the tangents: refuse it."""
-    if forward_ad._current_level >= 0 and not torch.compiler.is_compiling():
-        if any(isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
-            raise NotImplementedError(f"{name} has no forward-mode derivative")
+    """Forward-mode differentiation of an op without a formula for it would drop the tangents: refuse it.  (A tangent below
+    a `vmap` cannot be looked at; the graph nodes of `torch.func` transforms refuse it where the batch is unpacked.)"""
+    if forward_ad._current_level >= 0 and not _is_compiling():
+        for t in tensors:
+            if isinstance(t, torch.Tensor) and not torch._C._functorch.is_batchedtensor(t):
+                if forward_ad.unpack_dual(t).tangent is not None:
+                    raise NotImplementedError(f"{name} has no forward-mode derivative")
+
+
+def no_tangents(name: str) -> Callable:
+    """The `jvp` of a graph node without one."""
+    def jvp(ctx, *tangents):
+        raise NotImplementedError(f"{name} has no forward-mode derivative")
+
+    return jvp
 
 
 class OpHandle:

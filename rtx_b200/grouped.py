@@ -21,7 +21,7 @@ from torch.autograd.function import once_differentiable
 
 from . import fp8 as _fp8
 from . import ops
-from ._oplib import call_without_derivative, custom_op, eager, refuse_tangents, transformed
+from ._oplib import call_without_derivative, custom_op, eager, no_tangents, refuse_tangents, transformed
 from .formats import (PACKED_OPERAND_SCHEMA_VERSION, SCALE_LAYOUT_CODES, MXFP8Tensor, make_mxfp8_tensor,
                       mxfp8_kernel_operands, mxfp8_qdata_2d, mxfp8_scales_for_kernel, mxfp8_state_for_kernel,
                       reject_packed_dtype_conversion)
@@ -181,8 +181,13 @@ class _TransformedGroupedLinear(torch.autograd.Function):
     def forward(x, weight, offsets):
         return mxfp8_grouped_linear_op(x, weight, offsets)
 
-    setup_context = staticmethod(_train_setup)
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        _train_setup(ctx, inputs, output)
+        ctx.save_for_forward(*inputs)      # a batched `jvp` looks for them
+
     backward = staticmethod(_dispatched_backward)
+    jvp = staticmethod(no_tangents("mxfp8_grouped_linear"))
 
 
 def _packed_group_shape(weight) -> Tuple[int, int, int]:

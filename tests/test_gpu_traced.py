@@ -214,3 +214,74 @@ def test_offsets_that_are_no_tensor_are_named(dev):
     for weight in (w, r.quantize_mxfp8(w)):
         with pytest.raises(TypeError, match="offsets must be a torch.Tensor"):
             r.mxfp8_grouped_linear(x, weight, [0, 4, 8])
+
+
+@pytest.mark.parametrize("act", ["none", "relu2"])
+def test_func_transforms_without_bias_and_residual(dev, act):
+    """What is left out is no operand of a transform; activation "none" keeps no z."""
+    import rtx_b200 as r
+
+    x, w, b, res = calls(dev)["epilogue"][1]
+    xs = torch.stack([x, x.flip(0)])
+    for bias, residual in ((None, None), (b, None), (None, res)):
+        f = lambda x, w: r.mxfp8_linear_epilogue(x, w, bias, residual, activation=act)
+        same(torch.func.vmap(f, (0, None))(xs, w), torch.stack([f(t, w) for t in xs]))
+        leaves = [x.clone().requires_grad_(True), w.clone().requires_grad_(True)]
+        loss = lambda x, w: f(x, w).float().sum()
+        want = torch.autograd.grad(loss(*leaves), leaves)
+        same(torch.func.grad(loss, argnums=(0, 1))(x, w), want)
+        each = torch.func.vmap(torch.func.grad(loss), (0, None))(xs, w)
+        same(each[0], want[0])
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_no_form_drops_a_tangent(dev, name):
+    """Forward-mode calls are refused, also where vmap hides the tangent from the function."""
+    f, first, _, _ = calls(dev)[name]
+    rest = first[1:]
+
+    def total(t):
+        out = f(t, *rest)
+        return sum(v.float().sum() for v in (out if isinstance(out, tuple) else (out,)))
+
+    x, t = first[0], torch.ones_like(first[0])
+    batched = lambda v: torch.func.vmap(total)(torch.stack([v, v])).sum()
+    for g in (total, batched):
+        with pytest.raises(NotImplementedError):
+            torch.func.jvp(g, (x,), (t,))
+    # constants of the transform, batched below it, have no tangent to drop
+    one = torch.ones((), device=dev)
+    part = lambda v: out[0] if isinstance(out := f(v, *rest), tuple) else out
+    got = torch.func.jvp(lambda s: torch.func.vmap(part)(torch.stack([x, x])) * s, (one,), (one,))
+    same(got[1][1], part(x))
+    if name in ("grouped", "epilogue"):
+        few = lambda v: f(v.bfloat16(), *rest).float().square().sum()
+        with pytest.raises(NotImplementedError):
+            torch.func.jvp(torch.func.grad(few), (x,), (t,))                 # forward over reverse
+
+
+@pytest.mark.parametrize("name", ["grouped", "epilogue"])
+def test_checkpointed_training(dev, name):
+    """Activation checkpointing, plain and by a policy that names the op, gives the bits of the plain step."""
+    import functools
+
+    from torch.utils.checkpoint import CheckpointPolicy, checkpoint, create_selective_checkpoint_contexts
+
+    f, first, _, _ = calls(dev)[name]
+    leaves = [t.requires_grad_(True) for t in first if t.is_floating_point()]
+    dy = torch.randn_like(f(*first))
+    want = torch.autograd.grad(f(*first) * 2, leaves, dy)
+    op = torch.ops.rtx.mxfp8_grouped_linear_train if name == "grouped" else torch.ops.rtx.mxfp8_linear_epilogue_train
+    named = []
+
+    def policy(ctx, func, *args, **kwargs):
+        if func is op.default:
+            named.append(func)
+            return CheckpointPolicy.MUST_SAVE
+        return CheckpointPolicy.PREFER_RECOMPUTE
+
+    run = lambda *args: f(*args) * 2
+    for kwargs in ({}, {"context_fn": functools.partial(create_selective_checkpoint_contexts, policy)}):
+        y = checkpoint(run, *first, use_reentrant=False, **kwargs)
+        same(torch.autograd.grad(y, leaves, dy), want)
+    assert named
