@@ -79,6 +79,14 @@ def call_without_derivative(op: "OpHandle", message: str, *args):
     return _Once.apply(op, message, *args) if transformed() else op(*args)
 
 
+def call_detached(op: "OpHandle", message: str, *args):
+    """The same for a function whose results carry no gradient, whatever its operands: as in an eager call, also where a
+    graph is recorded."""
+    if transformed():
+        return _Once.apply(op, message, *args)
+    return op(*(a.detach() if isinstance(a, torch.Tensor) else a for a in args))
+
+
 def refuse_tangents(name: str, *tensors) -> None:
     """Forward-mode differentiation of an op without a formula for it would drop the tangents: refuse it.  (A tangent below
     a `vmap` cannot be looked at; the graph nodes of `torch.func` transforms refuse it where the batch is unpacked.)"""

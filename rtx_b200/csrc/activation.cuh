@@ -92,9 +92,9 @@ __device__ __forceinline__ void relu_slope2(float& gx, float& gy, float x, float
 }
 
 // act'(-a), 0 <= a <= 128, of silu and the two gelus: the entries of the backward's table, a few thousand per block, so they
-// are made to FP32 accuracy (a few 2^-24 of the slope, also beside its zero).  A slope that is off by 3 2^-24 of 1/2 moves
-// dz across a BF16 rounding, and now and then an E4M3 code behind it, for every gradient of an unlucky z: in the training
-// step of 8192 x 4096 x 8192 that was 2.1e-4 of dx (2-norm), where the MMAs' accumulation is 1.2e-4 and these entries are 0.
+// are made to FP32 accuracy (a few 2^-24 of the slope, also beside its zero).  A slope that is off by 3e-7 moves dz across a
+// BF16 rounding, and now and then an E4M3 code behind it, for every gradient of an unlucky z: in the training step of
+// 8192 x 4096 x 8192 that was 2.1e-4 of dx (2-norm), where the MMAs' accumulation is 1.2e-4 and these entries are 0.
 //   silu, gelu_tanh  with s(-u) = q / (1 + q), q = e^-u:   q (1 - a u'(a) + q) / (1 + q)^2;  u = a,  or 2 A (a + B a^3)
 //   gelu             Phi(-a) - a phi(a) = e^(-a^2 / 2) (a0 - a) h(a): a0 its zero, in two parts, h a polynomial in
 //                    1 / (1 + 0.32 a) fitted as above on 0 <= a <= 14 (4.6e-8)

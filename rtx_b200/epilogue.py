@@ -17,7 +17,8 @@ from torch.autograd.function import once_differentiable
 
 from . import fp8 as _fp8
 from . import ops
-from ._oplib import call_without_derivative, custom_op, eager, no_tangents, refuse_tangents, transformed
+from ._oplib import (call_detached, call_without_derivative, custom_op, eager, no_tangents, refuse_tangents,
+                     transformed)
 from .formats import (PACKED_OPERAND_SCHEMA_VERSION, SCALE_LAYOUT_CODES, MXFP8Tensor, make_mxfp8_tensor,
                       mxfp8_kernel_operands, mxfp8_matrix_shape, mxfp8_qdata_2d, mxfp8_scales_for_kernel,
                       mxfp8_state_for_kernel, reject_packed_dtype_conversion)
@@ -264,7 +265,7 @@ def mxfp8_linear_epilogue_backward(grad_output: torch.Tensor, z: Optional[torch.
     if eager(x, grad_output, z2d, weight):
         dx, dw, db = mxfp8_linear_epilogue_bwd.fn(*args)
     else:
-        dx, dw, db = call_without_derivative(mxfp8_linear_epilogue_bwd, _TWICE, *args)
+        dx, dw, db = call_detached(mxfp8_linear_epilogue_bwd, _TWICE, *args)
     return dx.reshape(x.shape), dw, db if bias else None
 
 

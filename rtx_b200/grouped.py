@@ -21,7 +21,7 @@ from torch.autograd.function import once_differentiable
 
 from . import fp8 as _fp8
 from . import ops
-from ._oplib import call_without_derivative, custom_op, eager, no_tangents, refuse_tangents, transformed
+from ._oplib import call_detached, call_without_derivative, custom_op, eager, no_tangents, refuse_tangents, transformed
 from .formats import (PACKED_OPERAND_SCHEMA_VERSION, SCALE_LAYOUT_CODES, MXFP8Tensor, make_mxfp8_tensor,
                       mxfp8_kernel_operands, mxfp8_qdata_2d, mxfp8_scales_for_kernel, mxfp8_state_for_kernel,
                       reject_packed_dtype_conversion)
@@ -245,7 +245,7 @@ def mxfp8_grouped_linear_backward(grad_output: torch.Tensor, x: torch.Tensor, we
     refuse_tangents("mxfp8_grouped_linear_backward", grad_output, x, weight)
     if eager(x, grad_output, weight, offsets):
         return mxfp8_grouped_linear_bwd.fn(grad_output, x, weight, offsets)
-    return call_without_derivative(mxfp8_grouped_linear_bwd, _TWICE, grad_output, x, weight, offsets)
+    return call_detached(mxfp8_grouped_linear_bwd, _TWICE, grad_output, x, weight, offsets)
 
 
 class MXFP8GroupedLinear(nn.Module):

@@ -285,3 +285,16 @@ def test_checkpointed_training(dev, name):
         y = checkpoint(run, *first, use_reentrant=False, **kwargs)
         same(torch.autograd.grad(y, leaves, dy), want)
     assert named
+
+
+@pytest.mark.parametrize("name", ["grouped backward", "epilogue backward"])
+def test_backward_functions_carry_no_gradient(dev, name):
+    """With operands that require one, too: eager, compiled and recorded alike."""
+    f, first, other, _ = calls(dev)[name]
+    first, other = (tuple(t.requires_grad_(True) if t.is_floating_point() else t for t in v) for v in (first, other))
+    want = f(*other)
+    compiled = torch.compile(f, fullgraph=True)
+    for g in (f, compiled, make_fx(f)(*first), torch.jit.trace(f, first, check_trace=False)):
+        got = g(*other)
+        same(got, want)
+        assert not any(t.requires_grad for t in got)
